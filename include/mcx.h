@@ -13,7 +13,7 @@
  *   - `stream` is a hipStream_t passed as void*; NULL is the default stream.
  *     Calls only enqueue work; they never synchronise or allocate.
  *   - `dtype` selects the data scalar: MCX_F32, MCX_F64, or MCX_BF16
- *     (convolution entry points only; accumulation is fp32).  sample_map and
+ *     (convolution and attention entry points only; accumulation is fp32).  sample_map and
  *     interp_weights have the data's type for F32/F64 and are float for BF16.
  *   - `interp`: 0 nearest (also any other value), 1 bilinear, 2 bispherical
  *     (include/core/resample.h:62-90).
@@ -405,6 +405,86 @@ int mcx_planar_conv_operator(const float *samples, const float *vertices, const 
                              int64_t *face_idx, int64_t *vertex_idx, float *weights,
                              void *workspace, size_t workspace_bytes, int64_t N, int64_t V,
                              int64_t F, int nearest, void *stream);
+
+/* ---- Attention with a bias by relative-position buckets, and what goes with it ----------
+ * No counterpart in the reference.  Data is MCX_F32 or MCX_BF16; weights and bias tables have
+ * the data's type; every sum, statistic and accumulation is fp32. */
+
+/* Norm of queries and keys per head with the position rotation in the same pass.
+ * q [B, L, Hq, D], k [B, L, Hk, D], the last axis dense, the other strides (in values) given;
+ * wq, wk [D]; cos, sin float [places, F], F = rotated / 2;
+ * positions int64 [B, L], or NULL for the index along L.
+ *   n = x / sqrt(mean(x^2) + eps) * w;  of the first 2 F values, the pairs (f, f + F), or with
+ *   `adjacent` (2 f, 2 f + 1), are turned:  a c - b s, b c + a s.
+ * q_out, k_out are contiguous.  A position outside [0, places) gives NaN.  1 <= D <= 256. */
+int mcx_qk_norm_rotate_forward(const void *q, const void *k, const void *wq, const void *wk,
+                               const float *cos, const float *sin, const int64_t *positions,
+                               void *q_out, void *k_out, const int64_t *q_stride,
+                               const int64_t *k_stride, int64_t B, int64_t L, int64_t Hq,
+                               int64_t Hk, int64_t D, int64_t F, int64_t places, double eps,
+                               int adjacent, int dtype, void *stream);
+/* Gradients: gq, gk (contiguous, of q_out and k_out) -> gq_in, gk_in (contiguous), gwq, gwk [D]. */
+size_t mcx_qk_norm_rotate_backward_workspace(int64_t B, int64_t L, int64_t Hq, int64_t Hk,
+                                             int64_t D, int dtype);
+int mcx_qk_norm_rotate_backward(const void *gq, const void *gk, const void *q, const void *k,
+                                const void *wq, const void *wk, const float *cos, const float *sin,
+                                const int64_t *positions, void *gq_in, void *gk_in, void *gwq,
+                                void *gwk, void *workspace, size_t workspace_bytes,
+                                const int64_t *q_stride, const int64_t *k_stride, int64_t B,
+                                int64_t L, int64_t Hq, int64_t Hk, int64_t D, int64_t F,
+                                int64_t places, double eps, int adjacent, int dtype, void *stream);
+
+/* Sizes of an attention call.  Strides in values, of batch, token and head; the last axis is
+ * dense.  Any alignment goes; 16-byte aligned rows are read in 16-byte words.
+ * 1 <= D <= 128, Hk divides Hq, table_size <= 512 (0: no bias), scale in [1e-6, 1e6]. */
+typedef struct mcx_attention_desc {
+  int64_t B, Lq, Lk, Hq, Hk, D;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  int64_t bucket_count; /* entries of `buckets` */
+  int64_t bucket_zero;  /* the entry of difference 0 */
+  int64_t table_size;   /* buckets of a head */
+  double scale;
+  int32_t causal;
+  int32_t reserved; /* 0 */
+} mcx_attention_desc;
+
+/* out[b,i,h] = sum_j softmax_j(scale q[b,i,h].k[b,j,g] + table[h, buckets[x]]) v[b,j,g]
+ *   x = clamp(j - (query_start[b] + i) + bucket_zero, 0, bucket_count - 1),  g = h / (Hq / Hk)
+ * over the keys j < key_lengths[b] and, if causal, j <= query_start[b] + i.
+ *   q [B, Lq, Hq, D], k, v [B, Lk, Hk, D], table [Hq, table_size] and buckets int32 or both NULL,
+ *   query_start int32 [B] or NULL (zeros), key_lengths int32 [B] or NULL (Lk; clamped to [0, Lk]),
+ *   out [B, Lq, Hq, D] contiguous, stats float [B, Hq, Lq, 2] for the gradients, or NULL.
+ * A row that nothing is left of is zeros.  What lies at keys from key_lengths[b] on is not read.
+ * A bucket outside [0, table_size) has no bias; a bias of -inf takes its pairs out; a finite bias
+ * is held within 1e30.
+ * Few queries against many keys are split over the keys and joined; that takes a workspace of
+ * mcx_attention_forward_workspace() bytes (0: none). */
+size_t mcx_attention_forward_workspace(const mcx_attention_desc *desc, int dtype);
+int mcx_attention_forward(const void *q, const void *k, const void *v, const void *table,
+                          const int32_t *buckets, const int32_t *query_start,
+                          const int32_t *key_lengths, void *out, float *stats, void *workspace,
+                          size_t workspace_bytes, const mcx_attention_desc *desc, int dtype,
+                          void *stream);
+
+/* Gradients from gout (contiguous) and the forward call's out and stats: gq [B, Lq, Hq, D],
+ * gk, gv [B, Lk, Hk, D] (zeros at keys that are not in use), gtable [Hq, table_size], all
+ * contiguous; NULL for a gradient that is not wanted.  The same bits from call to call. */
+size_t mcx_attention_backward_workspace(const mcx_attention_desc *desc, int dtype);
+int mcx_attention_backward(const void *gout, const void *q, const void *k, const void *v,
+                           const void *out, const float *stats, const void *table,
+                           const int32_t *buckets, const int32_t *query_start,
+                           const int32_t *key_lengths, void *gq, void *gk, void *gv, void *gtable,
+                           void *workspace, size_t workspace_bytes, const mcx_attention_desc *desc,
+                           int dtype, void *stream);
+
+/* Clipping by the global norm: norm[0] = sqrt(sum of squares over all tensors), out = in *
+ * min(1, max_norm / (norm + eps)); out[t] may be in[t].  in, out, sizes (values) and dtypes are
+ * HOST arrays of `count` entries, read before the call returns; a NULL `out` asks for the norm
+ * alone.  max_norm >= 0. */
+size_t mcx_clip_grad_norm_workspace(const int64_t *sizes, int64_t count);
+int mcx_clip_grad_norm(const void *const *in, void *const *out, const int64_t *sizes,
+                       const int32_t *dtypes, int64_t count, double max_norm, double eps,
+                       float *norm, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -856,3 +856,273 @@ def planar_conv_operator_from_samples(samples, vertices, faces, keepdim=True, ne
                                           _stream(samples))
     _lib.check(rc, "planar_conv_operator_from_samples")
     return [face_idx, vertex_idx, weights]
+
+
+# ---- attention with a bias by relative-position buckets, and what goes with it -------------
+# (no counterpart in the reference)
+
+def _attention_dtype(data, **same):
+    """Data type code of the attention operators: float32 or bfloat16, one for all operands."""
+    if data.dtype != torch.float32 and data.dtype != torch.bfloat16:
+        raise RuntimeError("unsupported dtype %s (float32 or bfloat16)" % data.dtype)
+    for name, t in same.items():
+        if t is not None and t.dtype != data.dtype:
+            raise RuntimeError("%s is %s, expected %s" % (name, t.dtype, data.dtype))
+    return _DTYPES[data.dtype]
+
+
+def _heads(name, t, B=None, L=None, H=None, D=None):
+    """Shape of a [B, L, H, D] tensor whose last axis is dense."""
+    if t.dim() != 4:
+        raise RuntimeError("%s must have 4 dimensions [B, L, H, D], got %s" % (name, tuple(t.shape)))
+    for axis, (got, want) in enumerate(zip(t.shape, (B, L, H, D))):
+        if want is not None and got != want:
+            raise RuntimeError("%s has size %d in dimension %d, expected %d" %
+                               (name, got, axis, want))
+    return t.shape
+
+
+def _dense_last(t):
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+def _norm_args(query, key, query_weight, key_weight, cos, sin, positions, eps):
+    B, L, Hq, D = _heads("query", query)
+    _, _, Hk, _ = _heads("key", key, B, L, None, D)
+    dt = _attention_dtype(query, key=key, query_weight=query_weight, key_weight=key_weight)
+    _on_gpu("query", query, key=key, query_weight=query_weight, key_weight=key_weight, cos=cos,
+            sin=sin, positions=positions)
+    if Hq < 1 or Hk < 1 or not 1 <= D <= 256:
+        raise RuntimeError("heads of 1 to 256 values are supported (got %d heads, %d key heads, "
+                           "%d values)" % (Hq, Hk, D))
+    for name, w in (("query_weight", query_weight), ("key_weight", key_weight)):
+        if tuple(w.shape) != (D,):
+            raise RuntimeError("%s must have shape (%d,), got %s" % (name, D, tuple(w.shape)))
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise RuntimeError("cos and sin must be float32")
+    if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > D:
+        raise RuntimeError("cos and sin must have the same shape [places, F] with 2 F <= %d, got "
+                           "%s and %s" % (D, tuple(cos.shape), tuple(sin.shape)))
+    if positions is not None:
+        if positions.dtype != torch.int64 or tuple(positions.shape) != (B, L):
+            raise RuntimeError("positions must be int64 of shape (%d, %d), got %s %s" %
+                               (B, L, positions.dtype, tuple(positions.shape)))
+        positions = positions.contiguous()
+    elif cos.shape[0] < L:
+        raise RuntimeError("cos and sin have %d places for %d positions" % (cos.shape[0], L))
+    if not eps >= 0:
+        raise RuntimeError("eps must not be negative")
+    _contig(query_weight=query_weight, key_weight=key_weight)
+    return (dt, B, L, Hq, Hk, D, _dense_last(query), _dense_last(key), cos.contiguous(),
+            sin.contiguous(), positions)
+
+
+def _strides(t):
+    return (_lib._i64 * 3)(t.stride(0), t.stride(1), t.stride(2))
+
+
+def qk_norm_rotate_forward(query, key, query_weight, key_weight, cos, sin, positions=None,
+                           eps=1e-6, adjacent=False):
+    """Queries [B, L, Hq, D] and keys [B, L, Hk, D] (views of a packed projection go as they are),
+    every head of every token divided by its root mean square and multiplied by query_weight /
+    key_weight [D]; then the first 2 F values of each turned by the angles of the token's place:
+    cos, sin float32 [places, F], the place being `positions` [B, L] (int64) or the index along
+    L.  A pair is (f, f + F), or (2 f, 2 f + 1) if `adjacent`.  -> [query, key], contiguous.
+    A position outside the places gives NaN."""
+    dt, B, L, Hq, Hk, D, query, key, cos, sin, positions = _norm_args(
+        query, key, query_weight, key_weight, cos, sin, positions, eps)
+    q_out = torch.empty((B, L, Hq, D), dtype=query.dtype, device=query.device)
+    k_out = torch.empty((B, L, Hk, D), dtype=query.dtype, device=query.device)
+    with _device(query):
+        rc = _lib.load().mcx_qk_norm_rotate_forward(
+            _ptr(query), _ptr(key), _ptr(query_weight), _ptr(key_weight), _ptr(cos), _ptr(sin),
+            _ptr(positions), _ptr(q_out), _ptr(k_out), _strides(query), _strides(key), B, L, Hq,
+            Hk, D, cos.shape[1], cos.shape[0], float(eps), int(bool(adjacent)), dt, _stream(query))
+    _lib.check(rc, "qk_norm_rotate_forward")
+    return [q_out, k_out]
+
+
+def qk_norm_rotate_backward(grad_query, grad_key, query, key, query_weight, key_weight, cos, sin,
+                            positions=None, eps=1e-6, adjacent=False):
+    """-> [grad_query, grad_key, grad_query_weight, grad_key_weight] of qk_norm_rotate_forward
+    from the gradients of its outputs."""
+    dt, B, L, Hq, Hk, D, query, key, cos, sin, positions = _norm_args(
+        query, key, query_weight, key_weight, cos, sin, positions, eps)
+    _heads("grad_query", grad_query, B, L, Hq, D)
+    _heads("grad_key", grad_key, B, L, Hk, D)
+    _attention_dtype(query, grad_query=grad_query, grad_key=grad_key)
+    _on_gpu("query", query, grad_query=grad_query, grad_key=grad_key)
+    grad_query, grad_key = grad_query.contiguous(), grad_key.contiguous()
+    gq, gk = torch.empty_like(grad_query), torch.empty_like(grad_key)
+    gwq, gwk = torch.empty_like(query_weight), torch.empty_like(key_weight)
+    lib = _lib.load()
+    nbytes = lib.mcx_qk_norm_rotate_backward_workspace(B, L, Hq, Hk, D, dt)
+    ws = _workspace(nbytes, query.device)
+    with _device(query):
+        rc = lib.mcx_qk_norm_rotate_backward(
+            _ptr(grad_query), _ptr(grad_key), _ptr(query), _ptr(key), _ptr(query_weight),
+            _ptr(key_weight), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(gq), _ptr(gk), _ptr(gwq),
+            _ptr(gwk), _ptr(ws), nbytes, _strides(query), _strides(key), B, L, Hq, Hk, D,
+            cos.shape[1], cos.shape[0], float(eps), int(bool(adjacent)), dt, _stream(query))
+    _lib.check(rc, "qk_norm_rotate_backward")
+    return [gq, gk, gwq, gwk]
+
+
+def _attention_args(query, key, value, bias_table, buckets, bucket_zero, scale, causal,
+                    query_start, key_lengths):
+    """(dtype code, descriptor, the tensors as the library takes them) of an attention call."""
+    B, Lq, Hq, D = _heads("query", query)
+    _, Lk, Hk, _ = _heads("key", key, B, None, None, D)
+    _heads("value", value, B, Lk, Hk, D)
+    dt = _attention_dtype(query, key=key, value=value, bias_table=bias_table)
+    _on_gpu("query", query, key=key, value=value, bias_table=bias_table, buckets=buckets,
+            query_start=query_start, key_lengths=key_lengths)
+    if Hk < 1 or Hq % Hk or Hq < 1:
+        raise RuntimeError("%d query heads cannot share %d key heads" % (Hq, Hk))
+    if not 1 <= D <= 128:
+        raise RuntimeError("heads of 1 to 128 values are supported, got %d" % D)
+    if (bias_table is None) != (buckets is None):
+        raise RuntimeError("bias_table and buckets go together")
+    if bias_table is not None:
+        if bias_table.dim() != 2 or bias_table.shape[0] != Hq or \
+                not 1 <= bias_table.shape[1] <= 512:
+            raise RuntimeError("bias_table must be [%d, 1 to 512 buckets], got %s" %
+                               (Hq, tuple(bias_table.shape)))
+        if buckets.dtype != torch.int32 or buckets.dim() != 1:
+            raise RuntimeError("buckets must be a vector of int32, got %s %s" %
+                               (buckets.dtype, tuple(buckets.shape)))
+        if not 0 <= bucket_zero < buckets.shape[0]:
+            raise RuntimeError("bucket_zero %d is no entry of %d buckets" %
+                               (bucket_zero, buckets.shape[0]))
+        bias_table, buckets = bias_table.contiguous(), buckets.contiguous()
+    for name, t in (("query_start", query_start), ("key_lengths", key_lengths)):
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,)):
+            raise RuntimeError("%s must be int32 of shape (%d,), got %s %s" %
+                               (name, B, t.dtype, tuple(t.shape)))
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 1e-6 <= scale <= 1e6:
+        raise RuntimeError("scale must lie between 1e-6 and 1e6, got %g" % scale)
+    query, key, value = _dense_last(query), _dense_last(key), _dense_last(value)
+    if query_start is not None:
+        query_start = query_start.contiguous()
+    if key_lengths is not None:
+        key_lengths = key_lengths.contiguous()
+    n, size = (0, 0) if bias_table is None else (buckets.shape[0], bias_table.shape[1])
+    desc = _lib.AttentionDesc(B, Lq, Lk, Hq, Hk, D, _strides(query), _strides(key),
+                              _strides(value), n, int(bucket_zero) if n else 0, size, scale,
+                              int(bool(causal)), 0)
+    return dt, desc, (query, key, value, bias_table, buckets, query_start, key_lengths)
+
+
+def relative_attention_forward(query, key, value, bias_table=None, buckets=None, bucket_zero=0,
+                               scale=None, causal=False, query_start=None, key_lengths=None,
+                               for_backward=False):
+    """Attention of queries [B, Lq, Hq, D] over keys and values [B, Lk, Hk, D] (Hk divides Hq;
+    any strides with a dense last axis) with a learned bias by relative position:
+
+        out = softmax_j(scale q_i . k_j + bias_table[h, buckets[clamp(j - pos_i + bucket_zero)]]) v_j
+
+    query i standing at position pos_i = query_start[b] + i (0 + i by default) and key j at j.
+    bias_table [Hq, buckets of a head]; buckets int32, one entry a difference, the ends standing
+    for all beyond.  `causal` keeps the keys up to the query's own position; key_lengths int32 [B]
+    says how many keys are in use: what lies behind them is not read.  scale: D ** -0.5 by default.
+    A row that nothing is left of is zeros.  A bucket that the table does not have has no bias; a
+    bias of -inf takes its pairs out.
+    -> [out [B, Lq, Hq, D], stats]: stats, for relative_attention_backward, is None unless
+    `for_backward`.  Keys and values within key_lengths have to be finite."""
+    dt, desc, tensors = _attention_args(query, key, value, bias_table, buckets, bucket_zero, scale,
+                                        causal, query_start, key_lengths)
+    query = tensors[0]
+    B, Lq, Hq, D = query.shape
+    out = torch.empty((B, Lq, Hq, D), dtype=query.dtype, device=query.device)
+    stats = None
+    if for_backward:
+        stats = torch.empty((B, Hq, Lq, 2), dtype=torch.float32, device=query.device)
+    lib = _lib.load()
+    nbytes = lib.mcx_attention_forward_workspace(desc, dt)
+    ws = _workspace(nbytes, query.device) if nbytes else None
+    with _device(query):
+        rc = lib.mcx_attention_forward(*[_ptr(t) for t in tensors], _ptr(out), _ptr(stats),
+                                       _ptr(ws), nbytes, desc, dt, _stream(query))
+    _lib.check(rc, "relative_attention_forward")
+    return [out, stats]
+
+
+def relative_attention_backward(grad_output, query, key, value, output, stats, bias_table=None,
+                                buckets=None, bucket_zero=0, scale=None, causal=False,
+                                query_start=None, key_lengths=None,
+                                needs=(True, True, True, True)):
+    """-> [grad_query, grad_key, grad_value, grad_bias_table] of relative_attention_forward, called
+    with the same arguments and `for_backward`; a gradient that `needs` leaves out is None.  The
+    same bits from call to call."""
+    dt, desc, tensors = _attention_args(query, key, value, bias_table, buckets, bucket_zero, scale,
+                                        causal, query_start, key_lengths)
+    query, key, value, table = tensors[:4]
+    _heads("grad_output", grad_output, *query.shape)
+    _heads("output", output, *query.shape)
+    _attention_dtype(query, grad_output=grad_output, output=output)
+    _on_gpu("query", query, grad_output=grad_output, output=output, stats=stats)
+    B, Lq, Hq, D = query.shape
+    if stats is None or stats.dtype != torch.float32 or tuple(stats.shape) != (B, Hq, Lq, 2):
+        raise RuntimeError("stats must be what relative_attention_forward returned with for_backward")
+    grad_output, output, stats = grad_output.contiguous(), output.contiguous(), stats.contiguous()
+
+    def like(t, wanted):
+        return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None
+
+    gq, gk, gv = like(query, needs[0]), like(key, needs[1]), like(value, needs[2])
+    gt = like(table, needs[3]) if table is not None else None
+    if B == 0 or Lq == 0:
+        for t in (gk, gv, gt):
+            if t is not None:
+                t.zero_()
+        return [gq, gk, gv, gt]
+    lib = _lib.load()
+    nbytes = lib.mcx_attention_backward_workspace(desc, dt)
+    ws = _workspace(nbytes, query.device)
+    with _device(query):
+        rc = lib.mcx_attention_backward(_ptr(grad_output), *[_ptr(t) for t in tensors[:3]],
+                                        _ptr(output), _ptr(stats), *[_ptr(t) for t in tensors[3:]],
+                                        _ptr(gq), _ptr(gk), _ptr(gv), _ptr(gt), _ptr(ws), nbytes,
+                                        desc, dt, _stream(query))
+    _lib.check(rc, "relative_attention_backward")
+    return [gq, gk, gv, gt]
+
+
+def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
+    """The norm of all values of a list of tensors (float32 and bfloat16, contiguous, on one GPU),
+    as a float32 scalar; the tensors, or where `out` gives as many of the same sizes and types
+    those, hold min(1, max_norm / (norm + eps)) times the values then.  A norm that is no number
+    makes them all none."""
+    import ctypes
+    max_norm, eps = float(max_norm), float(eps)
+    if not max_norm >= 0 or not eps >= 0:
+        raise RuntimeError("max_norm and eps must not be negative")
+    tensors = list(tensors)
+    if not tensors:
+        raise RuntimeError("clip_grad_norm needs at least one tensor")
+    device, dtypes, n = tensors[0].device, [t.dtype for t in tensors], len(tensors)
+    to = tensors if out is None else list(out)
+    if [t.dtype for t in to] != dtypes or [t.shape for t in to] != [t.shape for t in tensors]:
+        raise RuntimeError("out must have the tensors' shapes and dtypes")
+    for t in tensors if out is None else tensors + to:
+        if t.device != device or not t.is_cuda:
+            raise RuntimeError("all tensors must be on one GPU")
+        if not t.is_contiguous():
+            raise RuntimeError("tensors must be contiguous")
+    codes = [_DTYPES.get(d, MCX_F64) for d in dtypes]
+    if MCX_F64 in codes:
+        raise RuntimeError("unsupported dtype %s (float32 or bfloat16)" % dtypes[codes.index(MCX_F64)])
+    pointers = ctypes.c_void_p * n
+    sizes = (_lib._i64 * n)(*[t.numel() for t in tensors])
+    inputs = pointers(*[t.data_ptr() for t in tensors])
+    outputs = inputs if out is None else pointers(*[t.data_ptr() for t in to])
+    lib = _lib.load()
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    nbytes = lib.mcx_clip_grad_norm_workspace(sizes, n)
+    ws = _workspace(nbytes, device)
+    with _device(norm):
+        rc = lib.mcx_clip_grad_norm(inputs, outputs, sizes, (ctypes.c_int32 * n)(*codes), n,
+                                    max_norm, eps, _ptr(norm), _ptr(ws), nbytes, _stream(norm))
+    _lib.check(rc, "clip_grad_norm")
+    return norm

@@ -27,6 +27,19 @@ class PlanDesc(ctypes.Structure):
 
 _desc = ctypes.POINTER(PlanDesc)
 
+
+class AttentionDesc(ctypes.Structure):
+    """mcx_attention_desc of include/mcx.h: the sizes of an attention call."""
+    _fields_ = [("B", _i64), ("Lq", _i64), ("Lk", _i64), ("Hq", _i64), ("Hk", _i64), ("D", _i64),
+                ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3),
+                ("bucket_count", _i64), ("bucket_zero", _i64), ("table_size", _i64),
+                ("scale", ctypes.c_double), ("causal", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+_adesc = ctypes.POINTER(AttentionDesc)
+_f64 = ctypes.c_double
+
 # name -> (restype, argtypes); mirrors include/mcx.h one to one.
 SIGNATURES = {
     "mcx_abi_version": (_i, []),
@@ -68,6 +81,16 @@ SIGNATURES = {
     "mcx_gnomonic_samples": (_i, [_p] * 2 + [_i64] * 3 + [ctypes.c_double] * 2 + [_p]),
     "mcx_planar_conv_operator_workspace": (_sz, [_i64]),
     "mcx_planar_conv_operator": (_i, [_p] * 7 + [_sz] + [_i64] * 3 + [_i, _p]),
+    "mcx_qk_norm_rotate_forward": (_i, [_p] * 9 + [_i64 * 3] * 2 + [_i64] * 7 + [_f64, _i, _i, _p]),
+    "mcx_qk_norm_rotate_backward_workspace": (_sz, [_i64] * 5 + [_i]),
+    "mcx_qk_norm_rotate_backward": (_i, [_p] * 14 + [_sz] + [_i64 * 3] * 2 + [_i64] * 7 +
+                                    [_f64, _i, _i, _p]),
+    "mcx_attention_forward_workspace": (_sz, [_adesc, _i]),
+    "mcx_attention_forward": (_i, [_p] * 10 + [_sz, _adesc, _i, _p]),
+    "mcx_attention_backward_workspace": (_sz, [_adesc, _i]),
+    "mcx_attention_backward": (_i, [_p] * 15 + [_sz, _adesc, _i, _p]),
+    "mcx_clip_grad_norm_workspace": (_sz, [_p, _i64]),
+    "mcx_clip_grad_norm": (_i, [_p] * 4 + [_i64, _f64, _f64, _p, _p, _sz, _p]),
 }
 
 _lib = None

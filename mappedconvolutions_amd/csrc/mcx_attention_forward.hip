@@ -1,0 +1,259 @@
+// Attention with a bias by relative-position buckets: the forward product and the C entry points.
+#include <algorithm>
+#include <cmath>
+
+#include "mcx_attention.h"
+
+namespace mcx {
+namespace attention {
+
+// One pass over the keys with a running reference and sum (both fp32): a workgroup holds 128
+// queries of one head, a wave 32 of them, and walks the keys 64 at a time through two LDS buffers,
+// the next tile's loads under way while the current one is multiplied.
+//   The reference is the row's maximum, but it follows it only when a score exceeds it by 2^8:
+// sums stay far inside fp32, and the accumulated output is seldom rescaled.
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * kWaves) void attention_forward_kernel(Params p, T *out,
+                                                                        float *stats, int nq) {
+  constexpr int P = pitch<T, DP>(), Chunks = DP / 16, Blocks = DP / 32;
+  __shared__ __attribute__((aligned(16))) T ks[2][kTile * P];
+  __shared__ __attribute__((aligned(16))) T vs[2][kTile * P];
+  __shared__ __attribute__((aligned(16))) Window window[2];
+  extern __shared__ float table[];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x);
+  const int bh = wg / nq, b = bh / p.Hq, h = bh % p.Hq;
+  // the longest rows of a causal map first
+  const int i0 = (nq - 1 - wg % nq) * kBlock;
+  const int kh = h / (p.Hq / p.Hk);
+  const int start = first_position(p, b), length = key_length(p, b);
+  const int local = wave * kLanesRows + (lane & 31), i = i0 + local;
+  const bool live = i < p.Lq;
+  const int limit = p.causal ? min(length, start + i + 1) : length;  // keys of this query
+  const int last = min(i0 + kBlock, p.Lq) - 1;
+  const int keys = p.causal ? max(0, min(length, start + last + 1)) : length;
+  const int wave_limit = p.causal ? min(length, start + i0 + wave * kLanesRows + 1) : length;
+
+  const T *q = (const T *)p.q + b * p.qs[0] + (int64_t)i * p.qs[1] + h * p.qs[2];
+  const T *k = (const T *)p.k + b * p.ks[0] + kh * p.ks[2];
+  const T *v = (const T *)p.v + b * p.vs[0] + kh * p.vs[2];
+  const bool biased = p.table != nullptr;
+
+  Frag<T> qf[Chunks];
+#pragma unroll
+  for (int c = 0; c < Chunks; c++) qf[c] = global_frag<T>(live ? q : nullptr, c, half, p.D, p.q_wide);
+
+  // window value t stands for the difference (first key of the tile) - (position of query
+  // i0 + kBlock - 1) + t
+  const int base = -(start + i0 + kBlock - 1);
+  if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
+  Tile<T, DP> kt, vt;
+  int bucket = 0;
+  const int tiles = (keys + kTile - 1) / kTile;
+  if (tiles > 0) {
+    kt.load(k, p.ks[1], keys, p.D, p.k_wide, tid);
+    vt.load(v, p.vs[1], keys, p.D, p.v_wide, tid);
+    if (biased) bucket = bucket_of(p, base + tid);
+  }
+  __syncthreads();  // the table
+  if (tiles > 0) {
+    kt.store(ks[0], tid);
+    vt.store(vs[0], tid);
+    if (biased && tid < kWindow) window[0].put(tid, bias_of(table, p.NB, bucket));
+  }
+  __syncthreads();
+
+  const float c = p.scale * kLog2e;
+  const int at = kBlock - 1 - local, shift = at & 3;
+  floatx16 o[Blocks];
+#pragma unroll
+  for (int d = 0; d < Blocks; d++) o[d] = (floatx16)(0.f);
+  float ref = -kInf, sum = 0.f;
+
+  for (int t = 0; t < tiles; t++) {
+    const int j0 = t * kTile, buf = t & 1;
+    if (t + 1 < tiles) {
+      const int64_t next = j0 + kTile;
+      kt.load(k + next * p.ks[1], p.ks[1], keys - (int)next, p.D, p.k_wide, tid);
+      vt.load(v + next * p.vs[1], p.vs[1], keys - (int)next, p.D, p.v_wide, tid);
+      if (biased) bucket = bucket_of(p, base + (int)next + tid);
+    }
+    floatx16 u[2];
+#pragma unroll
+    for (int blk = 0; blk < 2; blk++) {
+      if (biased) {
+        const floatx8 lo = window[buf].get(at + 32 * blk + 8 * half, shift);
+        const floatx8 hi = window[buf].get(at + 32 * blk + 16 + 8 * half, shift);
+        u[blk] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15);
+      } else {
+        u[blk] = (floatx16)(0.f);
+      }
+#pragma unroll
+      for (int ch = 0; ch < Chunks; ch++)
+        u[blk] = mma(row_frag<T, DP>(ks[buf], 32 * blk + row_of(lane & 31), ch, half), qf[ch], u[blk]);
+    }
+    if (j0 + kTile > wave_limit) {
+#pragma unroll
+      for (int blk = 0; blk < 2; blk++)
+#pragma unroll
+        for (int n = 0; n < 16; n++) {
+          const int j = j0 + 32 * blk + 16 * (n >> 3) + 8 * half + (n & 7);
+          if (j >= limit) u[blk][n] = -kInf;
+        }
+    }
+    float top = u[0][0];
+#pragma unroll
+    for (int blk = 0; blk < 2; blk++)
+#pragma unroll
+      for (int n = 0; n < 16; n++) top = fmaxf(top, u[blk][n]);
+    top = fmaxf(top, other_half(top));
+    if (__any((top - ref) * c > 8.f)) {  // (-inf against -inf is no number: not above)
+      const float next = fmaxf(ref, top);
+      const float keep = next == -kInf ? 1.f : exp2_fast((ref - next) * c);
+      ref = next;
+      sum *= keep;
+#pragma unroll
+      for (int d = 0; d < Blocks; d++) o[d] *= keep;
+    }
+    const float used = ref == -kInf ? 0.f : ref;
+    if (__any(fabsf(used) * c > kHugeStat)) {
+#pragma unroll
+      for (int blk = 0; blk < 2; blk++)
+#pragma unroll
+        for (int n = 0; n < 16; n++) u[blk][n] = exp2_fast((u[blk][n] - used) * c);
+    } else {
+      const float shiftc = -used * c;
+#pragma unroll
+      for (int blk = 0; blk < 2; blk++)
+#pragma unroll
+        for (int n = 0; n < 16; n++) u[blk][n] = exp2_fast(fmaf(u[blk][n], c, shiftc));
+    }
+    float part = 0.f;
+#pragma unroll
+    for (int blk = 0; blk < 2; blk++) {
+#pragma unroll
+      for (int n = 0; n < 16; n++) part += u[blk][n];
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        const floatx8 x = s == 0
+            ? __builtin_shufflevector(u[blk], u[blk], 0, 1, 2, 3, 4, 5, 6, 7)
+            : __builtin_shufflevector(u[blk], u[blk], 8, 9, 10, 11, 12, 13, 14, 15);
+        const Frag<T> pf = Frag<T>::pack(x);
+#pragma unroll
+        for (int d = 0; d < Blocks; d++)
+          o[d] = mma(col_frag<DP>(vs[buf], 32 * blk + 16 * s, d, lane), pf, o[d]);
+      }
+    }
+    sum += part;
+    if (t + 1 < tiles) {
+      kt.store(ks[buf ^ 1], tid);
+      vt.store(vs[buf ^ 1], tid);
+      if (biased && tid < kWindow) window[buf ^ 1].put(tid, bias_of(table, p.NB, bucket));
+    }
+    __syncthreads();
+  }
+  sum += other_half(sum);
+  if (!live) return;
+  const int64_t row = ((int64_t)b * p.Lq + i) * p.Hq + h;
+  store_column<T, Blocks>(out + row * p.D, o, sum == 0.f ? 0.f : 1.f / sum, p.D, half, p.D % 4 == 0);
+  if (stats && half == 0) {
+    float *s = stats + 2 * (((int64_t)b * p.Hq + h) * p.Lq + i);
+    s[0] = ref;
+    s[1] = sum;
+  }
+}
+
+template <typename T>
+static int launch_forward(const Params &p, void *out, float *stats, hipStream_t stream) {
+  const int nq = (p.Lq + kBlock - 1) / kBlock;
+  const dim3 grid((unsigned)((int64_t)p.B * p.Hq * nq)), threads(64 * kWaves);
+  const size_t lds = p.table ? p.NB * sizeof(float) : 0;
+#define MCX_FORWARD(DP)                                                                         \
+  hipLaunchKernelGGL((attention_forward_kernel<T, DP>), grid, threads, lds, stream, p, (T *)out, \
+                     stats, nq)
+  if (p.D <= 32) MCX_FORWARD(32);
+  else if (p.D <= 64) MCX_FORWARD(64);
+  else if (p.D <= 96) MCX_FORWARD(96);
+  else MCX_FORWARD(128);
+#undef MCX_FORWARD
+  MCX_HIP_CHECK_LAUNCH();
+  return MCX_OK;
+}
+
+static bool wide_loads(const void *p, const int64_t *strides, int64_t D, int64_t per16) {
+  return (uintptr_t)p % 16 == 0 && D % per16 == 0 && strides[0] % per16 == 0 &&
+         strides[1] % per16 == 0 && strides[2] % per16 == 0;
+}
+
+int make_params(Params &p, const void *q, const void *k, const void *v, const void *table,
+                const int32_t *buckets, const int32_t *query_start, const int32_t *key_lengths,
+                const mcx_attention_desc *d, int dtype) {
+  if (!d) return MCX_E_NULL;
+  if (dtype != MCX_F32 && dtype != MCX_BF16) return MCX_E_DTYPE;
+  const int64_t most = 1 << 28;
+  if (d->B < 0 || d->Lq < 0 || d->Lk < 0 || d->B > most || d->Lq > most || d->Lk > most)
+    return MCX_E_SHAPE;
+  if (d->D < 1 || d->D > kMaxD || d->Hk < 1 || d->Hq < 1 || d->Hq > 65536 || d->Hq % d->Hk)
+    return MCX_E_SHAPE;
+  if (!(d->scale >= 1e-6 && d->scale <= 1e6)) return MCX_E_SHAPE;
+  if (d->B && d->Lq && (!q || (d->Lk && (!k || !v)))) return MCX_E_NULL;
+  if ((table != nullptr) != (buckets != nullptr)) return MCX_E_NULL;
+  if (table && (d->table_size < 1 || d->table_size > kMaxTable || d->bucket_count < 1 ||
+                d->bucket_count > 4 * most || d->bucket_zero < 0 ||
+                d->bucket_zero >= d->bucket_count))
+    return MCX_E_SHAPE;
+  p.q = q, p.k = k, p.v = v, p.table = table;
+  p.buckets = buckets, p.start = query_start, p.lengths = key_lengths;
+  for (int n = 0; n < 3; n++)
+    p.qs[n] = d->q_stride[n], p.ks[n] = d->k_stride[n], p.vs[n] = d->v_stride[n];
+  p.B = (int)d->B, p.Lq = (int)d->Lq, p.Lk = (int)d->Lk;
+  p.Hq = (int)d->Hq, p.Hk = (int)d->Hk, p.D = (int)d->D;
+  p.R = table ? (int)d->bucket_count : 0, p.zero = table ? (int)d->bucket_zero : 0;
+  p.NB = table ? (int)d->table_size : 0, p.causal = d->causal != 0;
+  p.scale = (float)d->scale;
+  const int64_t per16 = dtype == MCX_BF16 ? 8 : 4;
+  p.q_wide = wide_loads(q, p.qs, p.D, per16);
+  p.k_wide = wide_loads(k, p.ks, p.D, per16);
+  p.v_wide = wide_loads(v, p.vs, p.D, per16);
+  return MCX_OK;
+}
+
+}  // namespace attention
+}  // namespace mcx
+
+extern "C" {
+
+size_t mcx_attention_forward_workspace(const mcx_attention_desc *desc, int dtype) {
+  using namespace mcx::attention;
+  Params p;
+  static const int32_t any = 0;  // (stands for pointers that are not read here)
+  const int32_t *table = desc && desc->table_size > 0 ? &any : nullptr;
+  if (make_params(p, &any, &any, &any, table, table, nullptr, nullptr, desc, dtype) != MCX_OK)
+    return 0;
+  return p.B && p.Lq ? split_bytes(p, split_parts(p)) : 0;
+}
+
+int mcx_attention_forward(const void *q, const void *k, const void *v, const void *table,
+                          const int32_t *buckets, const int32_t *query_start,
+                          const int32_t *key_lengths, void *out, float *stats, void *workspace,
+                          size_t workspace_bytes, const mcx_attention_desc *desc, int dtype,
+                          void *stream) {
+  using namespace mcx::attention;
+  Params p;
+  const int rc = make_params(p, q, k, v, table, buckets, query_start, key_lengths, desc, dtype);
+  if (rc != MCX_OK) return rc;
+  if (p.B == 0 || p.Lq == 0) return MCX_OK;
+  if (!out) return MCX_E_NULL;
+  const int parts = split_parts(p);
+  if (parts) {
+    if (split_bytes(p, parts) && (!workspace || workspace_bytes < split_bytes(p, parts)))
+      return MCX_E_WORKSPACE;
+    return launch_split(p, parts, out, stats, workspace, dtype, (hipStream_t)stream);
+  }
+  if ((int64_t)p.B * p.Hq * ((p.Lq + kBlock - 1) / kBlock) > 0x7fffffffLL) return MCX_E_SHAPE;
+  return dtype == MCX_BF16 ? launch_forward<__bf16>(p, out, stats, (hipStream_t)stream)
+                           : launch_forward<float>(p, out, stats, (hipStream_t)stream);
+}
+
+}  // extern "C"

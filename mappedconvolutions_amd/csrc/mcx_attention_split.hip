@@ -1,0 +1,346 @@
+// Attention of few queries over many keys: the keys are split over workgroups and the parts joined.
+//
+// Bound by memory: one token reads the whole cache once.  The query heads that share a key head
+// are rows of one product (row r = query r / group, head r % group), 32 to a workgroup, so their
+// keys are read once for all.  A wave takes every fourth 32 keys of its workgroup's part: the keys
+// come straight into the product's operand registers, the values through LDS that only this wave
+// uses, the next tile's loads under way meanwhile; there is no barrier in the loop.
+#include <algorithm>
+
+#include "mcx_attention.h"
+
+namespace mcx {
+namespace attention {
+
+constexpr int kRows = 32;       // rows of a workgroup
+constexpr int kStep = 32;       // keys of a wave's tile
+constexpr int kMostParts = 256;
+
+// What a wave's lanes have written to LDS is there for its other lanes: the hardware keeps a wave's
+// LDS instructions in order, and the compiler may not move them past this.
+__device__ inline void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+struct Split {
+  int parts;       // of the keys
+  int blocks;      // of 32 rows, of a key head
+  int rows;        // Lq * group
+  float *sums;     // [B * Hk * blocks][parts][32][2]: reference and sum
+  float *outs;     // [B * Hk * blocks][parts][32][D]
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, Split sp, T *out,
+                                                                      float *stats) {
+  constexpr int P = pitch<T, DP>(), Chunks = DP / 16, Blocks = DP / 32;
+  constexpr int E = 16 / (int)sizeof(T), PerRow = DP / E, N = kStep * PerRow / 64;
+  // a wave's values; at the end all waves' sums, four blocks of columns at a time
+  constexpr int kTileBytes = kStep * P * (int)sizeof(T);
+  __shared__ __attribute__((aligned(16))) char tiles_lds[kWaves * kTileBytes];
+  __shared__ int buckets_lds[kWaves][64];
+  __shared__ float merge[kWaves][kRows][2];
+  extern __shared__ float table[];  // [min(group, 32)][NB]
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x);
+  const int part = wg % sp.parts, unit = wg / sp.parts;
+  const int block = unit % sp.blocks, bk = unit / sp.blocks, b = bk / p.Hk, kh = bk % p.Hk;
+  const int group = p.Hq / p.Hk;
+  const int r = block * kRows + (lane & 31);
+  const bool live = r < sp.rows;
+  const int i = r / group, h = kh * group + r % group;
+  const int start = first_position(p, b), length = key_length(p, b);
+  const int limit = !live ? 0 : p.causal ? min(length, start + i + 1) : length;
+  const int first_i = block * kRows / group;
+  const int last_i = min(block * kRows + kRows - 1, sp.rows - 1) / group;
+  const int keys = p.causal ? max(0, min(length, start + last_i + 1)) : length;
+  const int wave_limit = p.causal ? min(length, start + first_i + 1) : length;
+
+  const bool biased = p.table != nullptr;
+  const int slots = min(group, kRows), slot = group <= kRows ? r % group : lane & 31;
+  if (biased) {
+    for (int n = tid; n < slots * p.NB; n += 64 * kWaves) {
+      const int s = n / p.NB, hs = kh * group + (group <= kRows ? s : (block * kRows + s) % group);
+      float x = to_float(((const T *)p.table)[(int64_t)hs * p.NB + n % p.NB]);
+      if (fabsf(x) < kInf) x = fminf(fmaxf(x, -kBiasLimit), kBiasLimit);
+      table[n] = x / p.scale;
+    }
+  }
+  __syncthreads();
+
+  const int total = (keys + kStep - 1) / kStep, each = (total + sp.parts - 1) / sp.parts;
+  const int t_end = min(total, (part + 1) * each);
+  int t = part * each + wave;
+
+  const T *k = (const T *)p.k + b * p.ks[0] + kh * p.ks[2];
+  const T *v = (const T *)p.v + b * p.vs[0] + kh * p.vs[2];
+  const T *q = (const T *)p.q + b * p.qs[0] + (int64_t)i * p.qs[1] + h * p.qs[2];
+  Frag<T> qf[Chunks], kf[Chunks];
+  uint4 vr[N];
+#pragma unroll
+  for (int c = 0; c < Chunks; c++) qf[c] = global_frag<T>(live ? q : nullptr, c, half, p.D, p.q_wide);
+
+  const int key_row = row_of(lane & 31);
+  // bias: difference x of a tile = j - (position of the block's last query)
+  const int origin = start + last_i, own = live ? last_i - i : 0;
+  int bucket = 0;
+  bool varied = false;  // whether the tile's pairs are of more than one bucket
+  auto fetch = [&](int tile) {
+    const int j0 = tile * kStep;
+    const T *row = j0 + key_row < keys ? k + (int64_t)(j0 + key_row) * p.ks[1] : nullptr;
+#pragma unroll
+    for (int c = 0; c < Chunks; c++) kf[c] = global_frag<T>(row, c, half, p.D, p.k_wide);
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const int id = lane + 64 * n, j = j0 + id / PerRow, d0 = (id % PerRow) * E;
+      vr[n] = j < keys ? load16(v + (int64_t)j * p.vs[1], d0, p.D, p.v_wide) : make_uint4(0, 0, 0, 0);
+    }
+    if (biased) bucket = bucket_of(p, j0 - origin + lane);
+  };
+  const float c = p.scale * kLog2e;
+  T *vs = (T *)(tiles_lds + wave * kTileBytes);
+  floatx16 o[Blocks];
+#pragma unroll
+  for (int d = 0; d < Blocks; d++) o[d] = (floatx16)(0.f);
+  float ref = -kInf, sum = 0.f;
+  if (t < t_end) fetch(t);
+  for (; t < t_end; t += kWaves) {
+    const int j0 = t * kStep;
+    Frag<T> now[Chunks];
+#pragma unroll
+    for (int n = 0; n < Chunks; n++) now[n] = kf[n];
+    wave_order();
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const int id = lane + 64 * n;
+      *(uint4 *)(vs + (id / PerRow) * P + (id % PerRow) * E) = vr[n];
+    }
+    buckets_lds[wave][lane] = bucket;
+    wave_order();
+    floatx16 u = (floatx16)(0.f);
+    if (biased) {
+      const int one = __builtin_amdgcn_readfirstlane(bucket);
+      varied = __any(bucket != one);
+      if (varied) {
+#pragma unroll
+        for (int n = 0; n < 16; n++) {
+          const int x = buckets_lds[wave][16 * (n >> 3) + 8 * half + (n & 7) + own];
+          u[n] = (unsigned)x < (unsigned)p.NB ? table[slot * p.NB + x] : 0.f;
+        }
+      } else {
+        u = (floatx16)((unsigned)one < (unsigned)p.NB ? table[slot * p.NB + one] : 0.f);
+      }
+    }
+    if (t + kWaves < t_end) fetch(t + kWaves);
+#pragma unroll
+    for (int n = 0; n < Chunks; n++) u = mma(now[n], qf[n], u);
+    if (j0 + kStep > wave_limit) {
+#pragma unroll
+      for (int n = 0; n < 16; n++)
+        if (j0 + 16 * (n >> 3) + 8 * half + (n & 7) >= limit) u[n] = -kInf;
+    }
+    float top = u[0];
+#pragma unroll
+    for (int n = 1; n < 16; n++) top = fmaxf(top, u[n]);
+    top = fmaxf(top, other_half(top));
+    if (__any((top - ref) * c > 8.f)) {
+      const float next = fmaxf(ref, top);
+      const float keep = next == -kInf ? 1.f : exp2_fast((ref - next) * c);
+      ref = next;
+      sum *= keep;
+#pragma unroll
+      for (int d = 0; d < Blocks; d++) o[d] *= keep;
+    }
+    const float used = ref == -kInf ? 0.f : ref;
+#pragma unroll
+    for (int n = 0; n < 16; n++) {
+      u[n] = exp2_fast((u[n] - used) * c);
+      sum += u[n];
+    }
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      const floatx8 x = s == 0 ? __builtin_shufflevector(u, u, 0, 1, 2, 3, 4, 5, 6, 7)
+                               : __builtin_shufflevector(u, u, 8, 9, 10, 11, 12, 13, 14, 15);
+      const Frag<T> pf = Frag<T>::pack(x);
+#pragma unroll
+      for (int d = 0; d < Blocks; d++) o[d] = mma(col_frag<DP>(vs, 16 * s, d, lane), pf, o[d]);
+    }
+  }
+  sum += other_half(sum);
+
+  // the four waves' parts: a common reference, then block by block of columns through LDS
+  if (half == 0) {
+    merge[wave][lane][0] = ref;
+    merge[wave][lane][1] = sum;
+  }
+  __syncthreads();
+  float top = -kInf;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) top = fmaxf(top, merge[w][lane & 31][0]);
+  float all = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    const float x = merge[w][lane & 31][0];
+    all += x == -kInf ? merge[w][lane & 31][1] : merge[w][lane & 31][1] * exp2_fast((x - top) * c);
+  }
+  const float factor = ref == -kInf ? 1.f : exp2_fast((ref - top) * c);
+  // wave w sums columns 32 d + 8 w .. 8 w + 7 of every block: [wave][32 columns][32 rows], a row
+  // of 33 values
+  float *part_lds = (float *)tiles_lds;
+  static_assert(kWaves * kTileBytes >= kWaves * 32 * 16 * 4, "a block's sums fit two halves");
+  const int64_t at = (int64_t)unit * sp.parts + part;
+#pragma unroll
+  for (int d = 0; d < Blocks; d++)
+#pragma unroll
+    for (int hh = 0; hh < 2; hh++) {  // 16 of the 32 columns at a time
+      __syncthreads();
+#pragma unroll
+      for (int g = 0; g < 2; g++)
+#pragma unroll
+        for (int a = 0; a < 4; a++)
+          part_lds[(wave * 16 + 8 * g + 4 * half + a) * 32 + (lane & 31)] =
+              o[d][8 * hh + 4 * g + a] * factor;
+      __syncthreads();
+      // 256 threads, 16 columns x 32 rows: two columns each
+#pragma unroll
+      for (int n = 0; n < 2; n++) {
+        const int column = 2 * (tid >> 5) + n, row = tid & 31, rr = block * kRows + row;
+        const int dd = 32 * d + 16 * hh + column;
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) x += part_lds[(w * 16 + column) * 32 + row];
+        if (rr < sp.rows && dd < p.D) {
+          if (sp.parts == 1) {
+            // (lane & 31 is this thread's row too, so `all` is its row's sum)
+            const int64_t to = ((int64_t)b * p.Lq + rr / group) * p.Hq + kh * group + rr % group;
+            out[to * p.D + dd] = (T)(all == 0.f ? 0.f : x / all);
+          } else {
+            sp.outs[(at * kRows + row) * p.D + dd] = x;
+          }
+        }
+      }
+    }
+  if (wave == 0 && half == 0 && live) {
+    if (sp.parts > 1) {
+      sp.sums[(at * kRows + lane) * 2] = top;
+      sp.sums[(at * kRows + lane) * 2 + 1] = all;
+    } else if (stats) {
+      float *s = stats + 2 * (((int64_t)b * p.Hq + h) * p.Lq + i);
+      s[0] = top;
+      s[1] = all;
+    }
+  }
+}
+
+// Joins the parts of a row: a workgroup has one row, its waves every fourth part.
+template <typename T>
+__global__ __launch_bounds__(64 * kWaves) void attention_join_kernel(Params p, Split sp, T *out,
+                                                                     float *stats) {
+  __shared__ float weight[kMostParts];
+  __shared__ float merge[kWaves][kMaxD];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int group = p.Hq / p.Hk;
+  const int bk = blockIdx.x / sp.rows, r = blockIdx.x % sp.rows, b = bk / p.Hk, kh = bk % p.Hk;
+  const int unit = bk * sp.blocks + r / kRows, row = r % kRows;
+  const float *sums = sp.sums + ((int64_t)unit * sp.parts * kRows + row) * 2;
+  const float c = p.scale * kLog2e;
+  // every wave finds the common reference and the sum by itself
+  float top = -kInf;
+  for (int n = lane; n < sp.parts; n += 64) top = fmaxf(top, sums[(int64_t)n * kRows * 2]);
+  for (int m = 32; m; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
+  float all = 0.f;
+  for (int n = lane; n < sp.parts; n += 64) {
+    const float ref = sums[(int64_t)n * kRows * 2];
+    const float w = ref == -kInf ? 1.f : exp2_fast((ref - top) * c);  // (a NaN part stays one)
+    all += w * sums[(int64_t)n * kRows * 2 + 1];
+    if (wave == 0) weight[n] = w;
+  }
+  for (int m = 32; m; m >>= 1) all += __shfl_xor(all, m);
+  __syncthreads();
+  const float *from = sp.outs + ((int64_t)unit * sp.parts * kRows + row) * p.D;
+  float x = 0.f, y = 0.f;
+  for (int n = wave; n < sp.parts; n += kWaves) {
+    const float w = weight[n];
+    const float *f = from + (int64_t)n * kRows * p.D;
+    if (lane < p.D) x = fmaf(w, f[lane], x);
+    if (lane + 64 < p.D) y = fmaf(w, f[lane + 64], y);
+  }
+  merge[wave][lane] = x;
+  merge[wave][lane + 64] = y;
+  __syncthreads();
+  const int h = kh * group + r % group, i = r / group;
+  if (tid < p.D) {
+    x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) x += merge[w][tid];
+    out[(((int64_t)b * p.Lq + i) * p.Hq + h) * p.D + tid] = (T)(all == 0.f ? 0.f : x / all);
+  }
+  if (stats && tid == 0) {
+    float *s = stats + 2 * (((int64_t)b * p.Hq + h) * p.Lq + i);
+    s[0] = top;
+    s[1] = all;
+  }
+}
+
+// 0: the other kernel is the better one.
+int split_parts(const Params &p) {
+  const int64_t group = p.Hq / p.Hk, rows = p.Lq * group;
+  const int64_t blocks = (rows + kRows - 1) / kRows, units = (int64_t)p.B * p.Hk * blocks;
+  const int64_t whole = (int64_t)p.B * p.Hq * ((p.Lq + kBlock - 1) / kBlock);
+  if (rows > 64 && !(whole <= 64 && p.Lk >= 1024)) return 0;
+  if (units > (1 << 24)) return 0;
+  const int64_t most = std::max<int64_t>(1, (p.Lk + kWaves * kStep - 1) / (kWaves * kStep));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + units - 1) / units, most, kMostParts}));
+}
+
+static Split split_of(const Params &p, int parts) {
+  Split sp = {};
+  sp.parts = parts;
+  sp.rows = p.Lq * (p.Hq / p.Hk);
+  sp.blocks = (sp.rows + kRows - 1) / kRows;
+  return sp;
+}
+
+size_t split_bytes(const Params &p, int parts) {
+  if (parts <= 1) return 0;
+  const Split sp = split_of(p, parts);
+  const size_t rows = (size_t)p.B * p.Hk * sp.blocks * parts * kRows;
+  return align256(rows * 2 * sizeof(float)) + align256(rows * p.D * sizeof(float));
+}
+
+template <typename T>
+static int launch(const Params &p, Split sp, void *out, float *stats, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)p.B * p.Hk * sp.blocks * sp.parts)), threads(64 * kWaves);
+  const size_t lds = p.table ? std::min(p.Hq / p.Hk, kRows) * p.NB * sizeof(float) : 0;
+#define MCX_SPLIT(DP) \
+  hipLaunchKernelGGL((attention_split_kernel<T, DP>), grid, threads, lds, stream, p, sp, (T *)out, stats)
+  if (p.D <= 32) MCX_SPLIT(32);
+  else if (p.D <= 64) MCX_SPLIT(64);
+  else if (p.D <= 96) MCX_SPLIT(96);
+  else MCX_SPLIT(128);
+#undef MCX_SPLIT
+  MCX_HIP_CHECK_LAUNCH();
+  if (sp.parts > 1) {
+    hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)((int64_t)p.B * p.Hk * sp.rows)),
+                       threads, 0, stream, p, sp, (T *)out, stats);
+    MCX_HIP_CHECK_LAUNCH();
+  }
+  return MCX_OK;
+}
+
+int launch_split(const Params &p, int parts, void *out, float *stats, void *workspace, int dtype,
+                 hipStream_t stream) {
+  Split sp = split_of(p, parts);
+  if (parts > 1) {
+    const size_t rows = (size_t)p.B * p.Hk * sp.blocks * parts * kRows;
+    sp.sums = (float *)workspace;
+    sp.outs = (float *)((char *)workspace + align256(rows * 2 * sizeof(float)));
+  }
+  return dtype == MCX_BF16 ? launch<__bf16>(p, sp, out, stats, stream)
+                           : launch<float>(p, sp, out, stats, stream);
+}
+
+}  // namespace attention
+}  // namespace mcx

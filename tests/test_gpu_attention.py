@@ -1,0 +1,343 @@
+"""Attention with a bias by relative-position buckets, its gradients and its form for few queries,
+against the same computed in float64 on the CPU.
+
+Tolerances, from the number formats.  float32: sums of at most a few thousand products of size one
+in fp32, 2e-5 of the result's largest value (several hundred roundings of 2^-24).  bfloat16: the
+inputs are the same bf16 values for both; probabilities and score gradients are rounded to bf16
+(2^-9 each) before a product, the result once more: each output is a sum whose terms are off by at
+most 2^-8 + 2^-9 of their size, 2e-2 of the result's largest value allows for the sum of the terms'
+sizes being some three times the result."""
+import math
+
+import pytest
+import torch
+
+from mappedconvolutions_amd import _C
+
+pytestmark = pytest.mark.gpu
+
+TOL = {torch.float32: 2e-5, torch.bfloat16: 2e-2}
+
+
+def reference(q, k, v, table=None, buckets=None, zero=0, scale=None, causal=False, start=None,
+              lengths=None, go=None):
+    """out, and with go the gradients of q, k, v and table, in float64 on the CPU."""
+    q, k, v = (t.detach().double().cpu().requires_grad_(go is not None) for t in (q, k, v))
+    B, Lq, Hq, D = q.shape
+    Lk, Hk = k.shape[1], k.shape[2]
+    scale = D ** -0.5 if scale is None else scale
+    kk, vv = (t.repeat_interleave(Hq // Hk, 2) for t in (k, v))
+    pos = torch.zeros(B, dtype=torch.int64) if start is None else start.cpu().long()
+    rel = torch.arange(Lk) - (pos[:, None, None] + torch.arange(Lq)[:, None])  # B Lq Lk
+    keep = torch.ones_like(rel, dtype=torch.bool)
+    if causal:
+        keep &= rel <= 0
+    if lengths is not None:
+        n = lengths.cpu().long().clamp(0, Lk)
+        keep &= (torch.arange(Lk) < n[:, None])[:, None]
+        used = (torch.arange(Lk) < n[:, None])[:, :, None, None]
+        kk, vv = torch.where(used, kk, 0.), torch.where(used, vv, 0.)
+    s = torch.einsum("bihd,bjhd->bhij", q, kk) * scale
+    if table is not None:
+        table = table.detach().double().cpu().requires_grad_(go is not None)
+        which = buckets.cpu().long()[(rel + zero).clamp(0, buckets.numel() - 1)]
+        known = (which >= 0) & (which < table.shape[1])
+        bias = table[:, which.clamp(0, table.shape[1] - 1)].transpose(0, 1)
+        s = s + torch.where(known[:, None], bias, 0.)
+    keep = keep[:, None] & (s > -math.inf)
+    top = torch.where(keep, s, -math.inf).amax(-1, keepdim=True) if Lk else s.new_zeros(B, Hq, Lq, 1)
+    top = torch.where(top == -math.inf, 0., top).detach()
+    e = torch.where(keep, torch.exp(torch.where(keep, s - top, 0.)), 0.)
+    total = e.sum(-1, keepdim=True)
+    p = e / torch.where(total == 0, 1., total)
+    out = torch.einsum("bhij,bjhd->bihd", p, vv)
+    if go is None:
+        return out
+    leaves = [q, k, v] + ([] if table is None else [table])
+    grads = torch.autograd.grad(out, leaves, go.detach().double().cpu(), allow_unused=True)
+    return [out.detach()] + [torch.zeros_like(t) if g is None else g for t, g in zip(leaves, grads)]
+
+
+def close(got, want, tol, what):
+    got = got.double().cpu()
+    assert got.shape == want.shape, what
+    assert torch.isfinite(got).all(), what + ": not finite"
+    if got.numel():
+        bound = tol * max(want.abs().max().item(), 1e-3)
+        off = (got - want).abs().max().item()
+        assert off <= bound, "%s: off by %g of %g" % (what, off, bound)
+
+
+def problem(seed, dtype, B, Lq, Lk, Hq, Hk, D, NB=16, reach=40, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    q, k, v = (spread * torch.randn(B, L, H, D, generator=g) for L, H in ((Lq, Hq), (Lk, Hk), (Lk, Hk)))
+    go = torch.randn(B, Lq, Hq, D, generator=g)
+    table = torch.randn(Hq, NB, generator=g)
+    buckets = torch.randint(0, NB, (2 * reach + 1,), generator=g).int()
+    q, k, v, go, table = (t.to(dtype).cuda() for t in (q, k, v, go, table))
+    return q, k, v, go, table, buckets.cuda(), reach
+
+
+def check(q, k, v, go, table, buckets, zero, train=True, **kw):
+    tol = TOL[q.dtype]
+    names = dict(bias_table=table, buckets=buckets, bucket_zero=zero,
+                 query_start=kw.get("start"), key_lengths=kw.get("lengths"),
+                 scale=kw.get("scale"), causal=kw.get("causal", False))
+    out, stats = _C.relative_attention_forward(q, k, v, for_backward=train, **names)
+    want = reference(q, k, v, table, buckets, zero, go=go if train else None, **kw)
+    if not train:
+        assert stats is None
+        close(out, want, tol, "out")
+        return out
+    close(out, want[0], tol, "out")
+    grads = _C.relative_attention_backward(go, q, k, v, out, stats, **names)
+    for name, got, w in zip(("grad_query", "grad_key", "grad_value", "grad_bias_table"), grads, want[1:]):
+        close(got, w, tol, name)
+    again = _C.relative_attention_backward(go, q, k, v, out, stats, **names)
+    for a, b in zip(grads, again):
+        assert a is None or torch.equal(a, b)
+    return out
+
+
+SIZES = [
+    # B, Lq, Lk, Hq, Hk, D
+    (1, 1, 1, 1, 1, 1),
+    (2, 5, 7, 2, 1, 8),
+    (1, 64, 64, 2, 2, 64),
+    (2, 128, 128, 4, 2, 64),
+    (1, 129, 65, 3, 1, 40),
+    (2, 200, 333, 6, 2, 48),
+    (1, 257, 191, 2, 2, 96),
+    (1, 300, 300, 4, 1, 128),
+    (3, 33, 31, 2, 1, 13),
+    (1, 700, 130, 2, 2, 32),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_forward_and_gradients(device, size, dtype, causal):
+    check(*problem(1, dtype, *size), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [(2, 100, 100, 2, 2, 32), (1, 190, 70, 4, 2, 128)])
+def test_without_bias(device, size, dtype):
+    q, k, v, go, _, _, _ = problem(2, dtype, *size)
+    check(q, k, v, go, None, None, 0, scale=0.3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_lengths_and_starts(device, dtype):
+    # no key, one, some, all, more than there are; positions before, amid and behind the keys
+    B, Lq, Lk = 6, 70, 150
+    lengths = torch.tensor([0, 1, 77, 150, 400, -3], dtype=torch.int32).cuda()
+    start = torch.tensor([0, -30, 20, 80, 149, 5], dtype=torch.int32).cuda()
+    args = problem(3, dtype, B, Lq, Lk, 4, 2, 32)
+    for causal in (False, True):
+        check(*args, causal=causal, lengths=lengths, start=start)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_unused_keys_may_hold_anything(device, dtype):
+    q, k, v, go, table, buckets, zero = problem(4, dtype, 3, 90, 200, 2, 1, 64)
+    lengths = torch.tensor([0, 130, 64], dtype=torch.int32).cuda()
+    for b, n in enumerate(lengths.tolist()):
+        k[b, n:], v[b, n:] = float("nan"), float("inf")
+        k[b, n + 1::2] = -float("inf")
+    check(q, k, v, go, table, buckets, zero, lengths=lengths)
+    # a single query takes the form that splits the keys
+    check(q[:, :1], k, v, go[:, :1], table, buckets, zero, lengths=lengths)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Lq", [1, 150])
+def test_buckets_taken_out_and_lowest_values(device, dtype, Lq):
+    q, k, v, go, table, buckets, zero = problem(5, dtype, 2, Lq, 150, 2, 1, 32, NB=8)
+    table[0, 3] = -float("inf")          # some pairs
+    table[1, :] = -float("inf")          # a head of which nothing is left
+    out = check(q, k, v, go, table, buckets, zero)
+    assert (out[:, :, 1] == 0).all()
+    table[0, 3] = torch.finfo(dtype).min  # swallows the scores it is added to
+    check(q, k, v, go, table, buckets, zero)
+    # rows with nothing but the lowest value: all their keys alike
+    low = torch.full_like(table, torch.finfo(dtype).min)
+    out, stats = _C.relative_attention_forward(q, k, v, low, buckets, zero, for_backward=True)
+    close(out, v.double().cpu().mean(1, keepdim=True).expand(2, 150, 1, 32)[:, :Lq].repeat(1, 1, 2, 1),
+          TOL[dtype], "mean of the values")
+    grads = _C.relative_attention_backward(go, q, k, v, out, stats, low, buckets, zero)
+    gv = (go.double().cpu().sum(1).sum(1) / 150)[:, None, None].expand(2, 150, 1, 32)
+    close(grads[2], gv, TOL[dtype], "gradient of the values")
+
+
+def test_unknown_buckets_have_no_bias(device):
+    q, k, v, go, table, buckets, zero = problem(6, torch.float32, 1, 140, 140, 2, 2, 32, NB=8)
+    buckets[::3] = -1
+    buckets[1::7] = 8
+    check(q, k, v, go, table, buckets, zero)
+    check(q[:, :2], k, v, go[:, :2], table, buckets, zero)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_and_alignment(device, dtype):
+    g = torch.Generator().manual_seed(7)
+    B, L, D = 2, 130, 32
+    packed = torch.randn(B, L, 8, D, generator=g).to(dtype).cuda()
+    q, k, v = packed[:, :, :4], packed[:, :, 4:6], packed[:, :, 6:]
+    go = torch.randn(B, L, 4, D, generator=g).to(dtype).cuda()
+    _, _, _, _, table, buckets, zero = problem(7, dtype, 1, 1, 1, 4, 2, D)
+    check(q, k, v, go, table, buckets, zero, causal=True)
+    # heads before tokens
+    heads = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    check(*heads, go.transpose(1, 2).contiguous().transpose(1, 2), table, buckets, zero)
+    # rows that start at any value
+    wide = torch.randn(B, L, 8, D + 5, generator=g).to(dtype).cuda()[..., 3:3 + D]
+    for n in (L, 1):
+        check(wide[:, :n, :4], wide[:, :, 4:6], wide[:, :, 6:], go[:, :n], table, buckets, zero)
+    # one row for all, and a head size that is dense in another axis
+    check(q, k.expand(2, L, 2, D)[:1].expand(B, L, 2, D), v, go, table, buckets, zero)
+    turned = [t.transpose(1, 3).contiguous().transpose(1, 3) for t in (q, k, v)]
+    check(*turned, go, table, buckets, zero)
+
+
+DECODE = [
+    # B, Lq, Lk, Hq, Hk, D
+    (1, 1, 1, 1, 1, 64),
+    (1, 1, 1000, 8, 8, 64),
+    (3, 1, 4097, 8, 2, 128),
+    (2, 5, 777, 12, 4, 40),
+    (1, 2, 3001, 64, 1, 32),
+    (2, 1, 130, 40, 1, 96),
+    (1, 40, 2000, 2, 1, 48),
+    (2, 3, 5, 3, 1, 7),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", DECODE)
+def test_few_queries_against_a_cache(device, size, dtype):
+    B, Lq, Lk = size[:3]
+    args = problem(8, dtype, *size)
+    check(*args, train=False)
+    lengths = torch.tensor([max(0, Lk - 61 * b) for b in range(B)], dtype=torch.int32).cuda()
+    check(*args, train=False, causal=True, lengths=lengths, start=lengths - Lq)
+    check(*args, causal=True, lengths=lengths, start=lengths - Lq)
+
+
+def test_a_cache_beyond_32_bits(device):
+    # one key head of 2^31 values and more between the batches: offsets need 64 bits
+    B, Lk, D = 3, 1 << 22, 128
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    cache = torch.zeros(B, 2, Lk, 1, D, dtype=torch.bfloat16, device="cuda")
+    k, v = cache[:, 0], cache[:, 1]
+    g = torch.Generator().manual_seed(9)
+    n = 300
+    for b in range(B):
+        k[b, -n:] = torch.randn(n, 1, D, generator=g).cuda().bfloat16() * 3
+        v[b, -n:] = torch.randn(n, 1, D, generator=g).cuda().bfloat16()
+    q = torch.randn(B, 1, 2, D, generator=g).cuda().bfloat16()
+    # all but the last 300 keys are taken out by their bucket
+    buckets = torch.ones(n, dtype=torch.int32, device="cuda")
+    buckets[0] = 0
+    table = torch.zeros(2, 2, dtype=torch.bfloat16, device="cuda")
+    table[:, 0] = -float("inf")
+    start = torch.full((B,), Lk - 1, dtype=torch.int32, device="cuda")
+    out, _ = _C.relative_attention_forward(q, k, v, table, buckets, n - 1, causal=True, query_start=start)
+    want = reference(q, k[:, -n + 1:], v[:, -n + 1:])
+    close(out, want, TOL[torch.bfloat16], "out")
+
+
+def test_gradient_against_differences(device):
+    # float32 steps of 1e-2: the difference is off by 2nd order terms (1e-4 of the curvature, size
+    # one here) and by roundings, 1e-5 / 1e-2; bound 5e-3 on derivatives of size one
+    q, k, v, go, table, buckets, zero = problem(10, torch.float32, 1, 40, 50, 2, 1, 16, NB=6)
+
+    def loss(*x):
+        out, _ = _C.relative_attention_forward(*x[:3], x[3], buckets, zero, causal=True,
+                                               query_start=torch.full((1,), 10, dtype=torch.int32).cuda())
+        return (out.double() * go.double()).sum()
+
+    start = torch.full((1,), 10, dtype=torch.int32).cuda()
+    out, stats = _C.relative_attention_forward(q, k, v, table, buckets, zero, causal=True,
+                                               query_start=start, for_backward=True)
+    grads = _C.relative_attention_backward(go, q, k, v, out, stats, table, buckets, zero,
+                                           causal=True, query_start=start)
+    g = torch.Generator().manual_seed(11)
+    for n in range(4):
+        x = [q, k, v, table]
+        way = torch.randn(x[n].shape, generator=g).cuda()
+        way /= way.norm()
+        ends = []
+        for sign in (1, -1):
+            y = list(x)
+            y[n] = x[n] + sign * 1e-2 * way
+            ends.append(loss(*y))
+        slope = ((ends[0] - ends[1]) / 2e-2).item()
+        assert abs(slope - (grads[n].double() * way.double()).sum().item()) < 5e-3
+
+
+def test_partial_gradients(device):
+    q, k, v, go, table, buckets, zero = problem(12, torch.bfloat16, 2, 100, 100, 4, 2, 64)
+    out, stats = _C.relative_attention_forward(q, k, v, table, buckets, zero, for_backward=True)
+    full = _C.relative_attention_backward(go, q, k, v, out, stats, table, buckets, zero)
+    for needs in ((True, False, False, False), (False, True, False, False),
+                  (False, False, True, False), (False, False, False, True), (False,) * 4):
+        got = _C.relative_attention_backward(go, q, k, v, out, stats, table, buckets, zero, needs=needs)
+        for a, b, n in zip(got, full, needs):
+            assert (a is None) if not n else torch.equal(a, b)
+
+
+def test_empty_sizes(device):
+    q, k, v, go, table, buckets, zero = problem(13, torch.float32, 2, 10, 12, 2, 1, 16)
+    out, stats = _C.relative_attention_forward(q, k[:, :0], v[:, :0], table, buckets, zero, for_backward=True)
+    assert (out == 0).all()
+    grads = _C.relative_attention_backward(go, q, k[:, :0], v[:, :0], out, stats, table, buckets, zero)
+    assert (grads[0] == 0).all() and (grads[3] == 0).all() and grads[1].shape == (2, 0, 1, 16)
+    out, stats = _C.relative_attention_forward(q[:, :0], k, v, table, buckets, zero, for_backward=True)
+    assert out.shape == (2, 0, 2, 16)
+    grads = _C.relative_attention_backward(go[:, :0], q[:, :0], k, v, out, stats, table, buckets, zero)
+    assert all((t == 0).all() for t in grads[1:])
+    out, _ = _C.relative_attention_forward(q[:0], k[:0], v[:0], table, buckets, zero)
+    assert out.shape == (0, 10, 2, 16)
+
+
+def test_another_stream(device):
+    q, k, v, go, table, buckets, zero = problem(14, torch.bfloat16, 2, 300, 300, 4, 2, 64)
+    want, _ = _C.relative_attention_forward(q, k, v, table, buckets, zero)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got, stats = _C.relative_attention_forward(q, k, v, table, buckets, zero, for_backward=True)
+        grads = _C.relative_attention_backward(go, q, k, v, got, stats, table, buckets, zero)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    for t in grads:
+        t.record_stream(torch.cuda.current_stream())
+        assert torch.isfinite(t.float()).all()
+
+
+def test_in_a_graph(device):
+    q, k, v, go, table, buckets, zero = problem(15, torch.bfloat16, 2, 150, 700, 4, 2, 64)
+
+    def step():
+        out, stats = _C.relative_attention_forward(q, k, v, table, buckets, zero, for_backward=True)
+        one, _ = _C.relative_attention_forward(q[:, :1], k, v, table, buckets, zero)
+        return [out, one] + _C.relative_attention_backward(go, q, k, v, out, stats, table, buckets, zero)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for n in range(3):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(n)).to(q))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
