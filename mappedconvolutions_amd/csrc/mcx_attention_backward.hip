@@ -22,6 +22,19 @@ __device__ inline floatx16 add_outer(float a, float b, floatx16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
 }
 
+// One step along the diagonals: ds plus the running sum of the lane below (lane 63's for lane 0),
+// none for the lane where `kept` is 0.  The wait is what a lane exchange needs after a write.
+__device__ inline float next_diagonals(float ds, float sum, float kept) {
+  asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 wave_ror:1 row_mask:0xf bank_mask:0xf"
+      : "+v"(ds) : "v"(sum), "v"(kept));
+  return ds;
+}
+// The upper half-wave's values in the lower, zeros in the upper.
+__device__ inline float upper_to_lower(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), 0u, false, false);
+  return __uint_as_float(r[1]);
+}
+
 // A probability from u: through lse = scale log2(e) ref + log2(sum), +inf for a row that nothing
 // is left of; or, where that is too large to hold its second term, from ref and 1 / sum.
 template <bool Huge>
@@ -32,19 +45,23 @@ __device__ inline float probability(float u, float c, float lse, float ref, floa
 
 // Queries' gradients, the sums per bucket, and the rows' statistics for the other kernel.  The
 // same walk as the forward product's: a wave holds 32 queries, their o gradient beside them.
-//   The bias' gradient: ds of a wave's 32 x 64 pairs goes by its difference j - i into a ring of
-// 128 sums that only this wave writes; the 64 differences that the next tile no longer meets are
-// then added to the wave's sums per bucket.
-template <typename T, int DP>
-__global__ __launch_bounds__(64 * kWaves) void attention_query_grad_kernel(
+//   The bias' gradient needs the sums of ds along the diagonals j - i.  A lane holds query lane & 31
+// and the keys 32 (lane >> 5) + n, n = 0 .. 31: from n to n + 1 a diagonal moves one lane up, so
+// one instruction a value adds it to its neighbour's running sum.  What reaches lane 31 is finished
+// and leaves (lane 32 starts anew); what leaves lane 63 is the part of a diagonal that lane 0 goes
+// on with.  The 64 diagonals that a tile finishes are added to the wave's sums per bucket.
+//   (Adding each ds to a sum in LDS costs about 3 clocks a value: 6.9 ms for 512 x 8 heads of 512 rows
+// of 64 bf16 values, which take 1.1 ms this way.)
+template <typename T, int DP, bool Wide>
+__global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void attention_query_grad_kernel(
     Params p, const T *out, const T *gout, const float *stats, float *lses, float *deltas, T *gq,
     float *partial, int nq) {
-  constexpr int P = pitch<T, DP>(), Chunks = DP / 16, Blocks = DP / 32;
-  __shared__ __attribute__((aligned(16))) T ks[2][kTile * P];
-  __shared__ __attribute__((aligned(16))) T vs[2][kTile * P];
+  constexpr int Chunks = DP / 16, Blocks = DP / 32;
+  __shared__ Word ks[2][kTile * words<T, DP>()];
+  __shared__ Word vs[2][kTile * words<T, DP>()];
   __shared__ __attribute__((aligned(16))) Window window[2];
   __shared__ int window_bucket[2][kWindow];
-  __shared__ float ring[kWaves][128];
+  __shared__ __attribute__((aligned(16))) float finished[kWaves][64];
   extern __shared__ float table[];  // NB values, then kWaves x NB sums
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
@@ -64,7 +81,6 @@ __global__ __launch_bounds__(64 * kWaves) void attention_query_grad_kernel(
   const T *k = (const T *)p.k + b * p.ks[0] + kh * p.ks[2];
   const T *v = (const T *)p.v + b * p.vs[0] + kh * p.vs[2];
   const int64_t row = ((int64_t)b * p.Lq + i) * p.Hq + h;
-  const bool out_wide = p.D % (16 / (int)sizeof(T)) == 0;
   const bool biased = p.table != nullptr, table_grad = partial != nullptr;
   float *sums = table + p.NB + wave * p.NB;
 
@@ -74,10 +90,9 @@ __global__ __launch_bounds__(64 * kWaves) void attention_query_grad_kernel(
   floatx16 products = (floatx16)(0.f);
 #pragma unroll
   for (int c = 0; c < Chunks; c++) {
-    qf[c] = global_frag<T>(live ? q : nullptr, c, half, p.D, p.q_wide);
-    gf[c] = global_frag<T>(live ? gout + row * p.D : nullptr, c, half, p.D, out_wide);
-    products = mma(global_frag<T>(live ? out + row * p.D : nullptr, c, half, p.D, out_wide), gf[c],
-                   products);
+    qf[c] = global_frag<Wide>(live ? q : nullptr, c, half, p.D);
+    gf[c] = global_frag<Wide>(live ? gout + row * p.D : nullptr, c, half, p.D);
+    products = mma(global_frag<Wide>(live ? out + row * p.D : nullptr, c, half, p.D), gf[c], products);
   }
   float delta = 0.f;
 #pragma unroll
@@ -99,24 +114,25 @@ __global__ __launch_bounds__(64 * kWaves) void attention_query_grad_kernel(
   }
   if (!gq && !table_grad) return;
 
-  const int base = -(start + i0 + kBlock - 1);
+  const int base = -(start + i0 + kBlock);
   if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
   if (table_grad) {
     for (int n = lane; n < p.NB; n += 64) sums[n] = 0.f;
-    ring[wave][lane] = ring[wave][64 + lane] = 0.f;
   }
-  Tile<T, DP> kt, vt;
+  Feed<T, DP, Wide> kt(p.ks[1], p.D, tid), vt(p.vs[1], p.D, tid);
   int bucket = 0;
   const int tiles = (keys + kTile - 1) / kTile;
   if (tiles > 0) {
-    kt.load(k, p.ks[1], keys, p.D, p.k_wide, tid);
-    vt.load(v, p.vs[1], keys, p.D, p.v_wide, tid);
+    kt.start(k, p.ks[1], keys, ks[0], p.D, tid);
+    vt.start(v, p.vs[1], keys, vs[0], p.D, tid);
     if (biased) bucket = bucket_of(p, base + tid);
   }
+  if (!biased) clear(window, tid);
+  loads_done();
   __syncthreads();
   if (tiles > 0) {
-    kt.store(ks[0], tid);
-    vt.store(vs[0], tid);
+    kt.finish(ks[0], tid);
+    vt.finish(vs[0], tid);
     if (biased && tid < kWindow) {
       window[0].put(tid, bias_of(table, p.NB, bucket));
       window_bucket[0][tid] = bucket;
@@ -124,8 +140,10 @@ __global__ __launch_bounds__(64 * kWaves) void attention_query_grad_kernel(
   }
   __syncthreads();
 
-  const int at = kBlock - 1 - local, shift = at & 3;
+  const int at = kBlock - local + 32 * half, shift = at & 3;
   const bool huge = __any(lse < kInf && fabsf(lse) > kHugeStat);
+  const float kept = lane == 32 ? 0.f : 1.f;
+  float diagonals = 0.f;
   floatx16 acc[Blocks];
 #pragma unroll
   for (int d = 0; d < Blocks; d++) acc[d] = (floatx16)(0.f);
@@ -134,31 +152,23 @@ __global__ __launch_bounds__(64 * kWaves) void attention_query_grad_kernel(
     const int j0 = t * kTile, buf = t & 1;
     if (t + 1 < tiles) {
       const int64_t next = j0 + kTile;
-      kt.load(k + next * p.ks[1], p.ks[1], keys - (int)next, p.D, p.k_wide, tid);
-      vt.load(v + next * p.vs[1], p.vs[1], keys - (int)next, p.D, p.v_wide, tid);
+      kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[buf ^ 1], p.D, tid);
+      vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[buf ^ 1], p.D, tid);
       if (biased) bucket = bucket_of(p, base + (int)next + tid);
     }
 #pragma unroll
     for (int blk = 0; blk < 2; blk++) {
       floatx16 u, dp;
-      if (biased) {
-        const floatx8 lo = window[buf].get(at + 32 * blk + 8 * half, shift);
-        const floatx8 hi = window[buf].get(at + 32 * blk + 16 + 8 * half, shift);
-        u = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15);
-      } else {
-        u = (floatx16)(0.f);
-      }
+      u = sixteen(window[buf].get(at + 16 * blk, shift), window[buf].get(at + 16 * blk + 8, shift));
       dp = (floatx16)(0.f);
 #pragma unroll
       for (int ch = 0; ch < Chunks; ch++) {
-        u = mma(row_frag<T, DP>(ks[buf], 32 * blk + row_of(lane & 31), ch, half), qf[ch], u);
-        dp = mma(row_frag<T, DP>(vs[buf], 32 * blk + row_of(lane & 31), ch, half), gf[ch], dp);
+        u = mma(row_frag<T, DP>(ks[buf], row_of(lane & 31, blk), ch, half), qf[ch], u);
+        dp = mma(row_frag<T, DP>(vs[buf], row_of(lane & 31, blk), ch, half), gf[ch], dp);
       }
       dp = add_outer(half ? 0.f : 1.f, -delta, dp);
       if (j0 + kTile > wave_limit) {
-#pragma unroll
-        for (int n = 0; n < 16; n++)
-          if (j0 + 32 * blk + 16 * (n >> 3) + 8 * half + (n & 7) >= limit) u[n] = -kInf;
+        keep_between(u, 0, limit - (j0 + 32 * half + 16 * blk));
       }
       if (huge) {
 #pragma unroll
@@ -167,35 +177,42 @@ __global__ __launch_bounds__(64 * kWaves) void attention_query_grad_kernel(
 #pragma unroll
         for (int n = 0; n < 16; n++) dp[n] *= probability<false>(u[n], c, lse, ref, inv);
       }
-      if (table_grad) {
-        // place of difference j - i in the ring: (j - j0) - (i - wave's first) + 64 t + 64, mod 128
-        const int place = 32 * blk + 8 * half - (lane & 31) + 64 * (t + 1);
-#pragma unroll
-        for (int n = 0; n < 16; n++)
-          atomicAdd(&ring[wave][(place + 16 * (n >> 3) + (n & 7)) & 127], dp[n]);
-      }
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-        const floatx8 x = s == 0
-            ? __builtin_shufflevector(dp, dp, 0, 1, 2, 3, 4, 5, 6, 7)
-            : __builtin_shufflevector(dp, dp, 8, 9, 10, 11, 12, 13, 14, 15);
-        const Frag<T> f = Frag<T>::pack(x);
+        const Frag<T> f = Frag<T>::pack(eight(dp, s));
 #pragma unroll
         for (int d = 0; d < Blocks; d++)
-          acc[d] = mma(col_frag<DP>(ks[buf], 32 * blk + 16 * s, d, lane), f, acc[d]);
+          acc[d] = mma(Column<T, DP, 32>::get(ks[buf], 16 * blk + 8 * s, d, lane), f, acc[d]);
+      }
+      if (table_grad) {
+        floatx16 left;  // what lane 31 held before each step: a finished diagonal
+#pragma unroll
+        for (int n = 0; n < 16; n++) {
+          left[n] = diagonals;
+          diagonals = next_diagonals(dp[n], diagonals, kept);
+        }
+        if (lane == 31) {
+          floatx4 *to = (floatx4 *)&finished[wave][16 * blk];
+#pragma unroll
+          for (int n = 0; n < 4; n++)
+            to[n] = floatx4{left[4 * n], left[4 * n + 1], left[4 * n + 2], left[4 * n + 3]};
+        }
       }
     }
     if (table_grad) {
-      // differences -31 .. 32 of the tile (from the wave's first query) are met no more
-      const int x = lane - 31, place = (x + 64 * (t + 1)) & 127;
-      const float value = ring[wave][place];
-      ring[wave][place] = 0.f;
-      const int n = window_bucket[buf][x + kBlock - 1 - wave * kLanesRows];
+      // the lower half-wave's sums are finished (difference 31 - lane), the upper half's go on in
+      // the next tile's lower half, one lane up
+      if (half == 0) finished[wave][63 - lane] = diagonals;
+      diagonals = upper_to_lower(diagonals);
+      wave_order();
+      const float value = finished[wave][lane];
+      const int n = window_bucket[buf][lane + kBlock - 32 - wave * kLanesRows];
       if ((unsigned)n < (unsigned)p.NB) atomicAdd(&sums[n], value);
+      wave_order();
     }
     if (t + 1 < tiles) {
-      kt.store(ks[buf ^ 1], tid);
-      vt.store(vs[buf ^ 1], tid);
+      kt.finish(ks[buf ^ 1], tid);
+      vt.finish(vs[buf ^ 1], tid);
       if (biased && tid < kWindow) {
         window[buf ^ 1].put(tid, bias_of(table, p.NB, bucket));
         window_bucket[buf ^ 1][tid] = bucket;
@@ -204,10 +221,9 @@ __global__ __launch_bounds__(64 * kWaves) void attention_query_grad_kernel(
     __syncthreads();
   }
   if (table_grad) {
-    if (tiles > 0 && lane < 31) {  // differences 33 .. 63 of the last tile
-      const int x = lane + 33, place = (x + 64 * tiles) & 127;
-      const int n = window_bucket[(tiles - 1) & 1][x + kBlock - 1 - wave * kLanesRows];
-      if ((unsigned)n < (unsigned)p.NB) atomicAdd(&sums[n], ring[wave][place]);
+    if (tiles > 0 && half == 0) {  // differences 63 - lane of the last tile
+      const int n = window_bucket[(tiles - 1) & 1][63 - lane + kBlock - wave * kLanesRows];
+      if ((unsigned)n < (unsigned)p.NB) atomicAdd(&sums[n], diagonals);
     }
     __syncthreads();
     float *to = partial + ((int64_t)bh * nq + block) * p.NB;
@@ -218,18 +234,18 @@ __global__ __launch_bounds__(64 * kWaves) void attention_query_grad_kernel(
       to[n] = x;
     }
   }
-  if (live && gq) store_column<T, Blocks>(gq + row * p.D, acc, p.scale, p.D, half, p.D % 4 == 0);
+  if (live && gq) store_column<Wide, T, Blocks>(gq + row * p.D, acc, p.scale, p.D, half);
 }
 
 // Keys' and values' gradients: a workgroup holds 128 keys of a key head, a wave 32 of them as
 // columns, and walks the queries of all heads that share them, 64 at a time.
-template <typename T, int DP>
-__global__ __launch_bounds__(64 * kWaves) void attention_key_grad_kernel(
+template <typename T, int DP, bool Wide>
+__global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void attention_key_grad_kernel(
     Params p, const T *gout, const float *stats, const float *lses, const float *deltas, T *gk,
     T *gv, int nk) {
-  constexpr int P = pitch<T, DP>(), Chunks = DP / 16, Blocks = DP / 32;
-  __shared__ __attribute__((aligned(16))) T qs[2][kTile * P];
-  __shared__ __attribute__((aligned(16))) T gs[2][kTile * P];
+  constexpr int Chunks = DP / 16, Blocks = DP / 32;
+  __shared__ Word qs[2][kTile * words<T, DP>()];
+  __shared__ Word gs[2][kTile * words<T, DP>()];
   __shared__ __attribute__((aligned(16))) Window window[2];
   __shared__ __attribute__((aligned(16))) float row_lse[2][kTile], row_delta[2][kTile],
       row_ref[2][kTile], row_inv[2][kTile];
@@ -251,36 +267,37 @@ __global__ __launch_bounds__(64 * kWaves) void attention_key_grad_kernel(
 
   const T *k = (const T *)p.k + b * p.ks[0] + (int64_t)j * p.ks[1] + kh * p.ks[2];
   const T *v = (const T *)p.v + b * p.vs[0] + (int64_t)j * p.vs[1] + kh * p.vs[2];
-  const bool out_wide = p.D % (16 / (int)sizeof(T)) == 0;
   const bool biased = p.table != nullptr;
   Frag<T> kf[Chunks], vf[Chunks];
 #pragma unroll
   for (int c = 0; c < Chunks; c++) {
-    kf[c] = global_frag<T>(used ? k : nullptr, c, half, p.D, p.k_wide);
-    vf[c] = global_frag<T>(used ? v : nullptr, c, half, p.D, p.v_wide);
+    kf[c] = global_frag<Wide>(used ? k : nullptr, c, half, p.D);
+    vf[c] = global_frag<Wide>(used ? v : nullptr, c, half, p.D);
   }
   const float c = p.scale * kLog2e;
-  const int at = kBlock - 1 - local, shift = at & 3;
+  const int at = kBlock - local + 32 * half, shift = at & 3;
   floatx16 dk[Blocks], dv[Blocks];
 #pragma unroll
   for (int d = 0; d < Blocks; d++) dk[d] = dv[d] = (floatx16)(0.f);
 
-  Tile<T, DP> qt, gt;
+  const int64_t go_row = (int64_t)p.Hq * p.D;
+  Feed<T, DP, Wide> qt(p.qs[1], p.D, tid), gt(go_row, p.D, tid);
   int bucket = 0;
   float lse = 0.f, delta = 0.f, ref = 0.f, sum = 1.f;
+  if (!biased) clear(window, tid);
+  loads_done();
   for (int g = 0; g < group && t0 < t1; g++) {
     const int h = kh * group + g;
     const T *q = (const T *)p.q + b * p.qs[0] + h * p.qs[2];
     const T *go = gout + ((int64_t)b * p.Lq * p.Hq + h) * p.D;
-    const int64_t go_row = (int64_t)p.Hq * p.D;
     const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq;
-    // window value x: query - key = (first query of the tile) - (j0 + kBlock - 1) + x, so the
-    // bucket's difference is j0 + kBlock - 1 - start - first query - x
-    const int base = j0 + kBlock - 1 - start;
-    auto fetch = [&](int t) {
+    // window value x: query - key = (first query of the tile) - (j0 + kBlock) + x, so the bucket's
+    // difference is j0 + kBlock - start - first query - x
+    const int base = j0 + kBlock - start;
+    auto fetch = [&](int t, int buf) {
       const int64_t i = (int64_t)t * kTile;
-      qt.load(q + i * p.qs[1], p.qs[1], p.Lq - (int)i, p.D, p.q_wide, tid);
-      gt.load(go + i * go_row, go_row, p.Lq - (int)i, p.D, out_wide, tid);
+      qt.start(q + i * p.qs[1], p.qs[1], p.Lq - (int)i, qs[buf], p.D, tid);
+      gt.start(go + i * go_row, go_row, p.Lq - (int)i, gs[buf], p.D, tid);
       if (biased) bucket = bucket_of(p, base - (int)i - tid);
       if (tid < kTile) {
         const bool in = i + tid < p.Lq;
@@ -291,8 +308,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_key_grad_kernel(
       }
     };
     auto put = [&](int buf) {
-      qt.store(qs[buf], tid);
-      gt.store(gs[buf], tid);
+      qt.finish(qs[buf], tid);
+      gt.finish(gs[buf], tid);
       if (biased && tid < kWindow) window[buf].put(tid, bias_of(table, p.NB, bucket));
       if (tid < kTile) {
         row_lse[buf][tid] = lse;
@@ -302,43 +319,34 @@ __global__ __launch_bounds__(64 * kWaves) void attention_key_grad_kernel(
       }
     };
     if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
-    fetch(t0);
+    fetch(t0, 0);
     __syncthreads();
     put(0);
     __syncthreads();
     for (int t = t0; t < t1; t++) {
       const int buf = (t - t0) & 1, i0 = t * kTile;
-      if (t + 1 < t1) fetch(t + 1);
+      if (t + 1 < t1) fetch(t + 1, buf ^ 1);
       const float mine = row_lse[buf][lane];
       const bool huge = __any(mine < kInf && fabsf(mine) > kHugeStat);
 #pragma unroll
       for (int blk = 0; blk < 2; blk++) {
         floatx16 u, dp;
-        if (biased) {
-          const floatx8 lo = window[buf].get(at + 32 * blk + 8 * half, shift);
-          const floatx8 hi = window[buf].get(at + 32 * blk + 16 + 8 * half, shift);
-          u = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15);
-        } else {
-          u = (floatx16)(0.f);
-        }
+        u = sixteen(window[buf].get(at + 16 * blk, shift), window[buf].get(at + 16 * blk + 8, shift));
         auto rows8 = [&](const float *x, int s) {
-          const floatx4 *w = (const floatx4 *)(x + 32 * blk + 16 * s + 8 * half);
+          const floatx4 *w = (const floatx4 *)(x + 32 * half + 16 * blk + 8 * s);
           const floatx4 lo = w[0], hi = w[1];
           return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         };
         dp = (floatx16)(0.f);
 #pragma unroll
         for (int ch = 0; ch < Chunks; ch++) {
-          u = mma(row_frag<T, DP>(qs[buf], 32 * blk + row_of(lane & 31), ch, half), kf[ch], u);
-          dp = mma(row_frag<T, DP>(gs[buf], 32 * blk + row_of(lane & 31), ch, half), vf[ch], dp);
+          u = mma(row_frag<T, DP>(qs[buf], row_of(lane & 31, blk), ch, half), kf[ch], u);
+          dp = mma(row_frag<T, DP>(gs[buf], row_of(lane & 31, blk), ch, half), vf[ch], dp);
         }
-        dp = add_outer(half ? 0.f : row_delta[buf][32 * blk + row_of(lane & 31)], 1.f, dp);
+        dp = add_outer(half ? 0.f : row_delta[buf][row_of(lane & 31, blk)], 1.f, dp);
         if (i0 < wave_safe || i0 + kTile > p.Lq) {
-#pragma unroll
-          for (int n = 0; n < 16; n++) {
-            const int i = i0 + 32 * blk + 16 * (n >> 3) + 8 * half + (n & 7);
-            if (i < own_first || i >= p.Lq) u[n] = -kInf;
-          }
+          const int row0 = i0 + 32 * half + 16 * blk;
+          keep_between(u, own_first - row0, p.Lq - row0);
         }
 #pragma unroll
         for (int s = 0; s < 2; s++) {
@@ -357,8 +365,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_key_grad_kernel(
           const Frag<T> pf = Frag<T>::pack(x), sf = Frag<T>::pack(y);
 #pragma unroll
           for (int d = 0; d < Blocks; d++) {
-            dv[d] = mma(col_frag<DP>(gs[buf], 32 * blk + 16 * s, d, lane), pf, dv[d]);
-            dk[d] = mma(col_frag<DP>(qs[buf], 32 * blk + 16 * s, d, lane), sf, dk[d]);
+            dv[d] = mma(Column<T, DP, 32>::get(gs[buf], 16 * blk + 8 * s, d, lane), pf, dv[d]);
+            dk[d] = mma(Column<T, DP, 32>::get(qs[buf], 16 * blk + 8 * s, d, lane), sf, dk[d]);
           }
         }
       }
@@ -373,37 +381,42 @@ __global__ __launch_bounds__(64 * kWaves) void attention_key_grad_kernel(
 #pragma unroll
     for (int d = 0; d < Blocks; d++) dk[d] = dv[d] = (floatx16)(0.f);
   }
-  if (gk) store_column<T, Blocks>(gk + row * p.D, dk, p.scale, p.D, half, p.D % 4 == 0);
-  if (gv) store_column<T, Blocks>(gv + row * p.D, dv, 1.f, p.D, half, p.D % 4 == 0);
+  if (gk) store_column<Wide, T, Blocks>(gk + row * p.D, dk, p.scale, p.D, half);
+  if (gv) store_column<Wide, T, Blocks>(gv + row * p.D, dv, 1.f, p.D, half);
 }
 
-// Sums per bucket of a head over the batch and the blocks of queries, in a fixed order: a
-// workgroup has one head and 64 buckets, its waves every kWaves-th part.
+// Sums per bucket of a head, in a fixed order.  Of `rows` sums of a head ([B][Hq][nq] with rows =
+// B nq, or [Hq][rows] with nq = rows), slice blockIdx.z of gridDim.z takes every gridDim.z-th; a
+// workgroup has one head and 64 buckets, its waves every kWaves-th row of the slice.
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves) void attention_table_grad_kernel(const float *partial,
-                                                                           T *gtable, int B, int Hq,
-                                                                           int nq, int NB) {
+                                                                           T *to, int64_t rows,
+                                                                           int Hq, int nq, int NB) {
   __shared__ float part[kWaves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int h = blockIdx.y, n = blockIdx.x * 64 + lane;
   float x = 0.f;
   if (n < NB)
-    for (int64_t s = wave; s < (int64_t)B * nq; s += kWaves)
+#pragma unroll 4
+    for (int64_t s = blockIdx.z * kWaves + wave; s < rows; s += kWaves * gridDim.z)
       x += partial[((s / nq * Hq + h) * nq + s % nq) * NB + n];
   part[wave][lane] = x;
   __syncthreads();
   if (wave == 0 && n < NB) {
     for (int w = 1; w < kWaves; w++) x += part[w][lane];
-    gtable[(int64_t)h * NB + n] = (T)x;
+    to[((int64_t)h * gridDim.z + blockIdx.z) * NB + n] = (T)x;
   }
 }
+
+constexpr int kSlices = 64;  // of the sums per bucket, where there are many
 
 static int64_t query_blocks(const Params &p) { return (p.Lq + kBlock - 1) / kBlock; }
 
 static size_t backward_bytes(const Params &p) {
   const size_t rows = (size_t)p.B * p.Hq * p.Lq;
   return 2 * align256(rows * sizeof(float)) +
-         align256((size_t)p.B * p.Hq * query_blocks(p) * p.NB * sizeof(float));
+         align256((size_t)p.B * p.Hq * query_blocks(p) * p.NB * sizeof(float)) +
+         align256((size_t)kSlices * p.Hq * p.NB * sizeof(float));
 }
 
 template <typename T>
@@ -418,32 +431,36 @@ static int launch_backward(const Params &p, const void *gout, const void *out, c
   if (rows) {
     const dim3 grid((unsigned)((int64_t)p.B * p.Hq * nq));
     const size_t lds = (gtable ? 1 + kWaves : 1) * p.NB * sizeof(float);
-#define MCX_GRAD(DP)                                                                              \
-  hipLaunchKernelGGL((attention_query_grad_kernel<T, DP>), grid, threads, lds, stream, p,          \
+#define MCX_GRAD(DP, W)                                                                           \
+  hipLaunchKernelGGL((attention_query_grad_kernel<T, DP, W>), grid, threads, lds, stream, p,       \
                      (const T *)out, (const T *)gout, stats, lses, deltas, (T *)gq,               \
                      gtable ? partial : nullptr, nq)
-    if (p.D <= 32) MCX_GRAD(32);
-    else if (p.D <= 64) MCX_GRAD(64);
-    else if (p.D <= 96) MCX_GRAD(96);
-    else MCX_GRAD(128);
+    MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out) && aligned16(gout) && aligned16(gq), MCX_GRAD);
 #undef MCX_GRAD
     MCX_HIP_CHECK_LAUNCH();
   }
   if (gtable) {
-    hipLaunchKernelGGL((attention_table_grad_kernel<T>), dim3((p.NB + 63) / 64, p.Hq), threads, 0,
-                       stream, partial, (T *)gtable, p.B, p.Hq, nq, p.NB);
+    const int64_t count = (int64_t)p.B * nq;
+    const int wide = (p.NB + 63) / 64;
+    if (count <= 2 * kSlices) {
+      hipLaunchKernelGGL((attention_table_grad_kernel<T>), dim3(wide, p.Hq), threads, 0, stream,
+                         partial, (T *)gtable, count, p.Hq, nq, p.NB);
+    } else {
+      float *slices = (float *)((char *)partial + align256((size_t)p.B * p.Hq * nq * p.NB * sizeof(float)));
+      hipLaunchKernelGGL((attention_table_grad_kernel<float>), dim3(wide, p.Hq, kSlices), threads, 0,
+                         stream, partial, slices, count, p.Hq, nq, p.NB);
+      hipLaunchKernelGGL((attention_table_grad_kernel<T>), dim3(wide, p.Hq), threads, 0, stream,
+                         slices, (T *)gtable, (int64_t)kSlices, p.Hq, kSlices, p.NB);
+    }
     MCX_HIP_CHECK_LAUNCH();
   }
   if ((gk || gv) && p.B && p.Lk) {
     const dim3 grid((unsigned)((int64_t)p.B * p.Hk * nk));
     const size_t lds = p.NB * sizeof(float);
-#define MCX_GRAD(DP)                                                                          \
-  hipLaunchKernelGGL((attention_key_grad_kernel<T, DP>), grid, threads, lds, stream, p,        \
+#define MCX_GRAD(DP, W)                                                                      \
+  hipLaunchKernelGGL((attention_key_grad_kernel<T, DP, W>), grid, threads, lds, stream, p,    \
                      (const T *)gout, stats, lses, deltas, (T *)gk, (T *)gv, nk)
-    if (p.D <= 32) MCX_GRAD(32);
-    else if (p.D <= 64) MCX_GRAD(64);
-    else if (p.D <= 96) MCX_GRAD(96);
-    else MCX_GRAD(128);
+    MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(gout) && aligned16(gk) && aligned16(gv), MCX_GRAD);
 #undef MCX_GRAD
     MCX_HIP_CHECK_LAUNCH();
   }

@@ -12,12 +12,12 @@ namespace attention {
 // the next tile's loads under way while the current one is multiplied.
 //   The reference is the row's maximum, but it follows it only when a score exceeds it by 2^8:
 // sums stay far inside fp32, and the accumulated output is seldom rescaled.
-template <typename T, int DP>
-__global__ __launch_bounds__(64 * kWaves) void attention_forward_kernel(Params p, T *out,
-                                                                        float *stats, int nq) {
-  constexpr int P = pitch<T, DP>(), Chunks = DP / 16, Blocks = DP / 32;
-  __shared__ __attribute__((aligned(16))) T ks[2][kTile * P];
-  __shared__ __attribute__((aligned(16))) T vs[2][kTile * P];
+template <typename T, int DP, bool Wide>
+__global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void attention_forward_kernel(
+    Params p, T *out, float *stats, int nq) {
+  constexpr int Chunks = DP / 16, Blocks = DP / 32;
+  __shared__ Word ks[2][kTile * words<T, DP>()];
+  __shared__ Word vs[2][kTile * words<T, DP>()];
   __shared__ __attribute__((aligned(16))) Window window[2];
   extern __shared__ float table[];
 
@@ -42,30 +42,32 @@ __global__ __launch_bounds__(64 * kWaves) void attention_forward_kernel(Params p
 
   Frag<T> qf[Chunks];
 #pragma unroll
-  for (int c = 0; c < Chunks; c++) qf[c] = global_frag<T>(live ? q : nullptr, c, half, p.D, p.q_wide);
+  for (int c = 0; c < Chunks; c++) qf[c] = global_frag<Wide>(live ? q : nullptr, c, half, p.D);
 
   // window value t stands for the difference (first key of the tile) - (position of query
-  // i0 + kBlock - 1) + t
-  const int base = -(start + i0 + kBlock - 1);
+  // i0 + kBlock) + t
+  const int base = -(start + i0 + kBlock);
   if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
-  Tile<T, DP> kt, vt;
+  Feed<T, DP, Wide> kt(p.ks[1], p.D, tid), vt(p.vs[1], p.D, tid);
   int bucket = 0;
   const int tiles = (keys + kTile - 1) / kTile;
   if (tiles > 0) {
-    kt.load(k, p.ks[1], keys, p.D, p.k_wide, tid);
-    vt.load(v, p.vs[1], keys, p.D, p.v_wide, tid);
+    kt.start(k, p.ks[1], keys, ks[0], p.D, tid);
+    vt.start(v, p.vs[1], keys, vs[0], p.D, tid);
     if (biased) bucket = bucket_of(p, base + tid);
   }
+  if (!biased) clear(window, tid);
+  loads_done();
   __syncthreads();  // the table
   if (tiles > 0) {
-    kt.store(ks[0], tid);
-    vt.store(vs[0], tid);
+    kt.finish(ks[0], tid);
+    vt.finish(vs[0], tid);
     if (biased && tid < kWindow) window[0].put(tid, bias_of(table, p.NB, bucket));
   }
   __syncthreads();
 
   const float c = p.scale * kLog2e;
-  const int at = kBlock - 1 - local, shift = at & 3;
+  const int at = kBlock - local + 32 * half, shift = at & 3;
   floatx16 o[Blocks];
 #pragma unroll
   for (int d = 0; d < Blocks; d++) o[d] = (floatx16)(0.f);
@@ -75,32 +77,22 @@ __global__ __launch_bounds__(64 * kWaves) void attention_forward_kernel(Params p
     const int j0 = t * kTile, buf = t & 1;
     if (t + 1 < tiles) {
       const int64_t next = j0 + kTile;
-      kt.load(k + next * p.ks[1], p.ks[1], keys - (int)next, p.D, p.k_wide, tid);
-      vt.load(v + next * p.vs[1], p.vs[1], keys - (int)next, p.D, p.v_wide, tid);
+      kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[buf ^ 1], p.D, tid);
+      vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[buf ^ 1], p.D, tid);
       if (biased) bucket = bucket_of(p, base + (int)next + tid);
     }
     floatx16 u[2];
 #pragma unroll
     for (int blk = 0; blk < 2; blk++) {
-      if (biased) {
-        const floatx8 lo = window[buf].get(at + 32 * blk + 8 * half, shift);
-        const floatx8 hi = window[buf].get(at + 32 * blk + 16 + 8 * half, shift);
-        u[blk] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15);
-      } else {
-        u[blk] = (floatx16)(0.f);
-      }
+      u[blk] = sixteen(window[buf].get(at + 16 * blk, shift), window[buf].get(at + 16 * blk + 8, shift));
 #pragma unroll
       for (int ch = 0; ch < Chunks; ch++)
-        u[blk] = mma(row_frag<T, DP>(ks[buf], 32 * blk + row_of(lane & 31), ch, half), qf[ch], u[blk]);
+        u[blk] = mma(row_frag<T, DP>(ks[buf], row_of(lane & 31, blk), ch, half), qf[ch], u[blk]);
     }
     if (j0 + kTile > wave_limit) {
 #pragma unroll
       for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-        for (int n = 0; n < 16; n++) {
-          const int j = j0 + 32 * blk + 16 * (n >> 3) + 8 * half + (n & 7);
-          if (j >= limit) u[blk][n] = -kInf;
-        }
+        keep_between(u[blk], 0, limit - (j0 + 32 * half + 16 * blk));
     }
     float top = u[0][0];
 #pragma unroll
@@ -136,19 +128,16 @@ __global__ __launch_bounds__(64 * kWaves) void attention_forward_kernel(Params p
       for (int n = 0; n < 16; n++) part += u[blk][n];
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-        const floatx8 x = s == 0
-            ? __builtin_shufflevector(u[blk], u[blk], 0, 1, 2, 3, 4, 5, 6, 7)
-            : __builtin_shufflevector(u[blk], u[blk], 8, 9, 10, 11, 12, 13, 14, 15);
-        const Frag<T> pf = Frag<T>::pack(x);
+        const Frag<T> pf = Frag<T>::pack(eight(u[blk], s));
 #pragma unroll
         for (int d = 0; d < Blocks; d++)
-          o[d] = mma(col_frag<DP>(vs[buf], 32 * blk + 16 * s, d, lane), pf, o[d]);
+          o[d] = mma(Column<T, DP, 32>::get(vs[buf], 16 * blk + 8 * s, d, lane), pf, o[d]);
       }
     }
     sum += part;
     if (t + 1 < tiles) {
-      kt.store(ks[buf ^ 1], tid);
-      vt.store(vs[buf ^ 1], tid);
+      kt.finish(ks[buf ^ 1], tid);
+      vt.finish(vs[buf ^ 1], tid);
       if (biased && tid < kWindow) window[buf ^ 1].put(tid, bias_of(table, p.NB, bucket));
     }
     __syncthreads();
@@ -156,7 +145,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_forward_kernel(Params p
   sum += other_half(sum);
   if (!live) return;
   const int64_t row = ((int64_t)b * p.Lq + i) * p.Hq + h;
-  store_column<T, Blocks>(out + row * p.D, o, sum == 0.f ? 0.f : 1.f / sum, p.D, half, p.D % 4 == 0);
+  store_column<Wide, T, Blocks>(out + row * p.D, o, sum == 0.f ? 0.f : 1.f / sum, p.D, half);
   if (stats && half == 0) {
     float *s = stats + 2 * (((int64_t)b * p.Hq + h) * p.Lq + i);
     s[0] = ref;
@@ -169,21 +158,19 @@ static int launch_forward(const Params &p, void *out, float *stats, hipStream_t 
   const int nq = (p.Lq + kBlock - 1) / kBlock;
   const dim3 grid((unsigned)((int64_t)p.B * p.Hq * nq)), threads(64 * kWaves);
   const size_t lds = p.table ? p.NB * sizeof(float) : 0;
-#define MCX_FORWARD(DP)                                                                         \
-  hipLaunchKernelGGL((attention_forward_kernel<T, DP>), grid, threads, lds, stream, p, (T *)out, \
+#define MCX_FORWARD(DP, W)                                                                     \
+  hipLaunchKernelGGL((attention_forward_kernel<T, DP, W>), grid, threads, lds, stream, p, (T *)out, \
                      stats, nq)
-  if (p.D <= 32) MCX_FORWARD(32);
-  else if (p.D <= 64) MCX_FORWARD(64);
-  else if (p.D <= 96) MCX_FORWARD(96);
-  else MCX_FORWARD(128);
+  MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out), MCX_FORWARD);
 #undef MCX_FORWARD
   MCX_HIP_CHECK_LAUNCH();
   return MCX_OK;
 }
 
-static bool wide_loads(const void *p, const int64_t *strides, int64_t D, int64_t per16) {
-  return (uintptr_t)p % 16 == 0 && D % per16 == 0 && strides[0] % per16 == 0 &&
-         strides[1] % per16 == 0 && strides[2] % per16 == 0;
+// Whether rows are whole 16-byte words, and a tile's offsets fit 32 bits.
+static bool wide_rows(const void *p, const int64_t *strides, int64_t D, int64_t per16) {
+  return aligned16(p) && D % per16 == 0 && strides[0] % per16 == 0 && strides[1] % per16 == 0 &&
+         strides[2] % per16 == 0 && strides[1] >= 0 && strides[1] < (1 << 22);
 }
 
 int make_params(Params &p, const void *q, const void *k, const void *v, const void *table,
@@ -200,7 +187,7 @@ int make_params(Params &p, const void *q, const void *k, const void *v, const vo
   if (d->B && d->Lq && (!q || (d->Lk && (!k || !v)))) return MCX_E_NULL;
   if ((table != nullptr) != (buckets != nullptr)) return MCX_E_NULL;
   if (table && (d->table_size < 1 || d->table_size > kMaxTable || d->bucket_count < 1 ||
-                d->bucket_count > 4 * most || d->bucket_zero < 0 ||
+                d->bucket_count > kMostPosition || d->bucket_zero < 0 ||
                 d->bucket_zero >= d->bucket_count))
     return MCX_E_SHAPE;
   p.q = q, p.k = k, p.v = v, p.table = table;
@@ -213,9 +200,8 @@ int make_params(Params &p, const void *q, const void *k, const void *v, const vo
   p.NB = table ? (int)d->table_size : 0, p.causal = d->causal != 0;
   p.scale = (float)d->scale;
   const int64_t per16 = dtype == MCX_BF16 ? 8 : 4;
-  p.q_wide = wide_loads(q, p.qs, p.D, per16);
-  p.k_wide = wide_loads(k, p.ks, p.D, per16);
-  p.v_wide = wide_loads(v, p.vs, p.D, per16);
+  p.wide = wide_rows(q, p.qs, p.D, per16) && wide_rows(k, p.ks, p.D, per16) &&
+           wide_rows(v, p.vs, p.D, per16);
   return MCX_OK;
 }
 

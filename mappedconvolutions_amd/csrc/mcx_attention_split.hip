@@ -16,12 +16,8 @@ constexpr int kRows = 32;       // rows of a workgroup
 constexpr int kStep = 32;       // keys of a wave's tile
 constexpr int kMostParts = 256;
 
-// What a wave's lanes have written to LDS is there for its other lanes: the hardware keeps a wave's
-// LDS instructions in order, and the compiler may not move them past this.
-__device__ inline void wave_order() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
+// As `row_of`, for 32 rows: a lane gets rows 16 c + 8 (lane >> 5) + 0 .. 7 (bits 2 and 3 swapped).
+__device__ inline int row_of_32(int m) { return (m & 0x13) | ((m & 4) << 1) | ((m & 8) >> 1); }
 
 struct Split {
   int parts;       // of the keys
@@ -31,14 +27,14 @@ struct Split {
   float *outs;     // [B * Hk * blocks][parts][32][D]
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool Wide>
 __global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, Split sp, T *out,
                                                                       float *stats) {
-  constexpr int P = pitch<T, DP>(), Chunks = DP / 16, Blocks = DP / 32;
-  constexpr int E = 16 / (int)sizeof(T), PerRow = DP / E, N = kStep * PerRow / 64;
+  constexpr int Chunks = DP / 16, Blocks = DP / 32;
+  constexpr int E = 16 / (int)sizeof(T), PerRow = words<T, DP>(), N = kStep * PerRow / 64;
   // a wave's values; at the end all waves' sums, four blocks of columns at a time
-  constexpr int kTileBytes = kStep * P * (int)sizeof(T);
-  __shared__ __attribute__((aligned(16))) char tiles_lds[kWaves * kTileBytes];
+  constexpr int kTileWords = kStep * PerRow;
+  __shared__ Word tiles_lds[kWaves * kTileWords];
   __shared__ int buckets_lds[kWaves][64];
   __shared__ float merge[kWaves][kRows][2];
   extern __shared__ float table[];  // [min(group, 32)][NB]
@@ -78,29 +74,31 @@ __global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, 
   const T *v = (const T *)p.v + b * p.vs[0] + kh * p.vs[2];
   const T *q = (const T *)p.q + b * p.qs[0] + (int64_t)i * p.qs[1] + h * p.qs[2];
   Frag<T> qf[Chunks], kf[Chunks];
-  uint4 vr[N];
+  Word vr[N];
 #pragma unroll
-  for (int c = 0; c < Chunks; c++) qf[c] = global_frag<T>(live ? q : nullptr, c, half, p.D, p.q_wide);
+  for (int c = 0; c < Chunks; c++) qf[c] = global_frag<Wide>(live ? q : nullptr, c, half, p.D);
 
-  const int key_row = row_of(lane & 31);
+  const int key_row = row_of_32(lane & 31);
   // bias: difference x of a tile = j - (position of the block's last query)
   const int origin = start + last_i, own = live ? last_i - i : 0;
   int bucket = 0;
   bool varied = false;  // whether the tile's pairs are of more than one bucket
   auto fetch = [&](int tile) {
     const int j0 = tile * kStep;
-    const T *row = j0 + key_row < keys ? k + (int64_t)(j0 + key_row) * p.ks[1] : nullptr;
+    // (a key behind the last one is the last one: its pairs are taken out below)
+    const T *row = k + (int64_t)min(j0 + key_row, keys - 1) * p.ks[1];
 #pragma unroll
-    for (int c = 0; c < Chunks; c++) kf[c] = global_frag<T>(row, c, half, p.D, p.k_wide);
+    for (int c = 0; c < Chunks; c++) kf[c] = global_frag<Wide>(row, c, half, p.D);
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      const int id = lane + 64 * n, j = j0 + id / PerRow, d0 = (id % PerRow) * E;
-      vr[n] = j < keys ? load16(v + (int64_t)j * p.vs[1], d0, p.D, p.v_wide) : make_uint4(0, 0, 0, 0);
+      const int id = lane + 64 * n, j = min(j0 + id / PerRow, keys - 1), d0 = (id % PerRow) * E;
+      const T *vrow = v + (int64_t)j * p.vs[1];
+      vr[n] = Wide ? *(const Word *)(vrow + (d0 < p.D ? d0 : 0)) : load16<false>(vrow, d0, p.D);
     }
     if (biased) bucket = bucket_of(p, j0 - origin + lane);
   };
   const float c = p.scale * kLog2e;
-  T *vs = (T *)(tiles_lds + wave * kTileBytes);
+  Word *vs = tiles_lds + wave * kTileWords;
   floatx16 o[Blocks];
 #pragma unroll
   for (int d = 0; d < Blocks; d++) o[d] = (floatx16)(0.f);
@@ -115,7 +113,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, 
 #pragma unroll
     for (int n = 0; n < N; n++) {
       const int id = lane + 64 * n;
-      *(uint4 *)(vs + (id / PerRow) * P + (id % PerRow) * E) = vr[n];
+      vs[word_at<T, DP>(id / PerRow, id % PerRow)] = vr[n];
     }
     buckets_lds[wave][lane] = bucket;
     wave_order();
@@ -161,11 +159,9 @@ __global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, 
     }
 #pragma unroll
     for (int s = 0; s < 2; s++) {
-      const floatx8 x = s == 0 ? __builtin_shufflevector(u, u, 0, 1, 2, 3, 4, 5, 6, 7)
-                               : __builtin_shufflevector(u, u, 8, 9, 10, 11, 12, 13, 14, 15);
-      const Frag<T> pf = Frag<T>::pack(x);
+      const Frag<T> pf = Frag<T>::pack(eight(u, s));
 #pragma unroll
-      for (int d = 0; d < Blocks; d++) o[d] = mma(col_frag<DP>(vs, 16 * s, d, lane), pf, o[d]);
+      for (int d = 0; d < Blocks; d++) o[d] = mma(Column<T, DP, 8>::get(vs, 16 * s, d, lane), pf, o[d]);
     }
   }
   sum += other_half(sum);
@@ -189,7 +185,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, 
   // wave w sums columns 32 d + 8 w .. 8 w + 7 of every block: [wave][32 columns][32 rows], a row
   // of 33 values
   float *part_lds = (float *)tiles_lds;
-  static_assert(kWaves * kTileBytes >= kWaves * 32 * 16 * 4, "a block's sums fit two halves");
+  static_assert(kTileWords * 16 >= 32 * 16 * 4, "a block's sums fit two halves");
   const int64_t at = (int64_t)unit * sp.parts + part;
 #pragma unroll
   for (int d = 0; d < Blocks; d++)
@@ -314,12 +310,10 @@ template <typename T>
 static int launch(const Params &p, Split sp, void *out, float *stats, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)p.B * p.Hk * sp.blocks * sp.parts)), threads(64 * kWaves);
   const size_t lds = p.table ? std::min(p.Hq / p.Hk, kRows) * p.NB * sizeof(float) : 0;
-#define MCX_SPLIT(DP) \
-  hipLaunchKernelGGL((attention_split_kernel<T, DP>), grid, threads, lds, stream, p, sp, (T *)out, stats)
-  if (p.D <= 32) MCX_SPLIT(32);
-  else if (p.D <= 64) MCX_SPLIT(64);
-  else if (p.D <= 96) MCX_SPLIT(96);
-  else MCX_SPLIT(128);
+#define MCX_SPLIT(DP, W)                                                                           \
+  hipLaunchKernelGGL((attention_split_kernel<T, DP, W>), grid, threads, lds, stream, p, sp, (T *)out, \
+                     stats)
+  MCX_ATTENTION_DISPATCH(p.D, p.wide, MCX_SPLIT);
 #undef MCX_SPLIT
   MCX_HIP_CHECK_LAUNCH();
   if (sp.parts > 1) {
