@@ -366,9 +366,16 @@ int make_params(Params &p, const void *q, const void *k, const void *v, const vo
                 const int32_t *buckets, const int32_t *query_start, const int32_t *key_lengths,
                 const mcx_attention_desc *desc, int dtype);
 
+// Work for fewer workgroups than there are compute units is split along the walked axis, in parts
+// of four tiles at least, whose results are joined afterwards: into how many parts.
+// 384 workgroups in all: gradients and output of 2 x 1250 float32 rows of 6 heads of 48 sharing 2
+// take 831 us with no parts, and 349, 286, 299, 324 us with 256, 384, 512, 1024; of 2562 bf16 rows
+// of 4 heads of 128 sharing one 236, 208, 249, 261 us.
+int parts_of(int64_t units, int64_t tiles);
+
 // The form for few queries against many keys (mcx_attention_split.hip): over how many parts of the
 // keys (0: not the form for these sizes), its workspace, and its launch.
-int split_parts(const Params &p);
+int split_parts(const Params &p, int dtype);
 size_t split_bytes(const Params &p, int parts);
 int launch_split(const Params &p, int parts, void *out, float *stats, void *workspace, int dtype,
                  hipStream_t stream);

@@ -55,7 +55,7 @@ __device__ inline float probability(float u, float c, float lse, float ref, floa
 template <typename T, int DP, bool Wide>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void attention_query_grad_kernel(
     Params p, const T *out, const T *gout, const float *stats, float *lses, float *deltas, T *gq,
-    float *partial, int nq) {
+    float *gq_parts, float *partial, int nq, int parts) {
   constexpr int Chunks = DP / 16, Blocks = DP / 32;
   __shared__ Word ks[2][kTile * words<T, DP>()];
   __shared__ Word vs[2][kTile * words<T, DP>()];
@@ -65,9 +65,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   extern __shared__ float table[];  // NB values, then kWaves x NB sums
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x);
-  const int bh = wg / nq, b = bh / p.Hq, h = bh % p.Hq;
-  const int block = nq - 1 - wg % nq, i0 = block * kBlock;
+  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
+  const int bh = unit / nq, b = bh / p.Hq, h = bh % p.Hq;
+  const int block = nq - 1 - unit % nq, i0 = block * kBlock;
   const int kh = h / (p.Hq / p.Hk);
   const int start = first_position(p, b), length = key_length(p, b);
   const int local = wave * kLanesRows + (lane & 31), i = i0 + local;
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   }
   const float lse = ref == -kInf ? kInf : fmaf(ref, c, __log2f(sum));
   const float inv = 1.f / sum;
-  if (live && half == 0) {
+  if (live && half == 0 && part == 0) {
     lses[stat] = lse;
     deltas[stat] = -delta;
   }
@@ -121,21 +121,23 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   }
   Feed<T, DP, Wide> kt(p.ks[1], p.D, tid), vt(p.vs[1], p.D, tid);
   int bucket = 0;
-  const int tiles = (keys + kTile - 1) / kTile;
-  if (tiles > 0) {
-    kt.start(k, p.ks[1], keys, ks[0], p.D, tid);
-    vt.start(v, p.vs[1], keys, vs[0], p.D, tid);
-    if (biased) bucket = bucket_of(p, base + tid);
+  const int all = (keys + kTile - 1) / kTile, each = (all + parts - 1) / parts;
+  const int first = part * each, tiles = min(all, first + each);  // of this part
+  if (first < tiles) {
+    const int64_t next = (int64_t)first * kTile;
+    kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[first & 1], p.D, tid);
+    vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[first & 1], p.D, tid);
+    if (biased) bucket = bucket_of(p, base + (int)next + tid);
   }
   if (!biased) clear(window, tid);
   loads_done();
   __syncthreads();
-  if (tiles > 0) {
-    kt.finish(ks[0], tid);
-    vt.finish(vs[0], tid);
+  if (first < tiles) {
+    kt.finish(ks[first & 1], tid);
+    vt.finish(vs[first & 1], tid);
     if (biased && tid < kWindow) {
-      window[0].put(tid, bias_of(table, p.NB, bucket));
-      window_bucket[0][tid] = bucket;
+      window[first & 1].put(tid, bias_of(table, p.NB, bucket));
+      window_bucket[first & 1][tid] = bucket;
     }
   }
   __syncthreads();
@@ -148,7 +150,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
 #pragma unroll
   for (int d = 0; d < Blocks; d++) acc[d] = (floatx16)(0.f);
 
-  for (int t = 0; t < tiles; t++) {
+  for (int t = first; t < tiles; t++) {
     const int j0 = t * kTile, buf = t & 1;
     if (t + 1 < tiles) {
       const int64_t next = j0 + kTile;
@@ -221,12 +223,12 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
     __syncthreads();
   }
   if (table_grad) {
-    if (tiles > 0 && half == 0) {  // differences 63 - lane of the last tile
+    if (first < tiles && half == 0) {  // differences 63 - lane of the last tile
       const int n = window_bucket[(tiles - 1) & 1][63 - lane + kBlock - wave * kLanesRows];
       if ((unsigned)n < (unsigned)p.NB) atomicAdd(&sums[n], diagonals);
     }
     __syncthreads();
-    float *to = partial + ((int64_t)bh * nq + block) * p.NB;
+    float *to = partial + (((int64_t)bh * nq + block) * parts + part) * p.NB;
     for (int n = tid; n < p.NB; n += 64 * kWaves) {
       float x = 0.f;
 #pragma unroll
@@ -234,7 +236,13 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
       to[n] = x;
     }
   }
-  if (live && gq) store_column<Wide, T, Blocks>(gq + row * p.D, acc, p.scale, p.D, half);
+  if (!live || !gq) return;
+  if (parts == 1) {
+    store_column<Wide, T, Blocks>(gq + row * p.D, acc, p.scale, p.D, half);
+  } else {
+    const int64_t size = (int64_t)p.B * p.Lq * p.Hq;
+    store_column<Wide, float, Blocks>(gq_parts + (part * size + row) * p.D, acc, p.scale, p.D, half);
+  }
 }
 
 // Keys' and values' gradients: a workgroup holds 128 keys of a key head, a wave 32 of them as
@@ -242,7 +250,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
 template <typename T, int DP, bool Wide>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void attention_key_grad_kernel(
     Params p, const T *gout, const float *stats, const float *lses, const float *deltas, T *gk,
-    T *gv, int nk) {
+    T *gv, float *gk_parts, float *gv_parts, int nk, int parts) {
   constexpr int Chunks = DP / 16, Blocks = DP / 32;
   __shared__ Word qs[2][kTile * words<T, DP>()];
   __shared__ Word gs[2][kTile * words<T, DP>()];
@@ -252,9 +260,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
   extern __shared__ float table[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x);
-  const int bh = wg / nk, b = bh / p.Hk, kh = bh % p.Hk;
-  const int j0 = (wg % nk) * kBlock;  // the longest columns of a causal map first
+  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
+  const int bh = unit / nk, b = bh / p.Hk, kh = bh % p.Hk;
+  const int j0 = (unit % nk) * kBlock;  // the longest columns of a causal map first
   const int group = p.Hq / p.Hk;
   const int start = first_position(p, b), length = key_length(p, b);
   const int local = wave * kLanesRows + (lane & 31), j = j0 + local;
@@ -262,7 +270,10 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
   // the first query that sees a key of this workgroup, and of this lane
   const int first = p.causal ? max(0, j0 - start) : 0;
   const int own_first = p.causal ? j - start : 0;
-  const int t0 = first / kTile, t1 = j0 < length ? (p.Lq + kTile - 1) / kTile : 0;
+  const int tf = first / kTile, per_head = j0 < length ? max(0, (p.Lq + kTile - 1) / kTile - tf) : 0;
+  // this part's of the tiles of all heads, one head after the other
+  const int each = (group * per_head + parts - 1) / parts, from = part * each;
+  const int upto = min(group * per_head, from + each);
   const int wave_safe = p.causal ? j0 + wave * kLanesRows + kLanesRows - 1 - start : 0;
 
   const T *k = (const T *)p.k + b * p.ks[0] + (int64_t)j * p.ks[1] + kh * p.ks[2];
@@ -286,7 +297,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
   float lse = 0.f, delta = 0.f, ref = 0.f, sum = 1.f;
   if (!biased) clear(window, tid);
   loads_done();
-  for (int g = 0; g < group && t0 < t1; g++) {
+  for (int g = 0; g < group; g++) {
+    const int t0 = tf + max(0, from - g * per_head), t1 = tf + min(per_head, upto - g * per_head);
+    if (t0 >= t1) continue;
     const int h = kh * group + g;
     const T *q = (const T *)p.q + b * p.qs[0] + h * p.qs[2];
     const T *go = gout + ((int64_t)b * p.Lq * p.Hq + h) * p.D;
@@ -381,8 +394,25 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
 #pragma unroll
     for (int d = 0; d < Blocks; d++) dk[d] = dv[d] = (floatx16)(0.f);
   }
-  if (gk) store_column<Wide, T, Blocks>(gk + row * p.D, dk, p.scale, p.D, half);
-  if (gv) store_column<Wide, T, Blocks>(gv + row * p.D, dv, 1.f, p.D, half);
+  if (parts == 1) {
+    if (gk) store_column<Wide, T, Blocks>(gk + row * p.D, dk, p.scale, p.D, half);
+    if (gv) store_column<Wide, T, Blocks>(gv + row * p.D, dv, 1.f, p.D, half);
+  } else {
+    const int64_t at = ((int64_t)part * p.B * p.Lk * p.Hk + row) * p.D;
+    if (gk) store_column<Wide, float, Blocks>(gk_parts + at, dk, p.scale, p.D, half);
+    if (gv) store_column<Wide, float, Blocks>(gv_parts + at, dv, 1.f, p.D, half);
+  }
+}
+
+// The sum of a gradient's parts, in order.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_sum_parts_kernel(const float *parts, T *to,
+                                                                  int64_t size, int count) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= size) return;
+  float x = parts[i];
+  for (int n = 1; n < count; n++) x += parts[n * size + i];
+  to[i] = (T)x;
 }
 
 // Sums per bucket of a head, in a fixed order.  Of `rows` sums of a head ([B][Hq][nq] with rows =
@@ -410,43 +440,72 @@ __global__ __launch_bounds__(64 * kWaves) void attention_table_grad_kernel(const
 
 constexpr int kSlices = 64;  // of the sums per bucket, where there are many
 
-static int64_t query_blocks(const Params &p) { return (p.Lq + kBlock - 1) / kBlock; }
+// How the work is split (`parts_of`): the query gradients' over the keys, the key gradients' over
+// the queries and the heads that share them.
+struct Plan {
+  int64_t nq, nk, q_units, k_units;
+  int q_parts, k_parts;
+  size_t rows_at, partial_at, slices_at, q_at, k_at, v_at, bytes;  // in the workspace
+};
 
-static size_t backward_bytes(const Params &p) {
-  const size_t rows = (size_t)p.B * p.Hq * p.Lq;
-  return 2 * align256(rows * sizeof(float)) +
-         align256((size_t)p.B * p.Hq * query_blocks(p) * p.NB * sizeof(float)) +
-         align256((size_t)kSlices * p.Hq * p.NB * sizeof(float));
+static Plan plan_of(const Params &p) {
+  Plan n = {};
+  n.nq = (p.Lq + kBlock - 1) / kBlock, n.nk = (p.Lk + kBlock - 1) / kBlock;
+  n.q_units = (int64_t)p.B * p.Hq * n.nq, n.k_units = (int64_t)p.B * p.Hk * n.nk;
+  const int64_t q_tiles = (p.Lq + kTile - 1) / kTile, k_tiles = (p.Lk + kTile - 1) / kTile;
+  n.q_parts = n.q_units ? parts_of(n.q_units, k_tiles) : 1;
+  n.k_parts = n.k_units ? parts_of(n.k_units, q_tiles * (p.Hq / p.Hk)) : 1;
+  const size_t rows = (size_t)p.B * p.Hq * p.Lq, keys = (size_t)p.B * p.Hk * p.Lk, f = sizeof(float);
+  n.rows_at = align256(rows * f);
+  n.partial_at = n.rows_at + align256(rows * f);
+  n.slices_at = n.partial_at + align256((size_t)n.q_units * n.q_parts * p.NB * f);
+  n.q_at = n.slices_at + align256((size_t)kSlices * p.Hq * p.NB * f);
+  n.k_at = n.q_at + (n.q_parts > 1 ? align256(n.q_parts * rows * p.D * f) : 0);
+  n.v_at = n.k_at + (n.k_parts > 1 ? align256(n.k_parts * keys * p.D * f) : 0);
+  n.bytes = n.v_at + (n.k_parts > 1 ? align256(n.k_parts * keys * p.D * f) : 0);
+  return n;
 }
 
 template <typename T>
-static int launch_backward(const Params &p, const void *gout, const void *out, const float *stats,
-                           void *gq, void *gk, void *gv, void *gtable, char *ws,
+static int sum_parts(const float *parts, void *to, int64_t size, int count, hipStream_t stream) {
+  hipLaunchKernelGGL((attention_sum_parts_kernel<T>), dim3((unsigned)((size + 255) / 256)), dim3(256),
+                     0, stream, parts, (T *)to, size, count);
+  MCX_HIP_CHECK_LAUNCH();
+  return MCX_OK;
+}
+
+template <typename T>
+static int launch_backward(const Params &p, const Plan &n, const void *gout, const void *out,
+                           const float *stats, void *gq, void *gk, void *gv, void *gtable, char *ws,
                            hipStream_t stream) {
-  const size_t rows = (size_t)p.B * p.Hq * p.Lq;
-  float *lses = (float *)ws, *deltas = (float *)(ws + align256(rows * sizeof(float)));
-  float *partial = (float *)(ws + 2 * align256(rows * sizeof(float)));
-  const int nq = (int)query_blocks(p), nk = (p.Lk + kBlock - 1) / kBlock;
+  float *lses = (float *)ws, *deltas = (float *)(ws + n.rows_at);
+  float *partial = (float *)(ws + n.partial_at), *slices = (float *)(ws + n.slices_at);
+  float *q_parts = (float *)(ws + n.q_at);
+  float *k_parts = (float *)(ws + n.k_at), *v_parts = (float *)(ws + n.v_at);
   const dim3 threads(64 * kWaves);
-  if (rows) {
-    const dim3 grid((unsigned)((int64_t)p.B * p.Hq * nq));
+  if (n.q_units) {
+    const int parts = gq || gtable ? n.q_parts : 1;
+    const dim3 grid((unsigned)(n.q_units * parts));
     const size_t lds = (gtable ? 1 + kWaves : 1) * p.NB * sizeof(float);
 #define MCX_GRAD(DP, W)                                                                           \
   hipLaunchKernelGGL((attention_query_grad_kernel<T, DP, W>), grid, threads, lds, stream, p,       \
-                     (const T *)out, (const T *)gout, stats, lses, deltas, (T *)gq,               \
-                     gtable ? partial : nullptr, nq)
+                     (const T *)out, (const T *)gout, stats, lses, deltas, (T *)gq, q_parts,      \
+                     gtable ? partial : nullptr, (int)n.nq, parts)
     MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out) && aligned16(gout) && aligned16(gq), MCX_GRAD);
 #undef MCX_GRAD
     MCX_HIP_CHECK_LAUNCH();
+    if (gq && parts > 1) {
+      const int rc = sum_parts<T>(q_parts, gq, (int64_t)p.B * p.Lq * p.Hq * p.D, parts, stream);
+      if (rc != MCX_OK) return rc;
+    }
   }
   if (gtable) {
-    const int64_t count = (int64_t)p.B * nq;
-    const int wide = (p.NB + 63) / 64;
+    const int64_t count = (int64_t)p.B * n.nq * n.q_parts;
+    const int nq = std::max(1, (int)n.nq * n.q_parts), wide = (p.NB + 63) / 64;
     if (count <= 2 * kSlices) {
       hipLaunchKernelGGL((attention_table_grad_kernel<T>), dim3(wide, p.Hq), threads, 0, stream,
                          partial, (T *)gtable, count, p.Hq, nq, p.NB);
     } else {
-      float *slices = (float *)((char *)partial + align256((size_t)p.B * p.Hq * nq * p.NB * sizeof(float)));
       hipLaunchKernelGGL((attention_table_grad_kernel<float>), dim3(wide, p.Hq, kSlices), threads, 0,
                          stream, partial, slices, count, p.Hq, nq, p.NB);
       hipLaunchKernelGGL((attention_table_grad_kernel<T>), dim3(wide, p.Hq), threads, 0, stream,
@@ -454,15 +513,22 @@ static int launch_backward(const Params &p, const void *gout, const void *out, c
     }
     MCX_HIP_CHECK_LAUNCH();
   }
-  if ((gk || gv) && p.B && p.Lk) {
-    const dim3 grid((unsigned)((int64_t)p.B * p.Hk * nk));
+  if ((gk || gv) && n.k_units) {
+    const dim3 grid((unsigned)(n.k_units * n.k_parts));
     const size_t lds = p.NB * sizeof(float);
 #define MCX_GRAD(DP, W)                                                                      \
   hipLaunchKernelGGL((attention_key_grad_kernel<T, DP, W>), grid, threads, lds, stream, p,    \
-                     (const T *)gout, stats, lses, deltas, (T *)gk, (T *)gv, nk)
+                     (const T *)gout, stats, lses, deltas, (T *)gk, (T *)gv, k_parts, v_parts, \
+                     (int)n.nk, n.k_parts)
     MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(gout) && aligned16(gk) && aligned16(gv), MCX_GRAD);
 #undef MCX_GRAD
     MCX_HIP_CHECK_LAUNCH();
+    if (n.k_parts > 1) {
+      const int64_t size = (int64_t)p.B * p.Lk * p.Hk * p.D;
+      int rc = gk ? sum_parts<T>(k_parts, gk, size, n.k_parts, stream) : MCX_OK;
+      if (rc == MCX_OK && gv) rc = sum_parts<T>(v_parts, gv, size, n.k_parts, stream);
+      if (rc != MCX_OK) return rc;
+    }
   }
   return MCX_OK;
 }
@@ -480,7 +546,7 @@ size_t mcx_attention_backward_workspace(const mcx_attention_desc *desc, int dtyp
   if (make_params(p, &any, &any, &any, biased ? &any : nullptr, biased ? &any : nullptr, nullptr,
                   nullptr, desc, dtype) != MCX_OK)
     return 0;
-  return backward_bytes(p);
+  return plan_of(p).bytes;
 }
 
 int mcx_attention_backward(const void *gout, const void *q, const void *k, const void *v,
@@ -496,15 +562,13 @@ int mcx_attention_backward(const void *gout, const void *q, const void *k, const
   if (gtable && !table) return MCX_E_NULL;
   if (!gq && !gk && !gv && !gtable) return MCX_OK;
   if (p.B && p.Lq && (!gout || !out || !stats)) return MCX_E_NULL;
-  if ((int64_t)p.B * p.Hq * query_blocks(p) > 0x7fffffffLL ||
-      (int64_t)p.B * p.Hk * ((p.Lk + kBlock - 1) / kBlock) > 0x7fffffffLL)
-    return MCX_E_SHAPE;
-  const size_t need = backward_bytes(p);
-  if (need && (!workspace || workspace_bytes < need)) return MCX_E_WORKSPACE;
+  const Plan n = plan_of(p);
+  if (n.q_units > 0x7fffffffLL || n.k_units > 0x7fffffffLL) return MCX_E_SHAPE;
+  if (n.bytes && (!workspace || workspace_bytes < n.bytes)) return MCX_E_WORKSPACE;
   return dtype == MCX_BF16
-             ? launch_backward<__bf16>(p, gout, out, stats, gq, gk, gv, gtable, (char *)workspace,
+             ? launch_backward<__bf16>(p, n, gout, out, stats, gq, gk, gv, gtable, (char *)workspace,
                                        (hipStream_t)stream)
-             : launch_backward<float>(p, gout, out, stats, gq, gk, gv, gtable, (char *)workspace,
+             : launch_backward<float>(p, n, gout, out, stats, gq, gk, gv, gtable, (char *)workspace,
                                       (hipStream_t)stream);
 }
 

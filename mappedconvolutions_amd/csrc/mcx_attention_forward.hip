@@ -14,7 +14,7 @@ namespace attention {
 // sums stay far inside fp32, and the accumulated output is seldom rescaled.
 template <typename T, int DP, bool Wide>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void attention_forward_kernel(
-    Params p, T *out, float *stats, int nq) {
+    Params p, T *out, float *stats, float *outs, float *sums, int nq, int parts) {
   constexpr int Chunks = DP / 16, Blocks = DP / 32;
   __shared__ Word ks[2][kTile * words<T, DP>()];
   __shared__ Word vs[2][kTile * words<T, DP>()];
@@ -22,10 +22,10 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   extern __shared__ float table[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x);
-  const int bh = wg / nq, b = bh / p.Hq, h = bh % p.Hq;
+  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
+  const int bh = unit / nq, b = bh / p.Hq, h = bh % p.Hq;
   // the longest rows of a causal map first
-  const int i0 = (nq - 1 - wg % nq) * kBlock;
+  const int i0 = (nq - 1 - unit % nq) * kBlock;
   const int kh = h / (p.Hq / p.Hk);
   const int start = first_position(p, b), length = key_length(p, b);
   const int local = wave * kLanesRows + (lane & 31), i = i0 + local;
@@ -50,19 +50,21 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
   Feed<T, DP, Wide> kt(p.ks[1], p.D, tid), vt(p.vs[1], p.D, tid);
   int bucket = 0;
-  const int tiles = (keys + kTile - 1) / kTile;
-  if (tiles > 0) {
-    kt.start(k, p.ks[1], keys, ks[0], p.D, tid);
-    vt.start(v, p.vs[1], keys, vs[0], p.D, tid);
-    if (biased) bucket = bucket_of(p, base + tid);
+  const int all = (keys + kTile - 1) / kTile, each = (all + parts - 1) / parts;
+  const int first = part * each, tiles = min(all, first + each);  // of this part
+  if (first < tiles) {
+    const int64_t next = (int64_t)first * kTile;
+    kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[first & 1], p.D, tid);
+    vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[first & 1], p.D, tid);
+    if (biased) bucket = bucket_of(p, base + (int)next + tid);
   }
   if (!biased) clear(window, tid);
   loads_done();
   __syncthreads();  // the table
-  if (tiles > 0) {
-    kt.finish(ks[0], tid);
-    vt.finish(vs[0], tid);
-    if (biased && tid < kWindow) window[0].put(tid, bias_of(table, p.NB, bucket));
+  if (first < tiles) {
+    kt.finish(ks[first & 1], tid);
+    vt.finish(vs[first & 1], tid);
+    if (biased && tid < kWindow) window[first & 1].put(tid, bias_of(table, p.NB, bucket));
   }
   __syncthreads();
 
@@ -73,7 +75,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   for (int d = 0; d < Blocks; d++) o[d] = (floatx16)(0.f);
   float ref = -kInf, sum = 0.f;
 
-  for (int t = 0; t < tiles; t++) {
+  for (int t = first; t < tiles; t++) {
     const int j0 = t * kTile, buf = t & 1;
     if (t + 1 < tiles) {
       const int64_t next = j0 + kTile;
@@ -145,25 +147,78 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   sum += other_half(sum);
   if (!live) return;
   const int64_t row = ((int64_t)b * p.Lq + i) * p.Hq + h;
-  store_column<Wide, T, Blocks>(out + row * p.D, o, sum == 0.f ? 0.f : 1.f / sum, p.D, half);
+  const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
+  if (parts > 1) {
+    const int64_t rows = (int64_t)p.B * p.Lq * p.Hq;
+    store_column<Wide, float, Blocks>(outs + (part * rows + row) * p.D, o, 1.f, p.D, half);
+    stats = sums + part * rows * 2;
+  } else {
+    store_column<Wide, T, Blocks>(out + row * p.D, o, sum == 0.f ? 0.f : 1.f / sum, p.D, half);
+  }
   if (stats && half == 0) {
-    float *s = stats + 2 * (((int64_t)b * p.Hq + h) * p.Lq + i);
-    s[0] = ref;
-    s[1] = sum;
+    stats[2 * stat] = ref;
+    stats[2 * stat + 1] = sum;
   }
 }
 
+// Joins the parts of the keys: a thread has one value of the output.
 template <typename T>
-static int launch_forward(const Params &p, void *out, float *stats, hipStream_t stream) {
-  const int nq = (p.Lq + kBlock - 1) / kBlock;
-  const dim3 grid((unsigned)((int64_t)p.B * p.Hq * nq)), threads(64 * kWaves);
+__global__ __launch_bounds__(256) void attention_join_values_kernel(Params p, const float *outs,
+                                                                    const float *sums, T *out,
+                                                                    float *stats, int parts) {
+  const int64_t rows = (int64_t)p.B * p.Lq * p.Hq, n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= rows * p.D) return;
+  const int64_t row = n / p.D, bi = row / p.Hq, b = bi / p.Lq;
+  const int64_t stat = (b * p.Hq + row % p.Hq) * p.Lq + bi % p.Lq;
+  const float c = p.scale * kLog2e;
+  float top = -kInf, all = 0.f, x = 0.f;
+  for (int s = 0; s < parts; s++) top = fmaxf(top, sums[(s * rows + stat) * 2]);
+  for (int s = 0; s < parts; s++) {
+    const float ref = sums[(s * rows + stat) * 2];
+    const float w = ref == -kInf ? 1.f : exp2_fast((ref - top) * c);  // (a NaN part stays one)
+    all = fmaf(w, sums[(s * rows + stat) * 2 + 1], all);
+    x = fmaf(w, outs[s * rows * p.D + n], x);
+  }
+  out[n] = (T)(all == 0.f ? 0.f : x / all);
+  if (stats && n % p.D == 0) {
+    stats[2 * stat] = top;
+    stats[2 * stat + 1] = all;
+  }
+}
+
+static int64_t query_units(const Params &p) {
+  return (int64_t)p.B * p.Hq * ((p.Lq + kBlock - 1) / kBlock);
+}
+static int forward_parts(const Params &p) {
+  return parts_of(query_units(p), (p.Lk + kTile - 1) / kTile);
+}
+static size_t forward_bytes(const Params &p) {
+  const int parts = forward_parts(p);
+  if (parts == 1) return 0;
+  const size_t rows = (size_t)p.B * p.Hq * p.Lq * parts;
+  return align256(rows * 2 * sizeof(float)) + align256(rows * p.D * sizeof(float));
+}
+
+template <typename T>
+static int launch_forward(const Params &p, void *out, float *stats, void *workspace,
+                          hipStream_t stream) {
+  const int nq = (p.Lq + kBlock - 1) / kBlock, parts = forward_parts(p);
+  const dim3 grid((unsigned)(query_units(p) * parts)), threads(64 * kWaves);
+  const int64_t rows = (int64_t)p.B * p.Hq * p.Lq;
+  float *sums = (float *)workspace;
+  float *outs = (float *)((char *)workspace + align256((size_t)rows * parts * 2 * sizeof(float)));
   const size_t lds = p.table ? p.NB * sizeof(float) : 0;
 #define MCX_FORWARD(DP, W)                                                                     \
   hipLaunchKernelGGL((attention_forward_kernel<T, DP, W>), grid, threads, lds, stream, p, (T *)out, \
-                     stats, nq)
+                     stats, outs, sums, nq, parts)
   MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out), MCX_FORWARD);
 #undef MCX_FORWARD
   MCX_HIP_CHECK_LAUNCH();
+  if (parts > 1) {
+    hipLaunchKernelGGL((attention_join_values_kernel<T>), dim3((unsigned)((rows * p.D + 255) / 256)),
+                       dim3(256), 0, stream, p, outs, sums, (T *)out, stats, parts);
+    MCX_HIP_CHECK_LAUNCH();
+  }
   return MCX_OK;
 }
 
@@ -171,6 +226,11 @@ static int launch_forward(const Params &p, void *out, float *stats, hipStream_t 
 static bool wide_rows(const void *p, const int64_t *strides, int64_t D, int64_t per16) {
   return aligned16(p) && D % per16 == 0 && strides[0] % per16 == 0 && strides[1] % per16 == 0 &&
          strides[2] % per16 == 0 && strides[1] >= 0 && strides[1] < (1 << 22);
+}
+
+int parts_of(int64_t units, int64_t tiles) {
+  if (units >= 256) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((384 + units - 1) / units, tiles / 4));
 }
 
 int make_params(Params &p, const void *q, const void *k, const void *v, const void *table,
@@ -217,7 +277,9 @@ size_t mcx_attention_forward_workspace(const mcx_attention_desc *desc, int dtype
   const int32_t *table = desc && desc->table_size > 0 ? &any : nullptr;
   if (make_params(p, &any, &any, &any, table, table, nullptr, nullptr, desc, dtype) != MCX_OK)
     return 0;
-  return p.B && p.Lq ? split_bytes(p, split_parts(p)) : 0;
+  if (p.B == 0 || p.Lq == 0) return 0;
+  const int parts = split_parts(p, dtype);
+  return parts ? split_bytes(p, parts) : forward_bytes(p);
 }
 
 int mcx_attention_forward(const void *q, const void *k, const void *v, const void *table,
@@ -231,15 +293,17 @@ int mcx_attention_forward(const void *q, const void *k, const void *v, const voi
   if (rc != MCX_OK) return rc;
   if (p.B == 0 || p.Lq == 0) return MCX_OK;
   if (!out) return MCX_E_NULL;
-  const int parts = split_parts(p);
+  const int parts = split_parts(p, dtype);
   if (parts) {
     if (split_bytes(p, parts) && (!workspace || workspace_bytes < split_bytes(p, parts)))
       return MCX_E_WORKSPACE;
     return launch_split(p, parts, out, stats, workspace, dtype, (hipStream_t)stream);
   }
-  if ((int64_t)p.B * p.Hq * ((p.Lq + kBlock - 1) / kBlock) > 0x7fffffffLL) return MCX_E_SHAPE;
-  return dtype == MCX_BF16 ? launch_forward<__bf16>(p, out, stats, (hipStream_t)stream)
-                           : launch_forward<float>(p, out, stats, (hipStream_t)stream);
+  if (query_units(p) > 0x7fffffffLL) return MCX_E_SHAPE;
+  if (forward_bytes(p) && (!workspace || workspace_bytes < forward_bytes(p))) return MCX_E_WORKSPACE;
+  return dtype == MCX_BF16
+             ? launch_forward<__bf16>(p, out, stats, workspace, (hipStream_t)stream)
+             : launch_forward<float>(p, out, stats, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -28,8 +28,8 @@ struct Split {
 };
 
 template <typename T, int DP, bool Wide>
-__global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, Split sp, T *out,
-                                                                      float *stats) {
+__global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void attention_split_kernel(
+    Params p, Split sp, T *out, float *stats) {
   constexpr int Chunks = DP / 16, Blocks = DP / 32;
   constexpr int E = 16 / (int)sizeof(T), PerRow = words<T, DP>(), N = kStep * PerRow / 64;
   // a wave's values; at the end all waves' sums, four blocks of columns at a time
@@ -83,19 +83,21 @@ __global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, 
   const int origin = start + last_i, own = live ? last_i - i : 0;
   int bucket = 0;
   bool varied = false;  // whether the tile's pairs are of more than one bucket
-  auto fetch = [&](int tile) {
-    const int j0 = tile * kStep;
-    // (a key behind the last one is the last one: its pairs are taken out below)
-    const T *row = k + (int64_t)min(j0 + key_row, keys - 1) * p.ks[1];
+  // (a key behind the last one is the last one: its pairs are taken out below)
+  auto fetch_keys = [&](int tile) {
+    const T *row = k + (int64_t)min(tile * kStep + key_row, keys - 1) * p.ks[1];
 #pragma unroll
     for (int c = 0; c < Chunks; c++) kf[c] = global_frag<Wide>(row, c, half, p.D);
+  };
+  auto fetch_values = [&](int tile) {
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      const int id = lane + 64 * n, j = min(j0 + id / PerRow, keys - 1), d0 = (id % PerRow) * E;
+      const int id = lane + 64 * n, j = min(tile * kStep + id / PerRow, keys - 1);
+      const int d0 = (id % PerRow) * E;
       const T *vrow = v + (int64_t)j * p.vs[1];
       vr[n] = Wide ? *(const Word *)(vrow + (d0 < p.D ? d0 : 0)) : load16<false>(vrow, d0, p.D);
     }
-    if (biased) bucket = bucket_of(p, j0 - origin + lane);
+    if (biased) bucket = bucket_of(p, tile * kStep - origin + lane);
   };
   const float c = p.scale * kLog2e;
   Word *vs = tiles_lds + wave * kTileWords;
@@ -103,12 +105,12 @@ __global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, 
 #pragma unroll
   for (int d = 0; d < Blocks; d++) o[d] = (floatx16)(0.f);
   float ref = -kInf, sum = 0.f;
-  if (t < t_end) fetch(t);
+  if (t < t_end) {
+    fetch_keys(t);
+    fetch_values(t);
+  }
   for (; t < t_end; t += kWaves) {
     const int j0 = t * kStep;
-    Frag<T> now[Chunks];
-#pragma unroll
-    for (int n = 0; n < Chunks; n++) now[n] = kf[n];
     wave_order();
 #pragma unroll
     for (int n = 0; n < N; n++) {
@@ -131,9 +133,10 @@ __global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, 
         u = (floatx16)((unsigned)one < (unsigned)p.NB ? table[slot * p.NB + one] : 0.f);
       }
     }
-    if (t + kWaves < t_end) fetch(t + kWaves);
+    if (t + kWaves < t_end) fetch_values(t + kWaves);
 #pragma unroll
-    for (int n = 0; n < Chunks; n++) u = mma(now[n], qf[n], u);
+    for (int n = 0; n < Chunks; n++) u = mma(kf[n], qf[n], u);
+    if (t + kWaves < t_end) fetch_keys(t + kWaves);
     if (j0 + kStep > wave_limit) {
 #pragma unroll
       for (int n = 0; n < 16; n++)
@@ -230,39 +233,50 @@ __global__ __launch_bounds__(64 * kWaves) void attention_split_kernel(Params p, 
   }
 }
 
-// Joins the parts of a row: a workgroup has one row, its waves every fourth part.
+// Joins the parts of a row: a workgroup has one row, its waves every kJoinWaves-th part.  What it
+// costs is the time of its loads from the first to the last, so they are many at once.
+constexpr int kJoinWaves = 16;
 template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void attention_join_kernel(Params p, Split sp, T *out,
-                                                                     float *stats) {
-  __shared__ float weight[kMostParts];
-  __shared__ float merge[kWaves][kMaxD];
+__global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(Params p, Split sp, T *out,
+                                                                         float *stats) {
+  __shared__ float merge[kJoinWaves][kMaxD];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int group = p.Hq / p.Hk;
   const int bk = blockIdx.x / sp.rows, r = blockIdx.x % sp.rows, b = bk / p.Hk, kh = bk % p.Hk;
   const int unit = bk * sp.blocks + r / kRows, row = r % kRows;
   const float *sums = sp.sums + ((int64_t)unit * sp.parts * kRows + row) * 2;
+  const float *from = sp.outs + ((int64_t)unit * sp.parts * kRows + row) * p.D;
   const float c = p.scale * kLog2e;
-  // every wave finds the common reference and the sum by itself
-  float top = -kInf;
-  for (int n = lane; n < sp.parts; n += 64) top = fmaxf(top, sums[(int64_t)n * kRows * 2]);
+  // the wave's parts, eight at a time, are on their way while it finds the common reference
+  float ref[kMostParts / 64], part_sum[kMostParts / 64], top = -kInf, all = 0.f;
+#pragma unroll
+  for (int n = 0; n < kMostParts / 64; n++) {
+    const int s = lane + 64 * n;
+    ref[n] = s < sp.parts ? sums[(int64_t)s * kRows * 2] : -kInf;
+    part_sum[n] = s < sp.parts ? sums[(int64_t)s * kRows * 2 + 1] : 0.f;
+  }
+#pragma unroll
+  for (int n = 0; n < kMostParts / 64; n++) top = fmaxf(top, ref[n]);
   for (int m = 32; m; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
-  float all = 0.f;
-  for (int n = lane; n < sp.parts; n += 64) {
-    const float ref = sums[(int64_t)n * kRows * 2];
-    const float w = ref == -kInf ? 1.f : exp2_fast((ref - top) * c);  // (a NaN part stays one)
-    all += w * sums[(int64_t)n * kRows * 2 + 1];
-    if (wave == 0) weight[n] = w;
+#pragma unroll
+  for (int n = 0; n < kMostParts / 64; n++) {
+    ref[n] = ref[n] == -kInf ? 1.f : exp2_fast((ref[n] - top) * c);  // (a NaN part stays one)
+    all = fmaf(ref[n], part_sum[n], all);
   }
   for (int m = 32; m; m >>= 1) all += __shfl_xor(all, m);
-  __syncthreads();
-  const float *from = sp.outs + ((int64_t)unit * sp.parts * kRows + row) * p.D;
   float x = 0.f, y = 0.f;
-  for (int n = wave; n < sp.parts; n += kWaves) {
-    const float w = weight[n];
-    const float *f = from + (int64_t)n * kRows * p.D;
-    if (lane < p.D) x = fmaf(w, f[lane], x);
-    if (lane + 64 < p.D) y = fmaf(w, f[lane + 64], y);
-  }
+#pragma unroll
+  for (int n = 0; n < kMostParts / 64; n++)
+#pragma unroll
+    for (int q = 0; q < 64 / kJoinWaves; q++) {
+      const int s = 64 * n + q * kJoinWaves + wave;
+      if (s < sp.parts) {
+        const float w = __shfl(ref[n], q * kJoinWaves + wave);
+        const float *f = from + (int64_t)s * kRows * p.D;
+        if (lane < p.D) x = fmaf(w, f[lane], x);
+        if (lane + 64 < p.D) y = fmaf(w, f[lane + 64], y);
+      }
+    }
   merge[wave][lane] = x;
   merge[wave][lane + 64] = y;
   __syncthreads();
@@ -270,7 +284,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_join_kernel(Params p, S
   if (tid < p.D) {
     x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) x += merge[w][tid];
+    for (int w = 0; w < kJoinWaves; w++) x += merge[w][tid];
     out[(((int64_t)b * p.Lq + i) * p.Hq + h) * p.D + tid] = (T)(all == 0.f ? 0.f : x / all);
   }
   if (stats && tid == 0) {
@@ -280,15 +294,60 @@ __global__ __launch_bounds__(64 * kWaves) void attention_join_kernel(Params p, S
   }
 }
 
-// 0: the other kernel is the better one.
-int split_parts(const Params &p) {
+// The same for a few parts of many rows: a thread has one value of the output.
+constexpr int kFewParts = 16;
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join_few_kernel(Params p, Split sp, T *out,
+                                                                 float *stats, int64_t total) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;  // [bk][row][value]
+  if (n >= total) return;
+  const int64_t br = n / p.D;
+  const int d = (int)(n - br * p.D);
+  const int bk = (int)(br / sp.rows), r = (int)(br - (int64_t)bk * sp.rows);
+  const int group = p.Hq / p.Hk, b = bk / p.Hk, kh = bk % p.Hk;
+  const int64_t first = ((int64_t)bk * sp.blocks + r / kRows) * sp.parts * kRows + r % kRows;
+  const float c = p.scale * kLog2e;
+  float top = -kInf, all = 0.f, x = 0.f;
+  for (int s = 0; s < sp.parts; s++) top = fmaxf(top, sp.sums[(first + s * kRows) * 2]);
+  for (int s = 0; s < sp.parts; s++) {
+    const float ref = sp.sums[(first + s * kRows) * 2];
+    const float w = ref == -kInf ? 1.f : exp2_fast((ref - top) * c);  // (a NaN part stays one)
+    all = fmaf(w, sp.sums[(first + s * kRows) * 2 + 1], all);
+    x = fmaf(w, sp.outs[(first + s * kRows) * p.D + d], x);
+  }
+  const int64_t i = r / group, h = kh * group + r % group;
+  out[((b * (int64_t)p.Lq + i) * p.Hq + h) * p.D + d] = (T)(all == 0.f ? 0.f : x / all);
+  if (stats && d == 0) {
+    float *s = stats + 2 * (((int64_t)b * p.Hq + h) * p.Lq + i);
+    s[0] = top;
+    s[1] = all;
+  }
+}
+
+// 0: the other kernel is the better one.  Both work on blocks of 32 rows; this one shares a key's
+// loads among the heads of a group but not among blocks, and fills its blocks with a group's heads
+// where the other one leaves waves of a head's 128 without queries.  Its block of keys costs up to
+// three times the other's in bf16, where the other one reaches half the matrix rate, and 1.5 times
+// in fp32 (this, other, in us): 16 x 32 queries, 2000 keys, 32 heads sharing 8 of 64: bf16 31, 49,
+// fp32 96, 275; 16 x 64 queries of 32 heads of 128 sharing 8: bf16 88, 74, fp32 382, 566; 128 x 100
+// queries and keys, 8 heads of 64: bf16 54, 18, fp32 90, 50.
+int split_parts(const Params &p, int dtype) {
   const int64_t group = p.Hq / p.Hk, rows = p.Lq * group;
   const int64_t blocks = (rows + kRows - 1) / kRows, units = (int64_t)p.B * p.Hk * blocks;
-  const int64_t whole = (int64_t)p.B * p.Hq * ((p.Lq + kBlock - 1) / kBlock);
-  if (rows > 64 && !(whole <= 64 && p.Lk >= 1024)) return 0;
+  const int64_t here = p.Hk * blocks * ((p.Lk + kWaves * kStep - 1) / (kWaves * kStep)) * (kWaves * kStep);
+  const int64_t there = (int64_t)p.Hq * ((p.Lq + kBlock - 1) / kBlock) * kWaves *
+                        ((p.Lk + kTile - 1) / kTile) * kTile;
+  if ((dtype == MCX_BF16 ? 6 : 3) * here > 2 * there) return 0;
   if (units > (1 << 24)) return 0;
-  const int64_t most = std::max<int64_t>(1, (p.Lk + kWaves * kStep - 1) / (kWaves * kStep));
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + units - 1) / units, most, kMostParts}));
+  // One workgroup for every compute unit where there are fewer units of work: more parts cost more
+  // in their ends and in the join than they win (one bf16 token over 20000 keys of 8 heads of 128:
+  // 23.0, 25.8, 33.5 us with 256, 512, 1024 workgroups in all).  Where there are enough, parts of at
+  // least 2048 keys even out the last round (64 bf16 tokens over up to 8192 keys of 8 heads: 368,
+  // 338, 319 us with one, two, four parts).
+  const int64_t tiles = (p.Lk + kWaves * kStep - 1) / (kWaves * kStep);
+  const int64_t parts = units < 256 ? std::min<int64_t>((256 + units - 1) / units, tiles)
+                                    : std::min<int64_t>((2048 + units - 1) / units, p.Lk / 2048);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(parts, kMostParts));
 }
 
 static Split split_of(const Params &p, int parts) {
@@ -316,11 +375,15 @@ static int launch(const Params &p, Split sp, void *out, float *stats, hipStream_
   MCX_ATTENTION_DISPATCH(p.D, p.wide, MCX_SPLIT);
 #undef MCX_SPLIT
   MCX_HIP_CHECK_LAUNCH();
-  if (sp.parts > 1) {
-    hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)((int64_t)p.B * p.Hk * sp.rows)),
-                       threads, 0, stream, p, sp, (T *)out, stats);
-    MCX_HIP_CHECK_LAUNCH();
+  const int64_t rows = (int64_t)p.B * p.Hk * sp.rows, total = rows * p.D;
+  if (sp.parts > kFewParts) {
+    hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)rows), dim3(64 * kJoinWaves), 0,
+                       stream, p, sp, (T *)out, stats);
+  } else if (sp.parts > 1) {
+    hipLaunchKernelGGL((attention_join_few_kernel<T>), dim3((unsigned)((total + 255) / 256)),
+                       dim3(256), 0, stream, p, sp, (T *)out, stats, total);
   }
+  MCX_HIP_CHECK_LAUNCH();
   return MCX_OK;
 }
 
