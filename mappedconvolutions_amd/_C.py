@@ -7,6 +7,7 @@ include/nn/layers/*.h wrappers do, allocates the outputs with torch, and calls
 the C ABI of libmcx_hip.so on the current HIP stream.  Tensors must live on the
 GPU: there is no CPU implementation behind these names.
 """
+import array
 import contextlib
 
 import torch
@@ -872,14 +873,15 @@ def _attention_dtype(data, **same):
 
 
 def _heads(name, t, B=None, L=None, H=None, D=None):
-    """Shape of a [B, L, H, D] tensor whose last axis is dense."""
-    if t.dim() != 4:
-        raise RuntimeError("%s must have 4 dimensions [B, L, H, D], got %s" % (name, tuple(t.shape)))
-    for axis, (got, want) in enumerate(zip(t.shape, (B, L, H, D))):
-        if want is not None and got != want:
+    """Shape of a [B, L, H, D] tensor, after a check of the sizes that are given."""
+    shape = t.shape
+    if len(shape) != 4:
+        raise RuntimeError("%s must have 4 dimensions [B, L, H, D], got %s" % (name, tuple(shape)))
+    for axis, want in enumerate((B, L, H, D)):
+        if want is not None and shape[axis] != want:
             raise RuntimeError("%s has size %d in dimension %d, expected %d" %
-                               (name, got, axis, want))
-    return t.shape
+                               (name, shape[axis], axis, want))
+    return shape
 
 
 def _dense_last(t):
@@ -917,8 +919,11 @@ def _norm_args(query, key, query_weight, key_weight, cos, sin, positions, eps):
             sin.contiguous(), positions)
 
 
+_three = _lib._i64 * 3
+
+
 def _strides(t):
-    return (_lib._i64 * 3)(t.stride(0), t.stride(1), t.stride(2))
+    return _three(*t.stride()[:3])
 
 
 def qk_norm_rotate_forward(query, key, query_weight, key_weight, cos, sin, positions=None,
@@ -1089,40 +1094,47 @@ def relative_attention_backward(grad_output, query, key, value, output, stats, b
     return [gq, gk, gv, gt]
 
 
+_CLIP_DTYPES = {torch.float32: MCX_F32, torch.bfloat16: MCX_BF16}
+
+
 def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
     """The norm of all values of a list of tensors (float32 and bfloat16, contiguous, on one GPU),
     as a float32 scalar; the tensors, or where `out` gives as many of the same sizes and types
     those, hold min(1, max_norm / (norm + eps)) times the values then.  A norm that is no number
     makes them all none."""
-    import ctypes
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0 or not eps >= 0:
         raise RuntimeError("max_norm and eps must not be negative")
     tensors = list(tensors)
     if not tensors:
         raise RuntimeError("clip_grad_norm needs at least one tensor")
-    device, dtypes, n = tensors[0].device, [t.dtype for t in tensors], len(tensors)
-    to = tensors if out is None else list(out)
-    if [t.dtype for t in to] != dtypes or [t.shape for t in to] != [t.shape for t in tensors]:
-        raise RuntimeError("out must have the tensors' shapes and dtypes")
-    for t in tensors if out is None else tensors + to:
-        if t.device != device or not t.is_cuda:
-            raise RuntimeError("all tensors must be on one GPU")
-        if not t.is_contiguous():
-            raise RuntimeError("tensors must be contiguous")
-    codes = [_DTYPES.get(d, MCX_F64) for d in dtypes]
-    if MCX_F64 in codes:
-        raise RuntimeError("unsupported dtype %s (float32 or bfloat16)" % dtypes[codes.index(MCX_F64)])
-    pointers = ctypes.c_void_p * n
-    sizes = (_lib._i64 * n)(*[t.numel() for t in tensors])
-    inputs = pointers(*[t.data_ptr() for t in tensors])
-    outputs = inputs if out is None else pointers(*[t.data_ptr() for t in to])
+    # (hundreds of tensors: every look at them is one pass in C)
+    every, n = tensors if out is None else tensors + list(out), len(tensors)
+    if len(every) != (n if out is None else 2 * n):
+        raise RuntimeError("out must have as many tensors")
+    where = set(map(torch.Tensor.get_device, every))
+    if len(where) != 1 or not tensors[0].is_cuda:
+        raise RuntimeError("all tensors must be on one GPU")
+    if not all(map(torch.Tensor.is_contiguous, every)):
+        raise RuntimeError("tensors must be contiguous")
+    sizes = list(map(torch.Tensor.numel, every))
+    codes = [_CLIP_DTYPES.get(t.dtype, -1) for t in every]
+    if -1 in codes:
+        raise RuntimeError("unsupported dtype %s (float32 or bfloat16)" % every[codes.index(-1)].dtype)
+    if out is not None and (sizes[:n] != sizes[n:] or codes[:n] != codes[n:]):
+        raise RuntimeError("out must have the tensors' sizes and dtypes")
+    # (host arrays of the library's types; `inputs` and the others live until it has returned)
+    at = list(map(torch.Tensor.data_ptr, every))
+    inputs, outputs = array.array("Q", at[:n]), array.array("Q", at[-n:])
+    lengths, types = array.array("q", sizes[:n]), array.array("i", codes[:n])
+    hosts = [a.buffer_info()[0] for a in (inputs, outputs, lengths, types)]
+    device = tensors[0].device
     lib = _lib.load()
     norm = torch.empty((), dtype=torch.float32, device=device)
-    nbytes = lib.mcx_clip_grad_norm_workspace(sizes, n)
+    nbytes = lib.mcx_clip_grad_norm_workspace(hosts[2], n)
     ws = _workspace(nbytes, device)
     with _device(norm):
-        rc = lib.mcx_clip_grad_norm(inputs, outputs, sizes, (ctypes.c_int32 * n)(*codes), n,
-                                    max_norm, eps, _ptr(norm), _ptr(ws), nbytes, _stream(norm))
+        rc = lib.mcx_clip_grad_norm(*hosts, n, max_norm, eps, _ptr(norm), _ptr(ws), nbytes,
+                                    _stream(norm))
     _lib.check(rc, "clip_grad_norm")
     return norm

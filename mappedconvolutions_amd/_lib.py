@@ -14,6 +14,7 @@ MCX_F32, MCX_F64, MCX_BF16 = 0, 1, 2
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i = ctypes.c_int
+_i32 = ctypes.c_int32
 _sz = ctypes.c_size_t
 
 

@@ -5,6 +5,9 @@
 // tensors: their table travels in the launch's arguments (no copy to the device), a workgroup
 // takes chunks of them in turn, and the second launch's workgroups each add up the first's sums,
 // in the same order, instead of waiting for a third.
+//   300 tensors of 0.6 billion bf16 values: 82 us for the squares of 0.4 GB (4.9 TB/s), 661 us in
+// all for 3.6 GB (5.4 TB/s; a large copy reaches 4.9): 708 us with the products in the squares'
+// order and 696 us with results written through the cache.  30 small tensors take 10 us.
 #include <algorithm>
 #include <cmath>
 
@@ -18,6 +21,7 @@ constexpr int kMost = 128;         // tensors of a launch: 3.6 kB of arguments
 constexpr int kBlocks = 1024;      // workgroups of a launch
 constexpr int64_t kLeast = 2048;   // values of a chunk
 constexpr int64_t kLargest = 32768;
+constexpr int64_t kCacheBytes = 256 << 20;  // of the last-level cache
 
 struct List {
   const void *in[kMost];
@@ -62,6 +66,7 @@ template <typename T> struct Chunk {
     return s + (t[0] + t[1]) + (t[2] + t[3]);
   }
 
+  template <bool Passing>
   static __device__ inline void scale(const T *x, T *y, int64_t lo, int64_t hi, float factor) {
     const int tid = threadIdx.x;
     const int64_t skew = (int64_t)(((uintptr_t)(x + lo) & 15) / sizeof(T));
@@ -79,7 +84,8 @@ template <typename T> struct Chunk {
       for (int n = 0; n < 4; n++) {
 #pragma unroll
         for (int e = 0; e < E; e++) v[n][e] = (T)(value(v[n][e]) * factor);
-        *(Vec *)(y + i + n * kThreads * E) = v[n];
+        if (Passing) __builtin_nontemporal_store(v[n], (Vec *)(y + i + n * kThreads * E));
+        else *(Vec *)(y + i + n * kThreads * E) = v[n];
       }
     }
     for (; i < z; i += kThreads * E) {
@@ -128,6 +134,8 @@ __global__ __launch_bounds__(kThreads) void grad_squares_kernel(List l, double *
   if (threadIdx.x == 0) sums[blockIdx.x] = s;
 }
 
+// Passing: the results are more than the cache holds, and are written past it.
+template <bool Passing>
 __global__ __launch_bounds__(kThreads) void grad_scale_kernel(List l, const double *sums, int n,
                                                               double max_norm, double eps,
                                                               float *norm) {
@@ -143,9 +151,9 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(List l, const doub
     if (factor == 1.f && l.in[t] == l.out[t]) continue;  // in place, nothing changes
     const int64_t lo = (int64_t)(c - l.first[t]) * l.chunk, hi = min(l.size[t], lo + l.chunk);
     if ((l.bf16[t >> 5] >> (t & 31)) & 1)
-      Chunk<__bf16>::scale((const __bf16 *)l.in[t], (__bf16 *)l.out[t], lo, hi, factor);
+      Chunk<__bf16>::template scale<Passing>((const __bf16 *)l.in[t], (__bf16 *)l.out[t], lo, hi, factor);
     else
-      Chunk<float>::scale((const float *)l.in[t], (float *)l.out[t], lo, hi, factor);
+      Chunk<float>::template scale<Passing>((const float *)l.in[t], (float *)l.out[t], lo, hi, factor);
   }
 }
 
@@ -172,12 +180,13 @@ int mcx_clip_grad_norm(const void *const *in, void *const *out, const int64_t *s
   if (!norm || (count && (!in || !sizes || !dtypes))) return MCX_E_NULL;
   if (!workspace || workspace_bytes < mcx_clip_grad_norm_workspace(sizes, count))
     return MCX_E_WORKSPACE;
-  int64_t total = 0;
+  int64_t total = 0, bytes = 0;
   for (int64_t t = 0; t < count; t++) {
     if (dtypes[t] != MCX_F32 && dtypes[t] != MCX_BF16) return MCX_E_DTYPE;
     if (sizes[t] < 0 || sizes[t] > (1LL << 40)) return MCX_E_SHAPE;
     if (sizes[t] && (!in[t] || (out && !out[t]))) return MCX_E_NULL;
     total += sizes[t];
+    bytes += sizes[t] * (dtypes[t] == MCX_BF16 ? 2 : 4);
   }
   const int64_t chunk = chunk_of(total);
   if (total / chunk + count > 0x7fffffffLL) return MCX_E_SHAPE;
@@ -192,11 +201,13 @@ int mcx_clip_grad_norm(const void *const *in, void *const *out, const int64_t *s
       l.count = 0, l.chunk = (int)chunk, l.first[0] = 0;
       for (int w = 0; w < kMost / 32; w++) l.bf16[w] = 0;
       for (; t0 < count && l.count < kMost; t0++) {
-        if (!sizes[t0]) continue;
+        // the products begin with what the squares read last, which may still be cached
+        const int64_t t = pass == 0 ? t0 : count - 1 - t0;
+        if (!sizes[t]) continue;
         const int n = l.count++;
-        l.in[n] = in[t0], l.out[n] = out ? out[t0] : nullptr, l.size[n] = sizes[t0];
-        l.first[n + 1] = l.first[n] + (int)((sizes[t0] + chunk - 1) / chunk);
-        if (dtypes[t0] == MCX_BF16) l.bf16[n >> 5] |= 1u << (n & 31);
+        l.in[n] = in[t], l.out[n] = out ? out[t] : nullptr, l.size[n] = sizes[t];
+        l.first[n + 1] = l.first[n] + (int)((sizes[t] + chunk - 1) / chunk);
+        if (dtypes[t] == MCX_BF16) l.bf16[n >> 5] |= 1u << (n & 31);
       }
       const int chunks = l.first[l.count];
       if (pass == 0) {
@@ -209,8 +220,9 @@ int mcx_clip_grad_norm(const void *const *in, void *const *out, const int64_t *s
         if (!l.count) l.first[0] = 0;
         const int blocks = l.count ? std::min(chunks, 2 * kBlocks) : 1;
         if (l.count || !norm_done)
-          hipLaunchKernelGGL(grad_scale_kernel, dim3(blocks), dim3(kThreads), 0, s, l, sums, used,
-                             max_norm, eps, norm_done ? nullptr : norm);
+          hipLaunchKernelGGL(bytes > kCacheBytes ? grad_scale_kernel<true> : grad_scale_kernel<false>,
+                             dim3(blocks), dim3(kThreads), 0, s, l, sums, used, max_norm, eps,
+                             norm_done ? nullptr : norm);
         norm_done = true;
         if (!out) break;
       }
