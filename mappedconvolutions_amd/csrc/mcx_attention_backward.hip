@@ -1,6 +1,6 @@
 // Gradients of attention with a bias by relative-position buckets.
 //
-//   p_ij = exp(scale u_ij - lse_i),  dp_ij = do_i . v_j,  delta_i = do_i . o_i
+//   p_ij = exp(scale (u_ij - ref_i)) / sum_i,  dp_ij = do_i . v_j,  delta_i = do_i . o_i
 //   ds_ij = p_ij (dp_ij - delta_i)
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
 //   dT[h, n] = sum of ds over the pairs of bucket n
@@ -15,6 +15,12 @@
 namespace mcx {
 namespace attention {
 
+// What the two kernels share of every row: [B, Hq, Lq].  delta is negative; ref is +inf for a row
+// that nothing is left of.
+struct Rows {
+  float *ref, *log_sum, *delta;
+};
+
 // c + a b^T of a column a (rows) and a row b (columns), the upper half-wave's a being 0: takes
 // delta from dp in the matrix pipe, which has the time, and after dp's last addition: equal sums
 // of equal terms then leave nothing.
@@ -22,12 +28,40 @@ __device__ inline floatx16 add_outer(float a, float b, floatx16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
 }
 
-// One step along the diagonals: ds plus the running sum of the lane below (lane 63's for lane 0),
-// none for the lane where `kept` is 0.  The wait is what a lane exchange needs after a write.
-__device__ inline float next_diagonals(float ds, float sum, float kept) {
-  asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 wave_ror:1 row_mask:0xf bank_mask:0xf"
-      : "+v"(ds) : "v"(sum), "v"(kept));
-  return ds;
+// A step along two chains of diagonals: ds plus the running sum of the lane below (lane 63's for lane
+// 0), none for the lane where `kept` is 0.  The wait is what a lane exchange needs after a write of
+// its source: two chains share it.
+__device__ inline void next_diagonals(float &ds0, float sum0, float &ds1, float sum1, float kept) {
+  asm("s_nop 1\n\t"
+      "v_fmac_f32_dpp %0, %2, %4 wave_ror:1 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %1, %3, %4 wave_ror:1 row_mask:0xf bank_mask:0xf"
+      : "+&v"(ds0), "+v"(ds1) : "v"(sum0), "v"(sum1), "v"(kept));
+}
+
+// The sum of x over the lanes up to this one in its run of lanes with the same n, and whether the run
+// ends here.  (Neighbouring differences mostly share a bucket, and 64 lanes' additions to one
+// place in LDS take four clocks each.)
+template <int Control, int Rows> __device__ inline float from_lane(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), Control, Rows, 0xf, false));
+}
+__device__ inline float run_sum(float x, int n, int lane, bool &last) {
+  const int below = __builtin_amdgcn_update_dpp(0, n, 0x138, 0xf, 0xf, false);  // lane - 1
+  const uint64_t starts = __builtin_amdgcn_ballot_w64(lane == 0 || below != n);
+  last = lane == 63 || (starts >> (lane + 1)) & 1;
+  const int before = lane - (63 - __builtin_clzll(starts & (~0ull >> (63 - lane))));  // in the run
+  float y = from_lane<0x111, 0xf>(x);  // 1, 2, 4, 8 lanes down, within 16
+  x += before >= 1 ? y : 0.f;
+  y = from_lane<0x112, 0xf>(x);
+  x += before >= 2 ? y : 0.f;
+  y = from_lane<0x114, 0xf>(x);
+  x += before >= 4 ? y : 0.f;
+  y = from_lane<0x118, 0xf>(x);
+  x += before >= 8 ? y : 0.f;
+  y = from_lane<0x142, 0xa>(x);  // lane 15 to lanes 16 .. 31, lane 47 to 48 .. 63
+  x += before > (lane & 15) ? y : 0.f;
+  y = from_lane<0x143, 0xc>(x);  // lane 31 to lanes 32 .. 63
+  x += before > lane - 32 ? y : 0.f;
+  return x;
 }
 // The upper half-wave's values in the lower, zeros in the upper.
 __device__ inline float upper_to_lower(float x) {
@@ -35,13 +69,40 @@ __device__ inline float upper_to_lower(float x) {
   return __uint_as_float(r[1]);
 }
 
-// A probability from u: through lse = scale log2(e) ref + log2(sum), +inf for a row that nothing
-// is left of; or, where that is too large to hold its second term, from ref and 1 / sum.
-template <bool Huge>
-__device__ inline float probability(float u, float c, float lse, float ref, float inv) {
-  if (Huge) return ref == -kInf ? 0.f : exp2_fast((u - ref) * c) * inv;
-  return exp2_fast(fmaf(u, c, -lse));
+// x, which the compiler takes for new: what is computed from it is computed here, and not kept in
+// registers from before the loop.
+__device__ inline int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
+
+// A step of a pipeline ends here: the compiler's scheduler keeps its instructions together.
+__device__ inline void step_end() { __builtin_amdgcn_sched_barrier(0); }
+
+// u += rows of `a` times x, dp += rows of `b` times y, for one 32 x 32 block of a tile's pairs.  The
+// operands are loaded `Ahead` chunks before their products, and `beside(n)`, n = 0 .. Chunks - 1, is
+// vector work that the matrix pipe's time is long enough for.
+template <typename T, int DP, int Ahead, typename F>
+__device__ inline void scores(const Word *a, const Word *b, int blk, int lane, const Frag<T> *x,
+                              const Frag<T> *y, floatx16 &u, floatx16 &dp, F beside) {
+  constexpr int Chunks = DP / 16;
+  const int row = row_of(lane & 31, blk), half = lane >> 5;
+  Frag<T> fa[Chunks], fb[Chunks];
+#pragma unroll
+  for (int ch = -Ahead; ch < Chunks; ch++) {
+    if (ch + Ahead < Chunks) {
+      fa[ch + Ahead] = row_frag<T, DP>(a, row, ch + Ahead, half);
+      fb[ch + Ahead] = row_frag<T, DP>(b, row, ch + Ahead, half);
+    }
+    if (ch < 0) continue;
+    u = mma(fa[ch], x[ch], u);
+    dp = mma(fb[ch], y[ch], dp);
+    beside(ch);
+    step_end();
+  }
+}
+// The part [n of steps) of the 16 values of a block.
+__device__ inline constexpr int part_start(int n, int steps) { return 16 * n / steps; }
 
 // Queries' gradients, the sums per bucket, and the rows' statistics for the other kernel.  The
 // same walk as the forward product's: a wave holds 32 queries, their o gradient beside them.
@@ -49,22 +110,26 @@ __device__ inline float probability(float u, float c, float lse, float ref, floa
 // and the keys 32 (lane >> 5) + n, n = 0 .. 31: from n to n + 1 a diagonal moves one lane up, so
 // one instruction a value adds it to its neighbour's running sum.  What reaches lane 31 is finished
 // and leaves (lane 32 starts anew); what leaves lane 63 is the part of a diagonal that lane 0 goes
-// on with.  The 64 diagonals that a tile finishes are added to the wave's sums per bucket.
+// on with.  Two chains, over n < 16 and n >= 16, run side by side, and the first one's ends are added
+// where their 16 further steps would have taken them: lane l to lane l + 16, or, past lane 31, out at
+// step 47 - l.  The 64 diagonals that a tile finishes are added to the wave's sums per bucket.
 //   (Adding each ds to a sum in LDS costs about 3 clocks a value: 6.9 ms for 512 x 8 heads of 512 rows
 // of 64 bf16 values, which take 1.1 ms this way.)
-template <typename T, int DP, bool Wide>
+template <typename T, int DP, bool Wide, bool Table>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void attention_query_grad_kernel(
-    Params p, const T *out, const T *gout, const float *stats, float *lses, float *deltas, T *gq,
-    float *gq_parts, float *partial, int nq, int parts) {
+    Params p, const T *out, const T *gout, const float *stats, Rows rows, T *gq, float *gq_parts,
+    float *partial, int nq, int parts) {
   constexpr int Chunks = DP / 16, Blocks = DP / 32;
+  constexpr int Ahead = DP * (int)sizeof(T) > 128 ? 1 : 2;  // (registers: two waves a SIMD)
   __shared__ Word ks[2][kTile * words<T, DP>()];
   __shared__ Word vs[2][kTile * words<T, DP>()];
   __shared__ __attribute__((aligned(16))) Window window[2];
   __shared__ int window_bucket[2][kWindow];
   __shared__ __attribute__((aligned(16))) float finished[kWaves][64];
+  __shared__ float chain_end[kWaves][64];
   extern __shared__ float table[];  // NB values, then kWaves x NB sums
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
   const int bh = unit / nq, b = bh / p.Hq, h = bh % p.Hq;
   const int block = nq - 1 - unit % nq, i0 = block * kBlock;
@@ -81,7 +146,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   const T *k = (const T *)p.k + b * p.ks[0] + kh * p.ks[2];
   const T *v = (const T *)p.v + b * p.vs[0] + kh * p.vs[2];
   const int64_t row = ((int64_t)b * p.Lq + i) * p.Hq + h;
-  const bool biased = p.table != nullptr, table_grad = partial != nullptr;
+  const bool biased = p.table != nullptr;
   float *sums = table + p.NB + wave * p.NB;
 
   Frag<T> qf[Chunks], gf[Chunks];
@@ -100,24 +165,25 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
     if ((lane & 31) == 8 * (n >> 2) + 4 * half + (n & 3)) delta = products[n];
   delta += other_half(delta);
   const float c = p.scale * kLog2e;
-  float ref = -kInf, sum = 0.f;
+  // (a row that nothing is left of: every difference from ref is -inf)
+  float ref = kInf, log_sum = 0.f;
   const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
-  if (live) {
+  if (live && stats[2 * stat] != -kInf) {
     ref = stats[2 * stat];
-    sum = stats[2 * stat + 1];
+    log_sum = __log2f(stats[2 * stat + 1]);
   }
-  const float lse = ref == -kInf ? kInf : fmaf(ref, c, __log2f(sum));
-  const float inv = 1.f / sum;
   if (live && half == 0 && part == 0) {
-    lses[stat] = lse;
-    deltas[stat] = -delta;
+    rows.ref[stat] = ref;
+    rows.log_sum[stat] = log_sum;
+    rows.delta[stat] = -delta;
   }
-  if (!gq && !table_grad) return;
+  if (!gq && !Table) return;
 
   const int base = -(start + i0 + kBlock);
   if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
-  if (table_grad) {
+  if (Table) {
     for (int n = lane; n < p.NB; n += 64) sums[n] = 0.f;
+    finished[wave][lane] = chain_end[wave][lane] = 0.f;
   }
   Feed<T, DP, Wide> kt(p.ks[1], p.D, tid), vt(p.vs[1], p.D, tid);
   int bucket = 0;
@@ -143,9 +209,21 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   __syncthreads();
 
   const int at = kBlock - local + 32 * half, shift = at & 3;
-  const bool huge = __any(lse < kInf && fabsf(lse) > kHugeStat);
   const float kept = lane == 32 ? 0.f : 1.f;
-  float diagonals = 0.f;
+  float diagonals = 0.f, second = 0.f;  // the two chains
+  int finished_bucket = -1;
+  // What a tile has finished goes to the sums while the next one's products are under way; what its
+  // upper half-wave holds goes on in that one's lower half, one lane up.
+  auto finish_diagonals = [&] {
+    const float above = chain_end[wave][(lane - 16) & 63];
+    const float first_chain = chain_end[wave][(47 - lane) & 63];
+    diagonals = upper_to_lower(second + (lane >= 48 ? above : 0.f));
+    bool last;
+    const float value = run_sum(finished[wave][lane] + (lane >= 16 ? first_chain : 0.f),
+                                finished_bucket, lane, last);
+    if (last && (unsigned)finished_bucket < (unsigned)p.NB) atomicAdd(&sums[finished_bucket], value);
+    wave_order();
+  };
   floatx16 acc[Blocks];
 #pragma unroll
   for (int d = 0; d < Blocks; d++) acc[d] = (floatx16)(0.f);
@@ -158,59 +236,72 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
       vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[buf ^ 1], p.D, tid);
       if (biased) bucket = bucket_of(p, base + (int)next + tid);
     }
+    floatx16 u[2], dp[2];
 #pragma unroll
     for (int blk = 0; blk < 2; blk++) {
-      floatx16 u, dp;
-      u = sixteen(window[buf].get(at + 16 * blk, shift), window[buf].get(at + 16 * blk + 8, shift));
-      dp = (floatx16)(0.f);
-#pragma unroll
-      for (int ch = 0; ch < Chunks; ch++) {
-        u = mma(row_frag<T, DP>(ks[buf], row_of(lane & 31, blk), ch, half), qf[ch], u);
-        dp = mma(row_frag<T, DP>(vs[buf], row_of(lane & 31, blk), ch, half), gf[ch], dp);
-      }
-      dp = add_outer(half ? 0.f : 1.f, -delta, dp);
-      if (j0 + kTile > wave_limit) {
-        keep_between(u, 0, limit - (j0 + 32 * half + 16 * blk));
-      }
-      if (huge) {
-#pragma unroll
-        for (int n = 0; n < 16; n++) dp[n] *= probability<true>(u[n], c, lse, ref, inv);
-      } else {
-#pragma unroll
-        for (int n = 0; n < 16; n++) dp[n] *= probability<false>(u[n], c, lse, ref, inv);
-      }
-#pragma unroll
-      for (int s = 0; s < 2; s++) {
-        const Frag<T> f = Frag<T>::pack(eight(dp, s));
-#pragma unroll
-        for (int d = 0; d < Blocks; d++)
-          acc[d] = mma(Column<T, DP, 32>::get(ks[buf], 16 * blk + 8 * s, d, lane), f, acc[d]);
-      }
-      if (table_grad) {
-        floatx16 left;  // what lane 31 held before each step: a finished diagonal
-#pragma unroll
-        for (int n = 0; n < 16; n++) {
-          left[n] = diagonals;
-          diagonals = next_diagonals(dp[n], diagonals, kept);
-        }
-        if (lane == 31) {
-          floatx4 *to = (floatx4 *)&finished[wave][16 * blk];
-#pragma unroll
-          for (int n = 0; n < 4; n++)
-            to[n] = floatx4{left[4 * n], left[4 * n + 1], left[4 * n + 2], left[4 * n + 3]};
-        }
-      }
+      u[blk] = sixteen(window[buf].get(at + 16 * blk, shift), window[buf].get(at + 16 * blk + 8, shift));
+      dp[blk] = (floatx16)(0.f);
+      // (what is -inf before the product stays it)
+      if (j0 + kTile > wave_limit) keep_between(u[blk], 0, limit - (j0 + 32 * half + 16 * blk));
     }
-    if (table_grad) {
-      // the lower half-wave's sums are finished (difference 31 - lane), the upper half's go on in
-      // the next tile's lower half, one lane up
-      if (half == 0) finished[wave][63 - lane] = diagonals;
-      diagonals = upper_to_lower(diagonals);
-      wave_order();
-      const float value = finished[wave][lane];
-      const int n = window_bucket[buf][lane + kBlock - 32 - wave * kLanesRows];
-      if ((unsigned)n < (unsigned)p.NB) atomicAdd(&sums[n], value);
-      wave_order();
+    {
+      // A pipeline over the two blocks of 32 keys: the vector work of one stands beside the
+      // products of the other.
+      const int lane = here(threadIdx.x & 63), half = lane >> 5;
+      Frag<T> ds[2];
+      auto begin = [&](int blk, auto beside) {
+        scores<T, DP, Ahead>(ks[buf], vs[buf], blk, lane, qf, gf, u[blk], dp[blk], beside);
+        dp[blk] = add_outer(half ? 0.f : 1.f, -delta, dp[blk]);
+      };
+      auto gradients = [&](int blk, int n0, int n1) {
+#pragma unroll
+        for (int n = n0; n < n1; n++) dp[blk][n] *= exp2_fast(fmaf(u[blk][n] - ref, c, -log_sum));
+      };
+      auto to_queries = [&](int blk, auto beside) {
+        ds[0] = Frag<T>::pack(eight(dp[blk], 0));
+        ds[1] = Frag<T>::pack(eight(dp[blk], 1));
+        Frag<T> f[2 * Blocks];
+#pragma unroll
+        for (int n = -Ahead; n < 2 * Blocks; n++) {
+          if (const int m = n + Ahead; m < 2 * Blocks)
+            f[m] = Column<T, DP, 32>::get(ks[buf], 16 * blk + 8 * (m / Blocks), m % Blocks, lane);
+          if (n < 0) continue;
+          acc[n % Blocks] = mma(f[n], ds[n / Blocks], acc[n % Blocks]);
+          beside(n);
+          step_end();
+        }
+      };
+      begin(0, [](int) {});
+      if constexpr (Table) finish_diagonals();
+      begin(1, [&](int n) { gradients(0, part_start(n, Chunks), part_start(n + 1, Chunks)); });
+      to_queries(0, [&](int n) { gradients(1, part_start(n, 2 * Blocks), part_start(n + 1, 2 * Blocks)); });
+      floatx16 left[2];  // what lane 31 held before each step: a finished diagonal
+      second = 0.f;
+      to_queries(1, [&](int n) {
+        if constexpr (Table) {
+#pragma unroll
+          for (int m = part_start(n, 2 * Blocks); m < part_start(n + 1, 2 * Blocks); m++) {
+            left[0][m] = diagonals, left[1][m] = second;
+            float x = dp[0][m], y = dp[1][m];
+            next_diagonals(x, diagonals, y, second, kept);
+            diagonals = x, second = y;
+          }
+        }
+      });
+      if constexpr (Table) {
+        chain_end[wave][lane] = diagonals;
+        if (lane == 31) {
+          floatx4 *to = (floatx4 *)finished[wave];
+#pragma unroll
+          for (int n = 0; n < 8; n++)
+            to[n] = floatx4{left[n / 4][4 * (n % 4)], left[n / 4][4 * (n % 4) + 1],
+                            left[n / 4][4 * (n % 4) + 2], left[n / 4][4 * (n % 4) + 3]};
+        }
+        // the lower half-wave's sums are finished (difference 31 - lane)
+        if (half == 0) finished[wave][63 - lane] = second;
+        finished_bucket = window_bucket[buf][lane + kBlock - 32 - wave * kLanesRows];
+        wave_order();
+      }
     }
     if (t + 1 < tiles) {
       kt.finish(ks[buf ^ 1], tid);
@@ -222,7 +313,8 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
     }
     __syncthreads();
   }
-  if (table_grad) {
+  if constexpr (Table) {
+    finish_diagonals();
     if (first < tiles && half == 0) {  // differences 63 - lane of the last tile
       const int n = window_bucket[(tiles - 1) & 1][63 - lane + kBlock - wave * kLanesRows];
       if ((unsigned)n < (unsigned)p.NB) atomicAdd(&sums[n], diagonals);
@@ -249,17 +341,15 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
 // columns, and walks the queries of all heads that share them, 64 at a time.
 template <typename T, int DP, bool Wide>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void attention_key_grad_kernel(
-    Params p, const T *gout, const float *stats, const float *lses, const float *deltas, T *gk,
-    T *gv, float *gk_parts, float *gv_parts, int nk, int parts) {
-  constexpr int Chunks = DP / 16, Blocks = DP / 32;
+    Params p, const T *gout, Rows rows, T *gk, T *gv, float *gk_parts, float *gv_parts, int nk, int parts) {
+  constexpr int Chunks = DP / 16, Blocks = DP / 32, Ahead = 3;
   __shared__ Word qs[2][kTile * words<T, DP>()];
   __shared__ Word gs[2][kTile * words<T, DP>()];
   __shared__ __attribute__((aligned(16))) Window window[2];
-  __shared__ __attribute__((aligned(16))) float row_lse[2][kTile], row_delta[2][kTile],
-      row_ref[2][kTile], row_inv[2][kTile];
+  __shared__ __attribute__((aligned(16))) float row_ref[2][kTile], row_log[2][kTile], row_delta[2][kTile];
   extern __shared__ float table[];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
   const int bh = unit / nk, b = bh / p.Hk, kh = bh % p.Hk;
   const int j0 = (unit % nk) * kBlock;  // the longest columns of a causal map first
@@ -294,7 +384,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
   const int64_t go_row = (int64_t)p.Hq * p.D;
   Feed<T, DP, Wide> qt(p.qs[1], p.D, tid), gt(go_row, p.D, tid);
   int bucket = 0;
-  float lse = 0.f, delta = 0.f, ref = 0.f, sum = 1.f;
+  float ref = 0.f, log_sum = 0.f, delta = 0.f;
   if (!biased) clear(window, tid);
   loads_done();
   for (int g = 0; g < group; g++) {
@@ -314,10 +404,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
       if (biased) bucket = bucket_of(p, base - (int)i - tid);
       if (tid < kTile) {
         const bool in = i + tid < p.Lq;
-        lse = in ? lses[stat + i + tid] : kInf;
-        delta = in ? deltas[stat + i + tid] : 0.f;
-        ref = in ? stats[2 * (stat + i + tid)] : -kInf;
-        sum = in ? stats[2 * (stat + i + tid) + 1] : 1.f;
+        ref = in ? rows.ref[stat + i + tid] : kInf;
+        log_sum = in ? rows.log_sum[stat + i + tid] : 0.f;
+        delta = in ? rows.delta[stat + i + tid] : 0.f;
       }
     };
     auto put = [&](int buf) {
@@ -325,10 +414,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
       gt.finish(gs[buf], tid);
       if (biased && tid < kWindow) window[buf].put(tid, bias_of(table, p.NB, bucket));
       if (tid < kTile) {
-        row_lse[buf][tid] = lse;
-        row_delta[buf][tid] = delta;
         row_ref[buf][tid] = ref;
-        row_inv[buf][tid] = 1.f / sum;
+        row_log[buf][tid] = log_sum;
+        row_delta[buf][tid] = delta;
       }
     };
     if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
@@ -339,49 +427,63 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
     for (int t = t0; t < t1; t++) {
       const int buf = (t - t0) & 1, i0 = t * kTile;
       if (t + 1 < t1) fetch(t + 1, buf ^ 1);
-      const float mine = row_lse[buf][lane];
-      const bool huge = __any(mine < kInf && fabsf(mine) > kHugeStat);
+      floatx16 u[2], dp[2];
 #pragma unroll
       for (int blk = 0; blk < 2; blk++) {
-        floatx16 u, dp;
-        u = sixteen(window[buf].get(at + 16 * blk, shift), window[buf].get(at + 16 * blk + 8, shift));
-        auto rows8 = [&](const float *x, int s) {
+        u[blk] = sixteen(window[buf].get(at + 16 * blk, shift), window[buf].get(at + 16 * blk + 8, shift));
+        dp[blk] = (floatx16)(0.f);
+        if (i0 < wave_safe || i0 + kTile > p.Lq) {
+          const int row0 = i0 + 32 * half + 16 * blk;
+          keep_between(u[blk], own_first - row0, p.Lq - row0);
+        }
+      }
+      {
+        // (the same pipeline; the rows are queries here)
+        const int lane = here(threadIdx.x & 63), half = lane >> 5;
+        Frag<T> pf[2][2], sf[2][2];
+        auto rows8 = [&](const float *x, int blk, int s) {
           const floatx4 *w = (const floatx4 *)(x + 32 * half + 16 * blk + 8 * s);
           const floatx4 lo = w[0], hi = w[1];
           return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         };
-        dp = (floatx16)(0.f);
+        auto begin = [&](int blk, auto beside) {
+          scores<T, DP, Ahead>(qs[buf], gs[buf], blk, lane, kf, vf, u[blk], dp[blk], beside);
+          const float delta_row = row_delta[buf][row_of(lane & 31, blk)];
+          dp[blk] = add_outer(half ? 0.f : delta_row, 1.f, dp[blk]);
+        };
+        floatx8 ref8, log8;
+        auto gradients = [&](int blk, int n0, int n1) {
 #pragma unroll
-        for (int ch = 0; ch < Chunks; ch++) {
-          u = mma(row_frag<T, DP>(qs[buf], row_of(lane & 31, blk), ch, half), kf[ch], u);
-          dp = mma(row_frag<T, DP>(gs[buf], row_of(lane & 31, blk), ch, half), vf[ch], dp);
-        }
-        dp = add_outer(half ? 0.f : row_delta[buf][row_of(lane & 31, blk)], 1.f, dp);
-        if (i0 < wave_safe || i0 + kTile > p.Lq) {
-          const int row0 = i0 + 32 * half + 16 * blk;
-          keep_between(u, own_first - row0, p.Lq - row0);
-        }
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-          floatx8 x, y;
-          const floatx8 l8 = rows8(row_lse[buf], s);
-          if (huge) {
-            const floatx8 r8 = rows8(row_ref[buf], s), i8 = rows8(row_inv[buf], s);
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = probability<true>(u[8 * s + e], c, l8[e], r8[e], i8[e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = probability<false>(u[8 * s + e], c, l8[e], 0.f, 0.f);
+          for (int n = n0; n < n1; n++) {
+            if (n % 8 == 0) ref8 = rows8(row_ref[buf], blk, n / 8), log8 = rows8(row_log[buf], blk, n / 8);
+            const float x = exp2_fast(fmaf(u[blk][n] - ref8[n % 8], c, -log8[n % 8]));
+            u[blk][n] = x;
+            dp[blk][n] *= x;
+            if (n % 8 == 7) {
+              pf[blk][n / 8] = Frag<T>::pack(eight(u[blk], n / 8));
+              sf[blk][n / 8] = Frag<T>::pack(eight(dp[blk], n / 8));
+            }
           }
+        };
+        auto to_keys = [&](int blk, auto beside) {
+          Frag<T> fg[2 * Blocks], fq[2 * Blocks];
 #pragma unroll
-          for (int e = 0; e < 8; e++) y[e] = x[e] * dp[8 * s + e];
-          const Frag<T> pf = Frag<T>::pack(x), sf = Frag<T>::pack(y);
-#pragma unroll
-          for (int d = 0; d < Blocks; d++) {
-            dv[d] = mma(Column<T, DP, 32>::get(gs[buf], 16 * blk + 8 * s, d, lane), pf, dv[d]);
-            dk[d] = mma(Column<T, DP, 32>::get(qs[buf], 16 * blk + 8 * s, d, lane), sf, dk[d]);
+          for (int n = -Ahead; n < 2 * Blocks; n++) {
+            if (const int m = n + Ahead; m < 2 * Blocks) {
+              fg[m] = Column<T, DP, 32>::get(gs[buf], 16 * blk + 8 * (m / Blocks), m % Blocks, lane);
+              fq[m] = Column<T, DP, 32>::get(qs[buf], 16 * blk + 8 * (m / Blocks), m % Blocks, lane);
+            }
+            if (n < 0) continue;
+            dv[n % Blocks] = mma(fg[n], pf[blk][n / Blocks], dv[n % Blocks]);
+            dk[n % Blocks] = mma(fq[n], sf[blk][n / Blocks], dk[n % Blocks]);
+            beside(n);
+            step_end();
           }
-        }
+        };
+        begin(0, [](int) {});
+        begin(1, [&](int n) { gradients(0, part_start(n, Chunks), part_start(n + 1, Chunks)); });
+        to_keys(0, [&](int n) { gradients(1, part_start(n, 2 * Blocks), part_start(n + 1, 2 * Blocks)); });
+        to_keys(1, [](int) {});
       }
       if (t + 1 < t1) put(buf ^ 1);
       __syncthreads();
@@ -457,7 +559,7 @@ static Plan plan_of(const Params &p) {
   n.k_parts = n.k_units ? parts_of(n.k_units, q_tiles * (p.Hq / p.Hk)) : 1;
   const size_t rows = (size_t)p.B * p.Hq * p.Lq, keys = (size_t)p.B * p.Hk * p.Lk, f = sizeof(float);
   n.rows_at = align256(rows * f);
-  n.partial_at = n.rows_at + align256(rows * f);
+  n.partial_at = n.rows_at + 2 * align256(rows * f);
   n.slices_at = n.partial_at + align256((size_t)n.q_units * n.q_parts * p.NB * f);
   n.q_at = n.slices_at + align256((size_t)kSlices * p.Hq * p.NB * f);
   n.k_at = n.q_at + (n.q_parts > 1 ? align256(n.q_parts * rows * p.D * f) : 0);
@@ -478,7 +580,7 @@ template <typename T>
 static int launch_backward(const Params &p, const Plan &n, const void *gout, const void *out,
                            const float *stats, void *gq, void *gk, void *gv, void *gtable, char *ws,
                            hipStream_t stream) {
-  float *lses = (float *)ws, *deltas = (float *)(ws + n.rows_at);
+  const Rows rows = {(float *)ws, (float *)(ws + n.rows_at), (float *)(ws + 2 * n.rows_at)};
   float *partial = (float *)(ws + n.partial_at), *slices = (float *)(ws + n.slices_at);
   float *q_parts = (float *)(ws + n.q_at);
   float *k_parts = (float *)(ws + n.k_at), *v_parts = (float *)(ws + n.v_at);
@@ -488,8 +590,10 @@ static int launch_backward(const Params &p, const Plan &n, const void *gout, con
     const dim3 grid((unsigned)(n.q_units * parts));
     const size_t lds = (gtable ? 1 + kWaves : 1) * p.NB * sizeof(float);
 #define MCX_GRAD(DP, W)                                                                           \
-  hipLaunchKernelGGL((attention_query_grad_kernel<T, DP, W>), grid, threads, lds, stream, p,       \
-                     (const T *)out, (const T *)gout, stats, lses, deltas, (T *)gq, q_parts,      \
+  hipLaunchKernelGGL((gtable ? attention_query_grad_kernel<T, DP, W, true>                        \
+                             : attention_query_grad_kernel<T, DP, W, false>), grid, threads, lds, \
+                     stream, p,                                                                   \
+                     (const T *)out, (const T *)gout, stats, rows, (T *)gq, q_parts,              \
                      gtable ? partial : nullptr, (int)n.nq, parts)
     MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out) && aligned16(gout) && aligned16(gq), MCX_GRAD);
 #undef MCX_GRAD
@@ -518,7 +622,7 @@ static int launch_backward(const Params &p, const Plan &n, const void *gout, con
     const size_t lds = p.NB * sizeof(float);
 #define MCX_GRAD(DP, W)                                                                      \
   hipLaunchKernelGGL((attention_key_grad_kernel<T, DP, W>), grid, threads, lds, stream, p,    \
-                     (const T *)gout, stats, lses, deltas, (T *)gk, (T *)gv, k_parts, v_parts, \
+                     (const T *)gout, rows, (T *)gk, (T *)gv, k_parts, v_parts,                \
                      (int)n.nk, n.k_parts)
     MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(gout) && aligned16(gk) && aligned16(gv), MCX_GRAD);
 #undef MCX_GRAD

@@ -21,7 +21,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   __shared__ __attribute__((aligned(16))) Window window[2];
   extern __shared__ float table[];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
   const int bh = unit / nq, b = bh / p.Hq, h = bh % p.Hq;
   // the longest rows of a causal map first

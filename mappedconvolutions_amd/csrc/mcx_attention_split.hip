@@ -39,7 +39,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   __shared__ float merge[kWaves][kRows][2];
   extern __shared__ float table[];  // [min(group, 32)][NB]
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x);
   const int part = wg % sp.parts, unit = wg / sp.parts;
   const int block = unit % sp.blocks, bk = unit / sp.blocks, b = bk / p.Hk, kh = bk % p.Hk;
@@ -240,7 +240,7 @@ template <typename T>
 __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(Params p, Split sp, T *out,
                                                                          float *stats) {
   __shared__ float merge[kJoinWaves][kMaxD];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = p.Hq / p.Hk;
   const int bk = blockIdx.x / sp.rows, r = blockIdx.x % sp.rows, b = bk / p.Hk, kh = bk % p.Hk;
   const int unit = bk * sp.blocks + r / kRows, row = r % kRows;
