@@ -453,7 +453,8 @@ typedef struct mcx_attention_desc {
  * over the keys j < key_lengths[b] and, if causal, j <= query_start[b] + i.
  *   q [B, Lq, Hq, D], k, v [B, Lk, Hk, D], table [Hq, table_size] and buckets int32 or both NULL,
  *   query_start int32 [B] or NULL (zeros), key_lengths int32 [B] or NULL (Lk; clamped to [0, Lk]),
- *   out [B, Lq, Hq, D] contiguous, stats float [B, Hq, Lq, 2] for the gradients, or NULL.
+ *   out [B, Lq, Hq, D] contiguous; for the gradients, or NULL: stats float [B, Hq, Lq, 2] (a row's
+ *   reference and sum), and for bf16 out_rest, like out: what rounding took from it.
  * A row that nothing is left of is zeros.  What lies at keys from key_lengths[b] on is not read.
  * A bucket outside [0, table_size) has no bias; a bias of -inf takes its pairs out; a finite bias
  * is held within 1e30.
@@ -462,17 +463,18 @@ typedef struct mcx_attention_desc {
 size_t mcx_attention_forward_workspace(const mcx_attention_desc *desc, int dtype);
 int mcx_attention_forward(const void *q, const void *k, const void *v, const void *table,
                           const int32_t *buckets, const int32_t *query_start,
-                          const int32_t *key_lengths, void *out, float *stats, void *workspace,
-                          size_t workspace_bytes, const mcx_attention_desc *desc, int dtype,
-                          void *stream);
+                          const int32_t *key_lengths, void *out, float *stats, void *out_rest,
+                          void *workspace, size_t workspace_bytes, const mcx_attention_desc *desc,
+                          int dtype, void *stream);
 
-/* Gradients from gout (contiguous) and the forward call's out and stats: gq [B, Lq, Hq, D],
+/* Gradients from gout (contiguous) and the forward call's out, out_rest (or NULL: delta = gout . out
+ * is then formed from the rounded output) and stats: gq [B, Lq, Hq, D],
  * gk, gv [B, Lk, Hk, D] (zeros at keys that are not in use), gtable [Hq, table_size], all
  * contiguous; NULL for a gradient that is not wanted.  The same bits from call to call. */
 size_t mcx_attention_backward_workspace(const mcx_attention_desc *desc, int dtype);
 int mcx_attention_backward(const void *gout, const void *q, const void *k, const void *v,
-                           const void *out, const float *stats, const void *table,
-                           const int32_t *buckets, const int32_t *query_start,
+                           const void *out, const void *out_rest, const float *stats,
+                           const void *table, const int32_t *buckets, const int32_t *query_start,
                            const int32_t *key_lengths, void *gq, void *gk, void *gv, void *gtable,
                            void *workspace, size_t workspace_bytes, const mcx_attention_desc *desc,
                            int dtype, void *stream);

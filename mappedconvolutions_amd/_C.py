@@ -1033,27 +1033,29 @@ def relative_attention_forward(query, key, value, bias_table=None, buckets=None,
     says how many keys are in use: what lies behind them is not read.  scale: D ** -0.5 by default.
     A row that nothing is left of is zeros.  A bucket that the table does not have has no bias; a
     bias of -inf takes its pairs out.
-    -> [out [B, Lq, Hq, D], stats]: stats, for relative_attention_backward, is None unless
-    `for_backward`.  Keys and values within key_lengths have to be finite."""
+    -> [out [B, Lq, Hq, D], saved]: `saved`, for relative_attention_backward, is None unless
+    `for_backward`: a list of the rows' statistics (float32) and, for bfloat16, of what rounding took
+    from the output.  Keys and values within key_lengths have to be finite."""
     dt, desc, tensors = _attention_args(query, key, value, bias_table, buckets, bucket_zero, scale,
                                         causal, query_start, key_lengths)
     query = tensors[0]
     B, Lq, Hq, D = query.shape
     out = torch.empty((B, Lq, Hq, D), dtype=query.dtype, device=query.device)
-    stats = None
+    stats = rest = None
     if for_backward:
         stats = torch.empty((B, Hq, Lq, 2), dtype=torch.float32, device=query.device)
+        rest = torch.empty_like(out) if dt == MCX_BF16 else None
     lib = _lib.load()
     nbytes = lib.mcx_attention_forward_workspace(desc, dt)
     ws = _workspace(nbytes, query.device) if nbytes else None
     with _device(query):
         rc = lib.mcx_attention_forward(*[_ptr(t) for t in tensors], _ptr(out), _ptr(stats),
-                                       _ptr(ws), nbytes, desc, dt, _stream(query))
+                                       _ptr(rest), _ptr(ws), nbytes, desc, dt, _stream(query))
     _lib.check(rc, "relative_attention_forward")
-    return [out, stats]
+    return [out, [stats, rest] if for_backward else None]
 
 
-def relative_attention_backward(grad_output, query, key, value, output, stats, bias_table=None,
+def relative_attention_backward(grad_output, query, key, value, output, saved, bias_table=None,
                                 buckets=None, bucket_zero=0, scale=None, causal=False,
                                 query_start=None, key_lengths=None,
                                 needs=(True, True, True, True)):
@@ -1066,11 +1068,14 @@ def relative_attention_backward(grad_output, query, key, value, output, stats, b
     _heads("grad_output", grad_output, *query.shape)
     _heads("output", output, *query.shape)
     _attention_dtype(query, grad_output=grad_output, output=output)
-    _on_gpu("query", query, grad_output=grad_output, output=output, stats=stats)
     B, Lq, Hq, D = query.shape
-    if stats is None or stats.dtype != torch.float32 or tuple(stats.shape) != (B, Hq, Lq, 2):
-        raise RuntimeError("stats must be what relative_attention_forward returned with for_backward")
-    grad_output, output, stats = grad_output.contiguous(), output.contiguous(), stats.contiguous()
+    stats, rest = saved if saved is not None else (None, None)
+    if stats is None or stats.dtype != torch.float32 or tuple(stats.shape) != (B, Hq, Lq, 2) or \
+            (rest is not None and (rest.dtype != query.dtype or rest.shape != query.shape)):
+        raise RuntimeError("saved must be what relative_attention_forward returned with for_backward")
+    _on_gpu("query", query, grad_output=grad_output, output=output, stats=stats, rest=rest)
+    _contig(stats=stats, rest=rest)
+    grad_output, output = grad_output.contiguous(), output.contiguous()
 
     def like(t, wanted):
         return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None
@@ -1087,7 +1092,8 @@ def relative_attention_backward(grad_output, query, key, value, output, stats, b
     ws = _workspace(nbytes, query.device)
     with _device(query):
         rc = lib.mcx_attention_backward(_ptr(grad_output), *[_ptr(t) for t in tensors[:3]],
-                                        _ptr(output), _ptr(stats), *[_ptr(t) for t in tensors[3:]],
+                                        _ptr(output), _ptr(rest), _ptr(stats),
+                                        *[_ptr(t) for t in tensors[3:]],
                                         _ptr(gq), _ptr(gk), _ptr(gv), _ptr(gt), _ptr(ws), nbytes,
                                         desc, dt, _stream(query))
     _lib.check(rc, "relative_attention_backward")

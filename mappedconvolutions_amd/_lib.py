@@ -87,9 +87,9 @@ SIGNATURES = {
     "mcx_qk_norm_rotate_backward": (_i, [_p] * 14 + [_sz] + [_i64 * 3] * 2 + [_i64] * 7 +
                                     [_f64, _i, _i, _p]),
     "mcx_attention_forward_workspace": (_sz, [_adesc, _i]),
-    "mcx_attention_forward": (_i, [_p] * 10 + [_sz, _adesc, _i, _p]),
+    "mcx_attention_forward": (_i, [_p] * 11 + [_sz, _adesc, _i, _p]),
     "mcx_attention_backward_workspace": (_sz, [_adesc, _i]),
-    "mcx_attention_backward": (_i, [_p] * 15 + [_sz, _adesc, _i, _p]),
+    "mcx_attention_backward": (_i, [_p] * 16 + [_sz, _adesc, _i, _p]),
     "mcx_clip_grad_norm_workspace": (_sz, [_p, _i64]),
     "mcx_clip_grad_norm": (_i, [_p] * 4 + [_i64, _f64, _f64, _p, _p, _sz, _p]),
 }

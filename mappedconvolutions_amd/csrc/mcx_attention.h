@@ -321,9 +321,11 @@ __device__ inline float other_half(float x) {
 }
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// A lane's column of a transposed result ([DP] values in blocks of 32) to a row of memory.
+// A lane's column of a transposed result ([DP] values in blocks of 32) to a row of memory, and what
+// rounding to T took from it to `rest`, where that is wanted.
 template <bool Wide, typename T, int NBlocks>
-__device__ inline void store_column(T *row, const floatx16 *acc, float factor, int D, int half) {
+__device__ inline void store_column(T *row, const floatx16 *acc, float factor, int D, int half,
+                                    T *rest = nullptr) {
 #pragma unroll
   for (int blk = 0; blk < NBlocks; blk++)
 #pragma unroll
@@ -333,14 +335,26 @@ __device__ inline void store_column(T *row, const floatx16 *acc, float factor, i
       floatx4 x = {acc[blk][4 * g] * factor, acc[blk][4 * g + 1] * factor,
                    acc[blk][4 * g + 2] * factor, acc[blk][4 * g + 3] * factor};
       const T4 y = __builtin_convertvector(x, T4);
+      const T4 z = __builtin_convertvector(x - __builtin_convertvector(y, floatx4), T4);
       if (Wide) {
         if (d0 < D) *(T4 *)(row + d0) = y;
+        if (rest && d0 < D) *(T4 *)(rest + d0) = z;
       } else {
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          if (d0 + e < D) row[d0 + e] = y[e];
+          if (d0 + e < D) {
+            row[d0 + e] = y[e];
+            if (rest) rest[d0 + e] = z[e];
+          }
       }
     }
+}
+
+// One value of the output, and what rounding took from it.
+template <typename T> __device__ inline void store_value(T *out, T *rest, int64_t at, float x) {
+  const T y = (T)x;
+  out[at] = y;
+  if (rest) rest[at] = (T)(x - (float)y);
 }
 
 // Eight of the sixteen values of a product, s = 0, 1; and two eights as the start of one.
@@ -377,8 +391,8 @@ int parts_of(int64_t units, int64_t tiles);
 // keys (0: not the form for these sizes), its workspace, and its launch.
 int split_parts(const Params &p, int dtype);
 size_t split_bytes(const Params &p, int parts);
-int launch_split(const Params &p, int parts, void *out, float *stats, void *workspace, int dtype,
-                 hipStream_t stream);
+int launch_split(const Params &p, int parts, void *out, float *stats, void *rest, void *workspace,
+                 int dtype, hipStream_t stream);
 
 }  // namespace attention
 }  // namespace mcx

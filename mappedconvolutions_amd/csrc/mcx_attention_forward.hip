@@ -14,7 +14,7 @@ namespace attention {
 // sums stay far inside fp32, and the accumulated output is seldom rescaled.
 template <typename T, int DP, bool Wide>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void attention_forward_kernel(
-    Params p, T *out, float *stats, float *outs, float *sums, int nq, int parts) {
+    Params p, T *out, float *stats, T *rest, float *outs, float *sums, int nq, int parts) {
   constexpr int Chunks = DP / 16, Blocks = DP / 32;
   __shared__ Word ks[2][kTile * words<T, DP>()];
   __shared__ Word vs[2][kTile * words<T, DP>()];
@@ -153,7 +153,8 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
     store_column<Wide, float, Blocks>(outs + (part * rows + row) * p.D, o, 1.f, p.D, half);
     stats = sums + part * rows * 2;
   } else {
-    store_column<Wide, T, Blocks>(out + row * p.D, o, sum == 0.f ? 0.f : 1.f / sum, p.D, half);
+    store_column<Wide, T, Blocks>(out + row * p.D, o, sum == 0.f ? 0.f : 1.f / sum, p.D, half,
+                                  rest ? rest + row * p.D : nullptr);
   }
   if (stats && half == 0) {
     stats[2 * stat] = ref;
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join_values_kernel(Params p, const float *outs,
                                                                     const float *sums, T *out,
-                                                                    float *stats, int parts) {
+                                                                    float *stats, T *rest, int parts) {
   const int64_t rows = (int64_t)p.B * p.Lq * p.Hq, n = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (n >= rows * p.D) return;
   const int64_t row = n / p.D, bi = row / p.Hq, b = bi / p.Lq;
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(256) void attention_join_values_kernel(Params p, co
     all = fmaf(w, sums[(s * rows + stat) * 2 + 1], all);
     x = fmaf(w, outs[s * rows * p.D + n], x);
   }
-  out[n] = (T)(all == 0.f ? 0.f : x / all);
+  store_value(out, rest, n, all == 0.f ? 0.f : x / all);
   if (stats && n % p.D == 0) {
     stats[2 * stat] = top;
     stats[2 * stat + 1] = all;
@@ -200,7 +201,7 @@ static size_t forward_bytes(const Params &p) {
 }
 
 template <typename T>
-static int launch_forward(const Params &p, void *out, float *stats, void *workspace,
+static int launch_forward(const Params &p, void *out, float *stats, void *rest, void *workspace,
                           hipStream_t stream) {
   const int nq = (p.Lq + kBlock - 1) / kBlock, parts = forward_parts(p);
   const dim3 grid((unsigned)(query_units(p) * parts)), threads(64 * kWaves);
@@ -210,13 +211,13 @@ static int launch_forward(const Params &p, void *out, float *stats, void *worksp
   const size_t lds = p.table ? p.NB * sizeof(float) : 0;
 #define MCX_FORWARD(DP, W)                                                                     \
   hipLaunchKernelGGL((attention_forward_kernel<T, DP, W>), grid, threads, lds, stream, p, (T *)out, \
-                     stats, outs, sums, nq, parts)
-  MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out), MCX_FORWARD);
+                     stats, (T *)rest, outs, sums, nq, parts)
+  MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out) && aligned16(rest), MCX_FORWARD);
 #undef MCX_FORWARD
   MCX_HIP_CHECK_LAUNCH();
   if (parts > 1) {
     hipLaunchKernelGGL((attention_join_values_kernel<T>), dim3((unsigned)((rows * p.D + 255) / 256)),
-                       dim3(256), 0, stream, p, outs, sums, (T *)out, stats, parts);
+                       dim3(256), 0, stream, p, outs, sums, (T *)out, stats, (T *)rest, parts);
     MCX_HIP_CHECK_LAUNCH();
   }
   return MCX_OK;
@@ -284,8 +285,8 @@ size_t mcx_attention_forward_workspace(const mcx_attention_desc *desc, int dtype
 
 int mcx_attention_forward(const void *q, const void *k, const void *v, const void *table,
                           const int32_t *buckets, const int32_t *query_start,
-                          const int32_t *key_lengths, void *out, float *stats, void *workspace,
-                          size_t workspace_bytes, const mcx_attention_desc *desc, int dtype,
+                          const int32_t *key_lengths, void *out, float *stats, void *out_rest,
+                          void *workspace, size_t workspace_bytes, const mcx_attention_desc *desc, int dtype,
                           void *stream) {
   using namespace mcx::attention;
   Params p;
@@ -297,13 +298,13 @@ int mcx_attention_forward(const void *q, const void *k, const void *v, const voi
   if (parts) {
     if (split_bytes(p, parts) && (!workspace || workspace_bytes < split_bytes(p, parts)))
       return MCX_E_WORKSPACE;
-    return launch_split(p, parts, out, stats, workspace, dtype, (hipStream_t)stream);
+    return launch_split(p, parts, out, stats, out_rest, workspace, dtype, (hipStream_t)stream);
   }
   if (query_units(p) > 0x7fffffffLL) return MCX_E_SHAPE;
   if (forward_bytes(p) && (!workspace || workspace_bytes < forward_bytes(p))) return MCX_E_WORKSPACE;
   return dtype == MCX_BF16
-             ? launch_forward<__bf16>(p, out, stats, workspace, (hipStream_t)stream)
-             : launch_forward<float>(p, out, stats, workspace, (hipStream_t)stream);
+             ? launch_forward<__bf16>(p, out, stats, out_rest, workspace, (hipStream_t)stream)
+             : launch_forward<float>(p, out, stats, nullptr, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

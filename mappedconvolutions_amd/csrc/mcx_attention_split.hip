@@ -29,7 +29,7 @@ struct Split {
 
 template <typename T, int DP, bool Wide>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void attention_split_kernel(
-    Params p, Split sp, T *out, float *stats) {
+    Params p, Split sp, T *out, float *stats, T *rest) {
   constexpr int Chunks = DP / 16, Blocks = DP / 32;
   constexpr int E = 16 / (int)sizeof(T), PerRow = words<T, DP>(), N = kStep * PerRow / 64;
   // a wave's values; at the end all waves' sums, four blocks of columns at a time
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
           if (sp.parts == 1) {
             // (lane & 31 is this thread's row too, so `all` is its row's sum)
             const int64_t to = ((int64_t)b * p.Lq + rr / group) * p.Hq + kh * group + rr % group;
-            out[to * p.D + dd] = (T)(all == 0.f ? 0.f : x / all);
+            store_value(out, rest, to * p.D + dd, all == 0.f ? 0.f : x / all);
           } else {
             sp.outs[(at * kRows + row) * p.D + dd] = x;
           }
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
 constexpr int kJoinWaves = 16;
 template <typename T>
 __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(Params p, Split sp, T *out,
-                                                                         float *stats) {
+                                                                         float *stats, T *rest) {
   __shared__ float merge[kJoinWaves][kMaxD];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = p.Hq / p.Hk;
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(Params 
     x = 0.f;
 #pragma unroll
     for (int w = 0; w < kJoinWaves; w++) x += merge[w][tid];
-    out[(((int64_t)b * p.Lq + i) * p.Hq + h) * p.D + tid] = (T)(all == 0.f ? 0.f : x / all);
+    store_value(out, rest, (((int64_t)b * p.Lq + i) * p.Hq + h) * p.D + tid, all == 0.f ? 0.f : x / all);
   }
   if (stats && tid == 0) {
     float *s = stats + 2 * (((int64_t)b * p.Hq + h) * p.Lq + i);
@@ -298,7 +298,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(Params 
 constexpr int kFewParts = 16;
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join_few_kernel(Params p, Split sp, T *out,
-                                                                 float *stats, int64_t total) {
+                                                                 float *stats, T *rest,
+                                                                 int64_t total) {
   const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;  // [bk][row][value]
   if (n >= total) return;
   const int64_t br = n / p.D;
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(256) void attention_join_few_kernel(Params p, Split
     x = fmaf(w, sp.outs[(first + s * kRows) * p.D + d], x);
   }
   const int64_t i = r / group, h = kh * group + r % group;
-  out[((b * (int64_t)p.Lq + i) * p.Hq + h) * p.D + d] = (T)(all == 0.f ? 0.f : x / all);
+  store_value(out, rest, ((b * (int64_t)p.Lq + i) * p.Hq + h) * p.D + d, all == 0.f ? 0.f : x / all);
   if (stats && d == 0) {
     float *s = stats + 2 * (((int64_t)b * p.Hq + h) * p.Lq + i);
     s[0] = top;
@@ -366,37 +367,38 @@ size_t split_bytes(const Params &p, int parts) {
 }
 
 template <typename T>
-static int launch(const Params &p, Split sp, void *out, float *stats, hipStream_t stream) {
+static int launch(const Params &p, Split sp, void *out, float *stats, void *rest,
+                  hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)p.B * p.Hk * sp.blocks * sp.parts)), threads(64 * kWaves);
   const size_t lds = p.table ? std::min(p.Hq / p.Hk, kRows) * p.NB * sizeof(float) : 0;
 #define MCX_SPLIT(DP, W)                                                                           \
   hipLaunchKernelGGL((attention_split_kernel<T, DP, W>), grid, threads, lds, stream, p, sp, (T *)out, \
-                     stats)
+                     stats, (T *)rest)
   MCX_ATTENTION_DISPATCH(p.D, p.wide, MCX_SPLIT);
 #undef MCX_SPLIT
   MCX_HIP_CHECK_LAUNCH();
   const int64_t rows = (int64_t)p.B * p.Hk * sp.rows, total = rows * p.D;
   if (sp.parts > kFewParts) {
     hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)rows), dim3(64 * kJoinWaves), 0,
-                       stream, p, sp, (T *)out, stats);
+                       stream, p, sp, (T *)out, stats, (T *)rest);
   } else if (sp.parts > 1) {
     hipLaunchKernelGGL((attention_join_few_kernel<T>), dim3((unsigned)((total + 255) / 256)),
-                       dim3(256), 0, stream, p, sp, (T *)out, stats, total);
+                       dim3(256), 0, stream, p, sp, (T *)out, stats, (T *)rest, total);
   }
   MCX_HIP_CHECK_LAUNCH();
   return MCX_OK;
 }
 
-int launch_split(const Params &p, int parts, void *out, float *stats, void *workspace, int dtype,
-                 hipStream_t stream) {
+int launch_split(const Params &p, int parts, void *out, float *stats, void *rest, void *workspace,
+                 int dtype, hipStream_t stream) {
   Split sp = split_of(p, parts);
   if (parts > 1) {
     const size_t rows = (size_t)p.B * p.Hk * sp.blocks * parts * kRows;
     sp.sums = (float *)workspace;
     sp.outs = (float *)((char *)workspace + align256(rows * 2 * sizeof(float)));
   }
-  return dtype == MCX_BF16 ? launch<__bf16>(p, sp, out, stats, stream)
-                           : launch<float>(p, sp, out, stats, stream);
+  return dtype == MCX_BF16 ? launch<__bf16>(p, sp, out, stats, rest, stream)
+                           : launch<float>(p, sp, out, stats, nullptr, stream);
 }
 
 }  // namespace attention
