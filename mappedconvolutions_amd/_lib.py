@@ -40,6 +40,7 @@ class AttentionDesc(ctypes.Structure):
 
 _adesc = ctypes.POINTER(AttentionDesc)
 _f64 = ctypes.c_double
+_pi64 = ctypes.POINTER(_i64)
 
 # name -> (restype, argtypes); mirrors include/mcx.h one to one.
 SIGNATURES = {
@@ -82,9 +83,9 @@ SIGNATURES = {
     "mcx_gnomonic_samples": (_i, [_p] * 2 + [_i64] * 3 + [ctypes.c_double] * 2 + [_p]),
     "mcx_planar_conv_operator_workspace": (_sz, [_i64]),
     "mcx_planar_conv_operator": (_i, [_p] * 7 + [_sz] + [_i64] * 3 + [_i, _p]),
-    "mcx_qk_norm_rotate_forward": (_i, [_p] * 9 + [_i64 * 3] * 2 + [_i64] * 7 + [_f64, _i, _i, _p]),
+    "mcx_qk_norm_rotate_forward": (_i, [_p] * 9 + [_pi64] * 2 + [_i64] * 7 + [_f64, _i, _i, _p]),
     "mcx_qk_norm_rotate_backward_workspace": (_sz, [_i64] * 5 + [_i]),
-    "mcx_qk_norm_rotate_backward": (_i, [_p] * 14 + [_sz] + [_i64 * 3] * 2 + [_i64] * 7 +
+    "mcx_qk_norm_rotate_backward": (_i, [_p] * 14 + [_sz] + [_pi64] * 2 + [_i64] * 7 +
                                     [_f64, _i, _i, _p]),
     "mcx_attention_forward_workspace": (_sz, [_adesc, _i]),
     "mcx_attention_forward": (_i, [_p] * 11 + [_sz, _adesc, _i, _p]),

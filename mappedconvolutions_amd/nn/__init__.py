@@ -9,6 +9,7 @@ from .mapped_transposed_convolution_layer import MappedTransposedConvolution
 from .mapped_max_pooling_layer import MappedMaxPool
 from .mapped_avg_pooling_layer import MappedAvgPool, MappedAvgUnpool
 from .resample_layer import Resample, Unresample
+from .relative_attention_layer import QKNormRotation, RelativeAttention
 
 __all__ = ['MappedConvolution', 'MappedTransposedConvolution', 'MappedMaxPool', 'MappedAvgPool',
-           'MappedAvgUnpool', 'Resample', 'Unresample']
+           'MappedAvgUnpool', 'Resample', 'Unresample', 'QKNormRotation', 'RelativeAttention']
