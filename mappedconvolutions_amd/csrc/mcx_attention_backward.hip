@@ -9,6 +9,7 @@
 // gradient then has one owner, who sums it in registers in a fixed order.  No atomics on memory,
 // the same bits each time.
 #include <algorithm>
+#include <type_traits>
 
 #include "mcx_attention.h"
 
@@ -196,19 +197,19 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   const int first = part * each, tiles = min(all, first + each);  // of this part
   if (first < tiles) {
     const int64_t next = (int64_t)first * kTile;
-    kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[first & 1], p.D, tid);
-    vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[first & 1], p.D, tid);
+    kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[0], p.D, tid);
+    vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[0], p.D, tid);
     if (biased) bucket = bucket_of(p, base + (int)next + tid);
   }
   if (!biased) clear(window, tid);
   loads_done();
   __syncthreads();
   if (first < tiles) {
-    kt.finish(ks[first & 1], tid);
-    vt.finish(vs[first & 1], tid);
+    kt.finish(ks[0], tid);
+    vt.finish(vs[0], tid);
     if (biased && tid < kWindow) {
-      window[first & 1].put(tid, bias_of(table, p.NB, bucket));
-      window_bucket[first & 1][tid] = bucket;
+      window[0].put(tid, bias_of(table, p.NB, bucket));
+      window_bucket[0][tid] = bucket;
     }
   }
   __syncthreads();
@@ -233,8 +234,10 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
 #pragma unroll
   for (int d = 0; d < Blocks; d++) acc[d] = (floatx16)(0.f);
 
-  for (int t = first; t < tiles; t++) {
-    const int j0 = t * kTile, buf = t & 1;
+  // (one copy for each buffer: its place is then part of the instructions)
+  auto tile = [&](int t, auto which) {
+    constexpr int buf = decltype(which)::value;
+    const int j0 = t * kTile;
     if (t + 1 < tiles) {
       const int64_t next = j0 + kTile;
       kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[buf ^ 1], p.D, tid);
@@ -317,11 +320,15 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
       }
     }
     __syncthreads();
+  };
+  for (int t = first; t < tiles; t += 2) {
+    tile(t, std::integral_constant<int, 0>{});
+    if (t + 1 < tiles) tile(t + 1, std::integral_constant<int, 1>{});
   }
   if constexpr (Table) {
     finish_diagonals();
     if (first < tiles && half == 0) {  // differences 63 - lane of the last tile
-      const int n = window_bucket[(tiles - 1) & 1][63 - lane + kBlock - wave * kLanesRows];
+      const int n = window_bucket[(tiles - 1 - first) & 1][63 - lane + kBlock - wave * kLanesRows];
       if ((unsigned)n < (unsigned)p.NB) atomicAdd(&sums[n], diagonals);
     }
     __syncthreads();
@@ -429,8 +436,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
     __syncthreads();
     put(0);
     __syncthreads();
-    for (int t = t0; t < t1; t++) {
-      const int buf = (t - t0) & 1, i0 = t * kTile;
+    auto tile = [&](int t, auto which) {
+      constexpr int buf = decltype(which)::value;
+      const int i0 = t * kTile;
       if (t + 1 < t1) fetch(t + 1, buf ^ 1);
       floatx16 u[2], dp[2];
 #pragma unroll
@@ -492,6 +500,10 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
       }
       if (t + 1 < t1) put(buf ^ 1);
       __syncthreads();
+    };
+    for (int t = t0; t < t1; t += 2) {
+      tile(t, std::integral_constant<int, 0>{});
+      if (t + 1 < t1) tile(t + 1, std::integral_constant<int, 1>{});
     }
   }
   if (!live) return;

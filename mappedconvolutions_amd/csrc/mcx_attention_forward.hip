@@ -1,6 +1,7 @@
 // Attention with a bias by relative-position buckets: the forward product and the C entry points.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "mcx_attention.h"
 
@@ -54,17 +55,17 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   const int first = part * each, tiles = min(all, first + each);  // of this part
   if (first < tiles) {
     const int64_t next = (int64_t)first * kTile;
-    kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[first & 1], p.D, tid);
-    vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[first & 1], p.D, tid);
+    kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[0], p.D, tid);
+    vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[0], p.D, tid);
     if (biased) bucket = bucket_of(p, base + (int)next + tid);
   }
   if (!biased) clear(window, tid);
   loads_done();
   __syncthreads();  // the table
   if (first < tiles) {
-    kt.finish(ks[first & 1], tid);
-    vt.finish(vs[first & 1], tid);
-    if (biased && tid < kWindow) window[first & 1].put(tid, bias_of(table, p.NB, bucket));
+    kt.finish(ks[0], tid);
+    vt.finish(vs[0], tid);
+    if (biased && tid < kWindow) window[0].put(tid, bias_of(table, p.NB, bucket));
   }
   __syncthreads();
 
@@ -75,8 +76,10 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   for (int d = 0; d < Blocks; d++) o[d] = (floatx16)(0.f);
   float ref = -kInf, sum = 0.f;
 
-  for (int t = first; t < tiles; t++) {
-    const int j0 = t * kTile, buf = t & 1;
+  // (one copy for each buffer: its place is then part of the instructions)
+  auto tile = [&](int t, auto which) {
+    constexpr int buf = decltype(which)::value;
+    const int j0 = t * kTile;
     if (t + 1 < tiles) {
       const int64_t next = j0 + kTile;
       kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[buf ^ 1], p.D, tid);
@@ -143,6 +146,10 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
       if (biased && tid < kWindow) window[buf ^ 1].put(tid, bias_of(table, p.NB, bucket));
     }
     __syncthreads();
+  };
+  for (int t = first; t < tiles; t += 2) {
+    tile(t, std::integral_constant<int, 0>{});
+    if (t + 1 < tiles) tile(t + 1, std::integral_constant<int, 1>{});
   }
   sum += other_half(sum);
   if (!live) return;
@@ -242,7 +249,7 @@ int make_params(Params &p, const void *q, const void *k, const void *v, const vo
   const int64_t most = 1 << 28;
   if (d->B < 0 || d->Lq < 0 || d->Lk < 0 || d->B > most || d->Lq > most || d->Lk > most)
     return MCX_E_SHAPE;
-  if (d->D < 1 || d->D > kMaxD || d->Hk < 1 || d->Hq < 1 || d->Hq > 65536 || d->Hq % d->Hk)
+  if (d->D < 1 || d->D > kMaxD || d->Hk < 1 || d->Hq < 1 || d->Hq > 65535 || d->Hq % d->Hk)
     return MCX_E_SHAPE;
   if (!(d->scale >= 1e-6 && d->scale <= 1e6)) return MCX_E_SHAPE;
   if (d->B && d->Lq && (!q || (d->Lk && (!k || !v)))) return MCX_E_NULL;

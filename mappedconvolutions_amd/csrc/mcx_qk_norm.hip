@@ -325,7 +325,7 @@ int norm_check(const void *q, const void *k, const void *wq, const void *wk, con
       places < 0 || !(eps >= 0))
     return MCX_E_SHAPE;
   const int64_t most = 0x7fffffffLL;
-  if (B > most || L > most || (L && B > (1LL << 40) / L) || Hq > 65536 || Hk > 65536)
+  if (B > most || L > most || (L && B > (1LL << 40) / L) || Hq > 65535 || Hk > 65535)
     return MCX_E_SHAPE;
   if (!q_stride || !k_stride || !wq || !wk) return MCX_E_NULL;
   if (B && L && (!q || !k)) return MCX_E_NULL;

@@ -341,3 +341,38 @@ def test_in_a_graph(device):
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [(1, 1100, 1000, 2, 1, 64), (1, 520, 1700, 3, 3, 40), (2, 900, 600, 2, 1, 128)])
+def test_small_grids_are_split_and_joined(device, size, dtype):
+    # fewer workgroups than compute units: parts of the keys, of the queries, some of them empty
+    args = problem(16, dtype, *size, NB=24, reach=200)
+    B, Lq, Lk = size[:3]
+    check(*args)
+    check(*args, causal=True)
+    lengths = torch.tensor([Lk // 3, 1][:B], dtype=torch.int32).cuda()
+    start = torch.tensor([Lk // 2 - Lq, -5][:B], dtype=torch.int32).cuda()
+    check(*args, causal=True, lengths=lengths, start=start)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [16, 64, 96, 128])
+def test_largest_table(device, dtype, D):
+    check(*problem(17, dtype, 1, 200, 260, 2, 1, D, NB=512, reach=300), causal=True)
+    check(*problem(18, dtype, 2, 1, 700, 40, 1, D, NB=512, reach=300), train=False)
+
+
+def test_one_bucket_and_many_runs(device):
+    # a new bucket every difference; and all differences in one, which shifts a row's scores alike
+    # (its gradient is a sum that comes to nothing, so it is not asked for)
+    q, k, v, go, table, buckets, zero = problem(19, torch.float32, 2, 250, 270, 2, 2, 32, NB=500, reach=240)
+    each = torch.arange(buckets.numel(), dtype=torch.int32).cuda()
+    check(q, k, v, go, table, each, zero)
+    want = reference(q, k, v, go=go)
+    for one, at in ((torch.full_like(buckets, 7), zero), (each[:1].clone(), 0)):
+        out, saved = _C.relative_attention_forward(q, k, v, table, one, at, for_backward=True)
+        grads = _C.relative_attention_backward(go, q, k, v, out, saved, table, one, at,
+                                               needs=(True, True, True, False))
+        for got, w in zip([out] + grads[:3], want):
+            close(got, w, TOL[torch.float32], "one bucket")
