@@ -57,7 +57,44 @@ struct Params {
   int R, zero, NB, causal;
   float scale;
   int wide;  // rows are whole 16-byte words
+  int order;  // of the work: below
+  int run;    // key heads that an XCD takes in a row
 };
+
+// Which head (of B x the call's `per_key` heads of each of Hk key heads) and which block a unit of
+// work is.  An XCD works on a run of an eighth of all units.
+//   kPlain: one head after the other, the block with the longest rows of a causal map first.
+//   kMixed: where sequences differ in length, an XCD gets every eighth run of key heads, so that all
+// have long and short ones.
+//   kTogether: and the longest blocks of all these heads come first, so that the short ones even out
+// the end.
+enum { kPlain, kMixed, kTogether };
+struct Unit {
+  int b, kh, g, block;  // key head; which of the heads that share it; block in the order of work
+};
+__device__ inline Unit unit_of(const Params &p, int unit, int per_key, int blocks) {
+  int kv, g, block;
+  if (p.order == kPlain) {
+    block = unit % blocks, unit /= blocks;
+    g = unit % per_key, kv = unit / per_key;
+  } else {
+    const int runs = p.B * p.Hk / p.run, q = runs / 8, r = runs % 8, each = per_key * blocks;
+    int xcd, in, count = (q + 1) * p.run;  // key heads of this XCD
+    if (unit < r * count * each) {
+      xcd = unit / (count * each), in = unit % (count * each);
+    } else {
+      unit -= r * count * each, count = q * p.run;
+      xcd = r + unit / (count * each), in = unit % (count * each);
+    }
+    int first = 0;
+    if (p.order == kMixed) first = in / each, in %= each, count = 1;
+    const int place = in % (count * per_key);
+    block = in / (count * per_key);
+    first += place / per_key;
+    g = place % per_key, kv = (xcd + 8 * (first / p.run)) * p.run + first % p.run;
+  }
+  return Unit{kv / p.Hk, kv % p.Hk, g, block};
+}
 
 __device__ inline int first_position(const Params &p, int b) {
   if (!p.start) return 0;
@@ -373,7 +410,20 @@ __device__ inline void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 inline bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
 // Calls f with the padded head size and whether rows are whole words, as constants.
-#define MCX_ATTENTION_DISPATCH(D, wide, F)   do {                                         if (wide) {                                  if ((D) <= 32) F(32, true);                else if ((D) <= 64) F(64, true);           else if ((D) <= 96) F(96, true);           else F(128, true);                       } else {                                     if ((D) <= 32) F(32, false);               else if ((D) <= 64) F(64, false);          else if ((D) <= 96) F(96, false);          else F(128, false);                      }                                        } while (0)
+#define MCX_ATTENTION_DISPATCH(D, wide, F)   \
+  do {                                       \
+    if (wide) {                              \
+      if ((D) <= 32) F(32, true);            \
+      else if ((D) <= 64) F(64, true);       \
+      else if ((D) <= 96) F(96, true);       \
+      else F(128, true);                     \
+    } else {                                 \
+      if ((D) <= 32) F(32, false);           \
+      else if ((D) <= 64) F(64, false);      \
+      else if ((D) <= 96) F(96, false);      \
+      else F(128, false);                    \
+    }                                        \
+  } while (0)
 
 // Checks the arguments of an entry point and fills in `p`: MCX_OK, or what is wrong with them.
 int make_params(Params &p, const void *q, const void *k, const void *v, const void *table,

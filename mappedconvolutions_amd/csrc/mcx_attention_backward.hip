@@ -115,7 +115,10 @@ __device__ inline constexpr int part_start(int n, int steps) { return 16 * n / s
 // where their 16 further steps would have taken them: lane l to lane l + 16, or, past lane 31, out at
 // step 47 - l.  The 64 diagonals that a tile finishes are added to the wave's sums per bucket.
 //   (Adding each ds to a sum in LDS costs about 3 clocks a value: 6.9 ms for 512 x 8 heads of 512 rows
-// of 64 bf16 values, which take 1.1 ms this way.)
+// of 64 bf16 values, which take 0.90 ms this way.)
+//   Bound by vector and matrix instructions that mostly take turns: these 0.90 ms are 457 TFLOP/s of
+// three products (vector instructions 48 %, matrix 25 %, LDS 30 % of the time), 16 heads of 8192 rows
+// of 128 sharing 4 take 0.96 ms, 862 TFLOP/s.
 template <typename T, int DP, bool Wide, bool Table>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void attention_query_grad_kernel(
     Params p, const T *out, const T *rest, const T *gout, const float *stats, Rows rows, T *gq, float *gq_parts,
@@ -132,9 +135,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
-  const int bh = unit / nq, b = bh / p.Hq, h = bh % p.Hq;
-  const int block = nq - 1 - unit % nq, i0 = block * kBlock;
-  const int kh = h / (p.Hq / p.Hk);
+  const Unit u0 = unit_of(p, unit, p.Hq / p.Hk, nq);
+  const int b = u0.b, kh = u0.kh, h = kh * (p.Hq / p.Hk) + u0.g, bh = b * p.Hq + h;
+  const int block = nq - 1 - u0.block, i0 = block * kBlock;
   const int start = first_position(p, b), length = key_length(p, b);
   const int local = wave * kLanesRows + (lane & 31), i = i0 + local;
   const bool live = i < p.Lq;
@@ -149,6 +152,20 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   const int64_t row = ((int64_t)b * p.Lq + i) * p.Hq + h;
   const bool biased = p.table != nullptr;
   float *sums = table + p.NB + wave * p.NB;
+
+  // the first tile is on its way while the rows' own values are loaded; none where only the
+  // statistics are asked for
+  const int base = -(start + i0 + kBlock);
+  Feed<T, DP, Wide> kt(p.ks[1], p.D, tid), vt(p.vs[1], p.D, tid);
+  int bucket = 0;
+  const int all = (keys + kTile - 1) / kTile, each = (all + parts - 1) / parts;
+  const int first = part * each, tiles = gq || Table ? min(all, first + each) : 0;  // of this part
+  if (first < tiles) {
+    const int64_t next = (int64_t)first * kTile;
+    kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[0], p.D, tid);
+    vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[0], p.D, tid);
+    if (biased) bucket = bucket_of(p, base + (int)next + tid);
+  }
 
   Frag<T> qf[Chunks], gf[Chunks];
   // delta is the diagonal of a product of the same kind as dp's: where a row's output is one of
@@ -174,9 +191,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   // (a row that nothing is left of: every difference from ref is -inf)
   float ref = kInf, log_sum = 0.f;
   const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
-  if (live && stats[2 * stat] != -kInf) {
-    ref = stats[2 * stat];
-    log_sum = __log2f(stats[2 * stat + 1]);
+  if (live) {
+    const float row_ref = stats[2 * stat], row_sum = stats[2 * stat + 1];
+    if (row_ref != -kInf) ref = row_ref, log_sum = __log2f(row_sum);
   }
   if (live && half == 0 && part == 0) {
     rows.ref[stat] = ref;
@@ -185,23 +202,12 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   }
   if (!gq && !Table) return;
 
-  const int base = -(start + i0 + kBlock);
-  if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
   if (Table) {
     for (int n = lane; n < p.NB; n += 64) sums[n] = 0.f;
     finished[wave][lane] = chain_end[wave][lane] = 0.f;
   }
-  Feed<T, DP, Wide> kt(p.ks[1], p.D, tid), vt(p.vs[1], p.D, tid);
-  int bucket = 0;
-  const int all = (keys + kTile - 1) / kTile, each = (all + parts - 1) / parts;
-  const int first = part * each, tiles = min(all, first + each);  // of this part
-  if (first < tiles) {
-    const int64_t next = (int64_t)first * kTile;
-    kt.start(k + next * p.ks[1], p.ks[1], keys - (int)next, ks[0], p.D, tid);
-    vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[0], p.D, tid);
-    if (biased) bucket = bucket_of(p, base + (int)next + tid);
-  }
-  if (!biased) clear(window, tid);
+  if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
+  else clear(window, tid);
   loads_done();
   __syncthreads();
   if (first < tiles) {
@@ -351,6 +357,10 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
 
 // Keys' and values' gradients: a workgroup holds 128 keys of a key head, a wave 32 of them as
 // columns, and walks the queries of all heads that share them, 64 at a time.
+//   Bound as the others: 512 x 8 heads of 512 rows of 64 bf16 values take 0.89 ms, 618 TFLOP/s of four
+// products (vector instructions 40 %, matrix 32 %, LDS 30 % of the time), 16 heads of 8192 rows of 128
+// sharing 4 take 1.34 ms, 818 TFLOP/s, with one wave a SIMD: two sums, the held keys and values fill
+// its registers.
 template <typename T, int DP, bool Wide>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void attention_key_grad_kernel(
     Params p, const T *gout, Rows rows, T *gk, T *gv, float *gk_parts, float *gv_parts, int nk, int parts) {
@@ -363,8 +373,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
-  const int bh = unit / nk, b = bh / p.Hk, kh = bh % p.Hk;
-  const int j0 = (unit % nk) * kBlock;  // the longest columns of a causal map first
+  const Unit u0 = unit_of(p, unit, 1, nk);
+  const int b = u0.b, kh = u0.kh;
+  const int j0 = u0.block * kBlock;  // the longest columns of a causal map first
   const int group = p.Hq / p.Hk;
   const int start = first_position(p, b), length = key_length(p, b);
   const int local = wave * kLanesRows + (lane & 31), j = j0 + local;
@@ -398,7 +409,6 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
   int bucket = 0;
   float ref = 0.f, log_sum = 0.f, delta = 0.f;
   if (!biased) clear(window, tid);
-  loads_done();
   for (int g = 0; g < group; g++) {
     const int t0 = tf + max(0, from - g * per_head), t1 = tf + min(per_head, upto - g * per_head);
     if (t0 >= t1) continue;
@@ -431,8 +441,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
         row_delta[buf][tid] = delta;
       }
     };
-    if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
     fetch(t0, 0);
+    if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
+    loads_done();
     __syncthreads();
     put(0);
     __syncthreads();

@@ -13,6 +13,10 @@ namespace attention {
 // the next tile's loads under way while the current one is multiplied.
 //   The reference is the row's maximum, but it follows it only when a score exceeds it by 2^8:
 // sums stay far inside fp32, and the accumulated output is seldom rescaled.
+//   Bound by vector and matrix instructions that mostly take turns.  512 x 8 heads of 512 rows of 64
+// bf16 values: 0.50 ms, 548 TFLOP/s, vector instructions 56 % of the time (a score's exponent,
+// maximum, sum and conversion), matrix instructions 26 %, LDS 27 %; 16 heads of 8192 rows of 128
+// sharing 4: 0.58 ms, 950 TFLOP/s, 44 and 45 %.  A large bf16 product reaches 1244 TFLOP/s.
 template <typename T, int DP, bool Wide>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void attention_forward_kernel(
     Params p, T *out, float *stats, T *rest, float *outs, float *sums, int nq, int parts) {
@@ -24,10 +28,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
-  const int bh = unit / nq, b = bh / p.Hq, h = bh % p.Hq;
-  // the longest rows of a causal map first
-  const int i0 = (nq - 1 - unit % nq) * kBlock;
-  const int kh = h / (p.Hq / p.Hk);
+  const Unit u0 = unit_of(p, unit, p.Hq / p.Hk, nq);
+  const int b = u0.b, kh = u0.kh, h = kh * (p.Hq / p.Hk) + u0.g;
+  const int i0 = (nq - 1 - u0.block) * kBlock;  // the longest rows of a causal map first
   const int start = first_position(p, b), length = key_length(p, b);
   const int local = wave * kLanesRows + (lane & 31), i = i0 + local;
   const bool live = i < p.Lq;
@@ -48,7 +51,6 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   // window value t stands for the difference (first key of the tile) - (position of query
   // i0 + kBlock) + t
   const int base = -(start + i0 + kBlock);
-  if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
   Feed<T, DP, Wide> kt(p.ks[1], p.D, tid), vt(p.vs[1], p.D, tid);
   int bucket = 0;
   const int all = (keys + kTile - 1) / kTile, each = (all + parts - 1) / parts;
@@ -59,7 +61,8 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
     vt.start(v + next * p.vs[1], p.vs[1], keys - (int)next, vs[0], p.D, tid);
     if (biased) bucket = bucket_of(p, base + (int)next + tid);
   }
-  if (!biased) clear(window, tid);
+  if (biased) load_table<T>(p, h, table, tid, 64 * kWaves);
+  else clear(window, tid);
   loads_done();
   __syncthreads();  // the table
   if (first < tiles) {
@@ -270,6 +273,17 @@ int make_params(Params &p, const void *q, const void *k, const void *v, const vo
   const int64_t per16 = dtype == MCX_BF16 ? 8 : 4;
   p.wide = wide_rows(q, p.qs, p.D, per16) && wide_rows(k, p.ks, p.D, per16) &&
            wide_rows(v, p.vs, p.D, per16);
+  // The order of the work (plain, this, in us; bf16, forward and gradients where not said): 16
+  // heads of 64 sharing 4, 4 causal sequences of 2048: 438, 379; forward over up to 2562: 100, 85;
+  // 16 x 8 heads of up to 1024 rows: 231, 168; 8 x 8 heads of up to 1024, not causal: 134, 124.
+  //   All heads of an XCD together where their keys and values fit its 4 MB of L2, since all of them
+  // are then read again and again.  8 x 32 heads of 128 sharing 8 over up to 8192: forward 4770, 4310
+  // with one key head after the other.
+  //   From 32 sequences on, an XCD's own are mixed enough, and all heads of one stay with it: their
+  // rows lie side by side (64 x 16 heads of up to 512: 520 plain, 541 with every eighth head, 513).
+  const int64_t held = ((int64_t)p.B * p.Hk + 7) / 8 * 2 * p.Lk * p.D * (16 / per16);
+  p.order = !p.causal && !p.lengths ? kPlain : p.causal && held <= (4 << 20) ? kTogether : kMixed;
+  p.run = p.B >= 32 ? p.Hk : 1;
   return MCX_OK;
 }
 

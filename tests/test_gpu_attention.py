@@ -376,3 +376,16 @@ def test_one_bucket_and_many_runs(device):
                                                needs=(True, True, True, False))
         for got, w in zip([out] + grads[:3], want):
             close(got, w, TOL[torch.float32], "one bucket")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [(3, 300, 300, 6, 3, 32), (35, 140, 150, 4, 2, 32), (5, 260, 260, 5, 1, 64),
+                                  (1, 200, 4200, 2, 1, 128)])
+def test_orders_of_work(device, size, dtype):
+    # key heads that the XCDs share unevenly, one and several in a row, more than an L2 holds
+    B, Lk = size[0], size[2]
+    args = problem(21, dtype, *size)
+    lengths = torch.tensor([Lk - 37 * b % Lk for b in range(B)], dtype=torch.int32).cuda()
+    start = torch.full((B,), Lk - size[1], dtype=torch.int32).cuda()
+    check(*args, lengths=lengths)
+    check(*args, causal=True, lengths=lengths, start=start)
