@@ -456,6 +456,7 @@ typedef struct mcx_attention_desc {
  *   out [B, Lq, Hq, D] contiguous; for the gradients, or NULL: stats float [B, Hq, Lq, 2] (a row's
  *   reference and sum), and for bf16 out_rest, like out: what rounding took from it.
  * A row that nothing is left of is zeros.  What lies at keys from key_lengths[b] on is not read.
+ * (Keys in use have to be finite: a value of probability zero is still a factor.)
  * A bucket outside [0, table_size) has no bias; a bias of -inf takes its pairs out; a finite bias
  * is held within 1e30.
  * Few queries against many keys are split over the keys and joined; that takes a workspace of

@@ -936,8 +936,7 @@ def qk_norm_rotate_forward(query, key, query_weight, key_weight, cos, sin, posit
     A position outside the places gives NaN."""
     dt, B, L, Hq, Hk, D, query, key, cos, sin, positions = _norm_args(
         query, key, query_weight, key_weight, cos, sin, positions, eps)
-    q_out = torch.empty((B, L, Hq, D), dtype=query.dtype, device=query.device)
-    k_out = torch.empty((B, L, Hk, D), dtype=query.dtype, device=query.device)
+    q_out, k_out = query.new_empty((B, L, Hq, D)), query.new_empty((B, L, Hk, D))
     with _device(query):
         rc = _lib.load().mcx_qk_norm_rotate_forward(
             _ptr(query), _ptr(key), _ptr(query_weight), _ptr(key_weight), _ptr(cos), _ptr(sin),
@@ -1040,7 +1039,7 @@ def relative_attention_forward(query, key, value, bias_table=None, buckets=None,
                                         causal, query_start, key_lengths)
     query = tensors[0]
     B, Lq, Hq, D = query.shape
-    out = torch.empty((B, Lq, Hq, D), dtype=query.dtype, device=query.device)
+    out = query.new_empty((B, Lq, Hq, D))
     stats = rest = None
     if for_backward:
         stats = torch.empty((B, Hq, Lq, 2), dtype=torch.float32, device=query.device)
