@@ -47,9 +47,9 @@ class RelativeAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, query, key, value, table, buckets, zero, scale, causal, query_start,
-                key_lengths):
+                key_lengths, recording):
         ctx.args = dict(bucket_zero=zero, scale=scale, causal=causal)
-        training = any(ctx.needs_input_grad[:4])
+        training = recording and any(ctx.needs_input_grad[:4])
         out, saved = _C.relative_attention_forward(
             query, key, value, table, buckets, query_start=query_start, key_lengths=key_lengths,
             for_backward=training, **ctx.args)
@@ -65,7 +65,7 @@ class RelativeAttentionFunction(torch.autograd.Function):
         grads = _C.relative_attention_backward(
             grad_output, query, key, value, out, saved, table, buckets, query_start=start,
             key_lengths=lengths, needs=needs, **ctx.args)
-        return tuple(grads) + (None,) * 6
+        return tuple(grads) + (None,) * 7
 
 
 class RelativeAttention(nn.Module):
@@ -93,4 +93,5 @@ class RelativeAttention(nn.Module):
         -> [B, Lq, H, D]."""
         table = None if self.table is None else self.table.to(query.dtype)
         return RelativeAttentionFunction.apply(query, key, value, table, self.buckets, self.zero,
-                                               self.scale, self.causal, query_start, key_lengths)
+                                               self.scale, self.causal, query_start, key_lengths,
+                                               torch.is_grad_enabled())

@@ -116,3 +116,20 @@ def test_example_serves(device, dtype):
     # up to 4, after a product over 128 channels that may turn one rounding into another)
     bound = 1e-4 if dtype == torch.float32 else 6e-2
     assert (whole - one_by_one).abs().max().item() <= bound
+
+
+def test_nothing_is_saved_without_a_graph(device, monkeypatch):
+    asked, forward = [], _C.relative_attention_forward
+
+    def watched(*args, for_backward=False, **kw):
+        asked.append(for_backward)
+        return forward(*args, for_backward=for_backward, **kw)
+
+    monkeypatch.setattr(_C, "relative_attention_forward", watched)
+    buckets, zero = util.distance_buckets(8, reach=20)
+    layer = nn.RelativeAttention(2, buckets, zero).to(device)
+    q = torch.randn(1, 9, 2, 16, device=device)
+    with torch.no_grad():
+        served = layer(q, q, q)
+    assert torch.equal(layer(q, q, q), served)
+    assert asked == [False, True]
