@@ -349,6 +349,11 @@ int split_parts(const Params &p, int dtype) {
   // least 2048 keys even out the last round (64 bf16 tokens over up to 8192 keys of 8 heads: 368,
   // 338, 319 us with one, two, four parts).
   const int64_t tiles = (p.Lk + kWaves * kStep - 1) / (kWaves * kStep);
+  // A short cache takes less time in one part than the join's launch (one token, 8 heads, a call
+  // through the binding, one part and split, in us): bf16, 1000 keys of 64 14.3, 18.9; 500 of 128
+  // 15.3, 18.9; 1000 of 128 19.6, 19.1; 2000 of 64 21.0, 18.9; fp32, 256 of 64 14.1, 18.7; 500 of 64
+  // 19.1, 18.8; 1000 of 64 30.0, 18.9.
+  if ((int64_t)p.Lk * p.D <= (dtype == MCX_BF16 ? 64 << 10 : 16 << 10)) return 1;
   const int64_t parts = units < 256 ? std::min<int64_t>((256 + units - 1) / units, tiles)
                                     : std::min<int64_t>((2048 + units - 1) / units, p.Lk / 2048);
   return (int)std::max<int64_t>(1, std::min<int64_t>(parts, kMostParts));
