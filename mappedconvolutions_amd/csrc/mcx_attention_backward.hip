@@ -534,15 +534,29 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
   }
 }
 
-// The sum of a gradient's parts, in order.
+// The sums of up to three gradients' parts, each in order.
+struct PartSums {
+  const float *parts[3];
+  void *to[3];
+  int64_t size[3];
+  unsigned first[4];  // workgroups before each
+  int count[3], n;
+  void add(const float *from, void *gradient, int64_t values, int parts_of_it) {
+    parts[n] = from, to[n] = gradient, size[n] = values, count[n] = parts_of_it;
+    first[n + 1] = first[n] + (unsigned)((values + 255) / 256);
+    n++;
+  }
+};
 template <typename T>
-__global__ __launch_bounds__(256) void attention_sum_parts_kernel(const float *parts, T *to,
-                                                                  int64_t size, int count) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void attention_sum_parts_kernel(PartSums sums) {
+  int s = 0;
+  while (s + 1 < sums.n && blockIdx.x >= sums.first[s + 1]) s++;
+  const int64_t size = sums.size[s], i = (int64_t)(blockIdx.x - sums.first[s]) * 256 + threadIdx.x;
   if (i >= size) return;
+  const float *parts = sums.parts[s];
   float x = parts[i];
-  for (int n = 1; n < count; n++) x += parts[n * size + i];
-  to[i] = (T)x;
+  for (int n = 1; n < sums.count[s]; n++) x += parts[n * size + i];
+  ((T *)sums.to[s])[i] = (T)x;
 }
 
 // Sums per bucket of a head, in a fixed order.  Of `rows` sums of a head ([B][Hq][nq] with rows =
@@ -597,14 +611,6 @@ static Plan plan_of(const Params &p) {
 }
 
 template <typename T>
-static int sum_parts(const float *parts, void *to, int64_t size, int count, hipStream_t stream) {
-  hipLaunchKernelGGL((attention_sum_parts_kernel<T>), dim3((unsigned)((size + 255) / 256)), dim3(256),
-                     0, stream, parts, (T *)to, size, count);
-  MCX_HIP_CHECK_LAUNCH();
-  return MCX_OK;
-}
-
-template <typename T>
 static int launch_backward(const Params &p, const Plan &n, const void *gout, const void *out,
                            const void *rest, const float *stats, void *gq, void *gk, void *gv, void *gtable, char *ws,
                            hipStream_t stream) {
@@ -613,6 +619,7 @@ static int launch_backward(const Params &p, const Plan &n, const void *gout, con
   float *q_parts = (float *)(ws + n.q_at);
   float *k_parts = (float *)(ws + n.k_at), *v_parts = (float *)(ws + n.v_at);
   const dim3 threads(64 * kWaves);
+  PartSums sums = {};
   if (n.q_units) {
     const int parts = gq || gtable ? n.q_parts : 1;
     const dim3 grid((unsigned)(n.q_units * parts));
@@ -628,10 +635,7 @@ static int launch_backward(const Params &p, const Plan &n, const void *gout, con
                            MCX_GRAD);
 #undef MCX_GRAD
     MCX_HIP_CHECK_LAUNCH();
-    if (gq && parts > 1) {
-      const int rc = sum_parts<T>(q_parts, gq, (int64_t)p.B * p.Lq * p.Hq * p.D, parts, stream);
-      if (rc != MCX_OK) return rc;
-    }
+    if (gq && parts > 1) sums.add(q_parts, gq, (int64_t)p.B * p.Lq * p.Hq * p.D, parts);
   }
   if (gtable) {
     const int64_t count = (int64_t)p.B * n.nq * n.q_parts;
@@ -659,10 +663,14 @@ static int launch_backward(const Params &p, const Plan &n, const void *gout, con
     MCX_HIP_CHECK_LAUNCH();
     if (n.k_parts > 1) {
       const int64_t size = (int64_t)p.B * p.Lk * p.Hk * p.D;
-      int rc = gk ? sum_parts<T>(k_parts, gk, size, n.k_parts, stream) : MCX_OK;
-      if (rc == MCX_OK && gv) rc = sum_parts<T>(v_parts, gv, size, n.k_parts, stream);
-      if (rc != MCX_OK) return rc;
+      if (gk) sums.add(k_parts, gk, size, n.k_parts);
+      if (gv) sums.add(v_parts, gv, size, n.k_parts);
     }
+  }
+  if (sums.n) {
+    hipLaunchKernelGGL((attention_sum_parts_kernel<T>), dim3(sums.first[sums.n]), dim3(256), 0, stream,
+                       sums);
+    MCX_HIP_CHECK_LAUNCH();
   }
   return MCX_OK;
 }
