@@ -598,7 +598,16 @@ static Plan plan_of(const Params &p) {
   n.q_units = (int64_t)p.B * p.Hq * n.nq, n.k_units = (int64_t)p.B * p.Hk * n.nk;
   const int64_t q_tiles = (p.Lq + kTile - 1) / kTile, k_tiles = (p.Lk + kTile - 1) / kTile;
   n.q_parts = n.q_units ? parts_of(n.q_units, k_tiles) : 1;
-  n.k_parts = n.k_units ? parts_of(n.k_units, q_tiles * (p.Hq / p.Hk)) : 1;
+  n.k_parts = 1;
+  if (n.k_units) {
+    n.k_parts = parts_of(n.k_units, q_tiles * (p.Hq / p.Hk));
+    // The key kernel mostly has a compute unit's registers for itself: parts of the same length in
+    // one round (256 workgroups at most instead of 384 at least, forward and gradients in us: 2562
+    // bf16 rows of 4 heads of 128 sharing one 158, 179; 2 x 1000 float32 rows of 8 heads of 32 148,
+    // 163).  A causal map's parts differ, and more of them even out (3000 bf16 rows of 8 heads of 128
+    // sharing 4 279, 266).
+    if (!p.causal) n.k_parts = std::max(1, std::min(n.k_parts, (int)(256 / n.k_units)));
+  }
   const size_t rows = (size_t)p.B * p.Hq * p.Lq, keys = (size_t)p.B * p.Hk * p.Lk, f = sizeof(float);
   n.rows_at = align256(rows * f);
   n.partial_at = n.rows_at + 2 * align256(rows * f);
