@@ -37,7 +37,8 @@ constexpr int kMaxTable = 512;     // buckets of a head: their values and sums s
 // A finite bias is held within this: its sum with a score then swallows the score, as the
 // lowest value of the type does, and neither the scale nor log2(e) takes it to infinity.
 constexpr float kBiasLimit = 1e30f;
-// Where a row's statistic is beyond this, one fma no longer holds the difference in the exponent.
+// The forward kernel's exponents share an error of half a unit in the last place of a row's reference
+// (32 here): beyond this it could take sums out of fp32, and differences are formed first.
 constexpr float kHugeStat = 1e9f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();

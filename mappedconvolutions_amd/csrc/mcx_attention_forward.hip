@@ -8,11 +8,21 @@
 namespace mcx {
 namespace attention {
 
+// What rounding takes from ref c (0 where the difference from ref is formed first).
+__device__ inline float residue_of(float ref, float c) {
+  const float shift = ref * c;
+  return fabsf(shift) > kHugeStat ? 0.f : fmaf(ref, c, -shift);
+}
+
 // One pass over the keys with a running reference and sum (both fp32): a workgroup holds 128
 // queries of one head, a wave 32 of them, and walks the keys 64 at a time through two LDS buffers,
 // the next tile's loads under way while the current one is multiplied.
 //   The reference is the row's maximum, but it follows it only when a score exceeds it by 2^8:
 // sums stay far inside fp32, and the accumulated output is seldom rescaled.
+//   Exponents are one fma, u c - shift, with shift = ref c rounded: against u - ref they are off by
+// residue = ref c - shift, the same for all keys.  It grows with the reference (0.03 at 10^6), so it is
+// taken account of where references meet: when one moves, and in the sum that the gradients and the
+// joining of parts take together with the reference itself.
 //   Bound by vector and matrix instructions that mostly take turns.  512 x 8 heads of 512 rows of 64
 // bf16 values: 0.50 ms, 548 TFLOP/s, vector instructions 56 % of the time (a score's exponent,
 // maximum, sum and conversion), matrix instructions 26 %, LDS 27 %; 16 heads of 8192 rows of 128
@@ -110,7 +120,8 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
     top = fmaxf(top, other_half(top));
     if (__any((top - ref) * c > 8.f)) {  // (-inf against -inf is no number: not above)
       const float next = fmaxf(ref, top);
-      const float keep = next == -kInf ? 1.f : exp2_fast((ref - next) * c);
+      const float moved = residue_of(next, c) - residue_of(ref, c);
+      const float keep = next == -kInf ? 1.f : exp2_fast(fmaf(ref - next, c, moved));
       ref = next;
       sum *= keep;
 #pragma unroll
@@ -118,10 +129,11 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
     }
     const float used = ref == -kInf ? 0.f : ref;
     if (__any(fabsf(used) * c > kHugeStat)) {
+      const float residue = residue_of(used, c);
 #pragma unroll
       for (int blk = 0; blk < 2; blk++)
 #pragma unroll
-        for (int n = 0; n < 16; n++) u[blk][n] = exp2_fast((u[blk][n] - used) * c);
+        for (int n = 0; n < 16; n++) u[blk][n] = exp2_fast(fmaf(u[blk][n] - used, c, residue));
     } else {
       const float shiftc = -used * c;
 #pragma unroll
@@ -158,9 +170,10 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   if (!live) return;
   const int64_t row = ((int64_t)b * p.Lq + i) * p.Hq + h;
   const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
+  const float of_ref = exp2_fast(-residue_of(ref, c));
   if (parts > 1) {
     const int64_t rows = (int64_t)p.B * p.Lq * p.Hq;
-    store_column<Wide, float, Blocks>(outs + (part * rows + row) * p.D, o, 1.f, p.D, half);
+    store_column<Wide, float, Blocks>(outs + (part * rows + row) * p.D, o, of_ref, p.D, half);
     stats = sums + part * rows * 2;
   } else {
     store_column<Wide, T, Blocks>(out + row * p.D, o, sum == 0.f ? 0.f : 1.f / sum, p.D, half,
@@ -168,7 +181,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   }
   if (stats && half == 0) {
     stats[2 * stat] = ref;
-    stats[2 * stat + 1] = sum;
+    stats[2 * stat + 1] = sum * of_ref;
   }
 }
 

@@ -389,3 +389,85 @@ def test_orders_of_work(device, size, dtype):
     start = torch.full((B,), Lk - size[1], dtype=torch.int32).cuda()
     check(*args, lengths=lengths)
     check(*args, causal=True, lengths=lengths, start=start)
+
+
+# ---- rows whose largest score is far from zero ----------------------------------------------
+# Zero queries (or whole numbers) make every score exact in both types, however large the bias, so the
+# tolerances above hold: what is left are the roundings of exponents of size one, of sums and products.
+
+FAR = [
+    # B, Lq, Lk, Hq, Hk, D: as many workgroups as compute units, and few, split along both axes
+    (64, 130, 130, 4, 2, 64),
+    (1, 260, 700, 2, 1, 64),
+    (1, 260, 700, 2, 1, 48),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", FAR)
+@pytest.mark.parametrize("bias", [-1e3, -1e4, -1e6, -1e8, -6e8, 3e4])
+def test_rows_under_one_large_bias(device, size, bias, dtype):
+    q, k, v, go, table, buckets, zero = problem(30, dtype, *size)
+    table = torch.full_like(table, bias)
+    check(torch.zeros_like(q), k, v, go, table, buckets, zero)
+    check(torch.zeros_like(q), k, v, go, table, buckets, zero, causal=True)
+
+
+@pytest.mark.parametrize("size", FAR[:2])
+@pytest.mark.parametrize("bias", [-1e3, -1e4, -1e6])
+def test_differences_of_large_biases(device, size, bias):
+    # (whole numbers: exact over the scale of 2^-3) the largest of a row lies in any of its tiles
+    q, k, v, go, table, buckets, zero = problem(31, torch.float32, *size, NB=64)
+    table = bias + torch.arange(64, device="cuda", dtype=torch.float32).div(8).floor().expand(size[3], 64)
+    check(torch.zeros_like(q), k, v, go, table, buckets, zero)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", FAR[:2])
+def test_large_scores(device, size, dtype):
+    # one value of 2^13 in every query makes scores of 1024 and a little; quarters: exact products
+    q, k, v, go, table, buckets, zero = problem(32, dtype, *size)
+    q, k = ((4 * t).round().clamp(-12, 12) / 4 for t in (q, k))
+    q[..., 0], k[..., 0] = 8192, 1
+    check(q, k, v, go, torch.zeros_like(table), buckets, zero)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("near", [0.0, -1e6, -6e8])
+def test_rows_of_different_size_in_a_wave(device, near, dtype):
+    # ten keys in use: the first rows see them under one bias, the last under the lowest value, those
+    # between under both
+    q, k, v, go, _, _, _ = problem(33, dtype, 2, 150, 600, 2, 1, 64)
+    buckets = torch.zeros(41, dtype=torch.int32, device="cuda")
+    buckets[:5] = 1  # differences of -16 and less
+    table = torch.tensor([near, torch.finfo(dtype).min]).to(dtype).cuda().expand(2, 2)
+    lengths = torch.tensor([10, 333], dtype=torch.int32).cuda()
+    # (a row sees one bucket or two of which one takes all: the table's gradient is a sum that comes to
+    # nothing, so it is not asked for)
+    q = torch.zeros_like(q)
+    want = reference(q, k, v, table, buckets, 20, lengths=lengths, go=go)
+    args = dict(bias_table=table, buckets=buckets, bucket_zero=20, key_lengths=lengths)
+    out, saved = _C.relative_attention_forward(q, k, v, for_backward=True, **args)
+    grads = _C.relative_attention_backward(go, q, k, v, out, saved, needs=(True, True, True, False), **args)
+    for got, w in zip([out] + grads[:3], want):
+        close(got, w, TOL[dtype], "two sizes")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", FAR)
+@pytest.mark.parametrize("bias", [0.0, -1e4, -1e6, -1e8, -6e8, -1e12])
+def test_probabilities_of_the_gradients_sum_to_one(device, size, bias, dtype):
+    # whatever a large bias leaves of the scores: sum_j grad_value_j = sum_i grad_output_i
+    q, k, v, go, table, buckets, zero = problem(34, dtype, *size)
+    Hq, Hk = size[3:5]
+    want = go.double().sum(1).unflatten(1, (Hk, Hq // Hk)).sum(2)
+    bound = TOL[dtype] * go.double().abs().sum(1).max().item()
+    for n in (size[1], 1):
+        if n == 1:  # the form for few queries
+            go = go[:, :1].contiguous()
+            want = go.double().sum(1).unflatten(1, (Hk, Hq // Hk)).sum(2)
+            bound = TOL[dtype] * go.double().abs().max().item()
+        args = (torch.full_like(table, bias), buckets, zero)
+        out, saved = _C.relative_attention_forward(q[:, :n], k, v, *args, for_backward=True)
+        gv = _C.relative_attention_backward(go, q[:, :n], k, v, out, saved, *args)[2]
+        assert ((gv.double().sum(1) - want).abs() <= bound).all()
