@@ -17,6 +17,8 @@
 // their lane, and neighbouring lanes hold neighbouring diagonals.
 #pragma once
 
+#include <algorithm>
+
 #include "mcx_mfma_common.h"
 
 namespace mcx {
@@ -60,6 +62,7 @@ struct Params {
   int wide;  // rows are whole 16-byte words
   int order;  // of the work: below
   int run;    // key heads that an XCD takes in a row
+  int first;  // workgroup of a call that a launch begins with: below
 };
 
 // Which head (of B x the call's `per_key` heads of each of Hk key heads) and which block a unit of
@@ -425,6 +428,23 @@ inline bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
       else F(128, false);                    \
     }                                        \
   } while (0)
+
+// A launch has at most 2^32 threads: more than a quarter of them go into launches of their own.
+// Calls f(the launch's parameters, its workgroups).
+constexpr int64_t kMostGroups = (int64_t)1 << 22;
+template <typename F> int launch_in_pieces(const Params &p, int64_t groups, F f) {
+  Params piece = p;
+  for (int64_t first = 0; first < groups; first += kMostGroups) {
+    piece.first = (int)first;
+    f(piece, dim3((unsigned)std::min(groups - first, kMostGroups)));
+    MCX_HIP_CHECK_LAUNCH();
+  }
+  return MCX_OK;
+}
+// The workgroup of the call that this one is.
+__device__ inline int group_of_call(const Params &p) {
+  return p.first + xcd_contiguous_tile(blockIdx.x, gridDim.x);
+}
 
 // Checks the arguments of an entry point and fills in `p`: MCX_OK, or what is wrong with them.
 int make_params(Params &p, const void *q, const void *k, const void *v, const void *table,

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   extern __shared__ float table[];  // NB values, then kWaves x NB sums
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
+  const int wg = group_of_call(p), part = wg % parts, unit = wg / parts;
   const Unit u0 = unit_of(p, unit, p.Hq / p.Hk, nq);
   const int b = u0.b, kh = u0.kh, h = kh * (p.Hq / p.Hk) + u0.g, bh = b * p.Hq + h;
   const int block = nq - 1 - u0.block, i0 = block * kBlock;
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(6))) void atten
   extern __shared__ float table[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
+  const int wg = group_of_call(p), part = wg % parts, unit = wg / parts;
   const Unit u0 = unit_of(p, unit, 1, nk);
   const int b = u0.b, kh = u0.kh;
   const int j0 = u0.block * kBlock;  // the longest columns of a causal map first
@@ -631,19 +631,20 @@ static int launch_backward(const Params &p, const Plan &n, const void *gout, con
   PartSums sums = {};
   if (n.q_units) {
     const int parts = gq || gtable ? n.q_parts : 1;
-    const dim3 grid((unsigned)(n.q_units * parts));
     const size_t lds = (gtable ? 1 + kWaves : 1) * p.NB * sizeof(float);
+    const int rc = launch_in_pieces(p, n.q_units * parts, [&](const Params &piece, dim3 grid) {
 #define MCX_GRAD(DP, W)                                                                           \
   hipLaunchKernelGGL((gtable ? attention_query_grad_kernel<T, DP, W, true>                        \
                              : attention_query_grad_kernel<T, DP, W, false>), grid, threads, lds, \
-                     stream, p,                                                                   \
+                     stream, piece,                                                               \
                      (const T *)out, (const T *)rest, (const T *)gout, stats, rows, (T *)gq,       \
                      q_parts,                                                                     \
                      gtable ? partial : nullptr, (int)n.nq, parts)
-    MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out) && aligned16(rest) && aligned16(gout) && aligned16(gq),
-                           MCX_GRAD);
+      MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out) && aligned16(rest) && aligned16(gout) && aligned16(gq),
+                             MCX_GRAD);
 #undef MCX_GRAD
-    MCX_HIP_CHECK_LAUNCH();
+    });
+    if (rc != MCX_OK) return rc;
     if (gq && parts > 1) sums.add(q_parts, gq, (int64_t)p.B * p.Lq * p.Hq * p.D, parts);
   }
   if (gtable) {
@@ -661,15 +662,16 @@ static int launch_backward(const Params &p, const Plan &n, const void *gout, con
     MCX_HIP_CHECK_LAUNCH();
   }
   if ((gk || gv) && n.k_units) {
-    const dim3 grid((unsigned)(n.k_units * n.k_parts));
     const size_t lds = p.NB * sizeof(float);
-#define MCX_GRAD(DP, W)                                                                      \
-  hipLaunchKernelGGL((attention_key_grad_kernel<T, DP, W>), grid, threads, lds, stream, p,    \
-                     (const T *)gout, rows, (T *)gk, (T *)gv, k_parts, v_parts,                \
+    const int rc = launch_in_pieces(p, n.k_units * n.k_parts, [&](const Params &piece, dim3 grid) {
+#define MCX_GRAD(DP, W)                                                                         \
+  hipLaunchKernelGGL((attention_key_grad_kernel<T, DP, W>), grid, threads, lds, stream, piece,   \
+                     (const T *)gout, rows, (T *)gk, (T *)gv, k_parts, v_parts,                   \
                      (int)n.nk, n.k_parts)
-    MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(gout) && aligned16(gk) && aligned16(gv), MCX_GRAD);
+      MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(gout) && aligned16(gk) && aligned16(gv), MCX_GRAD);
 #undef MCX_GRAD
-    MCX_HIP_CHECK_LAUNCH();
+    });
+    if (rc != MCX_OK) return rc;
     if (n.k_parts > 1) {
       const int64_t size = (int64_t)p.B * p.Lk * p.Hk * p.D;
       if (gk) sums.add(k_parts, gk, size, n.k_parts);

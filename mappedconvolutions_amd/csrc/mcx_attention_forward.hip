@@ -37,7 +37,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
   extern __shared__ float table[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-  const int wg = xcd_contiguous_tile(blockIdx.x, gridDim.x), part = wg % parts, unit = wg / parts;
+  const int wg = group_of_call(p), part = wg % parts, unit = wg / parts;
   const Unit u0 = unit_of(p, unit, p.Hq / p.Hk, nq);
   const int b = u0.b, kh = u0.kh, h = kh * (p.Hq / p.Hk) + u0.g;
   const int i0 = (nq - 1 - u0.block) * kBlock;  // the longest rows of a causal map first
@@ -227,17 +227,19 @@ template <typename T>
 static int launch_forward(const Params &p, void *out, float *stats, void *rest, void *workspace,
                           hipStream_t stream) {
   const int nq = (p.Lq + kBlock - 1) / kBlock, parts = forward_parts(p);
-  const dim3 grid((unsigned)(query_units(p) * parts)), threads(64 * kWaves);
+  const dim3 threads(64 * kWaves);
   const int64_t rows = (int64_t)p.B * p.Hq * p.Lq;
   float *sums = (float *)workspace;
   float *outs = (float *)((char *)workspace + align256((size_t)rows * parts * 2 * sizeof(float)));
   const size_t lds = p.table ? p.NB * sizeof(float) : 0;
-#define MCX_FORWARD(DP, W)                                                                     \
-  hipLaunchKernelGGL((attention_forward_kernel<T, DP, W>), grid, threads, lds, stream, p, (T *)out, \
+  const int rc = launch_in_pieces(p, query_units(p) * parts, [&](const Params &piece, dim3 grid) {
+#define MCX_FORWARD(DP, W)                                                                          \
+  hipLaunchKernelGGL((attention_forward_kernel<T, DP, W>), grid, threads, lds, stream, piece, (T *)out, \
                      stats, (T *)rest, outs, sums, nq, parts)
-  MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out) && aligned16(rest), MCX_FORWARD);
+    MCX_ATTENTION_DISPATCH(p.D, p.wide && aligned16(out) && aligned16(rest), MCX_FORWARD);
 #undef MCX_FORWARD
-  MCX_HIP_CHECK_LAUNCH();
+  });
+  if (rc != MCX_OK) return rc;
   if (parts > 1) {
     hipLaunchKernelGGL((attention_join_values_kernel<T>), dim3((unsigned)((rows * p.D + 255) / 256)),
                        dim3(256), 0, stream, p, outs, sums, (T *)out, stats, (T *)rest, parts);
@@ -297,6 +299,7 @@ int make_params(Params &p, const void *q, const void *k, const void *v, const vo
   const int64_t held = ((int64_t)p.B * p.Hk + 7) / 8 * 2 * p.Lk * p.D * (16 / per16);
   p.order = !p.causal && !p.lengths ? kPlain : p.causal && held <= (4 << 20) ? kTogether : kMixed;
   p.run = p.B >= 32 ? p.Hk : 1;
+  p.first = 0;
   return MCX_OK;
 }
 

@@ -342,7 +342,7 @@ int split_parts(const Params &p, int dtype) {
   const int64_t there = (int64_t)p.Hq * ((p.Lq + kBlock - 1) / kBlock) * kWaves *
                         ((p.Lk + kTile - 1) / kTile) * kTile;
   if ((dtype == MCX_BF16 ? 6 : 3) * here > 2 * there) return 0;
-  if (units > (1 << 24)) return 0;
+  if (units >= (1 << 24)) return 0;  // (more threads than a launch has)
   // One workgroup for every compute unit where there are fewer units of work: more parts cost more
   // in their ends and in the join than they win (one bf16 token over 20000 keys of 8 heads of 128:
   // 23.0, 25.8, 33.5 us with 256, 512, 1024 workgroups in all).  Where there are enough, parts of at

@@ -471,3 +471,23 @@ def test_probabilities_of_the_gradients_sum_to_one(device, size, bias, dtype):
         out, saved = _C.relative_attention_forward(q[:, :n], k, v, *args, for_backward=True)
         gv = _C.relative_attention_backward(go, q[:, :n], k, v, out, saved, *args)[2]
         assert ((gv.double().sum(1) - want).abs() <= bound).all()
+
+
+def test_more_workgroups_than_a_launch_takes(device):
+    # 2^24 workgroups of 256 threads are one thread more than a launch can have
+    if torch.cuda.mem_get_info()[0] < 32 << 30:
+        pytest.skip("needs 32 GB")
+    B, H, D = (1 << 20) + 3, 16, 8
+    g = torch.Generator(device="cuda").manual_seed(50)
+    q, k, v, go = (torch.randn(B, 2, H, D, generator=g, device="cuda").bfloat16() for _ in range(4))
+    table = torch.randn(H, 3, generator=g, device="cuda").bfloat16()
+    buckets = torch.arange(3, dtype=torch.int32, device="cuda")
+    args = dict(bias_table=table, buckets=buckets, bucket_zero=1)
+    out, saved = _C.relative_attention_forward(q, k, v, for_backward=True, **args)
+    gq, gk, gv, _ = _C.relative_attention_backward(go, q, k, v, out, saved, needs=(True, True, True, False),
+                                                   **args)
+    for at in (0, 1 << 18, 1 << 19, (1 << 20) - 2, B - 4):
+        part = slice(at, at + 4)
+        want = reference(q[part], k[part], v[part], table, buckets, 1, go=go[part])
+        for got, w, name in zip((out, gq, gk, gv), want, ("out", "grad_query", "grad_key", "grad_value")):
+            close(got[part], w, TOL[torch.bfloat16], name)
