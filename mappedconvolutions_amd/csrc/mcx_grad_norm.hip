@@ -34,36 +34,50 @@ struct List {
 
 template <typename T> __device__ inline float value(T x) { return (float)x; }
 
-// Calls f(first value, count in 16 bytes) over a chunk: whole words where the address allows it.
+// What a workgroup does to values [lo, hi) of a tensor, in 16-byte words where the address allows it.
 template <typename T> struct Chunk {
   static constexpr int E = 16 / (int)sizeof(T);
   typedef __attribute__((ext_vector_type(E))) T Vec;
 
-  static __device__ inline float squares(const T *x, int64_t lo, int64_t hi) {
+  // This thread's part of the sum of squares, in A; the bits that any of its values has go to `bits`.
+  template <typename A>
+  static __device__ inline A squares(const T *x, int64_t lo, int64_t hi, unsigned &bits) {
+    typedef __attribute__((ext_vector_type(4))) unsigned Words;
     const int tid = threadIdx.x;
     // values before the first whole word, and behind the last
     const int64_t skew = (int64_t)(((uintptr_t)(x + lo) & 15) / sizeof(T));
     const int64_t a = min(hi, lo + (skew ? E - skew : 0)), z = a + (hi - a) / E * E;
-    float s = 0.f;
-    for (int64_t i = lo + tid; i < a; i += kThreads) s = fmaf(value(x[i]), value(x[i]), s);
-    for (int64_t i = z + tid; i < hi; i += kThreads) s = fmaf(value(x[i]), value(x[i]), s);
-    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    A s = 0, t[4] = {0, 0, 0, 0};
+    const auto one = [&](T v) {
+      s = fma((A)value(v), (A)value(v), s);
+      bits |= __float_as_uint(value(v));
+    };
+    const auto word = [&](const Vec &v, A &sum) {
+#pragma unroll
+      for (int e = 0; e < E; e++) sum = fma((A)value(v[e]), (A)value(v[e]), sum);
+      const Words w = __builtin_bit_cast(Words, v);
+      bits |= w[0] | w[1] | w[2] | w[3];
+    };
+    for (int64_t i = lo + tid; i < a; i += kThreads) one(x[i]);
+    for (int64_t i = z + tid; i < hi; i += kThreads) one(x[i]);
     int64_t i = a + tid * E;
     for (; i + 3 * kThreads * E < z; i += 4 * kThreads * E) {
       Vec v[4];
 #pragma unroll
       for (int n = 0; n < 4; n++) v[n] = *(const Vec *)(x + i + n * kThreads * E);
 #pragma unroll
-      for (int n = 0; n < 4; n++)
-#pragma unroll
-        for (int e = 0; e < E; e++) t[n] = fmaf(value(v[n][e]), value(v[n][e]), t[n]);
+      for (int n = 0; n < 4; n++) word(v[n], t[n]);
     }
-    for (; i < z; i += kThreads * E) {
-      const Vec v = *(const Vec *)(x + i);
-#pragma unroll
-      for (int e = 0; e < E; e++) s = fmaf(value(v[e]), value(v[e]), s);
-    }
+    for (; i < z; i += kThreads * E) word(*(const Vec *)(x + i), s);
     return s + (t[0] + t[1]) + (t[2] + t[3]);
+  }
+  // In fp32 (a few hundred squares at most), and again in fp64 where that overflows (a value beyond
+  // 10^19) or is so small that squares may be lost below it.
+  static __device__ inline double squares(const T *x, int64_t lo, int64_t hi) {
+    unsigned bits = 0;
+    const float s = squares<float>(x, lo, hi, bits);
+    if ((s >= 0x1p-90f && s < __builtin_inff()) || !bits) return s;
+    return squares<double>(x, lo, hi, bits);
   }
 
   template <bool Passing>
@@ -119,8 +133,7 @@ __device__ inline double block_sum(double x) {
   return x;
 }
 
-// A thread's squares of a chunk are summed in fp32 (a few hundred at most), everything else in
-// fp64.
+// A thread's squares of a chunk are summed in fp32 where it holds them, everything else in fp64.
 __global__ __launch_bounds__(kThreads) void grad_squares_kernel(List l, double *sums) {
   double s = 0.;
   const int chunks = l.first[l.count];

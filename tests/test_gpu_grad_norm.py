@@ -129,3 +129,28 @@ def test_in_a_graph(device):
         for a, b in zip(eager, out):
             assert torch.equal(a, b)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("size", [1e25, 1e18, 1e-18, 1e-25, 1e-30])
+def test_values_whose_squares_leave_fp32(device, size, dtype):
+    # (values a thread walks in words, those before and behind them, and a part of zeros)
+    ts = [(size * t.double()).to(dtype) for t in tensors(8, [3, 5001, 300000], (dtype,))]
+    ts.insert(1, torch.zeros(70000, dtype=dtype, device="cuda"))
+    ts = [torch.cat((t[:1], t))[1:] for t in ts]
+    wide = [t.double().cpu() for t in ts]
+    norm = torch.sqrt(sum((t * t).sum() for t in wide)).item()
+    out = [torch.empty_like(t) for t in ts]
+    got = _C.clip_grad_norm(ts, 0.25 * norm, eps=0.0, out=out)
+    assert abs(got.item() - norm) <= 1e-6 * norm
+    for o, t in zip(out, wide):
+        off = (o.double().cpu() - 0.25 * t).abs()
+        assert (off <= TOL[dtype] * 0.25 * t.abs() + 1e-37).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_one_value_whose_square_leaves_fp32(device, dtype):
+    for at in (0, 12345, 99999):
+        ts = tensors(9, [50, 100000], (dtype,))
+        ts[1][at] = 1e22
+        check(ts, 1.0)
