@@ -481,7 +481,8 @@ int mcx_attention_backward(const void *gout, const void *q, const void *k, const
                            int dtype, void *stream);
 
 /* Clipping by the global norm: norm[0] = sqrt(sum of squares over all tensors), out = in *
- * min(1, max_norm / (norm + eps)); out[t] may be in[t].  in, out, sizes (values) and dtypes are
+ * min(1, max_norm / (norm + eps)); out[t] may be in[t], and shares no memory with any other tensor (the
+ * workgroups of two tensors would race; not checked here).  in, out, sizes (values) and dtypes are
  * HOST arrays of `count` entries, read before the call returns; a NULL `out` asks for the norm
  * alone.  max_norm >= 0. */
 size_t mcx_clip_grad_norm_workspace(const int64_t *sizes, int64_t count);

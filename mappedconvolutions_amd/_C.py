@@ -1102,11 +1102,22 @@ def relative_attention_backward(grad_output, query, key, value, output, saved, b
 _CLIP_DTYPES = {torch.float32: MCX_F32, torch.bfloat16: MCX_BF16}
 
 
+def _written_apart(read, write, tensors):
+    """Refuses a tensor that would be written while another one's work reads or writes it."""
+    # (tensors without values may share an address)
+    pairs = [(r, w) for r, w, t in zip(read, write, tensors) if t.numel()]
+    if len({w for _, w in pairs}) != len(pairs):
+        raise RuntimeError("a tensor that is written stands in the list twice")
+    if not {w for r, w in pairs if r != w}.isdisjoint(r for r, _ in pairs):
+        raise RuntimeError("a tensor of out is another one's input")
+
+
 def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
     """The norm of all values of a list of tensors (float32 and bfloat16, contiguous, on one GPU),
     as a float32 scalar; the tensors, or where `out` gives as many of the same sizes and types
     those, hold min(1, max_norm / (norm + eps)) times the values then.  A norm that is no number
-    makes them all none."""
+    makes them all none.  What is written must not share memory with any other tensor: one that
+    stands in the list twice is refused, parts that overlap are not looked for."""
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0 or not eps >= 0:
         raise RuntimeError("max_norm and eps must not be negative")
@@ -1117,6 +1128,9 @@ def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
     every, n = tensors if out is None else tensors + list(out), len(tensors)
     if len(every) != (n if out is None else 2 * n):
         raise RuntimeError("out must have as many tensors")
+    at = list(map(torch.Tensor.data_ptr, every))
+    if len(set(at)) != len(at):
+        _written_apart(at[:n], at[-n:], tensors)
     where = set(map(torch.Tensor.get_device, every))
     if len(where) != 1 or not tensors[0].is_cuda:
         raise RuntimeError("all tensors must be on one GPU")
@@ -1129,7 +1143,6 @@ def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
     if out is not None and (sizes[:n] != sizes[n:] or codes[:n] != codes[n:]):
         raise RuntimeError("out must have the tensors' sizes and dtypes")
     # (host arrays of the library's types; `inputs` and the others live until it has returned)
-    at = list(map(torch.Tensor.data_ptr, every))
     inputs, outputs = array.array("Q", at[:n]), array.array("Q", at[-n:])
     lengths, types = array.array("q", sizes[:n]), array.array("i", codes[:n])
     hosts = [a.buffer_info()[0] for a in (inputs, outputs, lengths, types)]

@@ -58,7 +58,8 @@ def clip_grad_norm_(parameters, max_norm, eps=1e-6):
     most max_norm; -> that norm before (float32 scalar on the GPU; 0 where there is no gradient).
     Gradients are float32 or bfloat16, on one GPU; one that is not contiguous is copied and back."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    grads = [p.grad for p in parameters if p.grad is not None]
+    # (a gradient that several have, or a parameter that is given twice, counts once)
+    grads = list(dict.fromkeys(p.grad for p in parameters if p.grad is not None))
     if not grads:
         return torch.zeros(())
     with torch.no_grad():

@@ -180,3 +180,27 @@ def test_rotation_table():
     # turning on from the last place comes to the first
     step = torch.complex(cos[1], sin[1])
     assert torch.allclose(torch.complex(cos[11], sin[11]) * step, torch.complex(cos[0], sin[0]), atol=1e-6)
+
+
+def test_clip_refuses_what_is_written_twice():
+    a, b, none = torch.ones(5), torch.ones(5), torch.empty(0)
+    for kw in (dict(tensors=[a, b, a]), dict(tensors=[a, b], out=[b, b.clone()]),
+               dict(tensors=[a, b], out=[none.new_ones(5)] * 2), dict(tensors=[a, b, none], out=[b, a, none])):
+        with pytest.raises(RuntimeError, match="twice|another one"):
+            _C.clip_grad_norm(max_norm=1.0, **kw)
+    # read twice, each its own, none with values: on to the next check
+    for kw in (dict(tensors=[a, a], out=[b, b.clone()]), dict(tensors=[a, b], out=[a, b]),
+               dict(tensors=[a, b], out=[a, b.clone()]), dict(tensors=[none, a, none.clone()])):
+        with pytest.raises(RuntimeError, match="one GPU"):
+            _C.clip_grad_norm(max_norm=1.0, **kw)
+
+
+def test_parameters_that_share_a_gradient_are_clipped_once(monkeypatch):
+    shared, other = torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(2))
+    tied = torch.nn.Parameter(torch.ones(3))
+    shared.grad, other.grad = torch.ones(3), torch.ones(2)
+    tied.grad = shared.grad
+    lists = []
+    monkeypatch.setattr(_C, "clip_grad_norm", lambda ts, *rest, **kw: lists.append(ts))
+    util.clip_grad_norm_([shared, other, shared, tied], 1.0)
+    assert len(lists[0]) == 2 and lists[0][0] is shared.grad and lists[0][1] is other.grad
