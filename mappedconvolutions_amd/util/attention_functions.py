@@ -55,13 +55,15 @@ def rotation_table(places, rotated, base=10000.0, circle=False, device=None):
 
 def clip_grad_norm_(parameters, max_norm, eps=1e-6):
     """Scales the gradients of the parameters in place so that the norm of all of them together is at
-    most max_norm; -> that norm before (float32 scalar on the GPU; 0 where there is no gradient).
+    most max_norm; -> that norm before (float32 scalar where the parameters are; 0 where there is no
+    gradient).
     Gradients are float32 or bfloat16, on one GPU; one that is not contiguous is copied and back."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     # (a gradient that several have, or a parameter that is given twice, counts once)
     grads = list(dict.fromkeys(p.grad for p in parameters if p.grad is not None))
     if not grads:
-        return torch.zeros(())
+        return torch.zeros((), dtype=torch.float32,
+                           device=parameters[0].device if parameters else None)
     with torch.no_grad():
         dense = [g if g.is_contiguous() else g.contiguous() for g in grads]
         norm = _C.clip_grad_norm(dense, max_norm, eps)

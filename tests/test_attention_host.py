@@ -204,3 +204,10 @@ def test_parameters_that_share_a_gradient_are_clipped_once(monkeypatch):
     monkeypatch.setattr(_C, "clip_grad_norm", lambda ts, *rest, **kw: lists.append(ts))
     util.clip_grad_norm_([shared, other, shared, tied], 1.0)
     assert len(lists[0]) == 2 and lists[0][0] is shared.grad and lists[0][1] is other.grad
+
+
+def test_norm_of_no_gradients_is_where_the_parameters_are():
+    parameters = [torch.nn.Parameter(torch.ones(3, device="meta"))]
+    norm = util.clip_grad_norm_(parameters, 1.0)
+    assert norm.device == parameters[0].device and norm.dtype == torch.float32 and norm.dim() == 0
+    assert util.clip_grad_norm_([], 1.0).item() == 0
