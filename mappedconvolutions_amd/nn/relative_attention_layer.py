@@ -8,6 +8,26 @@ import torch.nn as nn
 from .. import _C
 
 
+class FirstDerivative(torch.autograd.Function):
+    """A gradient that depends on what it was computed from in a way that is not differentiated
+    again.  (torch's once_differentiable says so only where the output's gradient is itself a
+    variable, which that of a plain sum is not.)"""
+
+    @staticmethod
+    def forward(ctx, gradient, *computed_from):
+        return gradient
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("second derivatives through the attention layers are not supported")
+
+
+def first_derivatives(gradients, *computed_from):
+    if not torch.is_grad_enabled():  # no graph of the backward pass is recorded
+        return tuple(gradients)
+    return tuple(None if g is None else FirstDerivative.apply(g, *computed_from) for g in gradients)
+
+
 class QKNormRotationFunction(torch.autograd.Function):
 
     @staticmethod
@@ -21,7 +41,7 @@ class QKNormRotationFunction(torch.autograd.Function):
     def backward(ctx, grad_query, grad_key):
         grads = _C.qk_norm_rotate_backward(grad_query, grad_key, *ctx.saved_tensors, ctx.eps,
                                            ctx.adjacent)
-        return tuple(grads) + (None,) * 5
+        return first_derivatives(grads, grad_query, grad_key, *ctx.saved_tensors[:4]) + (None,) * 5
 
 
 class QKNormRotation(nn.Module):
@@ -65,7 +85,7 @@ class RelativeAttentionFunction(torch.autograd.Function):
         grads = _C.relative_attention_backward(
             grad_output, query, key, value, out, saved, table, buckets, query_start=start,
             key_lengths=lengths, needs=needs, **ctx.args)
-        return tuple(grads) + (None,) * 7
+        return first_derivatives(grads, grad_output, query, key, value, table) + (None,) * 7
 
 
 class RelativeAttention(nn.Module):

@@ -211,3 +211,37 @@ def test_norm_of_no_gradients_is_where_the_parameters_are():
     norm = util.clip_grad_norm_(parameters, 1.0)
     assert norm.device == parameters[0].device and norm.dtype == torch.float32 and norm.dim() == 0
     assert util.clip_grad_norm_([], 1.0).item() == 0
+
+
+@pytest.fixture
+def without_kernels(monkeypatch):
+    """Stand-ins of the operators that compute nothing: what the layers do around them."""
+    asked = []
+
+    def norm_back(gq, gk, q, k, wq, wk, *rest, needs=(True,) * 4, **kw):
+        asked.append(tuple(needs))
+        return [torch.ones_like(t) if n else None for t, n in zip((q, k, wq, wk), needs)]
+
+    def attention_back(go, q, k, v, out, saved, table, *rest, needs, **kw):
+        return [torch.ones_like(t) if t is not None and n else None for t, n in zip((q, k, v, table), needs)]
+
+    monkeypatch.setattr(_C, "qk_norm_rotate_forward", lambda q, k, *rest, **kw: [q.clone(), k.clone()])
+    monkeypatch.setattr(_C, "qk_norm_rotate_backward", norm_back)
+    monkeypatch.setattr(_C, "relative_attention_forward",
+                        lambda q, *rest, **kw: [q.clone(), [torch.zeros(1), None]])
+    monkeypatch.setattr(_C, "relative_attention_backward", attention_back)
+    return asked
+
+
+def test_second_derivatives_are_refused(without_kernels):
+    # a penalty on the gradient beside the loss itself: its part must not be left out silently
+    q = torch.randn(1, 5, 2, 16).requires_grad_()
+    cos = torch.ones(5, 8)
+    for layer in (lambda x: nn.RelativeAttention(2)(x, x, x), lambda x: nn.QKNormRotation(16)(x, x, cos, cos)[0]):
+        loss = layer(q).sum()
+        gradient, = torch.autograd.grad(loss, q, create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            (loss + gradient.square().sum()).backward()
+        # a graph of the backward pass that nothing is asked of is no fault
+        torch.autograd.grad(layer(q).square().sum(), q, create_graph=True)
+        layer(q).sum().backward()
