@@ -52,14 +52,15 @@ class RowNetwork(nn.Module):
         buckets, zero = distance_buckets(num_buckets, circle=width)
         self.rows = HeadsOfTokens(channels, heads, key_heads, buckets, zero, num_buckets)
         self.read = nn.Linear(channels, 1)
-        cos, sin = rotation_table(width, channels // heads, circle=True)
-        self.register_buffer('cos', cos)
-        self.register_buffer('sin', sin)
+        # (their bits as whole numbers: a network that is cast keeps its angles in float32)
+        angles = torch.stack(rotation_table(width, channels // heads, circle=True))
+        self.register_buffer('angles', angles.view(torch.int32))
 
     def forward(self, images, sample_map):
         x = self.convolution(images, sample_map).permute(0, 2, 3, 1)      # B H W C
         B, H, W, C = x.shape
-        y = self.rows(x.reshape(B * H, W, C), self.cos, self.sin)
+        cos, sin = self.angles.view(torch.float32)
+        y = self.rows(x.reshape(B * H, W, C), cos, sin)
         return self.read(y).view(B, H, W)
 
 

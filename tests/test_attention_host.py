@@ -245,3 +245,19 @@ def test_second_derivatives_are_refused(without_kernels):
         # a graph of the backward pass that nothing is asked of is no fault
         torch.autograd.grad(layer(q).square().sum(), q, create_graph=True)
         layer(q).sum().backward()
+
+
+def test_example_keeps_its_angles_when_cast(without_kernels, monkeypatch):
+    from mappedconvolutions_amd.examples import row_attention
+    angles = []
+
+    def norm(q, k, wq, wk, cos, sin, *rest, **kw):
+        angles.append((cos, sin))
+        return [q.clone(), k.clone()]
+
+    monkeypatch.setattr(_C, "qk_norm_rotate_forward", norm)
+    net = row_attention.RowNetwork(8, channels=16).to(torch.bfloat16)
+    monkeypatch.setattr(net.convolution, "forward", lambda images, sample_map: images.expand(-1, 16, -1, -1))
+    net(torch.randn(1, 1, 2, 8).bfloat16(), None)
+    for got, want in zip(angles[0], util.rotation_table(8, 4, circle=True)):
+        assert got.dtype == torch.float32 and torch.equal(got, want)

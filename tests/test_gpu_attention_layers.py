@@ -133,3 +133,21 @@ def test_nothing_is_saved_without_a_graph(device, monkeypatch):
         served = layer(q, q, q)
     assert torch.equal(layer(q, q, q), served)
     assert asked == [False, True]
+
+
+def test_example_trains_in_bfloat16(device):
+    torch.manual_seed(3)
+    net = row_attention.RowNetwork(64).to(device, torch.bfloat16)
+    sample_map = util.latitude_map(16, 64).to(device)
+    optimizer = torch.optim.Adam(net.parameters(), lr=3e-3)
+    losses = []
+    for _ in range(40):
+        images = torch.randn(4, 1, 16, 64, device=device, dtype=torch.bfloat16)
+        optimizer.zero_grad()
+        loss = (net(images, sample_map).float() - images[:, 0].float().roll(16, -1)).square().mean()
+        loss.backward()
+        assert util.clip_grad_norm_(net.parameters(), 1.0).isfinite()
+        optimizer.step()
+        losses.append(loss.detach())
+    losses = torch.stack(losses).tolist()
+    assert losses[-1] < 0.8 * losses[0]
