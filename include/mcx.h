@@ -423,7 +423,8 @@ int mcx_qk_norm_rotate_forward(const void *q, const void *k, const void *wq, con
                                const int64_t *k_stride, int64_t B, int64_t L, int64_t Hq,
                                int64_t Hk, int64_t D, int64_t F, int64_t places, double eps,
                                int adjacent, int dtype, void *stream);
-/* Gradients: gq, gk (contiguous, of q_out and k_out) -> gq_in, gk_in (contiguous), gwq, gwk [D]. */
+/* Gradients: gq, gk (contiguous, of q_out and k_out) -> gq_in, gk_in (contiguous), gwq, gwk [D]; NULL
+ * for one that is not wanted. */
 size_t mcx_qk_norm_rotate_backward_workspace(int64_t B, int64_t L, int64_t Hq, int64_t Hk,
                                              int64_t D, int dtype);
 int mcx_qk_norm_rotate_backward(const void *gq, const void *gk, const void *q, const void *k,

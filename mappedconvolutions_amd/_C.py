@@ -947,9 +947,10 @@ def qk_norm_rotate_forward(query, key, query_weight, key_weight, cos, sin, posit
 
 
 def qk_norm_rotate_backward(grad_query, grad_key, query, key, query_weight, key_weight, cos, sin,
-                            positions=None, eps=1e-6, adjacent=False):
+                            positions=None, eps=1e-6, adjacent=False,
+                            needs=(True, True, True, True)):
     """-> [grad_query, grad_key, grad_query_weight, grad_key_weight] of qk_norm_rotate_forward
-    from the gradients of its outputs."""
+    from the gradients of its outputs; a gradient that `needs` leaves out is None."""
     dt, B, L, Hq, Hk, D, query, key, cos, sin, positions = _norm_args(
         query, key, query_weight, key_weight, cos, sin, positions, eps)
     _heads("grad_query", grad_query, B, L, Hq, D)
@@ -957,8 +958,8 @@ def qk_norm_rotate_backward(grad_query, grad_key, query, key, query_weight, key_
     _attention_dtype(query, grad_query=grad_query, grad_key=grad_key)
     _on_gpu("query", query, grad_query=grad_query, grad_key=grad_key)
     grad_query, grad_key = grad_query.contiguous(), grad_key.contiguous()
-    gq, gk = torch.empty_like(grad_query), torch.empty_like(grad_key)
-    gwq, gwk = torch.empty_like(query_weight), torch.empty_like(key_weight)
+    gq, gk, gwq, gwk = (torch.empty_like(t) if wanted else None for t, wanted in
+                        zip((grad_query, grad_key, query_weight, key_weight), needs))
     lib = _lib.load()
     nbytes = lib.mcx_qk_norm_rotate_backward_workspace(B, L, Hq, Hk, D, dt)
     ws = _workspace(nbytes, query.device)

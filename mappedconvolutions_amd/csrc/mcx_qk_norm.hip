@@ -32,6 +32,7 @@ struct NormParams {
   int64_t qs[3], ks[3];
   int64_t tokens;
   int L, Hq, Hk, D, F, adjacent, lanes;  // lanes of a row
+  int sums;        // the weights' gradients wanted: 1 the queries', 2 the keys'
   int64_t places;
   float eps;
 };
@@ -243,7 +244,7 @@ __device__ inline void norm_items(const NormParams &p, bool keys, int64_t first,
 #pragma unroll
         for (int e = 0; e < V; e++) y[e] = r * fmaf(-x[e], rest, y[e]);
       }
-      lane.store(o0 + dense + n * D, D, y);
+      if (!Grad || o0) lane.store(o0 + dense + n * D, D, y);
     }
   }
 }
@@ -265,10 +266,12 @@ __global__ __launch_bounds__(kThreads, 4) void qk_norm_rotate_kernel(NormParams 
   }
   __shared__ float sums[kThreads * V];
   for (int part = 0; part < 2; part++) {
+    if (!(part ? p.ok : p.oq) && !(p.sums >> part & 1)) continue;  // nothing of it is wanted
     float dw[V];
 #pragma unroll
     for (int e = 0; e < V; e++) dw[e] = 0.f;
     norm_items<T, Form, Grad>(p, part != 0, group, groups, lane, dw);
+    if (!(p.sums >> part & 1)) continue;
 #pragma unroll
     for (int e = 0; e < V; e++) sums[tid * V + e] = dw[e];
     __syncthreads();
@@ -282,23 +285,23 @@ __global__ __launch_bounds__(kThreads, 4) void qk_norm_rotate_kernel(NormParams 
   }
 }
 
-// gw[d] of the queries (part 0) and keys: the blocks' sums in a fixed order, four columns a
-// workgroup.
+// gw[d] of the queries (part 0) and keys, or of one of them: the blocks' sums in a fixed order, four
+// columns a workgroup.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void qk_norm_weight_grad_kernel(const float *partial, T *gwq,
                                                                        T *gwk, int blocks, int D) {
   __shared__ float sums[kThreads];
   const int column = blockIdx.x * 4 + (threadIdx.x & 3);
   float x = 0.f;
-  if (column < 2 * D)
+  if (column < 2 * D && (column < D ? gwq : gwk))
 #pragma unroll 8
     for (int n = threadIdx.x >> 2; n < blocks; n += kThreads / 4) x += partial[(int64_t)n * 2 * D + column];
   sums[threadIdx.x] = x;
   __syncthreads();
   if (threadIdx.x < 4 && column < 2 * D) {
     for (int n = 1; n < kThreads / 4; n++) x += sums[n * 4 + threadIdx.x];
-    if (column < D) gwq[column] = (T)x;
-    else gwk[column - D] = (T)x;
+    T *to = column < D ? gwq : gwk;
+    if (to) to[column < D ? column : column - D] = (T)x;
   }
 }
 
@@ -408,20 +411,22 @@ int mcx_qk_norm_rotate_backward(const void *gq, const void *gk, const void *q, c
   int rc = norm_check(q, k, wq, wk, cos, sin, q_stride, k_stride, B, L, Hq, Hk, D, F, places, eps,
                       dtype);
   if (rc != MCX_OK) return rc;
-  if (!gwq || !gwk || (B && L && (!gq || !gk || !gq_in || !gk_in))) return MCX_E_NULL;
+  if (B && L && (!gq || !gk)) return MCX_E_NULL;
+  if (!gwq && !gwk && (!B || !L || (!gq_in && !gk_in))) return MCX_OK;
   const size_t need = mcx_qk_norm_rotate_backward_workspace(B, L, Hq, Hk, D, dtype);
   if (!workspace || workspace_bytes < need) return MCX_E_WORKSPACE;
   NormParams p = {};
   p.q = q, p.k = k, p.wq = wq, p.wk = wk, p.gq = gq, p.gk = gk;
   p.cos = cos, p.sin = sin, p.positions = positions;
   p.oq = gq_in, p.ok = gk_in, p.partial = (float *)workspace;
+  p.sums = (gwq ? 1 : 0) | (gwk ? 2 : 0);
   for (int n = 0; n < 3; n++) p.qs[n] = q_stride[n], p.ks[n] = k_stride[n];
   p.tokens = B * L, p.L = (int)std::max<int64_t>(L, 1), p.Hq = (int)Hq, p.Hk = (int)Hk;
   p.D = (int)D, p.F = (int)F, p.places = places, p.eps = (float)eps, p.adjacent = adjacent != 0;
   int64_t blocks = grad_blocks(p.tokens, Hq, Hk);
   rc = dtype == MCX_BF16 ? norm_launch<__bf16, true>(p, &blocks, (hipStream_t)stream)
                          : norm_launch<float, true>(p, &blocks, (hipStream_t)stream);
-  if (rc != MCX_OK) return rc;
+  if (rc != MCX_OK || !p.sums) return rc;
   const dim3 grid((unsigned)((2 * D + 3) / 4));
   if (dtype == MCX_BF16)
     hipLaunchKernelGGL((qk_norm_weight_grad_kernel<__bf16>), grid, dim3(kThreads), 0,

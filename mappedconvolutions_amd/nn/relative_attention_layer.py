@@ -40,7 +40,7 @@ class QKNormRotationFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_query, grad_key):
         grads = _C.qk_norm_rotate_backward(grad_query, grad_key, *ctx.saved_tensors, ctx.eps,
-                                           ctx.adjacent)
+                                           ctx.adjacent, needs=tuple(ctx.needs_input_grad[:4]))
         return first_derivatives(grads, grad_query, grad_key, *ctx.saved_tensors[:4]) + (None,) * 5
 
 

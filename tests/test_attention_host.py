@@ -261,3 +261,23 @@ def test_example_keeps_its_angles_when_cast(without_kernels, monkeypatch):
     net(torch.randn(1, 1, 2, 8).bfloat16(), None)
     for got, want in zip(angles[0], util.rotation_table(8, 4, circle=True)):
         assert got.dtype == torch.float32 and torch.equal(got, want)
+
+
+def test_norm_asks_for_the_gradients_that_are_wanted(without_kernels):
+    norm, cos = nn.QKNormRotation(16), torch.ones(5, 8)
+    q, k = torch.randn(1, 5, 2, 16).requires_grad_(), torch.randn(1, 5, 2, 16)
+    norm.key_weight.requires_grad_(False)
+    sum(t.sum() for t in norm(q, k, cos, cos)).backward()
+    assert without_kernels == [(True, False, True, False)]
+
+
+def test_norm_gradients_that_are_not_wanted():
+    lib, three = _lib.load(), (_lib._i64 * 3)(64, 32, 16)
+
+    def call(gq=1, wanted=(1, 1, 1, 1), ws=None, B=1):
+        return lib.mcx_qk_norm_rotate_backward(gq, 1, 1, 1, 1, 1, 1, 1, None, *wanted, ws, 0, three, three,
+                                               B, 2, 2, 1, 16, 8, 2, 1e-6, 0, 0, None)
+
+    assert call(gq=None) == -3 and call() == -4
+    # nothing to do
+    assert call(wanted=(None,) * 4) == 0 and call(wanted=(1, 1, None, None), gq=None, B=0) == 0

@@ -155,3 +155,19 @@ def test_gradient_against_differences(device):
             ends.append(sum((a.double() * b.double()).sum() for a, b in zip(out, grads)))
         slope = ((ends[0] - ends[1]) / 2e-2).item()
         assert abs(slope - (back[n].double() * way.double()).sum().item()) < 1e-3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 37])
+def test_partial_gradients(device, dtype, D):
+    q, k, wq, wk, cos, sin, grads = problem(10, dtype, 2, 300, 6, 2, D, 16)
+    full = _C.qk_norm_rotate_backward(*grads, q, k, wq, wk, cos, sin)
+    for bits in range(16):
+        needs = tuple(bool(bits >> n & 1) for n in range(4))
+        got = _C.qk_norm_rotate_backward(*grads, q, k, wq, wk, cos, sin, needs=needs)
+        for a, b, n in zip(got, full, needs):
+            assert (a is None) if not n else torch.equal(a, b)
+    # no tokens: the weights' gradients are zeros
+    got = _C.qk_norm_rotate_backward(grads[0][:, :0], grads[1][:, :0], q[:, :0], k[:, :0], wq, wk, cos,
+                                     sin, needs=(True, False, False, True))
+    assert got[0].shape == (2, 0, 6, D) and got[1] is None and got[2] is None and (got[3] == 0).all()
