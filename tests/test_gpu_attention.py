@@ -491,3 +491,71 @@ def test_more_workgroups_than_a_launch_takes(device):
         want = reference(q[part], k[part], v[part], table, buckets, 1, go=go[part])
         for got, w, name in zip((out, gq, gk, gv), want, ("out", "grad_query", "grad_key", "grad_value")):
             close(got[part], w, TOL[torch.bfloat16], name)
+
+
+ANY_ROWS = [
+    # B, Lq, Lk, Hq, Hk, D: heads that are not whole 16-byte words, of every padded size
+    (1, 140, 150, 2, 1, 50),
+    (2, 131, 70, 2, 2, 61),
+    (1, 150, 200, 4, 2, 90),
+    (1, 129, 140, 2, 1, 100),
+    (1, 200, 90, 3, 1, 127),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", ANY_ROWS)
+def test_heads_of_any_size(device, size, dtype):
+    args = problem(40, dtype, *size)
+    B, Lq, Lk = size[:3]
+    lengths = torch.tensor([Lk - 31 * b - 5 for b in range(B)], dtype=torch.int32).cuda()
+    check(*args)
+    check(*args, causal=True, lengths=lengths)
+    # few queries over many keys, in one part and split
+    few = problem(41, dtype, 2, 2, 1500, *size[3:])
+    lengths = torch.tensor([1500, 900], dtype=torch.int32).cuda()
+    check(*few, train=False, causal=True, lengths=lengths, start=lengths - 2)
+    q, k, v, go, table, buckets, zero = few
+    check(q, k[:, :90], v[:, :90], go, table, buckets, zero)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 96, 128])
+def test_rows_at_any_address(device, D, dtype):
+    # whole heads of a packed projection that starts one value behind a 16-byte boundary, and the
+    # second case split along both axes
+    _, _, _, _, table, buckets, zero = problem(42, dtype, 1, 1, 1, 4, 2, D)
+    for B, L in ((2, 140), (1, 530)):
+        g = torch.Generator().manual_seed(43)
+        flat = torch.randn(B * L * 8 * D + 1, generator=g).to(dtype).cuda()
+        packed = flat[1:].view(B, L, 8, D)
+        q, k, v = packed[:, :, :4], packed[:, :, 4:6], packed[:, :, 6:]
+        go = torch.randn(B, L, 4, D, generator=g).to(dtype).cuda()
+        check(q, k, v, go, table, buckets, zero, causal=True)
+        check(q[:, :1], k, v, go[:, :1], table, buckets, zero)
+
+
+def test_another_stream_gives_the_same_bits(device):
+    # calls of different data on two streams at once, split along both axes, against each alone
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    calls = [problem(44 + n, torch.bfloat16, 1, 900, 800, 4, 2, 64) for n in range(2)]
+
+    def step(q, k, v, go, table, buckets, zero):
+        out, saved = _C.relative_attention_forward(q, k, v, table, buckets, zero, for_backward=True)
+        return [out] + _C.relative_attention_backward(go, q, k, v, out, saved, table, buckets, zero)
+
+    want = [step(*c) for c in calls]
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for s, c, g in zip(sides, calls, got):
+            with torch.cuda.stream(s):
+                g.append(step(*c))
+    for s in sides:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        for run in runs:
+            for a, b in zip(run, w):
+                assert torch.equal(a, b)
