@@ -5,6 +5,9 @@
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
 //   dT[h, n] = sum of ds over the pairs of bucket n
 //
+// bf16: p and ds are formed in fp32 and rounded to bf16 (2^-9 of each) as operands of the last three
+// products; the sums per bucket take ds before that.
+//
 // Scores are computed again in both kernels (seven products of a tile instead of five): every
 // gradient then has one owner, who sums it in registers in a fixed order.  No atomics on memory,
 // the same bits each time.

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
     Params p, Split sp, T *out, float *stats, T *rest) {
   constexpr int Chunks = DP / 16, Blocks = DP / 32;
   constexpr int E = 16 / (int)sizeof(T), PerRow = words<T, DP>(), N = kStep * PerRow / 64;
-  // a wave's values; at the end all waves' sums, four blocks of columns at a time
+  // a wave's values; at the end all waves' sums, half a block of columns at a time
   constexpr int kTileWords = kStep * PerRow;
   __shared__ Word tiles_lds[kWaves * kTileWords];
   __shared__ int buckets_lds[kWaves][64];
@@ -188,8 +188,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<T, DP>(3))) void atten
     all += x == -kInf ? merge[w][lane & 31][1] : merge[w][lane & 31][1] * exp2_fast((x - top) * c);
   }
   const float factor = ref == -kInf ? 1.f : exp2_fast((ref - top) * c);
-  // wave w sums columns 32 d + 8 w .. 8 w + 7 of every block: [wave][32 columns][32 rows], a row
-  // of 33 values
+  // 16 columns at a time: [wave][16 columns][32 rows], of which a thread sums two columns of a row
   float *part_lds = (float *)tiles_lds;
   static_assert(kTileWords * 16 >= 32 * 16 * 4, "a block's sums fit two halves");
   const int64_t at = (int64_t)unit * sp.parts + part;
