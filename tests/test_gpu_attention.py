@@ -477,6 +477,11 @@ def test_more_workgroups_than_a_launch_takes(device):
     # 2^24 workgroups of 256 threads are one thread more than a launch can have
     if torch.cuda.mem_get_info()[0] < 32 << 30:
         pytest.skip("needs 32 GB")
+    a_million_sequences()
+    torch.cuda.empty_cache()  # (blocks of gigabytes, that small tensors of later tests would hold)
+
+
+def a_million_sequences():
     B, H, D = (1 << 20) + 3, 16, 8
     g = torch.Generator(device="cuda").manual_seed(50)
     q, k, v, go = (torch.randn(B, 2, H, D, generator=g, device="cuda").bfloat16() for _ in range(4))
