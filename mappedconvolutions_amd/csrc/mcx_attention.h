@@ -31,8 +31,8 @@ constexpr int kTile = 64;          // rows walked at a time
 constexpr int kMaxD = 128;
 // Waves of a SIMD at once that the kernels' registers are fitted to: two where what a lane holds
 // (`values`: head sizes' worth of accumulators and operands) leaves room for the rest.  Registers that
-// go to scratch memory all the same: of the listed sizes' kernels 10 of the bf16 query gradient at 128
-// and 1 of the key gradient at 64; 110 of the float32 key gradient at 128 (gradients of 8 x 16 heads of
+// go to scratch memory all the same: 10 of the bf16 query gradient with a bias' at 128 and 1 of the bf16
+// key gradient at 64; 110 of the float32 key gradient at 128 (gradients of 8 x 16 heads of
 // 1024 rows sharing 4: 57 TFLOP/s, heads of 96 67); in the forms for rows that are not whole words up
 // to 87 (bf16, with a bias' gradient), 165 (without) and 312 (float32 keys), at 128.
 template <typename T, int DP> constexpr int waves_per_simd(int values) {

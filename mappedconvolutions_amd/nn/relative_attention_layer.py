@@ -10,8 +10,8 @@ from .. import _C
 
 class FirstDerivative(torch.autograd.Function):
     """A gradient that depends on what it was computed from in a way that is not differentiated
-    again.  (torch's once_differentiable says so only where the output's gradient is itself a
-    variable, which that of a plain sum is not.)"""
+    again: on the inputs too, since the output's gradient need not be a variable (that of a plain
+    sum is not)."""
 
     @staticmethod
     def forward(ctx, gradient, *computed_from):
