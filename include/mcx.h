@@ -494,6 +494,41 @@ int mcx_clip_grad_norm(const void *const *in, void *const *out, const int64_t *s
                        const int32_t *dtypes, int64_t count, double max_norm, double eps,
                        float *norm, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- The AdamW step -------------------------------------------------------------------
+ * No counterpart in the reference.  Parameters and gradients are MCX_F32 or MCX_BF16, each tensor
+ * with types of its own; the arithmetic is fp32.
+ *   g' = g min(1, max_norm / (norm + 1e-6)),  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+ *   p = p (1 - rate decay) - rate / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+ * bits 32: first and second moments are float.  bits 8: they are bytes, 256 values of a tensor
+ * sharing a float scale, a power of two (twice that of the block's largest value); a byte stands for
+ *   first:  s eeee mmm  (-1)^s (8 + m) 2^(e - 18), or for e = 0  (-1)^s m 2^-17
+ *   second: eeeee mmm          (8 + m) 2^(e - 34), or for e = 0         m 2^-33
+ * times it.  Values are rounded up with the probability of what is cut off, by 16 bits of a word that
+ * seed, step and the value's place in the list give (each tensor begins at a multiple of 256): the
+ * same bits from call to call with the same arguments.  A second moment above 0 stays above 0; a
+ * block with a value that is not finite has the scale NaN. */
+typedef struct mcx_adamw_options {
+  double rate, beta1, beta2, eps, weight_decay, max_norm;
+  int64_t step;               /* the number of this step, 1 for the first */
+  const int64_t *device_step; /* or NULL: the step is read from there */
+  const float *device_rate;   /* or NULL: the rate is read from there */
+  const float *grad_norm;     /* or NULL: gradients are clipped by this norm, see max_norm */
+  uint32_t seed;
+  int32_t bits; /* of the moments: 32 or 8 */
+} mcx_adamw_options;
+
+/* All arrays are HOST arrays of `count` entries, read before the call returns; the scales' (of
+ * tensors of (size + 255) / 256 floats) may be NULL with 32 bits.  Everything but the gradients is changed
+ * in place; tensors that are changed share no memory with others (not checked here). */
+int mcx_adamw_step(void *const *params, const void *const *grads, void *const *first,
+                   void *const *second, float *const *first_scales, float *const *second_scales,
+                   const int64_t *sizes, const int32_t *param_dtypes, const int32_t *grad_dtypes,
+                   int64_t count, const mcx_adamw_options *options, void *stream);
+/* The values that `size` bytes and their scales stand for; dtype F32 or BF16, which holds them
+ * exactly. */
+int mcx_adamw_moment(const void *codes, const float *scales, void *out, int64_t size, int second,
+                     int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1157,3 +1157,159 @@ def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
                                     _stream(norm))
     _lib.check(rc, "clip_grad_norm")
     return norm
+
+
+def grad_norm(tensors):
+    """The norm of all values of a list of tensors (float32 and bfloat16, contiguous, on one GPU), as
+    a float32 scalar; what clip_grad_norm multiplies by, without the products: adamw_step takes it."""
+    tensors = list(tensors)
+    if not tensors:
+        raise RuntimeError("grad_norm needs at least one tensor")
+    _one_gpu(tensors, tensors[0])
+    at, sizes, types = _host_lists(tensors)
+    device = tensors[0].device
+    lib = _lib.load()
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    nbytes = lib.mcx_clip_grad_norm_workspace(_host(sizes), len(tensors))
+    ws = _workspace(nbytes, device)
+    with _device(norm):
+        rc = lib.mcx_clip_grad_norm(_host(at), None, _host(sizes), _host(types), len(tensors), 0.0,
+                                    0.0, _ptr(norm), _ptr(ws), nbytes, _stream(norm))
+    _lib.check(rc, "grad_norm")
+    return norm
+
+
+def _one_gpu(tensors, first):
+    if len(set(map(torch.Tensor.get_device, tensors))) != 1 or not first.is_cuda:
+        raise RuntimeError("all tensors must be on one GPU")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise RuntimeError("tensors must be contiguous")
+
+
+def _host(a):
+    """The address of a host array (which has to live until the call returns)."""
+    return None if a is None else a.buffer_info()[0]
+
+
+def _host_lists(tensors):
+    """(addresses, sizes, type codes) of a list, as host arrays of the library's types."""
+    types = [_CLIP_DTYPES.get(t.dtype, -1) for t in tensors]
+    if -1 in types:
+        raise RuntimeError("unsupported dtype %s (float32 or bfloat16)" %
+                           tensors[types.index(-1)].dtype)
+    return (array.array("Q", map(torch.Tensor.data_ptr, tensors)),
+            array.array("q", map(torch.Tensor.numel, tensors)), array.array("i", types))
+
+
+ADAMW_BLOCK = 256  # values that share a scale where moments are held in 8 bits
+
+
+def _one_value(name, t, dtype, like):
+    if t.dtype != dtype or t.numel() != 1 or t.get_device() != like.get_device():
+        raise RuntimeError("%s must be one %s value on the parameters' GPU" % (name, dtype))
+    return t.data_ptr()
+
+
+def _moments(name, moments, scales, params, sizes):
+    """A check of the moments of one kind -> (addresses, the scales' addresses or None, all tensors)."""
+    dtype = torch.float32 if scales is None else torch.uint8
+    if len(moments) != len(params) or list(map(torch.Tensor.numel, moments)) != sizes:
+        raise RuntimeError("%s moments must have the parameters' number and sizes" % name)
+    if any(t.dtype != dtype for t in moments):
+        raise RuntimeError("%s moments must be %s" % (name, dtype))
+    at = array.array("Q", map(torch.Tensor.data_ptr, moments))
+    if scales is None:
+        return at, None, moments
+    if list(map(torch.Tensor.numel, scales)) != [-(-n // ADAMW_BLOCK) for n in sizes] or \
+            any(t.dtype != torch.float32 for t in scales):
+        raise RuntimeError("%s scales must be float32, one for %d values of a tensor" %
+                           (name, ADAMW_BLOCK))
+    return at, array.array("Q", map(torch.Tensor.data_ptr, scales)), moments + scales
+
+
+def adamw_step(params, grads, first_moments, second_moments, step, lr, betas=(0.9, 0.999), eps=1e-8,
+               weight_decay=0.0, first_scales=None, second_scales=None, seed=0, grad_norm=None,
+               max_norm=None):
+    """One AdamW step over lists of tensors on one GPU, in place:
+
+        g' = g min(1, max_norm / (grad_norm + 1e-6))        (g without grad_norm and max_norm)
+        m = b1 m + (1 - b1) g',   v = b2 v + (1 - b2) g'^2
+        p = p (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+
+    Parameters and gradients are float32 or bfloat16, each of its own type, contiguous.  The moments are
+    float32; or, with scales, uint8, which 256 values of a tensor share a float32 scale of
+    (first_scales, second_scales: (size + 255) // 256 values a tensor; zeros at the start): 3 bits
+    and an exponent each, rounded up with the probability of what is cut off, by words that `seed`, the
+    step and the value's place in the list give.
+    step: the number of this step from 1 on, or an int64 value on the GPU; lr: a number, or a float32
+    value on the GPU; both are read there when the kernels run, so that a captured step can be replayed.
+    What is changed must not share memory with any other tensor: one that stands in the lists twice
+    is refused, parts that overlap are not looked for."""
+    params, grads = list(params), list(grads)
+    first_moments, second_moments = list(first_moments), list(second_moments)
+    if (first_scales is None) != (second_scales is None):
+        raise RuntimeError("first_scales and second_scales go together")
+    if (grad_norm is None) != (max_norm is None):
+        raise RuntimeError("grad_norm and max_norm go together")
+    if len(grads) != len(params):
+        raise RuntimeError("%d gradients for %d parameters" % (len(grads), len(params)))
+    if first_scales is not None:
+        first_scales, second_scales = list(first_scales), list(second_scales)
+    beta1, beta2 = (float(b) for b in betas)
+    eps, weight_decay = float(eps), float(weight_decay)
+    if not (0 <= beta1 < 1 and 0 <= beta2 < 1 and eps >= 0 and weight_decay >= 0):
+        raise RuntimeError("betas must lie in [0, 1), eps and weight_decay must not be negative")
+    if max_norm is not None and not float(max_norm) >= 0:
+        raise RuntimeError("max_norm must not be negative")
+    if not isinstance(step, torch.Tensor) and int(step) < 1:
+        raise RuntimeError("step counts from 1, got %d" % step)
+    if not isinstance(lr, torch.Tensor) and not abs(float(lr)) < float("inf"):
+        raise RuntimeError("lr must be finite")
+    p_at, sizes, p_types = _host_lists(params)
+    g_at, g_sizes, g_types = _host_lists(grads)
+    if g_sizes != sizes:
+        raise RuntimeError("gradients must have the parameters' sizes")
+    counts = list(sizes)
+    m_at, ms_at, m_all = _moments("first", first_moments, first_scales, params, counts)
+    v_at, vs_at, v_all = _moments("second", second_moments, second_scales, params, counts)
+    if not params:
+        return
+    _one_gpu(params + grads + m_all + v_all, params[0])
+    written = [a for a in (*p_at, *m_at, *v_at, *(ms_at or ()), *(vs_at or ())) if a]
+    if len(set(written)) != len(written) or not set(written).isdisjoint(g_at):
+        # (tensors without values may share an address)
+        full = [t.data_ptr() for t in params + m_all + v_all if t.numel()]
+        if len(set(full)) != len(full) or \
+                not set(full).isdisjoint(t.data_ptr() for t in grads if t.numel()):
+            raise RuntimeError("a tensor that is changed stands in the lists twice")
+    device = params[0].device
+    options = _lib.AdamWOptions(
+        0.0 if isinstance(lr, torch.Tensor) else float(lr), beta1, beta2, eps, weight_decay,
+        0.0 if max_norm is None else float(max_norm), 1 if isinstance(step, torch.Tensor) else int(step),
+        _one_value("step", step, torch.int64, params[0]) if isinstance(step, torch.Tensor) else None,
+        _one_value("lr", lr, torch.float32, params[0]) if isinstance(lr, torch.Tensor) else None,
+        None if grad_norm is None else _one_value("grad_norm", grad_norm, torch.float32, params[0]),
+        int(seed) & 0xFFFFFFFF, 32 if first_scales is None else 8)
+    with _device(params[0]):
+        rc = _lib.load().mcx_adamw_step(_host(p_at), _host(g_at), _host(m_at), _host(v_at),
+                                        _host(ms_at), _host(vs_at), _host(sizes), _host(p_types),
+                                        _host(g_types), len(params), options, _stream(params[0]))
+    _lib.check(rc, "adamw_step")
+
+
+def adamw_moment(codes, scales, second, dtype=torch.float32):
+    """The values of moments that adamw_step holds in 8 bits (`second`: the second ones), in
+    codes' shape; float32 and bfloat16 hold them exactly."""
+    _contig(codes=codes, scales=scales)
+    _on_gpu("codes", codes, scales=scales)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.float32 or \
+            scales.numel() != -(-codes.numel() // ADAMW_BLOCK):
+        raise RuntimeError("codes must be uint8 and scales float32, one for %d of them" % ADAMW_BLOCK)
+    if dtype not in _CLIP_DTYPES:
+        raise RuntimeError("unsupported dtype %s (float32 or bfloat16)" % dtype)
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    with _device(codes):
+        rc = _lib.load().mcx_adamw_moment(_ptr(codes), _ptr(scales), _ptr(out), codes.numel(),
+                                          int(bool(second)), _CLIP_DTYPES[dtype], _stream(codes))
+    _lib.check(rc, "adamw_moment")
+    return out

@@ -38,6 +38,15 @@ class AttentionDesc(ctypes.Structure):
                 ("reserved", ctypes.c_int32)]
 
 
+class AdamWOptions(ctypes.Structure):
+    """mcx_adamw_options of include/mcx.h: the numbers of a step."""
+    _fields_ = [("rate", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double),
+                ("max_norm", ctypes.c_double), ("step", _i64), ("device_step", _p),
+                ("device_rate", _p), ("grad_norm", _p), ("seed", ctypes.c_uint32),
+                ("bits", ctypes.c_int32)]
+
+
 _adesc = ctypes.POINTER(AttentionDesc)
 _f64 = ctypes.c_double
 _pi64 = ctypes.POINTER(_i64)
@@ -93,6 +102,8 @@ SIGNATURES = {
     "mcx_attention_backward": (_i, [_p] * 16 + [_sz, _adesc, _i, _p]),
     "mcx_clip_grad_norm_workspace": (_sz, [_p, _i64]),
     "mcx_clip_grad_norm": (_i, [_p] * 4 + [_i64, _f64, _f64, _p, _p, _sz, _p]),
+    "mcx_adamw_step": (_i, [_p] * 9 + [_i64, ctypes.POINTER(AdamWOptions), _p]),
+    "mcx_adamw_moment": (_i, [_p] * 3 + [_i64, _i, _i, _p]),
 }
 
 _lib = None

@@ -1,0 +1,121 @@
+"""AdamW over all parameters at once, with moments in 32 or 8 bits.  No counterpart in the reference;
+the work is done by the HIP kernels behind `_C.adamw_step` and `_C.grad_norm`."""
+import torch
+
+from .. import _C
+
+
+class AdamW(torch.optim.Optimizer):
+    """Decoupled weight decay and bias-corrected moments, as the formula of _C.adamw_step says, in one
+    launch for several dozen parameters (float32 or bfloat16, on one GPU).
+
+    bits: of the moments, 32 or 8 (a quarter of the memory and a little over).
+    max_norm: gradients are clipped by the norm of all of them, which the step reads while it
+    updates: they are not changed themselves.  `grad_norm` holds the last step's norm.
+    capturable: steps are counted on the GPU, so that a captured step can be replayed; a learning
+    rate that changes between replays is a float32 value on the GPU then (a group's 'lr').  The first
+    step, which makes the moments, is not captured.
+    seed: of the rounding in 8 bits."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32,
+                 max_norm=None, capturable=False, seed=0):
+        if bits not in (32, 8):
+            raise ValueError('Moments are held in 32 or 8 bits')
+        self.max_norm, self.capturable, self.seed, self.grad_norm = max_norm, capturable, seed, None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                                      bits=bits))
+
+    def _state_of(self, p, bits, counter):
+        """The moments of a parameter, zeros when it first has a gradient."""
+        state = self.state[p]
+        if not state:
+            zeros = {32: torch.float32, 8: torch.uint8}[bits]
+            state['step'] = counter() if self.capturable else 0
+            for name in ('first', 'second'):
+                state[name] = torch.zeros(p.shape, dtype=zeros, device=p.device)
+                if bits == 8:
+                    state[name + '_scale'] = torch.zeros(-(-p.numel() // _C.ADAMW_BLOCK),
+                                                         device=p.device)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        # (the same gradient of several parameters is read, and counts in the norm, once)
+        dense = {}
+        for group in self.param_groups:
+            for p in group['params']:
+                if p.grad is not None and p.grad not in dense:
+                    if p.grad.is_sparse:
+                        raise RuntimeError('AdamW does not support sparse gradients')
+                    dense[p.grad] = p.grad.contiguous()
+        if not dense:
+            return loss
+        norm = None
+        if self.max_norm is not None:
+            norm = self.grad_norm = _C.grad_norm(list(dense.values()))
+        call = 0
+        for group in self.param_groups:
+            made = []
+
+            def counter():
+                # parameters that first have gradients in the same call share a counter
+                if not made:
+                    made.append(torch.zeros((), dtype=torch.int64, device=group['params'][0].device))
+                return made[0]
+
+            alike = {}
+            for p in group['params']:
+                if p.grad is None:
+                    continue
+                state = self._state_of(p, group['bits'], counter)
+                step = state['step']
+                key = id(step) if isinstance(step, torch.Tensor) else step
+                alike.setdefault(key, (step, []))[1].append((p, state))
+            for step, members in alike.values():
+                self._update(group, step, members, dense, norm, call)
+                call += 1
+        return loss
+
+    def _update(self, group, step, members, dense, norm, call):
+        if isinstance(step, torch.Tensor):
+            step += 1
+        else:
+            step += 1
+            for _, state in members:
+                state['step'] = step
+        params = [p if p.is_contiguous() else p.contiguous() for p, _ in members]
+        scales = {}
+        if group['bits'] == 8:
+            scales = dict(first_scales=[s['first_scale'] for _, s in members],
+                          second_scales=[s['second_scale'] for _, s in members],
+                          seed=self.seed + 0x9E3779B1 * call)
+        _C.adamw_step(params, [dense[p.grad] for p, _ in members], [s['first'] for _, s in members],
+                      [s['second'] for _, s in members], step, group['lr'], group['betas'],
+                      group['eps'], group['weight_decay'], grad_norm=norm,
+                      max_norm=None if norm is None else self.max_norm, **scales)
+        for changed, (p, _) in zip(params, members):
+            if changed is not p:
+                p.copy_(changed)
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # moments keep their own types (the base class casts them to the parameters')
+        ids = [i for group in state_dict['param_groups'] for i in group['params']]
+        for group in self.param_groups:
+            counters = {}
+            for p in group['params']:
+                saved = state_dict['state'].get(ids.pop(0))
+                if saved is None:
+                    continue
+                state = {name: value.to(p.device, copy=True) for name, value in saved.items()
+                         if name != 'step'}
+                state['step'] = int(saved['step'])
+                if self.capturable:  # as many counters in a group as there are numbers
+                    if state['step'] not in counters:
+                        counters[state['step']] = torch.tensor(state['step'], device=p.device)
+                    state['step'] = counters[state['step']]
+                self.state[p] = state
