@@ -494,6 +494,26 @@ int mcx_clip_grad_norm(const void *const *in, void *const *out, const int64_t *s
                        const int32_t *dtypes, int64_t count, double max_norm, double eps,
                        float *norm, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- Group norm with an activation, channels last --------------------------------------
+ * No counterpart in the reference.  F32 and BF16; weight and bias have the data's type; sums and
+ * statistics are fp32.  x [B, N, C], its last axis dense, x_stride (HOST): those of sample and token
+ * in values; G divides C.  Over the N tokens and the C / G channels of a group of a sample:
+ *   y = act((x - mean) / sqrt(var + eps) weight + bias);  weight, bias [C] or NULL
+ * activation: 0 none, 1 u / (1 + e^-u), 2 u (1 + erf(u / sqrt 2)) / 2.
+ * y [B, N, C] is contiguous; stats float [B, G, 2] (mean, 1 / sqrt(var + eps)) for the gradients, or
+ * NULL.  C <= 2^20, B G <= 2^23.  workspace: mcx_group_norm_workspace() bytes. */
+size_t mcx_group_norm_workspace(int64_t B, int64_t N, int64_t C, int64_t G, int backward, int dtype);
+int mcx_group_norm_forward(const void *x, const void *weight, const void *bias, void *y, float *stats,
+                           void *workspace, size_t workspace_bytes, const int64_t *x_stride, int64_t B,
+                           int64_t N, int64_t C, int64_t G, double eps, int activation, int dtype,
+                           void *stream);
+/* Gradients from gy (contiguous): gx [B, N, C] contiguous, gweight, gbias [C]; NULL for one that is
+ * not wanted.  The same bits from call to call.  Nothing is written where B or N is 0. */
+int mcx_group_norm_backward(const void *gy, const void *x, const float *stats, const void *weight,
+                            const void *bias, void *gx, void *gweight, void *gbias, void *workspace,
+                            size_t workspace_bytes, const int64_t *x_stride, int64_t B, int64_t N,
+                            int64_t C, int64_t G, int activation, int dtype, void *stream);
+
 /* ---- The AdamW step -------------------------------------------------------------------
  * No counterpart in the reference.  Parameters and gradients are MCX_F32 or MCX_BF16, each tensor
  * with types of its own; the arithmetic is fp32.

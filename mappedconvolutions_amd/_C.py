@@ -1159,6 +1159,96 @@ def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
     return norm
 
 
+# ---- group norm with an activation, channels last -----------------------------------------
+
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
+_two = _lib._i64 * 2
+
+
+def _group_args(x, groups, weight, bias, activation):
+    shape = x.shape
+    if len(shape) != 3:
+        raise RuntimeError("x must have 3 dimensions [B, N, C], got %s" % (tuple(shape),))
+    dt = _attention_dtype(x, weight=weight, bias=bias)
+    _on_gpu("x", x, weight=weight, bias=bias)
+    groups = int(groups)
+    if groups < 1 or shape[2] < 1 or shape[2] % groups:
+        raise RuntimeError("%d channels cannot be cut into %d groups" % (shape[2], groups))
+    if activation not in ACTIVATIONS:
+        raise RuntimeError("activation must be one of %s, got %r" %
+                           (", ".join(map(repr, ACTIVATIONS)), activation))
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and tuple(t.shape) != (shape[2],):
+            raise RuntimeError("%s must have shape (%d,), got %s" % (name, shape[2], tuple(t.shape)))
+    _contig(weight=weight, bias=bias)
+    if x.stride(2) != 1 and shape[2] != 1:
+        x = x.contiguous()
+    return dt, groups, ACTIVATIONS[activation], x
+
+
+def group_norm_forward(x, groups, weight=None, bias=None, eps=1e-5, activation=None,
+                       for_backward=False):
+    """x [B, N, C] (any strides with a dense last axis), every group of C / groups neighbouring channels of
+    a sample normed over the N tokens: y = act((x - mean) / sqrt(var + eps) * weight + bias), weight and
+    bias [C]; activation None, "silu" (u / (1 + e^-u)) or "gelu" (u (1 + erf(u / sqrt 2)) / 2).
+    -> [y, saved], y contiguous; `saved`, for group_norm_backward, is None unless `for_backward`:
+    mean and 1 / sqrt(var + eps) of every group, float32 [B, groups, 2]."""
+    dt, groups, act, x = _group_args(x, groups, weight, bias, activation)
+    eps = float(eps)
+    if not eps >= 0:
+        raise RuntimeError("eps must not be negative")
+    B, N, C = x.shape
+    y = x.new_empty((B, N, C))
+    stats = torch.empty((B, groups, 2), dtype=torch.float32, device=x.device) if for_backward else None
+    lib = _lib.load()
+    nbytes = lib.mcx_group_norm_workspace(B, N, C, groups, 0, dt)
+    ws = _workspace(nbytes, x.device)
+    with _device(x):
+        rc = lib.mcx_group_norm_forward(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(stats),
+                                        _ptr(ws), nbytes, _two(x.stride(0), x.stride(1)), B, N, C,
+                                        groups, eps, act, dt, _stream(x))
+    _lib.check(rc, "group_norm_forward")
+    return [y, stats]
+
+
+def group_norm_backward(grad_output, x, saved, groups, weight=None, bias=None, activation=None,
+                        needs=(True, True, True)):
+    """-> [grad_x, grad_weight, grad_bias] of group_norm_forward from the gradient of y and what it
+    saved; a gradient that `needs` leaves out, or whose parameter there is not, is None.  The same
+    bits from call to call."""
+    dt, groups, act, x = _group_args(x, groups, weight, bias, activation)
+    B, N, C = x.shape
+    if tuple(grad_output.shape) != (B, N, C):
+        raise RuntimeError("grad_output must have shape (%d, %d, %d), got %s" %
+                           (B, N, C, tuple(grad_output.shape)))
+    _attention_dtype(x, grad_output=grad_output)
+    if saved is None or saved.dtype != torch.float32 or tuple(saved.shape) != (B, groups, 2):
+        raise RuntimeError("saved must be what group_norm_forward returned with for_backward")
+    _on_gpu("x", x, grad_output=grad_output, saved=saved)
+    _contig(saved=saved)
+    grad_output = grad_output.contiguous()
+    gx = x.new_empty((B, N, C)) if needs[0] else None
+    gw = torch.empty_like(weight) if weight is not None and needs[1] else None
+    gb = torch.empty_like(bias) if bias is not None and needs[2] else None
+    if B == 0 or N == 0:
+        for t in (gw, gb):
+            if t is not None:
+                t.zero_()
+        return [gx, gw, gb]
+    lib = _lib.load()
+    nbytes = lib.mcx_group_norm_workspace(B, N, C, groups, 1, dt)
+    ws = _workspace(nbytes, x.device)
+    with _device(x):
+        rc = lib.mcx_group_norm_backward(_ptr(grad_output), _ptr(x), _ptr(saved), _ptr(weight),
+                                         _ptr(bias), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), nbytes,
+                                         _two(x.stride(0), x.stride(1)), B, N, C, groups, act, dt,
+                                         _stream(x))
+    _lib.check(rc, "group_norm_backward")
+    return [gx, gw, gb]
+
+
+# ---- clipping's norm alone, and the AdamW step ------------------------------------------------
+
 def grad_norm(tensors):
     """The norm of all values of a list of tensors (float32 and bfloat16, contiguous, on one GPU), as
     a float32 scalar; what clip_grad_norm multiplies by, without the products: adamw_step takes it."""

@@ -102,6 +102,9 @@ SIGNATURES = {
     "mcx_attention_backward": (_i, [_p] * 16 + [_sz, _adesc, _i, _p]),
     "mcx_clip_grad_norm_workspace": (_sz, [_p, _i64]),
     "mcx_clip_grad_norm": (_i, [_p] * 4 + [_i64, _f64, _f64, _p, _p, _sz, _p]),
+    "mcx_group_norm_workspace": (_sz, [_i64] * 4 + [_i, _i]),
+    "mcx_group_norm_forward": (_i, [_p] * 6 + [_sz, _pi64] + [_i64] * 4 + [_f64, _i, _i, _p]),
+    "mcx_group_norm_backward": (_i, [_p] * 9 + [_sz, _pi64] + [_i64] * 4 + [_i, _i, _p]),
     "mcx_adamw_step": (_i, [_p] * 9 + [_i64, ctypes.POINTER(AdamWOptions), _p]),
     "mcx_adamw_moment": (_i, [_p] * 3 + [_i64, _i, _i, _p]),
 }
