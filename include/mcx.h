@@ -494,6 +494,39 @@ int mcx_clip_grad_norm(const void *const *in, void *const *out, const int64_t *s
                        const int32_t *dtypes, int64_t count, double max_norm, double eps,
                        float *norm, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- A gated linear recurrence -----------------------------------------------------------
+ * No counterpart in the reference.  F32 and BF16; states are float and so is every sum.  Strides (of
+ * sequence and step, in values) of value, forget and gate [B, L, C], the last axis dense; any alignment
+ * goes, rows of whole 8-byte (BF16) or 16-byte words are read in those.  B * ceil(C / 16) <= 2^21. */
+typedef struct mcx_recurrence_desc {
+  int64_t B, L, C;
+  int64_t v_stride[2], f_stride[2], g_stride[2];
+  int32_t reverse;  /* from the last step in use to the first */
+  int32_t reserved; /* 0 */
+} mcx_recurrence_desc;
+
+/* a_t = sigmoid(forget_t),  h_t = a_t h_{t-1} + (1 - a_t) value_t,
+ * out_t = h_t gate_t sigmoid(gate_t), or h_t where gate is NULL
+ * over the steps t < lengths[b] (int32 [B], or NULL: L; clamped to [0, L]), from `initial` (float [B,
+ * C], or NULL: zeros).  What lies behind the steps in use is not read, and out is zero there.
+ * out [B, L, C] is contiguous; final float [B, C] is the state after the last step in use, and may be
+ * `initial` itself.  states float [B, mcx_gated_recurrence_spans(L), C] are for the gradients, or NULL.
+ * workspace: mcx_gated_recurrence_workspace() bytes (0: none).  Nothing is written where B or L is 0. */
+int64_t mcx_gated_recurrence_spans(int64_t L);
+size_t mcx_gated_recurrence_workspace(const mcx_recurrence_desc *desc, int dtype);
+int mcx_gated_recurrence_forward(const void *value, const void *forget, const void *gate,
+                                 const float *initial, const int32_t *lengths, void *out, float *final,
+                                 float *states, void *workspace, size_t workspace_bytes,
+                                 const mcx_recurrence_desc *desc, int dtype, void *stream);
+/* Gradients from gout [B, L, C] (contiguous), gfinal float [B, C] (or NULL: zeros) and the forward
+ * call's states: gvalue, gforget, ggate [B, L, C] contiguous (zeros at steps that are not in use),
+ * ginitial float [B, C]; NULL for one that is not wanted.  The same bits from call to call. */
+int mcx_gated_recurrence_backward(const void *gout, const float *gfinal, const void *value,
+                                  const void *forget, const void *gate, const float *states,
+                                  const int32_t *lengths, void *gvalue, void *gforget, void *ggate,
+                                  float *ginitial, void *workspace, size_t workspace_bytes,
+                                  const mcx_recurrence_desc *desc, int dtype, void *stream);
+
 /* ---- Group norm with an activation, channels last --------------------------------------
  * No counterpart in the reference.  F32 and BF16; weight and bias have the data's type; sums and
  * statistics are fp32.  x [B, N, C], its last axis dense, x_stride (HOST): those of sample and token

@@ -1159,10 +1159,133 @@ def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
     return norm
 
 
+# ---- a gated linear recurrence along a sequence ---------------------------------------------
+
+_two = _lib._i64 * 2
+
+
+def _pair(t):
+    return _two(t.stride(0), t.stride(1))
+
+
+def _recurrence_args(value, forget, gate, lengths, reverse):
+    """(dtype code, descriptor, the tensors as the library takes them) of a recurrence call."""
+    shape = value.shape
+    if len(shape) != 3 or shape[2] < 1:
+        raise RuntimeError("value must have 3 dimensions [B, L, C], got %s" % (tuple(shape),))
+    for name, t in (("forget", forget), ("gate", gate)):
+        if t is not None and t.shape != shape:
+            raise RuntimeError("%s must have value's shape %s, got %s" %
+                               (name, tuple(shape), tuple(t.shape)))
+    dt = _attention_dtype(value, forget=forget, gate=gate)
+    _on_gpu("value", value, forget=forget, gate=gate, lengths=lengths)
+    B, L, C = shape
+    if lengths is not None:
+        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,):
+            raise RuntimeError("lengths must be int32 of shape (%d,), got %s %s" %
+                               (B, lengths.dtype, tuple(lengths.shape)))
+        lengths = lengths.contiguous()
+    value, forget, gate = (t if t is None or t.stride(2) == 1 or C == 1 else t.contiguous()
+                           for t in (value, forget, gate))
+    desc = _lib.RecurrenceDesc(B, L, C, _pair(value), _pair(forget),
+                               _two(0, 0) if gate is None else _pair(gate), int(bool(reverse)), 0)
+    return dt, desc, value, forget, gate, lengths
+
+
+def _state(name, t, like):
+    if t is not None and (t.dtype != torch.float32 or t.shape != (like.shape[0], like.shape[2])):
+        raise RuntimeError("%s must be float32 of shape (%d, %d), got %s %s" %
+                           (name, like.shape[0], like.shape[2], t.dtype, tuple(t.shape)))
+
+
+def gated_recurrence_forward(value, forget, gate=None, initial=None, lengths=None, reverse=False,
+                             final=None, for_backward=False):
+    """A linear recurrence of every channel along the sequence, value, forget and gate [B, L, C] (any
+    strides with a dense last axis; parts of one projection go as they are):
+
+        a_t = sigmoid(forget_t),   h_t = a_t h_{t-1} + (1 - a_t) value_t
+        out_t = h_t gate_t sigmoid(gate_t)                          (h_t without a gate)
+
+    from the state `initial` float32 [B, C] (zeros by default).  lengths int32 [B] says how many steps
+    are in use: what lies behind them is not read, and out is zero there; `reverse` takes them from the
+    last one in use to the first.
+    -> [out [B, L, C], final, saved]: the state after the last step float32 [B, C], in the tensor `final`
+    where one is given (it may be `initial`, for a state that is kept from call to call); `saved`, for
+    gated_recurrence_backward, is None unless `for_backward`: states at some of the steps, float32."""
+    dt, desc, value, forget, gate, lengths = _recurrence_args(value, forget, gate, lengths, reverse)
+    B, L, C = value.shape
+    _state("initial", initial, value)
+    _state("final", final, value)
+    _on_gpu("value", value, initial=initial, final=final)
+    _contig(final=final)
+    if initial is not None:
+        initial = initial.contiguous()
+    out = value.new_empty((B, L, C))
+    if final is None:
+        final = torch.empty((B, C), dtype=torch.float32, device=value.device)
+    lib = _lib.load()
+    states = None
+    if for_backward:
+        states = torch.empty((B, lib.mcx_gated_recurrence_spans(L), C), dtype=torch.float32,
+                             device=value.device)
+    if B and not L:  # no step: the state stays as it is
+        if initial is None:
+            final.zero_()
+        elif final.data_ptr() != initial.data_ptr():
+            final.copy_(initial)
+    nbytes = lib.mcx_gated_recurrence_workspace(desc, dt)
+    ws = _workspace(nbytes, value.device) if nbytes else None
+    with _device(value):
+        rc = lib.mcx_gated_recurrence_forward(_ptr(value), _ptr(forget), _ptr(gate), _ptr(initial),
+                                              _ptr(lengths), _ptr(out), _ptr(final), _ptr(states),
+                                              _ptr(ws), nbytes, desc, dt, _stream(value))
+    _lib.check(rc, "gated_recurrence_forward")
+    return [out, final, states]
+
+
+def gated_recurrence_backward(grad_output, value, forget, gate, saved, grad_final=None, lengths=None,
+                              reverse=False, needs=(True, True, True, True)):
+    """-> [grad_value, grad_forget, grad_gate, grad_initial] of gated_recurrence_forward, called with the
+    same arguments and `for_backward`, from the gradients of out and (float32, zeros by default) of
+    final; a gradient that `needs` leaves out, or that of a gate that there is not, is None.  The same
+    bits from call to call."""
+    dt, desc, value, forget, gate, lengths = _recurrence_args(value, forget, gate, lengths, reverse)
+    B, L, C = value.shape
+    lib = _lib.load()
+    if grad_output.shape != value.shape:
+        raise RuntimeError("grad_output must have shape %s, got %s" %
+                           (tuple(value.shape), tuple(grad_output.shape)))
+    _attention_dtype(value, grad_output=grad_output)
+    _state("grad_final", grad_final, value)
+    if saved is None or saved.dtype != torch.float32 or \
+            tuple(saved.shape) != (B, lib.mcx_gated_recurrence_spans(L), C):
+        raise RuntimeError("saved must be what gated_recurrence_forward returned with for_backward")
+    _on_gpu("value", value, grad_output=grad_output, grad_final=grad_final, saved=saved)
+    _contig(saved=saved)
+    grad_output = grad_output.contiguous()
+    if grad_final is not None:
+        grad_final = grad_final.contiguous()
+    gv, gf, gg = (value.new_empty((B, L, C)) if wanted and t is not None else None
+                  for t, wanted in zip((value, forget, gate), needs))
+    gi = torch.empty((B, C), dtype=torch.float32, device=value.device) if needs[3] else None
+    if B and not L and gi is not None:
+        gi.zero_() if grad_final is None else gi.copy_(grad_final)
+    if not any(needs):
+        return [None, None, None, None]
+    nbytes = lib.mcx_gated_recurrence_workspace(desc, dt)
+    ws = _workspace(nbytes, value.device) if nbytes else None
+    with _device(value):
+        rc = lib.mcx_gated_recurrence_backward(
+            _ptr(grad_output), _ptr(grad_final), _ptr(value), _ptr(forget), _ptr(gate), _ptr(saved),
+            _ptr(lengths), _ptr(gv), _ptr(gf), _ptr(gg), _ptr(gi), _ptr(ws), nbytes, desc, dt,
+            _stream(value))
+    _lib.check(rc, "gated_recurrence_backward")
+    return [gv, gf, gg, gi]
+
+
 # ---- group norm with an activation, channels last -----------------------------------------
 
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
-_two = _lib._i64 * 2
 
 
 def _group_args(x, groups, weight, bias, activation):
@@ -1205,7 +1328,7 @@ def group_norm_forward(x, groups, weight=None, bias=None, eps=1e-5, activation=N
     ws = _workspace(nbytes, x.device)
     with _device(x):
         rc = lib.mcx_group_norm_forward(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(stats),
-                                        _ptr(ws), nbytes, _two(x.stride(0), x.stride(1)), B, N, C,
+                                        _ptr(ws), nbytes, _pair(x), B, N, C,
                                         groups, eps, act, dt, _stream(x))
     _lib.check(rc, "group_norm_forward")
     return [y, stats]
@@ -1241,7 +1364,7 @@ def group_norm_backward(grad_output, x, saved, groups, weight=None, bias=None, a
     with _device(x):
         rc = lib.mcx_group_norm_backward(_ptr(grad_output), _ptr(x), _ptr(saved), _ptr(weight),
                                          _ptr(bias), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), nbytes,
-                                         _two(x.stride(0), x.stride(1)), B, N, C, groups, act, dt,
+                                         _pair(x), B, N, C, groups, act, dt,
                                          _stream(x))
     _lib.check(rc, "group_norm_backward")
     return [gx, gw, gb]

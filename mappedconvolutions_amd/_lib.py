@@ -38,6 +38,13 @@ class AttentionDesc(ctypes.Structure):
                 ("reserved", ctypes.c_int32)]
 
 
+class RecurrenceDesc(ctypes.Structure):
+    """mcx_recurrence_desc of include/mcx.h: the sizes of a recurrence call."""
+    _fields_ = [("B", _i64), ("L", _i64), ("C", _i64), ("v_stride", _i64 * 2),
+                ("f_stride", _i64 * 2), ("g_stride", _i64 * 2), ("reverse", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
 class AdamWOptions(ctypes.Structure):
     """mcx_adamw_options of include/mcx.h: the numbers of a step."""
     _fields_ = [("rate", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
@@ -48,6 +55,7 @@ class AdamWOptions(ctypes.Structure):
 
 
 _adesc = ctypes.POINTER(AttentionDesc)
+_rdesc = ctypes.POINTER(RecurrenceDesc)
 _f64 = ctypes.c_double
 _pi64 = ctypes.POINTER(_i64)
 
@@ -102,6 +110,10 @@ SIGNATURES = {
     "mcx_attention_backward": (_i, [_p] * 16 + [_sz, _adesc, _i, _p]),
     "mcx_clip_grad_norm_workspace": (_sz, [_p, _i64]),
     "mcx_clip_grad_norm": (_i, [_p] * 4 + [_i64, _f64, _f64, _p, _p, _sz, _p]),
+    "mcx_gated_recurrence_spans": (_i64, [_i64]),
+    "mcx_gated_recurrence_workspace": (_sz, [_rdesc, _i]),
+    "mcx_gated_recurrence_forward": (_i, [_p] * 9 + [_sz, _rdesc, _i, _p]),
+    "mcx_gated_recurrence_backward": (_i, [_p] * 12 + [_sz, _rdesc, _i, _p]),
     "mcx_group_norm_workspace": (_sz, [_i64] * 4 + [_i, _i]),
     "mcx_group_norm_forward": (_i, [_p] * 6 + [_sz, _pi64] + [_i64] * 4 + [_f64, _i, _i, _p]),
     "mcx_group_norm_backward": (_i, [_p] * 9 + [_sz, _pi64] + [_i64] * 4 + [_i, _i, _p]),
