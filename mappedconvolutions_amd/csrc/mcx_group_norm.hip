@@ -11,6 +11,7 @@
 // mean far from zero costs nothing.  Statistics of the parts, then products: two launches forward, and
 // a third between them backward that joins the parts' sums.  No atomics: the same bits from call to call.
 #include <algorithm>
+#include <type_traits>
 
 #include "mcx_mfma_common.h"
 
@@ -21,6 +22,8 @@ constexpr int kThreads = 256;
 constexpr int kRows = 8;        // tokens of a block
 constexpr int kBlocks = 2048;   // workgroups aimed at
 constexpr int kMostParts = 256;
+constexpr int kAtOnce = 4;      // tokens whose loads are under way together
+constexpr int kJoin = 16;       // channels, or whole groups, of a workgroup that joins parts
 
 enum { kNone = 0, kSilu = 1, kGelu = 2 };
 
@@ -58,22 +61,53 @@ template <typename T> struct Word<T, 1> {
   static __device__ inline void store(T *p, const float *v) { *p = (T)v[0]; }
 };
 
-__device__ inline float logistic(float x) { return 1.f / (1.f + expf(-x)); }
+// e^x and 1 / (1 + e^-x), to a few units in the last place: the hardware's powers of two and reciprocals,
+// in single precision with what the product's rounding takes put back.
+template <bool Fine> __device__ inline float exponential(float x) {
+  constexpr float kLog2e = 1.44269504f, kRest = 1.92596299e-8f;
+  const float t = x * kLog2e;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return Fine ? fmaf(e, 0.69314718f * fmaf(x, kRest, fmaf(x, kLog2e, -t)), e) : e;
+}
+template <bool Fine> __device__ inline float logistic(float x) {
+  x = x < -80.f ? -80.f : x;  // (what is no number stays none)
+  if (Fine) x = x > 80.f ? 80.f : x;
+  return __builtin_amdgcn_rcpf(1.f + exponential<Fine>(-x));
+}
+// (1 + erf(u / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun, off by 7.5e-8 at most; `bell` is
+// e^(-u^2 / 2).  It costs a third of the library's erf, which the vector units took longer for than memory.
+template <bool Fine> __device__ inline float normal(float u, float &bell) {
+  const float x = fabsf(u) * 0.70710678f;
+  const float q = u * u;
+  bell = exponential<Fine>(q < 170.f ? -0.5f * q : -85.f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+  float s = fmaf(1.061405429f, t, -1.453152027f);
+  s = fmaf(s, t, 1.421413741f);
+  s = fmaf(s, t, -0.284496736f);
+  s = fmaf(s, t, 0.254829592f);
+  s = 0.5f * s * t * bell;
+  return u < 0.f ? s : 1.f - s;
+}
 
-template <int Act> __device__ inline float act(float u) {
-  if (Act == kSilu) return u * logistic(u);
-  if (Act == kGelu) return 0.5f * u * (1.f + erff(u * 0.70710678f));
+template <int Act, bool Fine> __device__ inline float act(float u) {
+  float bell;
+  if (Act == kSilu) return u * logistic<Fine>(u);
+  if (Act == kGelu) return u * normal<Fine>(u, bell);
   return u;
 }
-template <int Act> __device__ inline float act_slope(float u) {
+template <int Act, bool Fine> __device__ inline float act_slope(float u) {
   if (Act == kSilu) {
-    const float s = logistic(u);
-    return s * (1.f + u * (1.f - s));
+    const float s = logistic<Fine>(u);
+    return s * fmaf(u, 1.f - s, 1.f);
   }
-  if (Act == kGelu)
-    return 0.5f * (1.f + erff(u * 0.70710678f)) + u * expf(-0.5f * u * u) * 0.39894228f;
+  if (Act == kGelu) {
+    float bell;
+    const float n = normal<Fine>(u, bell);
+    return fmaf(u * bell, 0.39894228f, n);
+  }
   return 1.f;
 }
+template <typename T> constexpr bool kFine = sizeof(T) == 4;
 
 // Where a workgroup and its threads stand.
 struct Place {
@@ -95,6 +129,14 @@ template <int E> __device__ inline Place place_of(const GroupParams &p, int64_t 
   a.lane = threadIdx.x / a.across, a.col = threadIdx.x % a.across;
   a.row = (int64_t)a.part * p.rows, a.end = min(p.N, a.row + p.rows);
   return a;
+}
+
+// A thread's tokens of the part: f(count, first) for `Count` of them at a time, then one by one.
+template <int Count, typename F> __device__ inline void walk(const Place &a, F f) {
+  int64_t r = a.row + a.lane;
+  for (; r + (int64_t)(Count - 1) * a.lanes < a.end; r += (int64_t)Count * a.lanes)
+    f(std::integral_constant<int, Count>(), r);
+  for (; r < a.end; r += a.lanes) f(std::integral_constant<int, 1>(), r);
 }
 
 // Count, mean and squared deviations, and those of a block merged into them.
@@ -258,14 +300,19 @@ __global__ __launch_bounds__(kThreads) void group_apply_kernel(GroupParams p) {
     const Channels<T, E> ch(p, a, stats, col);
     const T *x = (const T *)p.x + a.b * p.xs[0] + a.c0 + col * E;
     T *y = (T *)p.y + (int64_t)a.b * p.N * p.C + a.c0 + col * E;
-    for (int64_t r = a.row + a.lane; r < a.end; r += a.lanes) {
-      float v[E];
-      Word<T, E>::load(x + r * p.xs[1], v);
+    walk<kAtOnce>(a, [&](auto count, int64_t r) {
+      constexpr int K = decltype(count)::value;
+      float v[K][E];
 #pragma unroll
-      for (int e = 0; e < E; e++)
-        v[e] = act<Act>(fmaf((v[e] - ch.mean[e]) * ch.r[e], ch.w[e], ch.b[e]));
-      Word<T, E>::store(y + r * p.C, v);
-    }
+      for (int k = 0; k < K; k++) Word<T, E>::load(x + (r + (int64_t)k * a.lanes) * p.xs[1], v[k]);
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          v[k][e] = act<Act, kFine<T>>(fmaf((v[k][e] - ch.mean[e]) * ch.r[e], ch.w[e], ch.b[e]));
+        Word<T, E>::store(y + (r + (int64_t)k * a.lanes) * p.C, v[k]);
+      }
+    });
   }
 }
 
@@ -284,17 +331,23 @@ __global__ __launch_bounds__(kThreads) void group_sums_kernel(GroupParams p) {
       const Channels<T, E> ch(p, a, stats, col);
       const T *x = (const T *)p.x + a.b * p.xs[0] + a.c0 + col * E;
       const T *gy = (const T *)p.gy + (int64_t)a.b * p.N * p.C + a.c0 + col * E;
-      for (int64_t r = a.row + a.lane; r < a.end; r += a.lanes) {
-        float v[E], g[E];
-        Word<T, E>::load(x + r * p.xs[1], v);
-        Word<T, E>::load(gy + r * p.C, g);
+      walk<kAtOnce>(a, [&](auto count, int64_t r) {
+        constexpr int K = decltype(count)::value;
+        float v[K][E], g[K][E];
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-          const float n = (v[e] - ch.mean[e]) * ch.r[e];
-          const float d = g[e] * act_slope<Act>(fmaf(n, ch.w[e], ch.b[e]));
-          s1[e] += d, s2[e] = fmaf(d, n, s2[e]);
+        for (int k = 0; k < K; k++) {
+          Word<T, E>::load(x + (r + (int64_t)k * a.lanes) * p.xs[1], v[k]);
+          Word<T, E>::load(gy + (r + (int64_t)k * a.lanes) * p.C, g[k]);
         }
-      }
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+          for (int e = 0; e < E; e++) {
+            const float n = (v[k][e] - ch.mean[e]) * ch.r[e];
+            const float d = g[k][e] * act_slope<Act, kFine<T>>(fmaf(n, ch.w[e], ch.b[e]));
+            s1[e] += d, s2[e] = fmaf(d, n, s2[e]);
+          }
+      });
     }
     __syncthreads();
 #pragma unroll
@@ -313,21 +366,30 @@ __global__ __launch_bounds__(kThreads) void group_sums_kernel(GroupParams p) {
   }
 }
 
-// The sums over the parts of a sample's slab, and the means of w g and w g n of its groups.
+// The sums over the parts of a sample's groups (kJoin channels of them, or one), and the means of w g and
+// w g n.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void group_join_kernel(GroupParams p) {
+__global__ __launch_bounds__(kThreads) void group_join_kernel(GroupParams p, int several, int jobs) {
   __shared__ float part[kThreads];
-  const int s = blockIdx.x % p.slabs, b = blockIdx.x / p.slabs;
-  const int g0 = s * p.slab, groups = min(p.slab, p.G - g0), c0 = g0 * p.per;
-  const int all = groups * p.per * 2;  // sums of the slab
+  const int b = blockIdx.x / jobs, g0 = blockIdx.x % jobs * several, groups = min(several, p.G - g0);
+  const int c0 = g0 * p.per, all = groups * p.per * 2;  // sums
   const int across = min(all, kThreads), lanes = kThreads / across;
   const int lane = threadIdx.x / across, col = threadIdx.x % across;
   float *sums = p.sums + ((int64_t)b * p.C + c0) * 2;
   for (int first = 0; first < all; first += across) {
     float x = 0.f;
-    if (lane < lanes && first + col < all)
-      for (int i = lane; i < p.parts; i += lanes)
-        x += p.partial[(((int64_t)b * p.parts + i) * p.C + c0) * 2 + first + col];
+    if (lane < lanes && first + col < all) {
+      const float *from = p.partial + ((int64_t)b * p.parts * p.C + c0) * 2 + first + col;
+      int i = lane;
+      for (; i + 7 * lanes < p.parts; i += 8 * lanes) {
+        float y[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) y[k] = from[(int64_t)(i + k * lanes) * p.C * 2];
+#pragma unroll
+        for (int k = 0; k < 8; k++) x += y[k];
+      }
+      for (; i < p.parts; i += lanes) x += from[(int64_t)i * p.C * 2];
+    }
     __syncthreads();
     part[threadIdx.x] = x;
     __syncthreads();
@@ -373,18 +435,25 @@ __global__ __launch_bounds__(kThreads) void group_gradient_kernel(GroupParams p)
       const int64_t from = (int64_t)a.b * p.N * p.C + a.c0 + col * E;
       const T *gy = (const T *)p.gy + from;
       T *gx = (T *)p.gx + from;
-      for (int64_t r = a.row + a.lane; r < a.end; r += a.lanes) {
-        float v[E], g[E];
-        Word<T, E>::load(x + r * p.xs[1], v);
-        Word<T, E>::load(gy + r * p.C, g);
+      walk<kAtOnce>(a, [&](auto count, int64_t r) {
+        constexpr int K = decltype(count)::value;
+        float v[K][E], g[K][E];
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-          const float n = (v[e] - ch.mean[e]) * ch.r[e];
-          const float d = g[e] * act_slope<Act>(fmaf(n, ch.w[e], ch.b[e])) * ch.w[e];
-          v[e] = ch.r[e] * (d - m1[e] - n * m2[e]);
+        for (int k = 0; k < K; k++) {
+          Word<T, E>::load(x + (r + (int64_t)k * a.lanes) * p.xs[1], v[k]);
+          Word<T, E>::load(gy + (r + (int64_t)k * a.lanes) * p.C, g[k]);
         }
-        Word<T, E>::store(gx + r * p.C, v);
-      }
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+          for (int e = 0; e < E; e++) {
+            const float n = (v[k][e] - ch.mean[e]) * ch.r[e];
+            const float d = g[k][e] * act_slope<Act, kFine<T>>(fmaf(n, ch.w[e], ch.b[e])) * ch.w[e];
+            v[k][e] = ch.r[e] * (d - m1[e] - n * m2[e]);
+          }
+          Word<T, E>::store(gx + (r + (int64_t)k * a.lanes) * p.C, v[k]);
+        }
+      });
     }
   // one workgroup of each slab: the sums over the samples
   if (a.b || a.part || (!p.gw && !p.gb)) return;
@@ -479,7 +548,8 @@ int launch_backward(const GroupParams &p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)p.B * p.slabs * p.parts)), threads(kThreads);
   hipLaunchKernelGGL((group_sums_kernel<T, E, Act>), grid, threads, 0, s, p);
   MCX_HIP_CHECK_LAUNCH();
-  hipLaunchKernelGGL((group_join_kernel<T>), dim3(p.B * p.slabs), threads, 0, s, p);
+  const int several = std::min(p.G, std::max(1, kJoin / p.per)), jobs = (p.G + several - 1) / several;
+  hipLaunchKernelGGL((group_join_kernel<T>), dim3((unsigned)(p.B * jobs)), threads, 0, s, p, several, jobs);
   MCX_HIP_CHECK_LAUNCH();
   hipLaunchKernelGGL((group_gradient_kernel<T, E, Act>), grid, threads, 0, s, p);
   MCX_HIP_CHECK_LAUNCH();
