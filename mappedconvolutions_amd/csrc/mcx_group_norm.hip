@@ -70,22 +70,23 @@ template <bool Fine> __device__ inline float exponential(float x) {
   return Fine ? fmaf(e, 0.69314718f * fmaf(x, kRest, fmaf(x, kLog2e, -t)), e) : e;
 }
 template <bool Fine> __device__ inline float logistic(float x) {
-  x = x < -80.f ? -80.f : x;  // (what is no number stays none)
-  if (Fine) x = x > 80.f ? 80.f : x;
+  if (Fine) {  // (an infinite power has no rounding to put back; what is no number stays none)
+    x = x < -80.f ? -80.f : x;
+    x = x > 80.f ? 80.f : x;
+  }
   return __builtin_amdgcn_rcpf(1.f + exponential<Fine>(-x));
 }
 // (1 + erf(u / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun, off by 7.5e-8 at most; `bell` is
 // e^(-u^2 / 2).  It costs a third of the library's erf, which the vector units took longer for than memory.
 template <bool Fine> __device__ inline float normal(float u, float &bell) {
-  const float x = fabsf(u) * 0.70710678f;
-  const float q = u * u;
-  bell = exponential<Fine>(q < 170.f ? -0.5f * q : -85.f);
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
-  float s = fmaf(1.061405429f, t, -1.453152027f);
-  s = fmaf(s, t, 1.421413741f);
-  s = fmaf(s, t, -0.284496736f);
-  s = fmaf(s, t, 0.254829592f);
-  s = 0.5f * s * t * bell;
+  const float q = Fine ? fminf(u * u, 170.f) : u * u;
+  bell = Fine ? exponential<true>(-0.5f * q) : __builtin_amdgcn_exp2f(-0.72134752f * q);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.23164190f, fabsf(u), 1.f));
+  float s = fmaf(0.5307027145f, t, -0.7265760135f);
+  s = fmaf(s, t, 0.7107068705f);
+  s = fmaf(s, t, -0.142248368f);
+  s = fmaf(s, t, 0.127414796f);
+  s = s * t * bell;
   return u < 0.f ? s : 1.f - s;
 }
 
@@ -270,14 +271,20 @@ __device__ inline void join_stats(const GroupParams &p, const Place &a, float *s
   }
 }
 
-// A thread's channels: mean, r, weight and bias of each.
+// A thread's channels.  n = x r - mean r in one step where x has few bits itself (its own are lost before
+// the product's rounding is); in single precision the difference first.
 template <typename T, int E> struct Channels {
   float mean[E], r[E], w[E], b[E];
+  __device__ inline float norm(float x, int e) const {
+    return kFine<T> ? (x - mean[e]) * r[e] : fmaf(x, r[e], mean[e]);
+  }
+  __device__ inline float scaled(float x, int e) const { return fmaf(norm(x, e), w[e], b[e]); }
   __device__ inline Channels(const GroupParams &p, const Place &a, const float *stats, int col) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const int c = col * E + e, g = c / p.per;
       mean[e] = stats[2 * g], r[e] = stats[2 * g + 1];
+      if (!kFine<T>) mean[e] *= -r[e];
       w[e] = p.w ? (float)((const T *)p.w)[a.c0 + c] : 1.f;
       b[e] = p.b ? (float)((const T *)p.b)[a.c0 + c] : 0.f;
     }
@@ -309,7 +316,7 @@ __global__ __launch_bounds__(kThreads) void group_apply_kernel(GroupParams p) {
       for (int k = 0; k < K; k++) {
 #pragma unroll
         for (int e = 0; e < E; e++)
-          v[k][e] = act<Act, kFine<T>>(fmaf((v[k][e] - ch.mean[e]) * ch.r[e], ch.w[e], ch.b[e]));
+          v[k][e] = act<Act, kFine<T>>(ch.scaled(v[k][e], e));
         Word<T, E>::store(y + (r + (int64_t)k * a.lanes) * p.C, v[k]);
       }
     });
@@ -343,7 +350,7 @@ __global__ __launch_bounds__(kThreads) void group_sums_kernel(GroupParams p) {
         for (int k = 0; k < K; k++)
 #pragma unroll
           for (int e = 0; e < E; e++) {
-            const float n = (v[k][e] - ch.mean[e]) * ch.r[e];
+            const float n = ch.norm(v[k][e], e);
             const float d = g[k][e] * act_slope<Act, kFine<T>>(fmaf(n, ch.w[e], ch.b[e]));
             s1[e] += d, s2[e] = fmaf(d, n, s2[e]);
           }
@@ -425,11 +432,12 @@ __global__ __launch_bounds__(kThreads) void group_gradient_kernel(GroupParams p)
   if (p.gx && a.lane < a.lanes)
     for (int col = a.col; col < a.words; col += a.across) {
       const Channels<T, E> ch(p, a, stats, col);
-      float m1[E], m2[E];
+      float m1[E], m2[E], wr[E];  // (times r in bf16)
 #pragma unroll
       for (int e = 0; e < E; e++) {
         const int g = (col * E + e) / p.per;
-        m1[e] = means[2 * g], m2[e] = means[2 * g + 1];
+        const float r = kFine<T> ? 1.f : ch.r[e];
+        m1[e] = -means[2 * g] * r, m2[e] = -means[2 * g + 1] * r, wr[e] = ch.w[e] * r;
       }
       const T *x = (const T *)p.x + a.b * p.xs[0] + a.c0 + col * E;
       const int64_t from = (int64_t)a.b * p.N * p.C + a.c0 + col * E;
@@ -447,9 +455,10 @@ __global__ __launch_bounds__(kThreads) void group_gradient_kernel(GroupParams p)
         for (int k = 0; k < K; k++) {
 #pragma unroll
           for (int e = 0; e < E; e++) {
-            const float n = (v[k][e] - ch.mean[e]) * ch.r[e];
-            const float d = g[k][e] * act_slope<Act, kFine<T>>(fmaf(n, ch.w[e], ch.b[e])) * ch.w[e];
-            v[k][e] = ch.r[e] * (d - m1[e] - n * m2[e]);
+            const float n = ch.norm(v[k][e], e);
+            const float d = g[k][e] * act_slope<Act, kFine<T>>(fmaf(n, ch.w[e], ch.b[e]));
+            v[k][e] = kFine<T> ? ch.r[e] * ((d * ch.w[e] + m1[e]) + n * m2[e])
+                               : fmaf(d, wr[e], fmaf(n, m2[e], m1[e]));
           }
           Word<T, E>::store(gx + (r + (int64_t)k * a.lanes) * p.C, v[k]);
         }
