@@ -20,9 +20,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRows = 8;        // tokens of a block
-constexpr int kBlocks = 2048;   // workgroups aimed at
+constexpr int kBlocks = 1024;   // workgroups aimed at (2048: 32 x 2048 tokens of 512 channels 142 -> 157 us)
 constexpr int kMostParts = 256;
 constexpr int kAtOnce = 4;      // tokens whose loads are under way together
+// Tensors of which two do not fit half the last-level cache: results that stay in it push out the input
+// that is read a second time (8 x 131072 tokens of 64 channels, forward and gradients 230 -> 211 us).
+constexpr int64_t kPassingBytes = 64 << 20;
 constexpr int kJoin = 16;       // channels, or whole groups, of a workgroup that joins parts
 
 enum { kNone = 0, kSilu = 1, kGelu = 2 };
@@ -49,16 +52,18 @@ template <typename T, int E> struct Word {
 #pragma unroll
     for (int e = 0; e < E; e++) v[e] = (float)w[e];
   }
-  static __device__ inline void store(T *p, const float *v) {
+  // Passing: past the cache
+  template <bool Passing> static __device__ inline void store(T *p, const float *v) {
     Vec w;
 #pragma unroll
     for (int e = 0; e < E; e++) w[e] = (T)v[e];
-    *(Vec *)p = w;
+    if (Passing) __builtin_nontemporal_store(w, (Vec *)p);
+    else *(Vec *)p = w;
   }
 };
 template <typename T> struct Word<T, 1> {
   static __device__ inline void load(const T *p, float *v) { v[0] = (float)*p; }
-  static __device__ inline void store(T *p, const float *v) { *p = (T)v[0]; }
+  template <bool> static __device__ inline void store(T *p, const float *v) { *p = (T)v[0]; }
 };
 
 // e^x and 1 / (1 + e^-x), to a few units in the last place: the hardware's powers of two and reciprocals,
@@ -271,29 +276,63 @@ __device__ inline void join_stats(const GroupParams &p, const Place &a, float *s
   }
 }
 
-// A thread's channels.  n = x r - mean r in one step where x has few bits itself (its own are lost before
-// the product's rounding is); in single precision the difference first.
-template <typename T, int E> struct Channels {
-  float mean[E], r[E], w[E], b[E];
+// A thread's channels (Own: of several groups).  n = x r - mean r in one step where x has few bits itself (its
+// own are lost before the product's rounding is); in single precision the difference first.
+template <typename T, int E, bool Own = true> struct Channels {
+  static constexpr int M = Own ? E : 1;
+  float mean[M], r[M], w[E], b[E];
   __device__ inline float norm(float x, int e) const {
-    return kFine<T> ? (x - mean[e]) * r[e] : fmaf(x, r[e], mean[e]);
+    const int m = Own ? e : 0;
+    return kFine<T> ? (x - mean[m]) * r[m] : fmaf(x, r[m], mean[m]);
   }
   __device__ inline float scaled(float x, int e) const { return fmaf(norm(x, e), w[e], b[e]); }
-  __device__ inline Channels(const GroupParams &p, const Place &a, const float *stats, int col) {
+  __device__ inline Channels(const GroupParams &p, const Place &a, int col) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const int c = col * E + e, g = c / p.per;
-      mean[e] = stats[2 * g], r[e] = stats[2 * g + 1];
-      if (!kFine<T>) mean[e] *= -r[e];
-      w[e] = p.w ? (float)((const T *)p.w)[a.c0 + c] : 1.f;
-      b[e] = p.b ? (float)((const T *)p.b)[a.c0 + c] : 0.f;
+      w[e] = p.w ? (float)((const T *)p.w)[a.c0 + col * E + e] : 1.f;
+      b[e] = p.b ? (float)((const T *)p.b)[a.c0 + col * E + e] : 0.f;
     }
+  }
+  __device__ inline Channels(const GroupParams &p, const Place &a, const float *stats, int col)
+      : Channels(p, a, col) {
+    take(p, stats, col);
+  }
+  __device__ inline void take(const GroupParams &p, const float *stats, int col) {
+    int g = col * E / p.per, rest = col * E - g * p.per;
+#pragma unroll
+    for (int m = 0; m < M; m++) {
+      mean[m] = stats[2 * g], r[m] = stats[2 * g + 1];
+      if (!kFine<T>) mean[m] *= -r[m];
+      if (++rest == p.per) rest = 0, g++;
+    }
+  }
+};
+
+// gx from n and g, for a thread's channels.
+template <typename T, int E, bool Own = true> struct Slope {
+  static constexpr int M = Own ? E : 1;
+  float m1[M], m2[M], wr[E];  // (times r in bf16)
+  __device__ inline Slope(const GroupParams &p, const Channels<T, E, Own> &ch, const float *means, int col) {
+    int g = col * E / p.per, rest = col * E - g * p.per;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const float r = kFine<T> ? 1.f : ch.r[Own ? e : 0];
+      if (e < M) {
+        m1[e] = -means[2 * g] * r, m2[e] = -means[2 * g + 1] * r;
+        if (++rest == p.per) rest = 0, g++;
+      }
+      wr[e] = ch.w[e] * r;
+    }
+  }
+  __device__ inline float value(const Channels<T, E, Own> &ch, float n, float d, int e) const {
+    const int m = Own ? e : 0;
+    return kFine<T> ? ch.r[m] * ((d * ch.w[e] + m1[m]) + n * m2[m]) : fmaf(d, wr[e], fmaf(n, m2[m], m1[m]));
   }
 };
 
 extern __shared__ float dynamic[];
 
-template <typename T, int E, int Act>
+template <typename T, int E, int Act, bool Passing>
 __global__ __launch_bounds__(kThreads) void group_apply_kernel(GroupParams p) {
   const Place a = place_of<E>(p, gridDim.x - 1 - (int64_t)blockIdx.x);
   float *stats = dynamic;  // [slab][2]
@@ -317,7 +356,7 @@ __global__ __launch_bounds__(kThreads) void group_apply_kernel(GroupParams p) {
 #pragma unroll
         for (int e = 0; e < E; e++)
           v[k][e] = act<Act, kFine<T>>(ch.scaled(v[k][e], e));
-        Word<T, E>::store(y + (r + (int64_t)k * a.lanes) * p.C, v[k]);
+        Word<T, E>::template store<Passing>(y + (r + (int64_t)k * a.lanes) * p.C, v[k]);
       }
     });
   }
@@ -423,7 +462,38 @@ __global__ __launch_bounds__(kThreads) void group_join_kernel(GroupParams p, int
   }
 }
 
-template <typename T, int E, int Act>
+// gw and gb of a slab's channels: the sums over the samples.
+template <typename T, int Threads>
+__device__ inline void sum_samples(const GroupParams &p, int c0, int channels, float *part) {
+  if (!p.gw && !p.gb) return;
+  const int across = min(channels, Threads), lanes = Threads / across;
+  const int lane = threadIdx.x / across, col = threadIdx.x % across;
+  for (int first = 0; first < channels; first += across) {
+    const int c = first + col;
+    float x1 = 0.f, x2 = 0.f;
+    if (lane < lanes && c < channels) {
+      const float *from = p.sums + (int64_t)(c0 + c) * 2;
+#pragma unroll 4
+      for (int b = lane; b < p.B; b += lanes) {
+        x1 += from[(int64_t)b * p.C * 2];
+        x2 += from[(int64_t)b * p.C * 2 + 1];
+      }
+    }
+    __syncthreads();
+    part[threadIdx.x] = x1, part[Threads + threadIdx.x] = x2;
+    __syncthreads();
+    if (lane == 0 && c < channels) {
+      for (int l = 1; l < lanes; l++) {
+        x1 += part[l * across + col];
+        x2 += part[Threads + l * across + col];
+      }
+      if (p.gb) ((T *)p.gb)[c0 + c] = (T)x1;
+      if (p.gw) ((T *)p.gw)[c0 + c] = (T)x2;
+    }
+  }
+}
+
+template <typename T, int E, int Act, bool Passing>
 __global__ __launch_bounds__(kThreads) void group_gradient_kernel(GroupParams p) {
   __shared__ float part[kThreads * 2];
   const Place a = place_of<E>(p, gridDim.x - 1 - (int64_t)blockIdx.x);
@@ -432,13 +502,7 @@ __global__ __launch_bounds__(kThreads) void group_gradient_kernel(GroupParams p)
   if (p.gx && a.lane < a.lanes)
     for (int col = a.col; col < a.words; col += a.across) {
       const Channels<T, E> ch(p, a, stats, col);
-      float m1[E], m2[E], wr[E];  // (times r in bf16)
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        const int g = (col * E + e) / p.per;
-        const float r = kFine<T> ? 1.f : ch.r[e];
-        m1[e] = -means[2 * g] * r, m2[e] = -means[2 * g + 1] * r, wr[e] = ch.w[e] * r;
-      }
+      const Slope<T, E> slope(p, ch, means, col);
       const T *x = (const T *)p.x + a.b * p.xs[0] + a.c0 + col * E;
       const int64_t from = (int64_t)a.b * p.N * p.C + a.c0 + col * E;
       const T *gy = (const T *)p.gy + from;
@@ -457,37 +521,228 @@ __global__ __launch_bounds__(kThreads) void group_gradient_kernel(GroupParams p)
           for (int e = 0; e < E; e++) {
             const float n = ch.norm(v[k][e], e);
             const float d = g[k][e] * act_slope<Act, kFine<T>>(fmaf(n, ch.w[e], ch.b[e]));
-            v[k][e] = kFine<T> ? ch.r[e] * ((d * ch.w[e] + m1[e]) + n * m2[e])
-                               : fmaf(d, wr[e], fmaf(n, m2[e], m1[e]));
+            v[k][e] = slope.value(ch, n, d, e);
           }
-          Word<T, E>::store(gx + (r + (int64_t)k * a.lanes) * p.C, v[k]);
+          Word<T, E>::template store<Passing>(gx + (r + (int64_t)k * a.lanes) * p.C, v[k]);
         }
       });
     }
-  // one workgroup of each slab: the sums over the samples
-  if (a.b || a.part || (!p.gw && !p.gb)) return;
-  const int across = min(a.channels, kThreads), lanes = kThreads / across;
-  const int lane = threadIdx.x / across, col = threadIdx.x % across;
-  for (int first = 0; first < a.channels; first += across) {
-    const int c = first + col;
-    float x1 = 0.f, x2 = 0.f;
-    if (lane < lanes && c < a.channels)
-      for (int b = lane; b < p.B; b += lanes) {
-        x1 += p.sums[((int64_t)b * p.C + a.c0 + c) * 2];
-        x2 += p.sums[((int64_t)b * p.C + a.c0 + c) * 2 + 1];
-      }
+  // one workgroup of each slab
+  if (a.b == 0 && a.part == 0) sum_samples<T, kThreads>(p, a.c0, a.channels, part);
+}
+
+// ---- samples whose slab a workgroup holds ----
+//
+// Up to kHeld words a thread stay in registers between the statistics and the products, so that everything
+// is read once, by one launch (and a second small one for the sums over the samples).
+
+constexpr int kHeld = 8;
+constexpr int kHeldWords = 32;            // words of a slab at most
+constexpr int kHeldSlots = kHeldWords * 8;
+
+template <typename T, int E> struct Kept {
+  typedef T Vec __attribute__((ext_vector_type(E)));
+  Vec x;
+  __device__ inline void load(const T *p) { x = *(const Vec *)p; }
+  __device__ inline float operator[](int e) const { return (float)x[e]; }
+};
+template <typename T> struct Kept<T, 1> {
+  T x;
+  __device__ inline void load(const T *p) { x = *p; }
+  __device__ inline float operator[](int) const { return (float)x; }
+};
+
+// The threads' values summed over the rows of threads into slots [across * M]: by lane exchange within a wave
+// where rows are a power of two of lanes, through LDS otherwise.
+template <int Threads, int M>
+__device__ inline void sum_rows(const Place &a, float *values, float *all, float *some, float *slots) {
+  const int n = a.across * M;
+  __syncthreads();
+  if ((a.across & (a.across - 1)) == 0) {
+    for (int d = a.across; d < 64; d <<= 1)
+#pragma unroll
+      for (int m = 0; m < M; m++) values[m] += __shfl_xor(values[m], d);
+    if ((threadIdx.x & 63) < a.across)
+#pragma unroll
+      for (int m = 0; m < M; m++) all[(threadIdx.x >> 6) * n + a.col * M + m] = values[m];
     __syncthreads();
-    part[threadIdx.x] = x1, part[kThreads + threadIdx.x] = x2;
+    for (int i = threadIdx.x; i < n; i += Threads) {
+      float x = all[i];
+#pragma unroll
+      for (int w = 1; w < Threads / 64; w++) x += all[w * n + i];
+      slots[i] = x;
+    }
     __syncthreads();
-    if (lane == 0 && c < a.channels) {
-      for (int l = 1; l < lanes; l++) {
-        x1 += part[l * across + col];
-        x2 += part[kThreads + l * across + col];
-      }
-      if (p.gb) ((T *)p.gb)[a.c0 + c] = (T)x1;
-      if (p.gw) ((T *)p.gw)[a.c0 + c] = (T)x2;
+    return;
+  }
+  // (two sums one after the other, of about as many values each)
+  const int several = max(1, min(Threads / n, 8));
+#pragma unroll
+  for (int m = 0; m < M; m++) all[threadIdx.x * M + m] = values[m];
+  __syncthreads();
+  for (int i = threadIdx.x; i < n * several; i += Threads) {
+    const int first = i / n, slot = i - first * n;
+    float x = 0.f;
+    for (int l = first; l < a.lanes; l += several) x += all[l * n + slot];
+    some[i] = x;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += Threads) {
+    float x = some[i];
+    for (int k = 1; k < several; k++) x += some[k * n + i];
+    slots[i] = x;
+  }
+  __syncthreads();
+}
+
+template <int Threads, int E> __device__ inline Place held_place(const GroupParams &p) {
+  Place a;
+  const int index = xcd_contiguous_tile(blockIdx.x, gridDim.x), s = index % p.slabs;
+  a.b = index / p.slabs, a.part = 0;
+  a.g0 = s * p.slab, a.groups = min(p.slab, p.G - a.g0);
+  a.c0 = a.g0 * p.per, a.channels = a.groups * p.per;
+  a.words = a.across = a.channels / E;
+  a.lanes = Threads / a.across;
+  a.lane = threadIdx.x / a.across, a.col = threadIdx.x % a.across;
+  a.row = 0, a.end = p.N;
+  return a;
+}
+
+template <int Threads, typename T, int E, int Act, bool Own>
+__global__ __launch_bounds__(Threads) void group_held_kernel(GroupParams p) {
+  constexpr int M = Own ? E : 1;
+  __shared__ float all[Threads * M], some[Threads > kHeldSlots ? Threads : kHeldSlots], slots[kHeldSlots];
+  __shared__ float stats[kHeldSlots * 2];
+  const Place a = held_place<Threads, E>(p);
+  const bool here = a.lane < a.lanes;
+  const T *x = (const T *)p.x + a.b * p.xs[0] + a.c0 + a.col * E;
+  Kept<T, E> v[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; k++) {
+    const int64_t r = a.lane + (int64_t)k * a.lanes;
+    if (here && r < p.N) v[k].load(x + r * p.xs[1]);
+  }
+  Channels<T, E, Own> ch(p, a, here ? a.col : 0);
+  const float count = (float)p.N * p.per;
+  const int each = p.per * M / E;  // slots of a group
+  const int group = a.col * E / p.per, rest = a.col * E - group * p.per;
+  // the means first, then the squares of what differs from them
+  for (int pass = 0; pass < 2; pass++) {
+    float sum[M], mean[M];
+    int g = group, at = rest;
+#pragma unroll
+    for (int m = 0; m < M; m++) {
+      sum[m] = 0.f;
+      mean[m] = pass && here ? stats[2 * g] : 0.f;
+      if (++at == p.per) at = 0, g++;
+    }
+#pragma unroll
+    for (int k = 0; k < kHeld; k++)
+      if (here && a.lane + (int64_t)k * a.lanes < p.N)
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const int m = Own ? e : 0;
+          const float d = v[k][e] - mean[m];
+          sum[m] = pass ? fmaf(d, d, sum[m]) : sum[m] + d;
+        }
+    sum_rows<Threads, M>(a, sum, all, some, slots);
+    for (int g = threadIdx.x; g < a.groups; g += Threads) {
+      float s = 0.f;
+      for (int i = 0; i < each; i++) s += slots[g * each + i];
+      stats[2 * g + pass] = pass ? 1.f / sqrtf(s / count + p.eps) : s / count;
+    }
+    __syncthreads();
+  }
+  if (p.stats)
+    for (int i = threadIdx.x; i < 2 * a.groups; i += Threads)
+      p.stats[((int64_t)a.b * p.G + a.g0) * 2 + i] = stats[i];
+  if (!here) return;
+  ch.take(p, stats, a.col);
+  T *y = (T *)p.y + (int64_t)a.b * p.N * p.C + a.c0 + a.col * E;
+#pragma unroll
+  for (int k = 0; k < kHeld; k++) {
+    const int64_t r = a.lane + (int64_t)k * a.lanes;
+    if (r < p.N) {
+      float o[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) o[e] = act<Act, kFine<T>>(ch.scaled(v[k][e], e));
+      Word<T, E>::template store<false>(y + r * p.C, o);
     }
   }
+}
+
+template <int Threads, typename T, int E, int Act, bool Own>
+__global__ __launch_bounds__(Threads) void group_held_gradient_kernel(GroupParams p) {
+  __shared__ float all[Threads * E], some[Threads > kHeldSlots ? Threads : kHeldSlots];
+  __shared__ float sums[2][kHeldSlots], means[kHeldSlots * 2];
+  const Place a = held_place<Threads, E>(p);
+  const bool here = a.lane < a.lanes;
+  const int64_t dense = (int64_t)a.b * p.N * p.C + a.c0 + a.col * E;
+  const T *x = (const T *)p.x + a.b * p.xs[0] + a.c0 + a.col * E, *gy = (const T *)p.gy + dense;
+  Kept<T, E> v[kHeld], g[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; k++) {
+    const int64_t r = a.lane + (int64_t)k * a.lanes;
+    if (here && r < p.N) v[k].load(x + r * p.xs[1]), g[k].load(gy + r * p.C);
+  }
+  const Channels<T, E, Own> ch(p, a, p.stats + ((int64_t)a.b * p.G + a.g0) * 2, here ? a.col : 0);
+  float s1[E], s2[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) s1[e] = s2[e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < kHeld; k++)
+    if (here && a.lane + (int64_t)k * a.lanes < p.N)
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float n = ch.norm(v[k][e], e);
+        const float d = g[k][e] * act_slope<Act, kFine<T>>(fmaf(n, ch.w[e], ch.b[e]));
+        s1[e] += d, s2[e] = fmaf(d, n, s2[e]);
+      }
+  sum_rows<Threads, E>(a, s1, all, some, sums[0]);
+  sum_rows<Threads, E>(a, s2, all, some, sums[1]);
+  for (int i = threadIdx.x; i < a.channels; i += Threads) {
+    const int c = a.c0 + i;
+    if (p.sums) {
+      float *to = p.sums + ((int64_t)a.b * p.C + c) * 2;
+      to[0] = sums[0][i], to[1] = sums[1][i];
+    } else {  // the only sample
+      if (p.gb) ((T *)p.gb)[c] = (T)sums[0][i];
+      if (p.gw) ((T *)p.gw)[c] = (T)sums[1][i];
+    }
+  }
+  if (!p.gx) return;
+  const float count = (float)p.N * p.per;
+  for (int k = threadIdx.x; k < 2 * a.groups; k += Threads) {
+    const float *from = sums[k & 1] + (k >> 1) * p.per;
+    float s = 0.f;
+    for (int i = 0; i < p.per; i++)
+      s = fmaf(p.w ? (float)((const T *)p.w)[a.c0 + (k >> 1) * p.per + i] : 1.f, from[i], s);
+    means[k] = s / count;
+  }
+  __syncthreads();
+  if (!here) return;
+  T *gx = (T *)p.gx + dense;
+  const Slope<T, E, Own> slope(p, ch, means, a.col);
+#pragma unroll
+  for (int k = 0; k < kHeld; k++) {
+    const int64_t r = a.lane + (int64_t)k * a.lanes;
+    if (r < p.N) {
+      float o[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float n = ch.norm(v[k][e], e);
+        const float d = g[k][e] * act_slope<Act, kFine<T>>(fmaf(n, ch.w[e], ch.b[e]));
+        o[e] = slope.value(ch, n, d, e);
+      }
+      Word<T, E>::template store<false>(gx + r * p.C, o);
+    }
+  }
+}
+
+template <typename T> __global__ __launch_bounds__(kThreads) void group_samples_kernel(GroupParams p) {
+  __shared__ float part[kThreads * 2];
+  const int c0 = blockIdx.x * kJoin;
+  sum_samples<T, kThreads>(p, c0, min(kJoin, p.C - c0), part);
 }
 
 // ---- host ----
@@ -527,6 +782,29 @@ Split split_of(int64_t B, int64_t N, int64_t C, int64_t G, int size, uint64_t by
   return s;
 }
 
+// The slab of the held form: as wide as a workgroup holds, but no wider than 128 bytes unless that leaves
+// more than kHeldGroups workgroups; 0: a sample does not fit.  threads: of that workgroup.
+// Workgroups of 1024 threads leave nothing to load beside those that compute: they are for calls that other-
+// wise wait for launches (forward and gradients of 4096 tokens of 256 channels 36 -> 32 us; 16 of them 80 -> 96).
+constexpr int kHeldGroups = 512, kHeldAlone = 128;
+int held_slab(int64_t B, int64_t N, int64_t C, int64_t G, int word, int size, int *threads) {
+  const int per = (int)(C / G), least = word / common(per % word ? per : word, word);
+  const int64_t unit = (int64_t)least * per / word;  // words
+  if (unit > kHeldWords || N > 1024 * kHeld || (int64_t)least > G) return 0;
+  int64_t best = 0;
+  for (int64_t k = 1; k * least < G + least && k * unit <= kHeldWords; k++) {
+    const int64_t words = std::min(k * unit, C / word);
+    if (N > 1024 / words * kHeld) break;
+    if (best && (words * word * size > 128 || B * ((G + k * least - 1) / (k * least)) < kHeldGroups)) break;
+    best = k;
+  }
+  if (!best) return 0;
+  const int64_t slab = std::min(best * least, G), words = slab * per / word;
+  *threads = N <= 256 / words * kHeld ? 256 : 1024;
+  if (*threads > 256 && B * ((G + slab - 1) / slab) > kHeldAlone) return 0;
+  return (int)slab;
+}
+
 int check_sizes(int64_t B, int64_t N, int64_t C, int64_t G, int dtype) {
   if (dtype != MCX_F32 && dtype != MCX_BF16) return MCX_E_DTYPE;
   if (B < 0 || N < 0 || C < 1 || G < 1 || C % G || C > (1 << 20) || N > 0x7fffffffLL ||
@@ -540,27 +818,66 @@ uint64_t address_bits(const void *x, const int64_t *stride, int64_t B, int64_t N
          (N > 1 ? (uint64_t)stride[1] * size : 0);
 }
 
+template <int Threads, typename T, int E, int Act> int launch_held(const GroupParams &p, hipStream_t s) {
+  const dim3 grid((unsigned)(p.B * p.slabs)), threads(Threads);
+  if (p.per % E == 0) {
+    hipLaunchKernelGGL((p.gy ? group_held_gradient_kernel<Threads, T, E, Act, false>
+                             : group_held_kernel<Threads, T, E, Act, false>), grid, threads, 0, s, p);
+  } else if constexpr (E > 1) {
+    hipLaunchKernelGGL((p.gy ? group_held_gradient_kernel<Threads, T, E, Act, true>
+                             : group_held_kernel<Threads, T, E, Act, true>), grid, threads, 0, s, p);
+  }
+  MCX_HIP_CHECK_LAUNCH();
+  if (p.gy && p.sums && (p.gw || p.gb)) {
+    hipLaunchKernelGGL((group_samples_kernel<T>), dim3((p.C + kJoin - 1) / kJoin), dim3(kThreads), 0, s, p);
+    MCX_HIP_CHECK_LAUNCH();
+  }
+  return MCX_OK;
+}
+template <typename T, int E, int Act> int try_held(GroupParams p, hipStream_t s, bool *done) {
+  int threads = 0;
+  const int slab = held_slab(p.B, p.N, p.C, p.G, E, sizeof(T), &threads);
+  *done = slab > 0;
+  if (!slab) return MCX_OK;
+  p.slab = slab, p.slabs = (p.G + slab - 1) / slab;
+  if (p.gy && p.B == 1) p.sums = nullptr;
+  return threads == 256 ? launch_held<256, T, E, Act>(p, s) : launch_held<1024, T, E, Act>(p, s);
+}
+
+template <typename T, int E> bool passing(const GroupParams &p) {
+  return (int64_t)p.B * p.N * p.C * (int64_t)sizeof(T) >= kPassingBytes;
+}
+
 template <typename T, int E, int Act>
 int launch_forward(const GroupParams &p, hipStream_t s) {
+  bool done;
+  if (int e = try_held<T, E, Act>(p, s, &done); e || done) return e;
   const dim3 grid((unsigned)((int64_t)p.B * p.slabs * p.parts)), threads(kThreads);
-  if (p.per % E == 0 || p.slab == 1)
+  if (p.per % E == 0) {
     hipLaunchKernelGGL((group_stats_kernel<T, E, false>), grid, threads, 0, s, p);
-  else
+  } else if constexpr (E > 1) {
     hipLaunchKernelGGL((group_stats_kernel<T, E, true>), grid, threads, 0, s, p);
+  }
   MCX_HIP_CHECK_LAUNCH();
-  hipLaunchKernelGGL((group_apply_kernel<T, E, Act>), grid, threads, sizeof(float) * 2 * p.slab, s, p);
+  hipLaunchKernelGGL((passing<T, E>(p) ? group_apply_kernel<T, E, Act, E * sizeof(T) == 16>
+                                       : group_apply_kernel<T, E, Act, false>),
+                     grid, threads, sizeof(float) * 2 * p.slab, s, p);
   MCX_HIP_CHECK_LAUNCH();
   return MCX_OK;
 }
 template <typename T, int E, int Act>
 int launch_backward(const GroupParams &p, hipStream_t s) {
+  bool done;
+  if (int e = try_held<T, E, Act>(p, s, &done); e || done) return e;
   const dim3 grid((unsigned)((int64_t)p.B * p.slabs * p.parts)), threads(kThreads);
   hipLaunchKernelGGL((group_sums_kernel<T, E, Act>), grid, threads, 0, s, p);
   MCX_HIP_CHECK_LAUNCH();
   const int several = std::min(p.G, std::max(1, kJoin / p.per)), jobs = (p.G + several - 1) / several;
   hipLaunchKernelGGL((group_join_kernel<T>), dim3((unsigned)(p.B * jobs)), threads, 0, s, p, several, jobs);
   MCX_HIP_CHECK_LAUNCH();
-  hipLaunchKernelGGL((group_gradient_kernel<T, E, Act>), grid, threads, 0, s, p);
+  hipLaunchKernelGGL((passing<T, E>(p) ? group_gradient_kernel<T, E, Act, E * sizeof(T) == 16>
+                                       : group_gradient_kernel<T, E, Act, false>),
+                     grid, threads, 0, s, p);
   MCX_HIP_CHECK_LAUNCH();
   return MCX_OK;
 }
