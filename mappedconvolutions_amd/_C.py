@@ -1168,6 +1168,9 @@ def _pair(t):
     return _two(t.stride(0), t.stride(1))
 
 
+_RECURRENCE_STRIDE = 1 << 22
+
+
 def _recurrence_args(value, forget, gate, lengths, reverse):
     """(dtype code, descriptor, the tensors as the library takes them) of a recurrence call."""
     shape = value.shape
@@ -1185,8 +1188,10 @@ def _recurrence_args(value, forget, gate, lengths, reverse):
             raise RuntimeError("lengths must be int32 of shape (%d,), got %s %s" %
                                (B, lengths.dtype, tuple(lengths.shape)))
         lengths = lengths.contiguous()
-    value, forget, gate = (t if t is None or t.stride(2) == 1 or C == 1 else t.contiguous()
-                           for t in (value, forget, gate))
+    # (steps further apart than the kernels' addresses reach are copied)
+    value, forget, gate = (
+        t if t is None or ((t.stride(2) == 1 or C == 1) and t.stride(1) <= _RECURRENCE_STRIDE)
+        else t.contiguous() for t in (value, forget, gate))
     desc = _lib.RecurrenceDesc(B, L, C, _pair(value), _pair(forget),
                                _two(0, 0) if gate is None else _pair(gate), int(bool(reverse)), 0)
     return dt, desc, value, forget, gate, lengths

@@ -5,28 +5,40 @@
 //   gv = (1 - a) D,  gf = a (1 - a) (h_{t-1} - v) D,  gg = go h silu'(g),  gh_0 = p_0
 //
 // Bound by memory: 4 streams forward, 7 backward, and a few dozen operations a value.  Channels are
-// independent; a workgroup has 16 lanes' words of them and walks the steps in tiles, each lane with T
-// steps of its own.  h_t of a run of steps is A h + H of the state before it; the lanes' (A, H) are joined
-// within a wave by lane exchange and between waves through LDS, so a tile costs one barrier forward and
-// two backward.  States are kept for the gradients every kSpan steps and the others recomputed.  Where
-// sequences and channels are too few to fill the card the steps are cut into segments, whose (A, H) a
-// first launch sums up.
+// independent; a workgroup has 16 lanes' words of them and walks the steps in tiles, each lane with a run
+// of steps of its own and the next tile's values under way.  h_t of a run is A h + H of the state before
+// it; the lanes' (A, H) are joined within a wave by lane exchange and between waves through LDS, so a tile
+// costs one barrier forward and two backward.  States are kept for the gradients every kSpan steps and the
+// others recomputed.
+//   Where sequences and channels are too few to fill the card the steps are cut into segments, and a first
+// launch sums up the (A, H) of each: it reads two streams of four, or three of seven, a second time.  (Tiles
+// that wait for the state of the tile before them read everything once and took longer: 2 sequences of 32768
+// steps of 1024 bf16 channels forward 165 us and backward 312.)
 #include <algorithm>
+#include <type_traits>
 
 #include "mcx_mfma_common.h"
 
 namespace mcx {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kRowLanes = 16;           // lanes of a step's channels
 constexpr int kRuns = kThreads / kRowLanes;  // runs of steps of a tile
-constexpr int kForward = 8, kBackward = 4;   // steps of a run
-constexpr int kTile = kRuns * kForward;      // 256 steps
+constexpr int kForward = 4, kBackward = 4;   // steps of a run
+constexpr int kTile = kRuns * kForward;
 constexpr int kSpan = kRuns * kBackward;     // steps from one kept state to the next
-constexpr int kGroups = 512;            // workgroups aimed at
 constexpr int kFew = 8;                 // steps that a thread walks alone
+// Workgroups aimed at by segments: as many as are resident at a time (forward, float32 backward, bf16 back-
+// ward; 768 there: 2 sequences of 32768 steps of 1024 channels 440 -> 542 us), and by the parts of the first
+// launch; workgroups from which on there are no segments.
+constexpr int kGroups = 768, kGroupsBf16Backward = 512, kSums = 8192, kAlone = 512;
+constexpr int kWideRow = 40;           // words of a row from which on the first launch reads rows of 64 lanes
+// Tensors whose results would push out of the last-level cache what is read a second time (2 sequences of
+// 32768 steps of 1024 channels 473 -> 440 us); only whole lines are written past it (rows of 360 bytes: 50 -> 66).
+constexpr int64_t kPassingBytes = 64 << 20;
+constexpr int kLine = 128;
 
 struct RecurParams {
   const void *v, *f, *g, *go;
@@ -34,9 +46,11 @@ struct RecurParams {
   const int32_t *lengths;
   void *out, *gv, *gf, *gg;
   float *final, *ginitial, *states;  // states [B, ceil(L / kSpan), C]
-  float *part;                       // [B, segments, 2, C]: A, H of a segment
+  float *part;                       // [B, parts + 1, 2, C]: A and H of a part; the initial state
   int64_t vs[2], fs[2], gs[2];       // strides of sequence and step
-  int L, C, tiles, segments, segment;  // tiles of channels; steps of a segment
+  int L, C, tiles;                   // tiles of channels
+  int segments, segment;             // steps of a segment
+  int parts, each, share;            // parts of all steps, their steps, parts of a segment
   int spans, reverse;
 };
 
@@ -44,14 +58,17 @@ template <typename T, int E> struct Raw {
   typedef T Vec __attribute__((ext_vector_type(E)));
   Vec x;
   __device__ inline void load(const T *p) { x = *(const Vec *)p; }
+  __device__ inline void fill(float v) { x = Vec((T)v); }
   __device__ inline float operator[](int e) const { return (float)x[e]; }
 };
 template <typename T> struct Raw<T, 1> {
   T x;
   __device__ inline void load(const T *p) { x = *p; }
+  __device__ inline void fill(float v) { x = (T)v; }
   __device__ inline float operator[](int) const { return (float)x; }
 };
-template <typename T, int E> __device__ inline void put(T *p, const float *v) {
+// Passing: past the cache
+template <typename T, int E, bool Passing = false> __device__ inline void put(T *p, const float *v) {
   if constexpr (E == 1) {
     *p = (T)v[0];
   } else {
@@ -59,50 +76,86 @@ template <typename T, int E> __device__ inline void put(T *p, const float *v) {
     Vec w;
 #pragma unroll
     for (int e = 0; e < E; e++) w[e] = (T)v[e];
-    *(Vec *)p = w;
+    if (Passing) __builtin_nontemporal_store(w, (Vec *)p);
+    else *(Vec *)p = w;
   }
 }
 
-// sigmoid(x), and in `away` 1 - sigmoid(x) without its cancellation.  Fine: what the roundings of the
-// product and of the reciprocal took is put back; factors, whose errors add up over hundreds of steps,
-// are always computed so (3 us of 330 on 134 million bf16 values), output gates in single precision.
-template <bool Fine> __device__ inline float logistic(float x, float &away) {
-  x = x < -80.f ? -80.f : x;  // (what is no number stays none)
-  if (Fine) x = x > 200.f ? 200.f : x;
+// sigmoid(x), and in `away` 1 - sigmoid(x) without its cancellation.  The reciprocal is corrected once: the
+// errors of factors add up over hundreds of steps.  Fine: what the exponent's rounding took is put back too.
+template <bool Fine> __device__ inline float exponential(float x) {  // e^-x
   constexpr float kLog2e = 1.44269504f, kRest = 1.92596299e-8f;
-  const float t = -x * kLog2e;
-  float e = __builtin_amdgcn_exp2f(t);
-  if (Fine) e = fmaf(e, 0.69314718f * fmaf(-x, kRest, fmaf(-x, kLog2e, -t)), e);
-  const float sum = 1.f + e;
-  float a = __builtin_amdgcn_rcpf(sum);
-  if (Fine) a = fmaf(fmaf(-sum, a, 1.f), a, a);
+  const float t = -x * kLog2e, e = __builtin_amdgcn_exp2f(t);
+  return Fine ? fmaf(e, 0.69314718f * fmaf(-x, kRest, fmaf(-x, kLog2e, -t)), e) : e;
+}
+__device__ inline float reciprocal(float x) {
+  const float r = __builtin_amdgcn_rcpf(x);
+  return fmaf(fmaf(-x, r, 1.f), r, r);
+}
+template <bool Fine> __device__ inline float logistic(float x, float &away) {
+  x = __builtin_elementwise_maximum(x, -80.f);  // (what is no number stays none)
+  if (Fine) x = __builtin_elementwise_minimum(x, 200.f);
+  const float e = exponential<Fine>(x), a = reciprocal(1.f + e);
   away = e * a;
   return a;
+}
+// The same for an output gate, which nothing adds up over.
+template <bool Fine> __device__ inline float sigmoid(float x) {
+  float away;
+  return Fine ? logistic<true>(x, away) : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504f));
 }
 template <typename T> constexpr bool kFine = sizeof(T) == 4;
 
 struct Place {
-  int b, c, segment, len;  // c: this lane's first channel; len: steps in use
+  int b, segment, len;  // len: steps in use
+  int c;                // this lane's first channel
   bool here;
-  int wave, row, run;      // the run of a tile that the lane has, row of its wave
 };
-template <int E> __device__ inline Place place_of(const RecurParams &p, int segments) {
+// (what all lanes have in common in scalar registers: the addresses are these, and 32 bits a lane)
+template <int E, int RowLanes = kRowLanes>
+__device__ inline Place place_of(const RecurParams &p, int index, int segments) {
   Place a;
-  int index = blockIdx.x;
-  const int tile = index % p.tiles;
-  index /= p.tiles;
-  a.segment = index % segments;
-  a.b = index / segments;
-  a.c = (tile * kRowLanes + (threadIdx.x & (kRowLanes - 1))) * E;
+  const int columns = gridDim.x / segments;  // (neighbours have the same steps)
+  a.segment = index / columns;
+  index -= a.segment * columns;
+  a.b = index / p.tiles;
+  a.c = ((index - a.b * p.tiles) * RowLanes + (threadIdx.x & (RowLanes - 1))) * E;
   a.here = a.c < p.C;
-  a.len = p.lengths ? min(max(p.lengths[a.b], 0), p.L) : p.L;
-  a.wave = threadIdx.x >> 6, a.row = (threadIdx.x & 63) / kRowLanes;
-  a.run = threadIdx.x / kRowLanes;
+  a.c = min(a.c, p.C - E);  // (lanes behind the last channel read it too, and write nothing)
+  a.len = p.lengths ? __builtin_amdgcn_readfirstlane(min(max(p.lengths[a.b], 0), p.L)) : p.L;
   return a;
 }
 // The token of step s (behind the last in use: the place of its zeros)
 __device__ inline int64_t token_of(const RecurParams &p, const Place &a, int s) {
   return p.reverse && s < a.len ? a.len - 1 - s : s;
+}
+// A tile of Tile steps in a tensor: the address of its first token, and from there in bytes that of a run's
+// first step and the way to the next step.
+template <typename T> struct Rows {
+  const char *base;
+  int first, step;
+  template <int Tile>
+  static __device__ inline Rows of(const RecurParams &p, const Place &a, int s0, const void *x,
+                                   int64_t sequence, int64_t stride, int j) {
+    const int64_t t0 = p.reverse ? (int64_t)a.len - Tile - s0 : s0;
+    const int bytes = (int)stride * (int)sizeof(T);
+    Rows r;
+    r.base = (const char *)x + (a.b * sequence + t0 * stride) * (int64_t)sizeof(T);
+    r.first = (p.reverse ? Tile - 1 - j : j) * bytes + a.c * (int)sizeof(T);
+    r.step = p.reverse ? -bytes : bytes;
+    return r;
+  }
+  __device__ inline T *at(int i) const { return (T *)(base + (unsigned)(first + i * step)); }
+};
+
+// Zeros at those of steps s to s + n that are not in use.
+template <typename T, int E>
+__device__ inline void put_zeros(const RecurParams &p, const Place &a, void *x, int s, int n) {
+  if (!a.here) return;
+  const float zeros[E] = {};
+#pragma unroll 1
+  for (int i = 0; i < n; i++)
+    if (s + i >= a.len && s + i < p.L) put<T, E>((T *)x + ((int64_t)a.b * p.L + s + i) * p.C + a.c, zeros);
 }
 
 // (A, H) of the runs before (Up) or behind a lane's in its wave, and of the whole wave in its
@@ -134,75 +187,206 @@ template <int E> struct Exchange {
   float a[kWaves][kRowLanes][E], h[kWaves][kRowLanes][E];
 };
 
-template <typename T, int E, bool Gated>
-__global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(RecurParams p) {
+// The state that a segment begins with: (A, H) of the parts before it (Backward: behind it) over `carry`.  A row of
+// lanes goes over some of them, then all over the rows.
+template <int E> struct Ranges {
+  float a[kRuns][kRowLanes][E], h[kRuns][kRowLanes][E];
+};
+template <int E, bool Backward>
+__device__ inline void carry_in(const RecurParams &p, const Place &at, Ranges<E> &x, float *carry) {
+  const int lane = threadIdx.x & (kRowLanes - 1), row = threadIdx.x / kRowLanes;
+  const int n = Backward ? max(0, p.parts - (at.segment + 1) * p.share) : at.segment * p.share;
+  const int each = (n + kRuns - 1) / kRuns;
+  const float *part = p.part + (int64_t)at.b * (p.parts + 1) * 2 * p.C + at.c;
+  float A[E], H[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
+#pragma unroll 4
+  for (int i = row * each; i < min(n, (row + 1) * each); i++) {
+    const float *of = part + (int64_t)(Backward ? p.parts - 1 - i : i) * 2 * p.C;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const float a = of[e];
+      H[e] = fmaf(a, H[e], of[p.C + e]);
+      A[e] *= a;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; e++) x.a[row][lane][e] = A[e], x.h[row][lane][e] = H[e];
+  __syncthreads();
+#pragma unroll 4
+  for (int k = 0; k < kRuns; k++)
+#pragma unroll
+    for (int e = 0; e < E; e++) carry[e] = fmaf(x.a[k][lane][e], carry[e], x.h[k][lane][e]);
+}
+
+// (A, H) of every part but those of the last segment, forward, and of the first, backward.  Gates below -20.79
+// count as that here: what they leave of the state, 10^-9, is below what 32 bits tell.
+template <typename T, int E, int RowLanes, bool Gated, bool Backward>
+__global__ __launch_bounds__(kThreads) void recurrence_parts_kernel(RecurParams p) {
+  constexpr int N = 4;  // steps under way
+  __shared__ float xa[kWaves][RowLanes][E], xh[kWaves][RowLanes][E];
+  const Place at = place_of<E, RowLanes>(p, blockIdx.x, Backward ? p.parts - p.share : (p.segments - 1) * p.share);
+  const int which = at.segment + (Backward ? p.share : 0), lane = threadIdx.x & (RowLanes - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = (threadIdx.x & 63) / RowLanes;
+  const int begin = which * p.each, end = min(at.len, begin + p.each);
+  const int run = p.each / (kThreads / RowLanes);  // steps of a run
+  const int lo = begin + threadIdx.x / RowLanes * run, hi = min(end, lo + run);
+  const int way = p.reverse != Backward ? -1 : 1;
+  float A[E], H[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
+  // from the run's first step on, or backward from its last
+  const int64_t t0 = token_of(p, at, Backward ? max(lo, hi - 1) : lo);
+  const T *f = (const T *)p.f + at.b * p.fs[0] + t0 * p.fs[1] + at.c;
+  const T *v = Backward ? (const T *)p.go + ((int64_t)at.b * p.L + t0) * p.C + at.c
+                        : (const T *)p.v + at.b * p.vs[0] + t0 * p.vs[1] + at.c;
+  const T *g = Backward && Gated ? (const T *)p.g + at.b * p.gs[0] + t0 * p.gs[1] + at.c : nullptr;
+  const int64_t fs = way * p.fs[1], vs = way * (Backward ? (int64_t)p.C : p.vs[1]), gs = way * p.gs[1];
+  const auto steps = [&](auto count, int i) {
+    constexpr int K = decltype(count)::value;
+    Raw<T, E> rf[K], rv[K], rg[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      rf[k].load(f + (i + k) * fs);
+      rv[k].load(v + (i + k) * vs);
+      if (Backward && Gated) rg[k].load(g + (i + k) * gs);
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      // over a common denominator, the product of all 1 / a = 1 + x, x = e^-f held below 2^30
+      float D = 1.f, M = H[e];
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        float f = __builtin_elementwise_maximum((float)rf[k][e], -20.79f);
+        if (kFine<T>) f = __builtin_elementwise_minimum(f, 200.f);
+        const float x = exponential<kFine<T>>(f);
+        float d = rv[k][e];
+        if (!Backward) d *= x;  // h = (h + x v) / (1 + x)
+        else if (Gated) d *= rg[k][e] * sigmoid<kFine<T>>(rg[k][e]);
+        M = fmaf(d, D, M), D = fmaf(x, D, D);
+      }
+      const float r = reciprocal(D);
+      H[e] = M * r, A[e] *= r;
+    }
+  };
+  int i = 0;
+  for (; i + N <= hi - lo; i += N) steps(std::integral_constant<int, N>(), i);
+  for (; i < hi - lo; i++) steps(std::integral_constant<int, 1>(), i);
+  if constexpr (RowLanes < 64) {
+    float before_a[E], before_h[E];
+    wave_scan<E, !Backward>(row, A, H, before_a, before_h);
+  }
+  if (row == (Backward ? 0 : 64 / RowLanes - 1))
+#pragma unroll
+    for (int e = 0; e < E; e++) xa[wave][lane][e] = A[e], xh[wave][lane][e] = H[e];
+  __syncthreads();
+  if (threadIdx.x >= RowLanes || !at.here) return;
+#pragma unroll
+  for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < kWaves; k++) {
+    const int w = Backward ? kWaves - 1 - k : k;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      H[e] = fmaf(xa[w][lane][e], H[e], xh[w][lane][e]);
+      A[e] *= xa[w][lane][e];
+    }
+  }
+  float *part = p.part + (int64_t)at.b * (p.parts + 1) * 2 * p.C + at.c;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    part[(int64_t)which * 2 * p.C + e] = A[e], part[((int64_t)which * 2 + 1) * p.C + e] = H[e];
+    // (the initial state too, since `final` may be the same memory)
+    if (!Backward && which == 0)
+      part[(int64_t)p.parts * 2 * p.C + e] = p.initial ? p.initial[(int64_t)at.b * p.C + at.c + e] : 0.f;
+  }
+}
+
+template <typename T, int E, bool Gated, bool Passing>
+__global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurParams p) {
   constexpr int N = kForward;
   __shared__ Exchange<E> both[2];
-  const Place at = place_of<E>(p, p.segments);
-  const int lane = threadIdx.x & (kRowLanes - 1);
+  __shared__ Ranges<E> ranges;
+  const int lane = threadIdx.x & (kRowLanes - 1), run = threadIdx.x / kRowLanes;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = (threadIdx.x & 63) / kRowLanes;
+  // (from the end, which the first launch read last)
+  const Place at = place_of<E>(p, gridDim.x - 1 - blockIdx.x, p.segments);
+  const int begin = at.segment * p.segment, end = min(p.L, begin + p.segment);
+  Raw<T, E> rv[N], rf[N], rz[N];
+  // the tile's values, the next one's while this one is worked on
+  const auto load = [&](int s0) {
+    const auto v = Rows<T>::template of<kTile>(p, at, s0, p.v, p.vs[0], p.vs[1], run * N);
+    const auto f = Rows<T>::template of<kTile>(p, at, s0, p.f, p.fs[0], p.fs[1], run * N);
+    const auto g = Rows<T>::template of<kTile>(p, at, s0, p.g, p.gs[0], p.gs[1], run * N);
+    const int s = s0 + run * N;
+    const bool whole = s0 + kTile <= at.len;
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        rv[i].load(v.at(i));
+        rf[i].load(f.at(i));
+        if (Gated) rz[i].load(g.at(i));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if (s + i < at.len) {
+        rv[i].load(v.at(i));
+        rf[i].load(f.at(i));
+        if (Gated) rz[i].load(g.at(i));
+      } else {  // a step that leaves the state as it is
+        rv[i].fill(0.f), rf[i].fill(__builtin_inff());
+        if (Gated) rz[i].fill(0.f);
+      }
+    }
+  };
+  load(begin);
   float carry[E];
 #pragma unroll
   for (int e = 0; e < E; e++) carry[e] = 0.f;
-  if (at.here) {
-    if (p.segments == 1) {
-      if (p.initial)
+  if (p.segments > 1) {
 #pragma unroll
-        for (int e = 0; e < E; e++) carry[e] = p.initial[(int64_t)at.b * p.C + at.c + e];
-    } else {
-      // the initial state lies in the last segment's place
-      const float *part = p.part + (int64_t)at.b * p.segments * 2 * p.C + at.c;
+    for (int e = 0; e < E; e++)
+      carry[e] = p.part[((int64_t)at.b * (p.parts + 1) + p.parts) * 2 * p.C + at.c + e];
+    carry_in<E, false>(p, at, ranges, carry);
+  } else if (p.initial) {
 #pragma unroll
-      for (int e = 0; e < E; e++) carry[e] = part[(int64_t)(p.segments - 1) * 2 * p.C + e];
-      for (int k = 0; k < at.segment; k++)
-#pragma unroll
-        for (int e = 0; e < E; e++)
-          carry[e] = fmaf(part[(int64_t)k * 2 * p.C + e], carry[e], part[((int64_t)k * 2 + 1) * p.C + e]);
-    }
+    for (int e = 0; e < E; e++) carry[e] = p.initial[(int64_t)at.b * p.C + at.c + e];
   }
-  const T *v = (const T *)p.v + at.b * p.vs[0] + at.c, *f = (const T *)p.f + at.b * p.fs[0] + at.c;
-  const T *g = Gated ? (const T *)p.g + at.b * p.gs[0] + at.c : nullptr;
-  T *out = (T *)p.out + (int64_t)at.b * p.L * p.C + at.c;
-  const int begin = at.segment * p.segment, end = min(p.L, begin + p.segment);
   int turn = 0;
   for (int s0 = begin; s0 < end; s0 += kTile, turn ^= 1) {
-    const int s = s0 + at.run * N;
+    const int s = s0 + run * N;
+    const bool whole = s0 + kTile <= at.len;
     float a[N][E], u[N][E], A[E], H[E], before_a[E], before_h[E];
     Raw<T, E> z[N];
 #pragma unroll
     for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
-    Raw<T, E> rv[N], rf[N];
-#pragma unroll
-    for (int i = 0; i < N; i++)
-      if (at.here && s + i < at.len) {
-        const int64_t t = token_of(p, at, s + i);
-        rv[i].load(v + t * p.vs[1]);
-        rf[i].load(f + t * p.fs[1]);
-        if (Gated) z[i].load(g + t * p.gs[1]);
-      }
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const bool live = at.here && s + i < at.len;
+      if (Gated) z[i] = rz[i];
 #pragma unroll
       for (int e = 0; e < E; e++) {
         float away;
-        a[i][e] = logistic<true>(rf[i][e], away);
+        a[i][e] = logistic<kFine<T>>(rf[i][e], away);
         u[i][e] = away * rv[i][e];
-        if (!live) a[i][e] = 1.f, u[i][e] = 0.f;
         A[e] *= a[i][e], H[e] = fmaf(a[i][e], H[e], u[i][e]);
       }
     }
-    wave_scan<E, true>(at.row, A, H, before_a, before_h);
+    wave_scan<E, true>(row, A, H, before_a, before_h);
     Exchange<E> &x = both[turn];
-    if (at.row == 64 / kRowLanes - 1)
+    if (row == 64 / kRowLanes - 1)
 #pragma unroll
-      for (int e = 0; e < E; e++) x.a[at.wave][lane][e] = A[e], x.h[at.wave][lane][e] = H[e];
+      for (int e = 0; e < E; e++) x.a[wave][lane][e] = A[e], x.h[wave][lane][e] = H[e];
     __syncthreads();
+    if (s0 + kTile < end) load(s0 + kTile);
     float h[E];
-#pragma unroll
+#pragma unroll 1
     for (int w = 0; w < kWaves; w++) {
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        if (w == at.wave) h[e] = carry[e];
+        if (w == wave) h[e] = carry[e];
         carry[e] = fmaf(x.a[w][lane][e], carry[e], x.h[w][lane][e]);
       }
     }
@@ -211,6 +395,7 @@ __global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(RecurParam
     if (p.states && at.here && s < p.L && s % kSpan == 0)
 #pragma unroll
       for (int e = 0; e < E; e++) p.states[((int64_t)at.b * p.spans + s / kSpan) * p.C + at.c + e] = h[e];
+    const auto out = Rows<T>::template of<kTile>(p, at, s0, p.out, (int64_t)p.L * p.C, p.C, run * N);
 #pragma unroll
     for (int i = 0; i < N; i++) {
       float y[E];
@@ -218,209 +403,159 @@ __global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(RecurParam
       for (int e = 0; e < E; e++) {
         h[e] = fmaf(a[i][e], h[e], u[i][e]);
         y[e] = h[e];
-        if (Gated) {
-          float away;
-          const float w = z[i][e];
-          y[e] *= w * logistic<kFine<T>>(w, away);
-        }
-        if (s + i >= at.len) y[e] = 0.f;
+        if (Gated) y[e] *= z[i][e] * sigmoid<kFine<T>>(z[i][e]);
       }
-      if (at.here && s + i < p.L) put<T, E>(out + token_of(p, at, s + i) * p.C, y);
+      if (at.here && (whole || s + i < at.len)) put<T, E, Passing>(out.at(i), y);
     }
+    if (!whole) put_zeros<T, E>(p, at, p.out, s, N);
   }
   if (at.here && at.segment == p.segments - 1 && threadIdx.x < kRowLanes)
 #pragma unroll
     for (int e = 0; e < E; e++) p.final[(int64_t)at.b * p.C + at.c + e] = carry[e];
 }
 
-// (A, H) of all segments but the last, forward, and of all but the first, backward.
-template <typename T, int E, bool Gated, bool Backward>
-__global__ __launch_bounds__(kThreads) void recurrence_segments_kernel(RecurParams p) {
-  __shared__ Exchange<E> x;
-  const Place at = place_of<E>(p, p.segments - 1);
-  const int segment = at.segment + (Backward ? 1 : 0), lane = threadIdx.x & (kRowLanes - 1);
-  const T *v = (const T *)p.v + at.b * p.vs[0] + at.c, *f = (const T *)p.f + at.b * p.fs[0] + at.c;
-  const T *g = Gated ? (const T *)p.g + at.b * p.gs[0] + at.c : nullptr;
-  const T *go = (const T *)p.go + (int64_t)at.b * p.L * p.C + at.c;
-  const int begin = segment * p.segment, end = min(at.len, begin + p.segment);
-  const int each = p.segment / kRuns;  // steps of a run
-  float A[E], H[E], before_a[E], before_h[E];
-#pragma unroll
-  for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
-  const int lo = begin + at.run * each, hi = min(end, lo + each);
-  if (at.here)
-    for (int i = lo; i < hi; i++) {
-      const int s = Backward ? hi - 1 - (i - lo) : i;
-      const int64_t t = token_of(p, at, s);
-      Raw<T, E> rf, rv, rg;
-      rf.load(f + t * p.fs[1]);
-      if (Backward) rv.load(go + t * p.C);
-      else rv.load(v + t * p.vs[1]);
-      if (Backward && Gated) rg.load(g + t * p.gs[1]);
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        float away;
-        const float a = logistic<true>(rf[e], away);
-        if (Backward) {
-          float d = rv[e], rest;
-          if (Gated) d *= rg[e] * logistic<kFine<T>>(rg[e], rest);
-          H[e] = a * (d + H[e]);
-        } else {
-          H[e] = fmaf(a, H[e], away * rv[e]);
-        }
-        A[e] *= a;
-      }
-    }
-  wave_scan<E, !Backward>(at.row, A, H, before_a, before_h);
-  if (at.row == (Backward ? 0 : 64 / kRowLanes - 1))
-#pragma unroll
-    for (int e = 0; e < E; e++) x.a[at.wave][lane][e] = A[e], x.h[at.wave][lane][e] = H[e];
-  __syncthreads();
-  if (threadIdx.x >= kRowLanes || !at.here) return;
-#pragma unroll
-  for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
-  for (int k = 0; k < kWaves; k++) {
-    const int w = Backward ? kWaves - 1 - k : k;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      H[e] = fmaf(x.a[w][lane][e], H[e], x.h[w][lane][e]);
-      A[e] *= x.a[w][lane][e];
-    }
-  }
-  float *part = p.part + (int64_t)at.b * p.segments * 2 * p.C + at.c;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    part[(int64_t)segment * 2 * p.C + e] = A[e], part[((int64_t)segment * 2 + 1) * p.C + e] = H[e];
-    // the initial state, in the place of the last segment's A: `final` may be the same memory
-    if (!Backward && segment == 0)
-      part[(int64_t)(p.segments - 1) * 2 * p.C + e] = p.initial ? p.initial[(int64_t)at.b * p.C + at.c + e] : 0.f;
-  }
-}
-
-template <typename T, int E, bool Gated>
-__global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(RecurParams p) {
+template <typename T, int E, bool Gated, bool Passing>
+__global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurParams p) {
   constexpr int N = kBackward;
   __shared__ Exchange<E> ahead[2], back[2];
-  const Place at = place_of<E>(p, p.segments);
-  const int lane = threadIdx.x & (kRowLanes - 1);
+  __shared__ Ranges<E> ranges;
+  const int lane = threadIdx.x & (kRowLanes - 1), run = threadIdx.x / kRowLanes;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = (threadIdx.x & 63) / kRowLanes;
+  // (from the beginning, which the first launch read last)
+  const Place at = place_of<E>(p, blockIdx.x, p.segments);
+  const int begin = at.segment * p.segment, end = min(p.L, begin + p.segment);
+  const int last = begin + (end - begin - 1) / kSpan * kSpan;
+  Raw<T, E> rv[N], rf[N], rg[N], ro[N];
+  float kept[E];
+  const auto load = [&](int s0) {
+    const auto v = Rows<T>::template of<kSpan>(p, at, s0, p.v, p.vs[0], p.vs[1], run * N);
+    const auto f = Rows<T>::template of<kSpan>(p, at, s0, p.f, p.fs[0], p.fs[1], run * N);
+    const auto g = Rows<T>::template of<kSpan>(p, at, s0, p.g, p.gs[0], p.gs[1], run * N);
+    const auto o = Rows<T>::template of<kSpan>(p, at, s0, p.go, (int64_t)p.L * p.C, p.C, run * N);
+    const int s = s0 + run * N;
+    const bool whole = s0 + kSpan <= at.len;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      kept[e] = p.states[((int64_t)at.b * p.spans + s0 / kSpan) * p.C + at.c + e];
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        rv[i].load(v.at(i));
+        rf[i].load(f.at(i));
+        if (Gated) rg[i].load(g.at(i));
+        ro[i].load(o.at(i));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if (s + i < at.len) {
+        rv[i].load(v.at(i));
+        rf[i].load(f.at(i));
+        if (Gated) rg[i].load(g.at(i));
+        ro[i].load(o.at(i));
+      } else {  // a step that leaves the state and its gradient as they are
+        rv[i].fill(0.f), rf[i].fill(__builtin_inff()), ro[i].fill(0.f);
+        if (Gated) rg[i].fill(0.f);
+      }
+    }
+  };
+  load(last);
   float carry[E];
 #pragma unroll
-  for (int e = 0; e < E; e++) carry[e] = 0.f;
-  if (at.here) {
-    if (p.gfinal)
-#pragma unroll
-      for (int e = 0; e < E; e++) carry[e] = p.gfinal[(int64_t)at.b * p.C + at.c + e];
-    const float *part = p.part + (int64_t)at.b * p.segments * 2 * p.C + at.c;
-    for (int k = p.segments - 1; k > at.segment; k--)
-#pragma unroll
-      for (int e = 0; e < E; e++)
-        carry[e] = fmaf(part[(int64_t)k * 2 * p.C + e], carry[e], part[((int64_t)k * 2 + 1) * p.C + e]);
-  }
-  const T *v = (const T *)p.v + at.b * p.vs[0] + at.c, *f = (const T *)p.f + at.b * p.fs[0] + at.c;
-  const T *g = Gated ? (const T *)p.g + at.b * p.gs[0] + at.c : nullptr;
-  const int64_t dense = (int64_t)at.b * p.L * p.C + at.c;
-  const T *go = (const T *)p.go + dense;
-  T *gv = (T *)p.gv, *gf = (T *)p.gf, *gg = (T *)p.gg;
-  const int begin = at.segment * p.segment, end = min(p.L, begin + p.segment);
+  for (int e = 0; e < E; e++) carry[e] = p.gfinal ? p.gfinal[(int64_t)at.b * p.C + at.c + e] : 0.f;
+  if (p.segments > 1) carry_in<E, true>(p, at, ranges, carry);
   int turn = 0;
-  for (int s0 = begin + (end - begin - 1) / kSpan * kSpan; s0 >= begin; s0 -= kSpan, turn ^= 1) {
-    const int s = s0 + at.run * N;
-    float a[N][E], away[N][E], h[N][E], d[N][E], A[E], H[E], before_a[E], before_h[E];
-    Raw<T, E> rv[N], rf[N], rg[N], ro[N];
-    float state[E];
-    if (at.here)
-#pragma unroll
-      for (int e = 0; e < E; e++) state[e] = p.states[((int64_t)at.b * p.spans + s0 / kSpan) * p.C + at.c + e];
-#pragma unroll
-    for (int i = 0; i < N; i++)
-      if (at.here && s + i < at.len) {
-        const int64_t t = token_of(p, at, s + i);
-        rv[i].load(v + t * p.vs[1]);
-        rf[i].load(f + t * p.fs[1]);
-        if (Gated) rg[i].load(g + t * p.gs[1]);
-        ro[i].load(go + t * p.C);
-      }
+  for (int s0 = last; s0 >= begin; s0 -= kSpan, turn ^= 1) {
+    const int s = s0 + run * N;
+    const bool whole = s0 + kSpan <= at.len;
+    float a[N][E], away[N][E], h[N][E], d[N][E], A[E], H[E], before_a[E], before_h[E], state[E];
 #pragma unroll
     for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const bool live = at.here && s + i < at.len;
+    for (int i = 0; i < N; i++)
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        a[i][e] = logistic<true>(rf[i][e], away[i][e]);
-        float u = away[i][e] * rv[i][e];
-        if (!live) a[i][e] = 1.f, u = 0.f;
-        A[e] *= a[i][e], H[e] = fmaf(a[i][e], H[e], u);
+        a[i][e] = logistic<kFine<T>>(rf[i][e], away[i][e]);
+        A[e] *= a[i][e], H[e] = fmaf(a[i][e], H[e], away[i][e] * rv[i][e]);
       }
-    }
-    wave_scan<E, true>(at.row, A, H, before_a, before_h);
+    wave_scan<E, true>(row, A, H, before_a, before_h);
     Exchange<E> &x = ahead[turn];
-    if (at.row == 64 / kRowLanes - 1)
+    if (row == 64 / kRowLanes - 1)
 #pragma unroll
-      for (int e = 0; e < E; e++) x.a[at.wave][lane][e] = A[e], x.h[at.wave][lane][e] = H[e];
+      for (int e = 0; e < E; e++) x.a[wave][lane][e] = A[e], x.h[wave][lane][e] = H[e];
     __syncthreads();
-    for (int w = 0; w < at.wave; w++)
+#pragma unroll
+    for (int e = 0; e < E; e++) state[e] = kept[e];
+#pragma unroll 1
+    for (int w = 0; w < wave; w++)
 #pragma unroll
       for (int e = 0; e < E; e++) state[e] = fmaf(x.a[w][lane][e], state[e], x.h[w][lane][e]);
 #pragma unroll
     for (int e = 0; e < E; e++) state[e] = fmaf(before_a[e], state[e], before_h[e]);
-    // from here on h: the state before a step
+    const auto gv = Rows<T>::template of<kSpan>(p, at, s0, p.gv, (int64_t)p.L * p.C, p.C, run * N);
+    const auto gf = Rows<T>::template of<kSpan>(p, at, s0, p.gf, (int64_t)p.L * p.C, p.C, run * N);
+    const auto gg = Rows<T>::template of<kSpan>(p, at, s0, p.gg, (int64_t)p.L * p.C, p.C, run * N);
+    // h: what the state before a step differs from its value by
 #pragma unroll
-    for (int i = 0; i < N; i++)
+    for (int i = 0; i < N; i++) {
+      float y[E];
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        h[i][e] = state[e];
-        state[e] = fmaf(a[i][e], state[e], away[i][e] * rv[i][e]);
-        float rest;
+        const float x = rv[i][e];
+        h[i][e] = state[e] - x;
+        state[e] = fmaf(a[i][e], state[e], away[i][e] * x);
         d[i][e] = ro[i][e];
-        if (Gated) d[i][e] *= rg[i][e] * logistic<kFine<T>>(rg[i][e], rest);
-        if (!(at.here && s + i < at.len)) d[i][e] = 0.f;
+        if (Gated) {
+          const float z = rg[i][e], sg = sigmoid<kFine<T>>(z);
+          y[e] = d[i][e] * state[e] * (sg * fmaf(z, 1.f - sg, 1.f));
+          d[i][e] *= z * sg;
+        }
       }
+      if (Gated && p.gg && at.here && (whole || s + i < at.len)) put<T, E, Passing>(gg.at(i), y);
+    }
+    if (s0 > begin) load(s0 - kSpan);
 #pragma unroll
     for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
 #pragma unroll
     for (int i = N - 1; i >= 0; i--)
 #pragma unroll
       for (int e = 0; e < E; e++) H[e] = a[i][e] * (d[i][e] + H[e]), A[e] *= a[i][e];
-    wave_scan<E, false>(at.row, A, H, before_a, before_h);
+    wave_scan<E, false>(row, A, H, before_a, before_h);
     Exchange<E> &y = back[turn];
-    if (at.row == 0)
+    if (row == 0)
 #pragma unroll
-      for (int e = 0; e < E; e++) y.a[at.wave][lane][e] = A[e], y.h[at.wave][lane][e] = H[e];
+      for (int e = 0; e < E; e++) y.a[wave][lane][e] = A[e], y.h[wave][lane][e] = H[e];
     __syncthreads();
     float push[E];
-#pragma unroll
+#pragma unroll 1
     for (int w = kWaves - 1; w >= 0; w--)
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        if (w == at.wave) push[e] = carry[e];
+        if (w == wave) push[e] = carry[e];
         carry[e] = fmaf(y.a[w][lane][e], carry[e], y.h[w][lane][e]);
       }
 #pragma unroll
     for (int e = 0; e < E; e++) push[e] = fmaf(before_a[e], push[e], before_h[e]);
 #pragma unroll
     for (int i = N - 1; i >= 0; i--) {
-      const bool live = s + i < at.len;
-      float y1[E], y2[E], y3[E];
+      float y1[E], y2[E];
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const float D = d[i][e] + push[e], x = rv[i][e];
+        const float D = d[i][e] + push[e];
         push[e] = a[i][e] * D;
         y1[e] = away[i][e] * D;
-        y2[e] = D * (h[i][e] - x) * (a[i][e] * away[i][e]);
-        if (Gated) {
-          float rest;
-          const float z = rg[i][e], sg = logistic<kFine<T>>(z, rest);
-          y3[e] = ro[i][e] * fmaf(a[i][e], h[i][e], away[i][e] * x) * (sg * fmaf(z, rest, 1.f));
-        }
-        if (!live) y1[e] = y2[e] = y3[e] = 0.f;
+        y2[e] = push[e] * (h[i][e] * away[i][e]);
       }
-      if (at.here && s + i < p.L) {
-        const int64_t to = dense + token_of(p, at, s + i) * p.C;
-        if (gv) put<T, E>(gv + to, y1);
-        if (gf) put<T, E>(gf + to, y2);
-        if (Gated && gg) put<T, E>(gg + to, y3);
+      if (at.here && (whole || s + i < at.len)) {
+        if (p.gv) put<T, E, Passing>(gv.at(i), y1);
+        if (p.gf) put<T, E, Passing>(gf.at(i), y2);
       }
+    }
+    if (!whole) {
+      if (p.gv) put_zeros<T, E>(p, at, p.gv, s, N);
+      if (p.gf) put_zeros<T, E>(p, at, p.gf, s, N);
+      if (Gated && p.gg) put_zeros<T, E>(p, at, p.gg, s, N);
     }
   }
   if (p.ginitial && at.here && at.segment == 0 && threadIdx.x < kRowLanes)
@@ -457,10 +592,10 @@ __global__ __launch_bounds__(256) void recurrence_few_kernel(RecurParams p, int6
 #pragma unroll
       for (int e = 0; e < E; e++) {
         float away;
-        const float a = logistic<true>(rf[e], away);
+        const float a = logistic<kFine<T>>(rf[e], away);
         h[e] = fmaf(a, h[e], away * rv[e]);
         y[e] = h[e];
-        if (Gated) y[e] *= rg[e] * logistic<kFine<T>>(rg[e], away);
+        if (Gated) y[e] *= rg[e] * sigmoid<kFine<T>>(rg[e]);
       }
     }
     put<T, E>((T *)p.out + ((int64_t)at.b * p.L + t) * p.C + at.c, y);
@@ -474,9 +609,12 @@ __global__ __launch_bounds__(256) void recurrence_few_kernel(RecurParams p, int6
 int check_desc(const mcx_recurrence_desc *d, int dtype) {
   if (!d) return MCX_E_NULL;
   if (dtype != MCX_F32 && dtype != MCX_BF16) return MCX_E_DTYPE;
-  if (d->B < 0 || d->L < 0 || d->C < 1 || d->L > 0x3fffffff || d->C > (1 << 24) || d->B > (1 << 24) ||
+  if (d->B < 0 || d->L < 0 || d->C < 1 || d->L > 0x3fffffff || d->C > (1 << 22) || d->B > (1 << 24) ||
       d->B * ((d->C + 15) / 16) > (1 << 21))
     return MCX_E_SHAPE;
+  // (a tile's addresses are 32 bits from its first)
+  for (int64_t stride : {d->v_stride[1], d->f_stride[1], d->g_stride[1]})
+    if (d->L > 1 && (stride < 0 || stride > (1 << 22))) return MCX_E_SHAPE;
   return MCX_OK;
 }
 int word_of(const mcx_recurrence_desc *d, int size, bool gated, uint64_t addresses) {
@@ -486,41 +624,74 @@ int word_of(const mcx_recurrence_desc *d, int size, bool gated, uint64_t address
     bits |= (uint64_t)d->v_stride[k] * size | (uint64_t)d->f_stride[k] * size;
     if (gated) bits |= (uint64_t)d->g_stride[k] * size;
   }
-  for (int w : {4, 2})
+  for (int w : {8 / size, 2})  // (of 8 bytes, or two values)
     if (d->C % w == 0 && bits % (w * size) == 0) return w;
   return 1;
 }
-// Segments of the steps: workgroups of `word` channels a lane are made kGroups, of two tiles at least.
-int segment_of(const mcx_recurrence_desc *d, int word) {
-  const int64_t tiles = (d->C + kRowLanes * word - 1) / (kRowLanes * word), groups = d->B * tiles;
-  int64_t n = groups * 4 >= kGroups * 3 ? 1 : (kGroups + groups - 1) / std::max<int64_t>(1, groups);
-  n = std::max<int64_t>(1, std::min(n, d->L / (2 * kTile)));
-  const int64_t each = (d->L + n - 1) / n;
-  return (int)((each + kTile - 1) / kTile * kTile);
+// Segments make kGroups workgroups of the second launch, parts of them kSums of the first, which has less to
+// do and so needs more under way; a tile at least.
+struct Cut {
+  int segments, segment, parts, each, share;
+};
+Cut cut_of(const mcx_recurrence_desc *d, int word, int groups) {
+  const int64_t columns = std::max<int64_t>(1, d->B * ((d->C + kRowLanes * word - 1) / (kRowLanes * word)));
+  int64_t n = columns >= kAlone ? 1 : (groups + columns - 1) / columns;
+  n = std::max<int64_t>(1, std::min(n, d->L / (4 * kTile)));
+  // in tiles
+  const int64_t segment = ((d->L + n - 1) / n + kTile - 1) / kTile;
+  const int64_t each = std::max<int64_t>(1, segment * columns * n / kSums);
+  Cut c;
+  c.share = (int)((segment + each - 1) / each), c.each = (int)(each * kTile), c.segment = c.share * c.each;
+  c.segments = (int)((d->L + c.segment - 1) / c.segment);
+  c.parts = (int)((d->L + c.each - 1) / c.each);
+  return c;
 }
 size_t part_bytes(const mcx_recurrence_desc *d) {
-  // (of the widest word, whose workgroups are the fewest)
-  int64_t n = 1;
-  for (int w : {1, 2, 4}) {
-    const int each = segment_of(d, w);
-    n = std::max<int64_t>(n, (d->L + each - 1) / each);
+  int64_t n = 0;
+  for (int w : {1, 2, 4}) {  // (whichever the alignment gives)
+    for (int groups : {kGroups, kGroupsBf16Backward}) {
+      const Cut c = cut_of(d, w, groups);
+      if (c.segments > 1) n = std::max<int64_t>(n, c.parts + 1);
+    }
   }
-  return n > 1 ? (size_t)(d->B * n * 2 * d->C) * sizeof(float) : 0;
+  return (size_t)(d->B * n * 2 * d->C) * sizeof(float);
 }
-RecurParams params_of(const mcx_recurrence_desc *d, int word) {
+RecurParams params_of(const mcx_recurrence_desc *d, int word, int groups, void *workspace) {
   RecurParams p = {};
   for (int k = 0; k < 2; k++) p.vs[k] = d->v_stride[k], p.fs[k] = d->f_stride[k], p.gs[k] = d->g_stride[k];
   p.L = (int)d->L, p.C = (int)d->C;
   p.tiles = (int)((d->C + kRowLanes * word - 1) / (kRowLanes * word));
-  p.segment = segment_of(d, word);
-  p.segments = (int)((d->L + p.segment - 1) / p.segment);
+  const Cut c = cut_of(d, word, groups);
+  p.segment = c.segment, p.segments = c.segments, p.parts = c.parts, p.each = c.each, p.share = c.share;
   p.spans = (int)((d->L + kSpan - 1) / kSpan);
   p.reverse = d->reverse != 0;
+  p.part = (float *)workspace;
   return p;
+}
+
+template <typename T, int E, int RowLanes, bool Gated, bool Backward>
+int launch_parts(RecurParams p, int64_t B, hipStream_t s) {
+  p.tiles = (p.C + RowLanes * E - 1) / (RowLanes * E);
+  const int64_t parts = Backward ? p.parts - p.share : (p.segments - 1) * p.share;
+  hipLaunchKernelGGL((recurrence_parts_kernel<T, E, RowLanes, Gated, Backward>), dim3((unsigned)(B * p.tiles * parts)),
+                     dim3(kThreads), 0, s, p);
+  MCX_HIP_CHECK_LAUNCH();
+  return MCX_OK;
+}
+template <typename T, int E, bool Gated, bool Backward>
+int sum_parts(const RecurParams &p, int64_t B, hipStream_t s) {
+  return p.C / E >= kWideRow ? launch_parts<T, E, 64, Gated, Backward>(p, B, s)
+                       : launch_parts<T, E, kRowLanes, Gated, Backward>(p, B, s);
+}
+
+template <typename T, int E> bool passing(const RecurParams &p, int64_t B) {
+  return p.C * (int)sizeof(T) % kLine == 0 && B * p.L * p.C * (int64_t)sizeof(T) >= kPassingBytes;
 }
 
 template <typename T, int E, bool Gated>
 int forward(const RecurParams &p, int64_t B, hipStream_t s) {
+  const unsigned groups = (unsigned)(B * p.tiles);
+  const dim3 threads(kThreads);
   if (p.L <= kFew) {
     const int64_t words = B * (p.C / E);
     hipLaunchKernelGGL((recurrence_few_kernel<T, E, Gated>), dim3((unsigned)((words + 255) / 256)), dim3(256),
@@ -528,27 +699,23 @@ int forward(const RecurParams &p, int64_t B, hipStream_t s) {
     MCX_HIP_CHECK_LAUNCH();
     return MCX_OK;
   }
-  const unsigned groups = (unsigned)(B * p.tiles);
-  if (p.segments > 1) {
-    hipLaunchKernelGGL((recurrence_segments_kernel<T, E, false, false>), dim3(groups * (p.segments - 1)),
-                       dim3(kThreads), 0, s, p);
-    MCX_HIP_CHECK_LAUNCH();
-  }
-  hipLaunchKernelGGL((recurrence_forward_kernel<T, E, Gated>), dim3(groups * p.segments), dim3(kThreads), 0,
-                     s, p);
+  if (p.segments > 1)
+    if (int e = sum_parts<T, E, false, false>(p, B, s)) return e;
+  hipLaunchKernelGGL((passing<T, E>(p, B) ? recurrence_forward_kernel<T, E, Gated, E * sizeof(T) == 8>
+                                          : recurrence_forward_kernel<T, E, Gated, false>),
+                     dim3(groups * p.segments), threads, 0, s, p);
   MCX_HIP_CHECK_LAUNCH();
   return MCX_OK;
 }
 template <typename T, int E, bool Gated>
 int backward(const RecurParams &p, int64_t B, hipStream_t s) {
   const unsigned groups = (unsigned)(B * p.tiles);
-  if (p.segments > 1) {
-    hipLaunchKernelGGL((recurrence_segments_kernel<T, E, Gated, true>), dim3(groups * (p.segments - 1)),
-                       dim3(kThreads), 0, s, p);
-    MCX_HIP_CHECK_LAUNCH();
-  }
-  hipLaunchKernelGGL((recurrence_backward_kernel<T, E, Gated>), dim3(groups * p.segments), dim3(kThreads), 0,
-                     s, p);
+  const dim3 threads(kThreads);
+  if (p.segments > 1)
+    if (int e = sum_parts<T, E, Gated, true>(p, B, s)) return e;
+  hipLaunchKernelGGL((passing<T, E>(p, B) ? recurrence_backward_kernel<T, E, Gated, E * sizeof(T) == 8>
+                                          : recurrence_backward_kernel<T, E, Gated, false>),
+                     dim3(groups * p.segments), threads, 0, s, p);
   MCX_HIP_CHECK_LAUNCH();
   return MCX_OK;
 }
@@ -557,7 +724,9 @@ int launch(const RecurParams &p, int64_t B, int word, hipStream_t s) {
 #define MCX_RECUR(E)                                                                                 \
   (Forward ? (p.g ? forward<T, E, true>(p, B, s) : forward<T, E, false>(p, B, s))                    \
            : (p.g ? backward<T, E, true>(p, B, s) : backward<T, E, false>(p, B, s)))
-  return word == 4 ? MCX_RECUR(4) : word == 2 ? MCX_RECUR(2) : MCX_RECUR(1);
+  if constexpr (sizeof(T) == 2)
+    if (word == 4) return MCX_RECUR(4);
+  return word == 2 ? MCX_RECUR(2) : MCX_RECUR(1);
 #undef MCX_RECUR
 }
 
@@ -586,9 +755,9 @@ int mcx_gated_recurrence_forward(const void *value, const void *forget, const vo
   if (need && (!workspace || workspace_bytes < need)) return MCX_E_WORKSPACE;
   const int word = word_of(desc, dtype == MCX_BF16 ? 2 : 4, gate != nullptr,
                            (uintptr_t)value | (uintptr_t)forget | (uintptr_t)gate | (uintptr_t)out);
-  RecurParams p = params_of(desc, word);
+  RecurParams p = params_of(desc, word, kGroups, workspace);
   p.v = value, p.f = forget, p.g = gate, p.initial = initial, p.lengths = lengths;
-  p.out = out, p.final = final, p.states = states, p.part = (float *)workspace;
+  p.out = out, p.final = final, p.states = states;
   return dtype == MCX_BF16 ? launch<__bf16, true>(p, desc->B, word, (hipStream_t)stream)
                            : launch<float, true>(p, desc->B, word, (hipStream_t)stream);
 }
@@ -607,10 +776,10 @@ int mcx_gated_recurrence_backward(const void *gout, const float *gfinal, const v
   const int word = word_of(desc, dtype == MCX_BF16 ? 2 : 4, gate != nullptr,
                            (uintptr_t)value | (uintptr_t)forget | (uintptr_t)gate | (uintptr_t)gout |
                                (uintptr_t)gvalue | (uintptr_t)gforget | (uintptr_t)ggate);
-  RecurParams p = params_of(desc, word);
+  RecurParams p = params_of(desc, word, dtype == MCX_BF16 ? kGroupsBf16Backward : kGroups, workspace);
   p.v = value, p.f = forget, p.g = gate, p.go = gout, p.gfinal = gfinal, p.lengths = lengths;
   p.gv = gvalue, p.gf = gforget, p.gg = ggate, p.ginitial = ginitial;
-  p.states = const_cast<float *>(states), p.part = (float *)workspace;
+  p.states = const_cast<float *>(states);
   return dtype == MCX_BF16 ? launch<__bf16, false>(p, desc->B, word, (hipStream_t)stream)
                            : launch<float, false>(p, desc->B, word, (hipStream_t)stream);
 }
