@@ -1377,46 +1377,44 @@ def group_norm_backward(grad_output, x, saved, groups, weight=None, bias=None, a
 
 # ---- clipping's norm alone, and the AdamW step ------------------------------------------------
 
+def _together(tensors):
+    """Addresses and sizes (lists) of tensors that have to be contiguous and on one GPU."""
+    # (hundreds of tensors: every look at them is one pass in C)
+    if len(set(map(torch.Tensor.get_device, tensors))) != 1 or not tensors[0].is_cuda:
+        raise RuntimeError("all tensors must be on one GPU")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise RuntimeError("tensors must be contiguous")
+    return list(map(torch.Tensor.data_ptr, tensors)), list(map(torch.Tensor.numel, tensors))
+
+
+def _type_codes(dtypes):
+    codes = list(map(_CLIP_DTYPES.get, dtypes))
+    if None in codes:
+        raise RuntimeError("unsupported dtype %s (float32 or bfloat16)" % dtypes[codes.index(None)])
+    return array.array("i", codes)
+
+
 def grad_norm(tensors):
     """The norm of all values of a list of tensors (float32 and bfloat16, contiguous, on one GPU), as
     a float32 scalar; what clip_grad_norm multiplies by, without the products: adamw_step takes it."""
     tensors = list(tensors)
     if not tensors:
         raise RuntimeError("grad_norm needs at least one tensor")
-    _one_gpu(tensors, tensors[0])
-    at, sizes, types = _host_lists(tensors)
+    at, sizes = _together(tensors)
+    types = _type_codes([t.dtype for t in tensors])
+    # (host arrays of the library's types, which live until it has returned)
+    at, sizes = array.array("Q", at), array.array("q", sizes)
+    hosts = [a.buffer_info()[0] for a in (at, sizes, types)]
     device = tensors[0].device
     lib = _lib.load()
     norm = torch.empty((), dtype=torch.float32, device=device)
-    nbytes = lib.mcx_clip_grad_norm_workspace(_host(sizes), len(tensors))
+    nbytes = lib.mcx_clip_grad_norm_workspace(hosts[1], len(tensors))
     ws = _workspace(nbytes, device)
     with _device(norm):
-        rc = lib.mcx_clip_grad_norm(_host(at), None, _host(sizes), _host(types), len(tensors), 0.0,
-                                    0.0, _ptr(norm), _ptr(ws), nbytes, _stream(norm))
+        rc = lib.mcx_clip_grad_norm(hosts[0], None, hosts[1], hosts[2], len(tensors), 0.0, 0.0,
+                                    _ptr(norm), _ptr(ws), nbytes, _stream(norm))
     _lib.check(rc, "grad_norm")
     return norm
-
-
-def _one_gpu(tensors, first):
-    if len(set(map(torch.Tensor.get_device, tensors))) != 1 or not first.is_cuda:
-        raise RuntimeError("all tensors must be on one GPU")
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
-        raise RuntimeError("tensors must be contiguous")
-
-
-def _host(a):
-    """The address of a host array (which has to live until the call returns)."""
-    return None if a is None else a.buffer_info()[0]
-
-
-def _host_lists(tensors):
-    """(addresses, sizes, type codes) of a list, as host arrays of the library's types."""
-    types = [_CLIP_DTYPES.get(t.dtype, -1) for t in tensors]
-    if -1 in types:
-        raise RuntimeError("unsupported dtype %s (float32 or bfloat16)" %
-                           tensors[types.index(-1)].dtype)
-    return (array.array("Q", map(torch.Tensor.data_ptr, tensors)),
-            array.array("q", map(torch.Tensor.numel, tensors)), array.array("i", types))
 
 
 ADAMW_BLOCK = 256  # values that share a scale where moments are held in 8 bits
@@ -1426,23 +1424,6 @@ def _one_value(name, t, dtype, like):
     if t.dtype != dtype or t.numel() != 1 or t.get_device() != like.get_device():
         raise RuntimeError("%s must be one %s value on the parameters' GPU" % (name, dtype))
     return t.data_ptr()
-
-
-def _moments(name, moments, scales, params, sizes):
-    """A check of the moments of one kind -> (addresses, the scales' addresses or None, all tensors)."""
-    dtype = torch.float32 if scales is None else torch.uint8
-    if len(moments) != len(params) or list(map(torch.Tensor.numel, moments)) != sizes:
-        raise RuntimeError("%s moments must have the parameters' number and sizes" % name)
-    if any(t.dtype != dtype for t in moments):
-        raise RuntimeError("%s moments must be %s" % (name, dtype))
-    at = array.array("Q", map(torch.Tensor.data_ptr, moments))
-    if scales is None:
-        return at, None, moments
-    if list(map(torch.Tensor.numel, scales)) != [-(-n // ADAMW_BLOCK) for n in sizes] or \
-            any(t.dtype != torch.float32 for t in scales):
-        raise RuntimeError("%s scales must be float32, one for %d values of a tensor" %
-                           (name, ADAMW_BLOCK))
-    return at, array.array("Q", map(torch.Tensor.data_ptr, scales)), moments + scales
 
 
 def adamw_step(params, grads, first_moments, second_moments, step, lr, betas=(0.9, 0.999), eps=1e-8,
@@ -1463,55 +1444,63 @@ def adamw_step(params, grads, first_moments, second_moments, step, lr, betas=(0.
     value on the GPU; both are read there when the kernels run, so that a captured step can be replayed.
     What is changed must not share memory with any other tensor: one that stands in the lists twice
     is refused, parts that overlap are not looked for."""
-    params, grads = list(params), list(grads)
-    first_moments, second_moments = list(first_moments), list(second_moments)
     if (first_scales is None) != (second_scales is None):
         raise RuntimeError("first_scales and second_scales go together")
     if (grad_norm is None) != (max_norm is None):
         raise RuntimeError("grad_norm and max_norm go together")
-    if len(grads) != len(params):
-        raise RuntimeError("%d gradients for %d parameters" % (len(grads), len(params)))
-    if first_scales is not None:
-        first_scales, second_scales = list(first_scales), list(second_scales)
-    beta1, beta2 = (float(b) for b in betas)
-    eps, weight_decay = float(eps), float(weight_decay)
-    if not (0 <= beta1 < 1 and 0 <= beta2 < 1 and eps >= 0 and weight_decay >= 0):
-        raise RuntimeError("betas must lie in [0, 1), eps and weight_decay must not be negative")
-    if max_norm is not None and not float(max_norm) >= 0:
-        raise RuntimeError("max_norm must not be negative")
-    if not isinstance(step, torch.Tensor) and int(step) < 1:
+    beta1, beta2 = betas
+    max_norm = 0.0 if max_norm is None else float(max_norm)
+    if not (0 <= beta1 < 1 and 0 <= beta2 < 1 and eps >= 0 and weight_decay >= 0 and max_norm >= 0):
+        raise RuntimeError("betas must lie in [0, 1), eps, weight_decay and max_norm must not be "
+                           "negative")
+    on_gpu = isinstance(step, torch.Tensor), isinstance(lr, torch.Tensor)
+    if not on_gpu[0] and int(step) < 1:
         raise RuntimeError("step counts from 1, got %d" % step)
-    if not isinstance(lr, torch.Tensor) and not abs(float(lr)) < float("inf"):
+    if not on_gpu[1] and not abs(float(lr)) < float("inf"):
         raise RuntimeError("lr must be finite")
-    p_at, sizes, p_types = _host_lists(params)
-    g_at, g_sizes, g_types = _host_lists(grads)
-    if g_sizes != sizes:
-        raise RuntimeError("gradients must have the parameters' sizes")
-    counts = list(sizes)
-    m_at, ms_at, m_all = _moments("first", first_moments, first_scales, params, counts)
-    v_at, vs_at, v_all = _moments("second", second_moments, second_scales, params, counts)
-    if not params:
+    lists = [list(params), list(grads), list(first_moments), list(second_moments)]
+    wide = first_scales is None
+    if not wide:
+        lists += [list(first_scales), list(second_scales)]
+    n = len(lists[0])
+    if set(map(len, lists)) != {n}:
+        raise RuntimeError("every list must have as many tensors: %s" % list(map(len, lists)))
+    if not n:
         return
-    _one_gpu(params + grads + m_all + v_all, params[0])
-    written = [a for a in (*p_at, *m_at, *v_at, *(ms_at or ()), *(vs_at or ())) if a]
-    if len(set(written)) != len(written) or not set(written).isdisjoint(g_at):
+    every = sum(lists, [])
+    at, sizes = _together(every)
+    dtypes = [t.dtype for t in every]
+    types = _type_codes(dtypes[:2 * n])
+    if set(dtypes[2 * n:4 * n]) != {torch.float32 if wide else torch.uint8}:
+        raise RuntimeError("moments must be float32, or uint8 with scales")
+    if set(dtypes[4 * n:]) - {torch.float32}:
+        raise RuntimeError("scales must be float32")
+    if sizes[:n] * 3 != sizes[n:4 * n]:
+        raise RuntimeError("gradients and moments must have the parameters' sizes")
+    if not wide and [-(-k // ADAMW_BLOCK) for k in sizes[:n]] * 2 != sizes[4 * n:]:
+        raise RuntimeError("there must be one scale for %d values of a tensor" % ADAMW_BLOCK)
+    written = at[:n] + at[2 * n:]
+    if len(set(written)) != len(written) or not set(written).isdisjoint(at[n:2 * n]):
         # (tensors without values may share an address)
-        full = [t.data_ptr() for t in params + m_all + v_all if t.numel()]
+        full = [a for a, k in zip(written, sizes[:n] + sizes[2 * n:]) if k]
         if len(set(full)) != len(full) or \
-                not set(full).isdisjoint(t.data_ptr() for t in grads if t.numel()):
+                not set(full).isdisjoint(a for a, k in zip(at[n:2 * n], sizes) if k):
             raise RuntimeError("a tensor that is changed stands in the lists twice")
-    device = params[0].device
+    first = every[0]
     options = _lib.AdamWOptions(
-        0.0 if isinstance(lr, torch.Tensor) else float(lr), beta1, beta2, eps, weight_decay,
-        0.0 if max_norm is None else float(max_norm), 1 if isinstance(step, torch.Tensor) else int(step),
-        _one_value("step", step, torch.int64, params[0]) if isinstance(step, torch.Tensor) else None,
-        _one_value("lr", lr, torch.float32, params[0]) if isinstance(lr, torch.Tensor) else None,
-        None if grad_norm is None else _one_value("grad_norm", grad_norm, torch.float32, params[0]),
-        int(seed) & 0xFFFFFFFF, 32 if first_scales is None else 8)
-    with _device(params[0]):
-        rc = _lib.load().mcx_adamw_step(_host(p_at), _host(g_at), _host(m_at), _host(v_at),
-                                        _host(ms_at), _host(vs_at), _host(sizes), _host(p_types),
-                                        _host(g_types), len(params), options, _stream(params[0]))
+        0.0 if on_gpu[1] else float(lr), beta1, beta2, eps, weight_decay, max_norm,
+        1 if on_gpu[0] else int(step),
+        _one_value("step", step, torch.int64, first) if on_gpu[0] else None,
+        _one_value("lr", lr, torch.float32, first) if on_gpu[1] else None,
+        None if grad_norm is None else _one_value("grad_norm", grad_norm, torch.float32, first),
+        int(seed) & 0xFFFFFFFF, 32 if wide else 8)
+    # (host arrays of the library's types, which live until it has returned)
+    at, sizes = array.array("Q", at), array.array("q", sizes[:n])
+    hosts = [at.buffer_info()[0] + 8 * n * k for k in range(4 if wide else 6)] + [None] * (2 * wide)
+    types_at = types.buffer_info()[0]
+    with _device(first):
+        rc = _lib.load().mcx_adamw_step(*hosts, sizes.buffer_info()[0], types_at, types_at + 4 * n, n,
+                                        options, _stream(first))
     _lib.check(rc, "adamw_step")
 
 

@@ -12,8 +12,10 @@
 // that keeps its place in the grid is not rounded anew when its block's largest changes.  A v above
 // zero stays above zero: it is divided by.
 //
-// Bound by memory: 26 to 28 bytes a value with moments in 32 bits, 14 to 16 in 8.  One launch for up
-// to kMost tensors, whose table travels in its arguments.
+// Bound by memory: 26 to 28 bytes a value with moments in 32 bits, 14 to 16 in 8, where the vector units have
+// nearly as much to do: a code's bits are shifted into a float's, subnormal where its exponent is 0, so that
+// one product decodes and one scaling rounds as the code's grid does.  One launch for up to kMost tensors,
+// whose table travels in its arguments.
 #include <algorithm>
 #include <cmath>
 
@@ -24,10 +26,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMost = 52;        // tensors of a launch: 3.6 kB of arguments
-constexpr int kBlocks = 2048;    // workgroups of a launch
+constexpr int kBlocks = 4096;    // workgroups of a launch
 constexpr int kBlock = 256;      // values that share a scale: those of a wave
 constexpr int64_t kLeast = 1024;     // values of a chunk
 constexpr int64_t kLargest = 16384;
+// Of the last-level cache: parameters, gradients and moments of 32 bits pass it by where there is more (0.6
+// billion values 3.27 -> 3.04 ms).  Bytes do not: words of 4 a lane are slower past it.
+constexpr int64_t kCacheBytes = 256 << 20;
 
 struct AdamTensors {
   void *p[kMost];
@@ -88,12 +93,12 @@ __device__ inline AdamFactors factors_of(const AdamNumbers &n) {
 }
 
 // Four values from i on, those below n.
-template <typename T, bool Whole>
+template <typename T, bool Whole, bool Passing = false>
 __device__ inline float4v four(const T *x, int64_t i, int64_t n) {
   float4v r = {0.f, 0.f, 0.f, 0.f};
   if (Whole) {
     typedef T Vec __attribute__((ext_vector_type(4)));
-    const Vec w = *(const Vec *)(x + i);
+    const Vec w = Passing ? __builtin_nontemporal_load((const Vec *)(x + i)) : *(const Vec *)(x + i);
 #pragma unroll
     for (int e = 0; e < 4; e++) r[e] = (float)w[e];
   } else {
@@ -103,14 +108,15 @@ __device__ inline float4v four(const T *x, int64_t i, int64_t n) {
   }
   return r;
 }
-template <typename T, bool Whole>
+template <typename T, bool Whole, bool Passing = false>
 __device__ inline void put_four(T *x, int64_t i, int64_t n, const float4v &r) {
   if (Whole) {
     typedef T Vec __attribute__((ext_vector_type(4)));
     Vec w;
 #pragma unroll
     for (int e = 0; e < 4; e++) w[e] = (T)r[e];
-    *(Vec *)(x + i) = w;
+    if (Passing) __builtin_nontemporal_store(w, (Vec *)(x + i));
+    else *(Vec *)(x + i) = w;
   } else {
 #pragma unroll
     for (int e = 0; e < 4; e++)
@@ -138,31 +144,38 @@ __device__ inline void put_four_codes(uint8_t *x, int64_t i, int64_t n, uint32_t
 }
 
 // Low: the exponent from which down the steps stay; a sign in the uppermost bit.
+constexpr float power(int e) {
+  float x = 1.f;
+  for (; e > 0; e--) x *= 2.f;
+  return x;
+}
 template <int Low, bool Signed>
 __device__ inline float value_of(uint32_t code) {
-  const uint32_t c = Signed ? code & 127 : code;
-  // a normal value's bits, or (with the leading bit that it lacks taken off again) a small one's
-  const float one = __uint_as_float((c << 20) + (uint32_t)((127 + Low - 1) << 23));
-  const float small = __uint_as_float((c << 20) + (uint32_t)((127 + Low) << 23)) -
-                      __uint_as_float((uint32_t)((127 + Low) << 23));
-  const float y = c < 8 ? small : one;
-  return Signed && code & 128 ? -y : y;
+  const uint32_t bits = Signed ? (code & 127) << 20 | (code & 128) << 24 : code << 20;
+  constexpr float up = power(126 + Low);
+  return __uint_as_float(bits) * up;
 }
-// y in [0, 2), 20 bits of chance
+// A value of a block whose power of two has this exponent; 20 bits of chance.
 template <int Low, bool Signed>
-__device__ inline uint32_t code_of(float y, uint32_t chance, bool negative) {
-  const float least = __uint_as_float((uint32_t)((127 + Low) << 23));
-  const bool tiny = y < least;
-  const uint32_t bits = __float_as_uint(tiny ? y + least : y);
-  uint32_t c = ((bits + chance) >> 20) - (uint32_t)((127 + Low) << 3) + (tiny ? 0 : 8);
-  if (Signed) return min(c, 127u) | (negative ? 128u : 0u);
-  return y > 0.f ? min(max(c, 1u), 255u) : 0u;
+__device__ inline uint32_t code_of(float x, int exponent, uint32_t chance) {
+  const float y = __builtin_amdgcn_ldexpf(fabsf(x), -exponent - 126 - Low);
+  const uint32_t c = (__float_as_uint(y) + chance) >> 20;
+  if (Signed) return min(c, 127u) | (x < 0.f ? 128u : 0u);
+  return x > 0.f ? min(max(c, 1u), 255u) : 0u;
 }
 
+// The largest of a wave's values: lanes of four, eight and sixteen exchange, then rows go on to rows.
+template <int Ctrl> __device__ inline uint32_t max_of(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, Ctrl, 0xf, 0xf, false));
+}
 __device__ inline uint32_t wave_max(uint32_t x) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, m));
-  return x;
+  x = max_of<0xb1>(x);   // quad_perm 1, 0, 3, 2
+  x = max_of<0x4e>(x);   // quad_perm 2, 3, 0, 1
+  x = max_of<0x141>(x);  // row_half_mirror
+  x = max_of<0x140>(x);  // row_mirror
+  x = max_of<0x142>(x);  // row_bcast 15
+  x = max_of<0x143>(x);  // row_bcast 31
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 // The exponent of a block's power of two from its largest value's bits.
 __device__ inline int exponent_of(uint32_t top) {
@@ -173,16 +186,16 @@ __device__ inline float scale_of(uint32_t top) {
   return top ? __builtin_amdgcn_ldexpf(1.f, exponent_of(top)) : 0.f;
 }
 
-template <int Bits, typename P, typename G, bool Whole>
+template <int Bits, typename P, typename G, bool Whole, bool Passing>
 __device__ inline void adam_four(const AdamFactors &f, const AdamTensors &l, int t, int64_t i,
                                  int64_t n) {
-  float4v p = four<P, Whole>((const P *)l.p[t], i, n), g = four<G, Whole>((const G *)l.g[t], i, n);
+  float4v p = four<P, Whole, Passing>((const P *)l.p[t], i, n), g = four<G, Whole, Passing>((const G *)l.g[t], i, n);
   float4v m, v;
   const int64_t block = i / kBlock;
   const bool here = i < n;
   if (Bits == 32) {
-    m = four<float, Whole>((const float *)l.m[t], i, n);
-    v = four<float, Whole>((const float *)l.v[t], i, n);
+    m = four<float, Whole, Passing>((const float *)l.m[t], i, n);
+    v = four<float, Whole, Passing>((const float *)l.v[t], i, n);
   } else {
     const uint32_t mc = four_codes<Whole>((const uint8_t *)l.m[t], i, n);
     const uint32_t vc = four_codes<Whole>((const uint8_t *)l.v[t], i, n);
@@ -198,12 +211,16 @@ __device__ inline void adam_four(const AdamFactors &f, const AdamTensors &l, int
     const float x = g[e] * f.clip;
     m[e] = m[e] * f.b1 + x * f.c1;
     v[e] = v[e] * f.b2 + (x * x) * f.c2;
-    p[e] = p[e] * f.keep - f.rate * (m[e] / (sqrtf(v[e]) * f.root + f.eps));
+    // (in 8 bits, where the vector units count, root and quotient to a unit in the last place)
+    const float root = Bits == 32 ? sqrtf(v[e]) : __builtin_amdgcn_sqrtf(v[e]);
+    const float below = root * f.root + f.eps;
+    const float ratio = Bits == 32 ? m[e] / below : m[e] * __builtin_amdgcn_rcpf(below);
+    p[e] = p[e] * f.keep - f.rate * ratio;
   }
-  put_four<P, Whole>((P *)l.p[t], i, n, p);
+  put_four<P, Whole, Passing>((P *)l.p[t], i, n, p);
   if (Bits == 32) {
-    put_four<float, Whole>((float *)l.m[t], i, n, m);
-    put_four<float, Whole>((float *)l.v[t], i, n, v);
+    put_four<float, Whole, Passing>((float *)l.m[t], i, n, m);
+    put_four<float, Whole, Passing>((float *)l.v[t], i, n, v);
     return;
   }
   uint32_t mt = 0, vt = 0;
@@ -215,17 +232,15 @@ __device__ inline void adam_four(const AdamFactors &f, const AdamTensors &l, int
   }
   mt = wave_max(mt), vt = wave_max(vt);
   const int me = exponent_of(mt), ve = exponent_of(vt);
+  // (i is a multiple of 4: the upper half of the place is that of all four)
   const uint64_t at = (uint64_t)(l.base[t] * kBlock + i);
+  const uint32_t upper = (uint32_t)(at >> 32) * 0x9E3779B1u;
   uint32_t mc = 0, vc = 0;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    const uint64_t k = at + e;
-    const uint32_t word = mix((((uint32_t)k) ^ ((uint32_t)(k >> 32) * 0x9E3779B1u)) + f.key);
-    mc |= code_of<-14, true>(__builtin_amdgcn_ldexpf(fabsf(m[e]), -me), ((word & 0xffff) << 4) | 8,
-                             m[e] < 0.f)
-          << (8 * e);
-    vc |= code_of<-30, false>(__builtin_amdgcn_ldexpf(v[e], -ve), ((word >> 16) << 4) | 8, false)
-          << (8 * e);
+    const uint32_t word = mix((((uint32_t)at + e) ^ upper) + f.key);
+    mc |= code_of<-14, true>(m[e], me, ((word & 0xffff) << 4) | 8) << (8 * e);
+    vc |= code_of<-30, false>(v[e], ve, ((word >> 16) << 4) | 8) << (8 * e);
   }
   put_four_codes<Whole>((uint8_t *)l.m[t], i, n, mc);
   put_four_codes<Whole>((uint8_t *)l.v[t], i, n, vc);
@@ -234,19 +249,19 @@ __device__ inline void adam_four(const AdamFactors &f, const AdamTensors &l, int
 
 // Values [lo, hi) of a tensor, lo a multiple of kBlock; every wave walks whole blocks, so that the
 // lanes behind the end are there for its sums.
-template <int Bits, typename P, typename G>
+template <int Bits, typename P, typename G, bool Passing>
 __device__ inline void adam_chunk(const AdamFactors &f, const AdamTensors &l, int t, int64_t lo,
                                   int64_t hi) {
   const bool wide = (l.wide >> t) & 1;
   const int64_t last = lo + (hi - lo + kBlock - 1) / kBlock * kBlock;
   for (int64_t i = lo + 4 * threadIdx.x; i < last; i += 4 * kThreads) {
     const int64_t block = i / kBlock * kBlock;
-    if (wide && block + kBlock <= hi) adam_four<Bits, P, G, true>(f, l, t, i, hi);
-    else adam_four<Bits, P, G, false>(f, l, t, i, hi);
+    if (wide && block + kBlock <= hi) adam_four<Bits, P, G, true, Passing>(f, l, t, i, hi);
+    else adam_four<Bits, P, G, false, Passing>(f, l, t, i, hi);
   }
 }
 
-template <int Bits>
+template <int Bits, bool Passing>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTensors l, AdamNumbers n) {
   const AdamFactors f = factors_of(n);
   const int chunks = l.first[l.count];
@@ -260,10 +275,10 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTensors l, AdamNumb
     const int t = lo;
     const int64_t a = (int64_t)(c - l.first[t]) * l.chunk, z = min(l.size[t], a + l.chunk);
     const bool pb = (l.p_bf16 >> t) & 1, gb = (l.g_bf16 >> t) & 1;
-    if (pb && gb) adam_chunk<Bits, __bf16, __bf16>(f, l, t, a, z);
-    else if (pb) adam_chunk<Bits, __bf16, float>(f, l, t, a, z);
-    else if (gb) adam_chunk<Bits, float, __bf16>(f, l, t, a, z);
-    else adam_chunk<Bits, float, float>(f, l, t, a, z);
+    if (pb && gb) adam_chunk<Bits, __bf16, __bf16, Passing>(f, l, t, a, z);
+    else if (pb) adam_chunk<Bits, __bf16, float, Passing>(f, l, t, a, z);
+    else if (gb) adam_chunk<Bits, float, __bf16, Passing>(f, l, t, a, z);
+    else adam_chunk<Bits, float, float, Passing>(f, l, t, a, z);
   }
 }
 
@@ -305,7 +320,7 @@ int mcx_adamw_step(void *const *params, const void *const *grads, void *const *f
   if (!params || !grads || !first || !second || !sizes || !param_dtypes || !grad_dtypes ||
       (o->bits == 8 && (!first_scales || !second_scales)))
     return MCX_E_NULL;
-  int64_t total = 0;
+  int64_t total = 0, bytes = 0;
   for (int64_t t = 0; t < count; t++) {
     if ((param_dtypes[t] != MCX_F32 && param_dtypes[t] != MCX_BF16) ||
         (grad_dtypes[t] != MCX_F32 && grad_dtypes[t] != MCX_BF16))
@@ -315,7 +330,9 @@ int mcx_adamw_step(void *const *params, const void *const *grads, void *const *f
                      (o->bits == 8 && (!first_scales[t] || !second_scales[t]))))
       return MCX_E_NULL;
     total += sizes[t];
+    bytes += sizes[t] * ((param_dtypes[t] == MCX_BF16 ? 2 : 4) + (grad_dtypes[t] == MCX_BF16 ? 2 : 4) + o->bits / 4);
   }
+  const bool passing = bytes > kCacheBytes;
   // two chunks a workgroup
   const int64_t even = ((total + 2 * kBlocks - 1) / (2 * kBlocks) + 1023) / 1024 * 1024;
   const int64_t chunk = std::max(kLeast, std::min(kLargest, even));
@@ -347,8 +364,9 @@ int mcx_adamw_step(void *const *params, const void *const *grads, void *const *f
     }
     if (!l.count) break;
     const int blocks = std::min(l.first[l.count], kBlocks);
-    hipLaunchKernelGGL(o->bits == 8 ? adamw_kernel<8> : adamw_kernel<32>, dim3(blocks), dim3(kThreads),
-                       0, (hipStream_t)stream, l, n);
+    const auto kernel = o->bits == 8 ? (passing ? adamw_kernel<8, true> : adamw_kernel<8, false>)
+                                     : (passing ? adamw_kernel<32, true> : adamw_kernel<32, false>);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, (hipStream_t)stream, l, n);
     MCX_HIP_CHECK_LAUNCH();
   }
   return MCX_OK;

@@ -10,6 +10,8 @@ from .mapped_max_pooling_layer import MappedMaxPool
 from .mapped_avg_pooling_layer import MappedAvgPool, MappedAvgUnpool
 from .resample_layer import Resample, Unresample
 from .relative_attention_layer import QKNormRotation, RelativeAttention
+from .recurrence_layer import GatedRecurrence, GroupNormActivation
 
 __all__ = ['MappedConvolution', 'MappedTransposedConvolution', 'MappedMaxPool', 'MappedAvgPool',
-           'MappedAvgUnpool', 'Resample', 'Unresample', 'QKNormRotation', 'RelativeAttention']
+           'MappedAvgUnpool', 'Resample', 'Unresample', 'QKNormRotation', 'RelativeAttention',
+           'GatedRecurrence', 'GroupNormActivation']

@@ -25,6 +25,10 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                                       bits=bits))
 
+    def __getstate__(self):
+        own = ('max_norm', 'capturable', 'seed', 'grad_norm')
+        return dict(super().__getstate__(), **{name: getattr(self, name) for name in own})
+
     def _state_of(self, p, bits, counter):
         """The moments of a parameter, zeros when it first has a gradient."""
         state = self.state[p]

@@ -3,7 +3,8 @@
 Tolerances, u = 2^-24.  m: two constants, two products and a sum, each rounded: 3 u of |b1 m| + |c1 g|
 and u of the result, 4 u in all; v: one product more, 5 u.  The change of p: m's 4 u, sqrt(v)'s half of 5 u
 and its own rounding, two constants, two products, a sum, a division: 12 u of its size before
-anything cancels; p's product and the difference: 3 u of p.  bf16 parameters: 2^-8 of the result
+anything cancels, and in 8 bits, where root and reciprocal are off by a unit in the last place (2 u) each
+and the quotient is a product more, 15 u; p's product and the difference: 3 u of p.  bf16 parameters: 2^-8 of the result
 besides.  Clipping: the factor is off by 1e-6 (the norm) and a rounding: 1.2e-6 of g, 2.4e-6 of v.
 In 8 bits what is held is equal to the definition's, but where the exact sum of value and chance lies
 nearer to a border than 32 bits tell (4 u of the parts over the step, and 2^-19 for up to 16 steps)."""
@@ -81,7 +82,7 @@ class Problem:
                                                    1.0 if factor is None else factor)
             more = 0.0 if factor is None else 1.2e-6
             half = 2.0 ** -8 if self.p[t].dtype == BF16 else 0.0
-            bound = 3 * U * p0.abs() + (12 * U + 2 * more) * change + half * p1.abs() + 1e-37
+            bound = 3 * U * p0.abs() + ((12 if self.bits == 32 else 15) * U + 2 * more) * change + half * p1.abs() + 1e-37
             off = (self.p[t].double().cpu() - p1).abs()
             assert (off <= bound).all(), (t, n, (off / bound).max())
             m_now, v_now = self.moments()[t]

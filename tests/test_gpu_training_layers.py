@@ -1,0 +1,364 @@
+"""The layers for recurrence and group norm, the optimizer, and the example that runs them together."""
+import copy
+import io
+
+import pytest
+import torch
+
+from mappedconvolutions_amd import _C, nn, util
+from mappedconvolutions_amd.examples import scan_recurrence
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layers_pass_gradients_to_float32_parameters(device, dtype):
+    torch.manual_seed(0)
+    norm = nn.GroupNormActivation(4, 24, activation="silu").to(device)
+    torch.nn.init.normal_(norm.weight)
+    torch.nn.init.normal_(norm.bias)
+    scan = nn.GatedRecurrence(reverse=True)
+    x = torch.randn(3, 5, 8, 24, device=device).to(dtype).requires_grad_()
+    first = torch.randn(3, 8, device=device, requires_grad=True)
+    lengths = torch.tensor([40, 0, 17], dtype=torch.int32, device=device)
+    y = norm(x)
+    packed = y.flatten(1, 2)
+    packed.retain_grad()
+    out, final = scan(*packed.split(8, 2), first, lengths)
+    g, gh = torch.randn_like(out), torch.randn_like(final)
+    torch.autograd.backward((out, final), (g, gh))
+    # the same by the operators
+    w, b = norm.weight.to(dtype), norm.bias.to(dtype)
+    want, saved = _C.group_norm_forward(x.flatten(1, 2), 4, w, b, activation="silu", for_backward=True)
+    assert torch.equal(y, want.view(y.shape))
+    parts = want.split(8, 2)
+    o, f, states = _C.gated_recurrence_forward(*parts, first, lengths, True, for_backward=True)
+    assert torch.equal(out, o) and torch.equal(final, f)
+    *grads, gi = _C.gated_recurrence_backward(g, *parts, states, gh, lengths, True)
+    assert torch.equal(packed.grad, torch.cat(grads, 2)) and torch.equal(first.grad, gi)
+    gx, gw, gb = _C.group_norm_backward(packed.grad, x.flatten(1, 2), saved, 4, w, b, activation="silu")
+    assert torch.equal(x.grad, gx.view(x.shape))
+    assert norm.weight.grad.dtype == F32
+    assert torch.equal(norm.weight.grad, gw.float()) and torch.equal(norm.bias.grad, gb.float())
+
+
+def test_gradients_of_one_output(device):
+    v, f, z = (torch.randn(2, 30, 8, device=device, requires_grad=True) for _ in range(3))
+    scan = nn.GatedRecurrence()
+    out, final = scan(v, f, z)
+    a = torch.autograd.grad(out.sum(), (v, f, z), retain_graph=True)
+    b = torch.autograd.grad(final.sum(), (v, f, z))
+    assert (b[2] == 0).all() and all(torch.isfinite(t).all() for t in a + b)
+    both = torch.autograd.grad(sum(t.sum() for t in scan(v, f, z)), (v, f, z))
+    for x, y, s in zip(a, b, both):
+        # two sums of the same numbers in another order: 64 roundings of values below 8
+        assert (x + y - s).abs().max().item() <= 64 * 8 * U
+    # a shared gate collects the gradients of all that it opens
+    one = torch.randn(2, 1, 8, device=device, requires_grad=True)
+    out, _ = scan(v, one.expand(2, 30, 8))
+    out.sum().backward()
+    wide = one.detach().expand(2, 30, 8).contiguous().requires_grad_()
+    scan(v.detach(), wide)[0].sum().backward()
+    assert torch.equal(one.grad, wide.grad.sum(1, keepdim=True))
+
+
+def test_second_derivatives_are_refused(device):
+    x = torch.randn(2, 20, 8, device=device, requires_grad=True)
+    for y in (nn.GatedRecurrence()(x, x, x)[0], nn.GatedRecurrence()(x, x)[1],
+              nn.GroupNormActivation(2, 8, activation="gelu").to(device)(x)):
+        gradient, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            gradient.sum().backward()
+
+
+def test_nothing_is_saved_without_a_graph(device, monkeypatch):
+    asked = []
+    for name in ("gated_recurrence_forward", "group_norm_forward"):
+        def watched(*args, _forward=getattr(_C, name), for_backward=False, **kw):
+            asked.append(for_backward)
+            return _forward(*args, for_backward=for_backward, **kw)
+        monkeypatch.setattr(_C, name, watched)
+    norm, scan = nn.GroupNormActivation(2, 8).to(device), nn.GatedRecurrence()
+    x = torch.randn(2, 20, 8, device=device)
+    with torch.no_grad():
+        norm(x), scan(x, x)
+    scan(x, x)
+    norm(x)
+    assert asked == [False, False, False, True]
+
+
+def test_shapes_and_memory_of_the_norm(device):
+    norm = nn.GroupNormActivation(4, 16, affine=False, activation="silu").to(device)
+    x = torch.randn(3, 16, 6, 10, device=device)
+    want = torch.nn.functional.silu(torch.nn.functional.group_norm(x.double(), 4)).float()
+    # 60 x 4 values: a few roundings of values up to 4
+    last = x.contiguous(memory_format=torch.channels_last)
+    for t in (x, last):
+        got = norm(t.permute(0, 2, 3, 1))
+        assert got.shape == (3, 6, 10, 16)
+        assert (got.permute(0, 3, 1, 2) - want).abs().max().item() <= 64 * 4 * U
+    assert norm(torch.randn(5, 16, device=device)).shape == (5, 16)
+    assert norm(torch.randn(0, 4, 16, device=device)).shape == (0, 4, 16)
+
+
+def test_refusals_on_the_gpu(device):
+    x = torch.zeros(2, 5, 16, device=device)
+    state = torch.zeros(2, 16, device=device)
+    for kw in (dict(initial=state.bfloat16()), dict(initial=state[:1]), dict(final=state[:, :8]),
+               dict(final=torch.zeros(16, 2, device=device).t()), dict(initial=state.cpu()),
+               dict(lengths=torch.zeros(2, dtype=torch.int64, device=device)),
+               dict(lengths=torch.zeros(3, dtype=torch.int32, device=device)),
+               dict(lengths=torch.zeros(2, dtype=torch.int32)), dict(gate=x[:, :, :8]),
+               dict(gate=x.cpu())):
+        with pytest.raises(RuntimeError):
+            _C.gated_recurrence_forward(x, x, **kw)
+    _, _, saved = _C.gated_recurrence_forward(x, x, for_backward=True)
+    for kw in (dict(saved=None), dict(saved=saved[:1]), dict(saved=saved.double()),
+               dict(grad_final=state[:1]), dict(grad_output=x.bfloat16()), dict(grad_output=x[:, :4])):
+        args = dict(grad_output=x, value=x, forget=x, gate=None, saved=saved)
+        args.update(kw)
+        with pytest.raises(RuntimeError):
+            _C.gated_recurrence_backward(**args)
+    w = torch.ones(16, device=device)
+    for args in ((x, 3), (x, 0), (x, 4, w[:8]), (x, 4, w.bfloat16()), (x, 4, w.cpu()), (x, 4, w, w, -1.0),
+                 (x, 4, w, w, 1e-5, "tanh"), (x, 4, torch.ones(32, device=device)[::2])):
+        with pytest.raises(RuntimeError):
+            _C.group_norm_forward(*args)
+    _, saved = _C.group_norm_forward(x, 4, for_backward=True)
+    for worse in (None, saved[:, :2], saved.double(), saved.cpu()):
+        with pytest.raises(RuntimeError):
+            _C.group_norm_backward(x, x, worse, 4)
+    with pytest.raises(RuntimeError):
+        _C.group_norm_backward(x[:, :3], x, saved, 4)
+    # the optimizer's step
+    p, g, m, v = (torch.zeros(300, device=device) for _ in range(4))
+    c, s = torch.zeros(300, dtype=torch.uint8, device=device), torch.zeros(2, device=device)
+    one = torch.tensor(1, device=device)
+    for args, kw in (
+            (([p], [g[:200]], [m], [v], 1, 1e-3), {}), (([p], [g.double()], [m], [v], 1, 1e-3), {}),
+            (([p], [g], [m.bfloat16()], [v], 1, 1e-3), {}), (([p], [g], [c], [c.clone()], 1, 1e-3), {}),
+            (([p], [g], [m], [v.cpu()], 1, 1e-3), {}), (([p], [g], [m], [m], 1, 1e-3), {}),
+            (([p], [p], [m], [v], 1, 1e-3), {}), (([p, p], [g, g], [m, v], [m, v], 1, 1e-3), {}),
+            (([p], [g], [c], [c.clone()], 1, 1e-3), dict(first_scales=[s], second_scales=[s[:1]])),
+            (([p], [g], [c], [c.clone()], 1, 1e-3), dict(first_scales=[s], second_scales=[s])),
+            (([p], [g], [m], [v], 1, 1e-3), dict(first_scales=[s], second_scales=[s.clone()])),
+            (([p], [g], [m], [v], one.int(), 1e-3), {}), (([p], [g], [m], [v], one.cpu(), 1e-3), {}),
+            (([p], [g], [m], [v], 1, one), {}),
+            (([p], [g], [m], [v], 1, 1e-3), dict(grad_norm=s, max_norm=1.0)),
+            (([torch.zeros(20, 20, device=device).t()], [g], [m], [v], 1, 1e-3), {})):
+        with pytest.raises(RuntimeError):
+            _C.adamw_step(*args, **kw)
+    for t in (p, m, v):
+        assert (t == 0).all()
+    with pytest.raises(RuntimeError):
+        _C.adamw_moment(c, s[:1], False)
+    with pytest.raises(RuntimeError):
+        _C.adamw_moment(c, s, False, torch.float16)
+    empty = [torch.zeros(0, device=device) for _ in range(4)]
+    _C.adamw_step([empty[0], p], [empty[1], g], [empty[2], m], [empty[3], v], 1, 1e-3)
+
+
+# ---- the optimizer ------------------------------------------------------------------------
+
+def parameters(dtype=F32, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    shapes = ((3, 5), (7,), (4, 6, 2, 2), (300,), ())
+    ps = [torch.randn(s, generator=g).to(dtype).cuda() for s in shapes]
+    ps[2] = ps[2].contiguous(memory_format=torch.channels_last)
+    return [torch.nn.Parameter(p) for p in ps]
+
+
+def give_gradients(params, seed, skip=()):
+    g = torch.Generator().manual_seed(seed)
+    for i, p in enumerate(params):
+        grad = torch.randn(p.shape, generator=g).to(p.device, p.dtype)
+        p.grad = None if i in skip else grad
+
+
+def test_optimizer_against_float64(device):
+    """Ten steps against torch's optimizer in 64 bits.  A step's change is off by 12 u of its size (up to
+    lr times a few), the moments by 4 u a step: 10 x 10 x 12 u of 0.1, and u of the parameters a step."""
+    ours = parameters()
+    wide = [torch.nn.Parameter(p.detach().double()) for p in ours]
+    args = dict(betas=(0.8, 0.95), eps=1e-6)
+    groups = lambda ps: [dict(params=ps[:2], lr=0.02, weight_decay=0.1), dict(params=ps[2:])]  # noqa: E731
+    optimizer = util.AdamW(groups(ours), lr=0.1, weight_decay=0.0, **args)
+    reference = torch.optim.AdamW(groups(wide), lr=0.1, weight_decay=0.0, **args)
+    for k in range(10):
+        give_gradients(ours, k, skip=(1,) if k < 3 else ())  # one parameter joins later
+        for p, w in zip(ours, wide):
+            w.grad = None if p.grad is None else p.grad.double()
+        optimizer.step()
+        reference.step()
+    for p, w in zip(ours, wide):
+        assert (p.double() - w).abs().max().item() <= 1200 * U * 0.1 + 40 * U * w.abs().max().item()
+    assert optimizer.state[ours[1]]["step"] == 7 and optimizer.state[ours[0]]["step"] == 10
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_optimizer_clips_as_clipping_does(device, dtype, bits):
+    ours, other = parameters(dtype), parameters(dtype)
+    a = util.AdamW(ours, lr=0.1, bits=bits, max_norm=0.5, eps=1e-3)
+    b = util.AdamW(other, lr=0.1, bits=bits, eps=1e-3)
+    give_gradients(ours, 1)
+    give_gradients(other, 1)
+    before = [p.grad.clone() for p in ours]
+    a.step()
+    norm = util.clip_grad_norm_(other, 0.5)
+    b.step()
+    assert torch.equal(a.grad_norm, norm)
+    for p, q, g in zip(ours, other, before):
+        assert torch.equal(p.grad, g)  # read, not changed
+        # clipped gradients are rounded to the parameters' type there (2^-8 or 2^-24 of them, and of the
+        # change, 0.1 at most), and are not here
+        half = 2.0 ** -8 if dtype == BF16 else U
+        assert (p.double() - q.double()).abs().max().item() <= 0.1 * 2 * half + 2 * half * p.abs().max().item()
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_optimizer_goes_on_from_a_file(device, dtype, bits, capturable):
+    ours = parameters(dtype)
+    make = lambda ps: util.AdamW(ps, lr=0.05, bits=bits, max_norm=1.0, capturable=capturable)  # noqa: E731
+    optimizer = make(ours)
+    for k in range(3):
+        give_gradients(ours, k, skip=(3,) if k == 0 else ())
+        optimizer.step()
+    file = io.BytesIO()
+    torch.save(optimizer.state_dict(), file)
+    file.seek(0)
+    again = [torch.nn.Parameter(p.detach().clone()) for p in ours]
+    loaded = make(again)
+    loaded.load_state_dict(torch.load(file, weights_only=True))
+    kinds = {n: v.dtype for n, v in optimizer.state[ours[0]].items() if isinstance(v, torch.Tensor)}
+    assert kinds == {n: v.dtype for n, v in loaded.state[again[0]].items() if isinstance(v, torch.Tensor)}
+    if capturable:  # counters are shared again
+        assert len({id(loaded.state[p]["step"]) for p in again}) == 2
+    for k in range(3, 6):
+        give_gradients(ours, k)
+        give_gradients(again, k)
+        optimizer.step()
+        loaded.step()
+    for p, q in zip(ours, again):
+        assert torch.equal(p, q)
+        for name, value in optimizer.state[p].items():
+            other = loaded.state[q][name]
+            assert value.equal(other) if isinstance(value, torch.Tensor) else value == other
+
+
+def test_optimizer_shares_a_gradient_and_copies(device):
+    a, b = (torch.nn.Parameter(torch.ones(10, device=device)) for _ in range(2))
+    a.grad = b.grad = torch.full((10,), 3.0, device=device)
+    optimizer = util.AdamW([a, b], lr=0.1, max_norm=1e9)
+    optimizer.step()
+    assert torch.equal(a, b) and abs(optimizer.grad_norm.item() - 90 ** 0.5) < 1e-5
+    other = copy.deepcopy(optimizer)
+    assert other.max_norm == 1e9 and len(other.state) == 2
+    with pytest.raises(RuntimeError, match="sparse"):
+        a.grad = torch.eye(10, device=device)[0].to_sparse()
+        optimizer.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_training_step(device, bits):
+    """Norm, recurrence, gradients, clipping and the step in one graph, replayed with other data and another
+    rate, against the same steps one by one."""
+    def make():
+        torch.manual_seed(5)
+        block = scan_recurrence.ScanBlock(32, 4).to(device)
+        params = list(block.parameters())
+        rate = torch.tensor(1e-2, device=device)
+        optimizer = util.AdamW(params, lr=rate, bits=bits, max_norm=0.5, capturable=True)
+        return block, params, rate, optimizer
+
+    x, wanted = torch.empty(2, 2, 500, 32, device=device).unbind()
+    lengths = torch.tensor([500, 333], dtype=torch.int32, device=device)
+
+    def gradients(block, params):
+        loss = (block(x, lengths) - wanted).square().mean()
+        for p, g in zip(params, torch.autograd.grad(loss, params)):
+            p.grad.copy_(g)
+
+    def fill(k):
+        g = torch.Generator(device=device).manual_seed(k)
+        for t in (x, wanted):
+            t.copy_(torch.randn(t.shape, generator=g, device=device))
+
+    sides = [make(), make()]
+    side = torch.cuda.Stream()
+    fill(0)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # the first step makes the moments
+        for block, params, _, optimizer in sides:
+            for p in params:
+                p.grad = torch.zeros_like(p)
+            gradients(block, params)
+            optimizer.step()
+    torch.cuda.current_stream().wait_stream(side)
+    block, params, rate, optimizer = sides[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gradients(block, params)
+        optimizer.step()
+    for k in range(1, 5):
+        fill(k)
+        for s in sides:
+            s[2].fill_(1e-2 / k)
+        graph.replay()
+        torch.cuda.synchronize()
+        gradients(sides[1][0], sides[1][1])
+        sides[1][3].step()
+        torch.cuda.synchronize()
+        for p, q in zip(params, sides[1][1]):
+            assert torch.equal(p, q)
+    assert optimizer.state[params[0]]["step"].item() == 5
+
+
+# ---- the example --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_example_trains(device, dtype, bits):
+    net, losses = scan_recurrence.train(steps=5, height=8, width=48, bits=bits, dtype=dtype)
+    assert len(losses) == 5 and all(torch.isfinite(torch.tensor(losses)))
+    for p in net.parameters():
+        assert torch.isfinite(p).all() and p.grad is not None and p.grad.abs().sum() > 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_example_serves(device, dtype):
+    whole, one_by_one = scan_recurrence.serve(dtype=dtype)
+    # the same numbers but for the order of sums; in bf16 two roundings of each value (2^-8 of values up to
+    # 8, after products over 128 channels that may turn one rounding into another)
+    bound = 1e-4 if dtype == F32 else 0.125
+    assert (whole - one_by_one).abs().max().item() <= bound
+
+
+def test_gradient_of_the_example_against_differences(device):
+    """One block, all its parts, along a direction: the loss is a mean of 2 x 40 x 16 squares in 32 bits (an
+    error of 10^-6 of it, over 2 h), the third derivative's share h^2."""
+    torch.manual_seed(3)
+    block = scan_recurrence.ScanBlock(16, 4, activation="gelu").to(device)
+    x, wanted = torch.randn(2, 2, 40, 16, device=device).unbind()
+    params = list(block.parameters())
+
+    def loss():
+        return (block(x) - wanted).double().square().mean()
+
+    grads = torch.autograd.grad(loss(), params)
+    way = [torch.randn_like(p) for p in params]
+    slope = sum((g.double() * w.double()).sum() for g, w in zip(grads, way)).item()
+    h, values = 2.0 ** -8, []
+    with torch.no_grad():
+        for sign in (1, -1):
+            for p, w in zip(params, way):
+                p.add_(w, alpha=sign * h)
+            values.append(loss().item())
+            for p, w in zip(params, way):
+                p.sub_(w, alpha=sign * h)
+    assert abs((values[0] - values[1]) / (2 * h) - slope) <= 1e-2 * (1 + abs(slope))
