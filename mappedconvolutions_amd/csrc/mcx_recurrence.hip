@@ -26,9 +26,10 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kRowLanes = 16;           // lanes of a step's channels
 constexpr int kRuns = kThreads / kRowLanes;  // runs of steps of a tile
-constexpr int kForward = 4, kBackward = 4;   // steps of a run
-constexpr int kTile = kRuns * kForward;
-constexpr int kSpan = kRuns * kBackward;     // steps from one kept state to the next
+// Steps of a run: 16 values a lane, 8 in single precision (whose words hold 2) and where no words can be read, so
+// that all fits the registers.
+constexpr int run_steps(int word, int size) { return word == 4 || size == 4 ? 4 : 8; }
+constexpr int kSpan = kRuns * 4;             // steps from one kept state to the next, a part of every tile
 constexpr int kFew = 8;                 // steps that a thread walks alone
 // Workgroups aimed at by segments: as many as are resident at a time (forward, float32 backward, bf16 back-
 // ward; 768 there: 2 sequences of 32768 steps of 1024 channels 440 -> 542 us), and by the parts of the first
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void recurrence_parts_kernel(RecurParams 
 
 template <typename T, int E, bool Gated, bool Passing>
 __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurParams p) {
-  constexpr int N = kForward;
+  constexpr int N = run_steps(E, sizeof(T)), kTile = kRuns * N;
   __shared__ Exchange<E> both[2];
   __shared__ Ranges<E> ranges;
   const int lane = threadIdx.x & (kRowLanes - 1), run = threadIdx.x / kRowLanes;
@@ -416,7 +417,7 @@ __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurPa
 
 template <typename T, int E, bool Gated, bool Passing>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurParams p) {
-  constexpr int N = kBackward;
+  constexpr int N = run_steps(E, sizeof(T)), kTile = kRuns * N;
   __shared__ Exchange<E> ahead[2], back[2];
   __shared__ Ranges<E> ranges;
   const int lane = threadIdx.x & (kRowLanes - 1), run = threadIdx.x / kRowLanes;
@@ -424,16 +425,16 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
   // (from the beginning, which the first launch read last)
   const Place at = place_of<E>(p, blockIdx.x, p.segments);
   const int begin = at.segment * p.segment, end = min(p.L, begin + p.segment);
-  const int last = begin + (end - begin - 1) / kSpan * kSpan;
+  const int last = begin + (end - begin - 1) / kTile * kTile;
   Raw<T, E> rv[N], rf[N], rg[N], ro[N];
   float kept[E];
   const auto load = [&](int s0) {
-    const auto v = Rows<T>::template of<kSpan>(p, at, s0, p.v, p.vs[0], p.vs[1], run * N);
-    const auto f = Rows<T>::template of<kSpan>(p, at, s0, p.f, p.fs[0], p.fs[1], run * N);
-    const auto g = Rows<T>::template of<kSpan>(p, at, s0, p.g, p.gs[0], p.gs[1], run * N);
-    const auto o = Rows<T>::template of<kSpan>(p, at, s0, p.go, (int64_t)p.L * p.C, p.C, run * N);
+    const auto v = Rows<T>::template of<kTile>(p, at, s0, p.v, p.vs[0], p.vs[1], run * N);
+    const auto f = Rows<T>::template of<kTile>(p, at, s0, p.f, p.fs[0], p.fs[1], run * N);
+    const auto g = Rows<T>::template of<kTile>(p, at, s0, p.g, p.gs[0], p.gs[1], run * N);
+    const auto o = Rows<T>::template of<kTile>(p, at, s0, p.go, (int64_t)p.L * p.C, p.C, run * N);
     const int s = s0 + run * N;
-    const bool whole = s0 + kSpan <= at.len;
+    const bool whole = s0 + kTile <= at.len;
 #pragma unroll
     for (int e = 0; e < E; e++)
       kept[e] = p.states[((int64_t)at.b * p.spans + s0 / kSpan) * p.C + at.c + e];
@@ -466,9 +467,9 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
   for (int e = 0; e < E; e++) carry[e] = p.gfinal ? p.gfinal[(int64_t)at.b * p.C + at.c + e] : 0.f;
   if (p.segments > 1) carry_in<E, true>(p, at, ranges, carry);
   int turn = 0;
-  for (int s0 = last; s0 >= begin; s0 -= kSpan, turn ^= 1) {
+  for (int s0 = last; s0 >= begin; s0 -= kTile, turn ^= 1) {
     const int s = s0 + run * N;
-    const bool whole = s0 + kSpan <= at.len;
+    const bool whole = s0 + kTile <= at.len;
     float a[N][E], away[N][E], h[N][E], d[N][E], A[E], H[E], before_a[E], before_h[E], state[E];
 #pragma unroll
     for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
@@ -493,9 +494,9 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
       for (int e = 0; e < E; e++) state[e] = fmaf(x.a[w][lane][e], state[e], x.h[w][lane][e]);
 #pragma unroll
     for (int e = 0; e < E; e++) state[e] = fmaf(before_a[e], state[e], before_h[e]);
-    const auto gv = Rows<T>::template of<kSpan>(p, at, s0, p.gv, (int64_t)p.L * p.C, p.C, run * N);
-    const auto gf = Rows<T>::template of<kSpan>(p, at, s0, p.gf, (int64_t)p.L * p.C, p.C, run * N);
-    const auto gg = Rows<T>::template of<kSpan>(p, at, s0, p.gg, (int64_t)p.L * p.C, p.C, run * N);
+    const auto gv = Rows<T>::template of<kTile>(p, at, s0, p.gv, (int64_t)p.L * p.C, p.C, run * N);
+    const auto gf = Rows<T>::template of<kTile>(p, at, s0, p.gf, (int64_t)p.L * p.C, p.C, run * N);
+    const auto gg = Rows<T>::template of<kTile>(p, at, s0, p.gg, (int64_t)p.L * p.C, p.C, run * N);
     // h: what the state before a step differs from its value by
 #pragma unroll
     for (int i = 0; i < N; i++) {
@@ -514,7 +515,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
       }
       if (Gated && p.gg && at.here && (whole || s + i < at.len)) put<T, E, Passing>(gg.at(i), y);
     }
-    if (s0 > begin) load(s0 - kSpan);
+    if (s0 > begin) load(s0 - kTile);
 #pragma unroll
     for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
 #pragma unroll
@@ -629,39 +630,40 @@ int word_of(const mcx_recurrence_desc *d, int size, bool gated, uint64_t address
   return 1;
 }
 // Segments make kGroups workgroups of the second launch, parts of them kSums of the first, which has less to
-// do and so needs more under way; a tile at least.
+// do and so needs more under way; two tiles and one at least.
 struct Cut {
   int segments, segment, parts, each, share;
 };
-Cut cut_of(const mcx_recurrence_desc *d, int word, int groups) {
+Cut cut_of(const mcx_recurrence_desc *d, int word, int size, int groups) {
   const int64_t columns = std::max<int64_t>(1, d->B * ((d->C + kRowLanes * word - 1) / (kRowLanes * word)));
   int64_t n = columns >= kAlone ? 1 : (groups + columns - 1) / columns;
-  n = std::max<int64_t>(1, std::min(n, d->L / (4 * kTile)));
+  const int64_t tile = kRuns * run_steps(word, size);
+  n = std::max<int64_t>(1, std::min(n, d->L / (2 * tile)));
   // in tiles
-  const int64_t segment = ((d->L + n - 1) / n + kTile - 1) / kTile;
+  const int64_t segment = ((d->L + n - 1) / n + tile - 1) / tile;
   const int64_t each = std::max<int64_t>(1, segment * columns * n / kSums);
   Cut c;
-  c.share = (int)((segment + each - 1) / each), c.each = (int)(each * kTile), c.segment = c.share * c.each;
+  c.share = (int)((segment + each - 1) / each), c.each = (int)(each * tile), c.segment = c.share * c.each;
   c.segments = (int)((d->L + c.segment - 1) / c.segment);
   c.parts = (int)((d->L + c.each - 1) / c.each);
   return c;
 }
-size_t part_bytes(const mcx_recurrence_desc *d) {
+size_t part_bytes(const mcx_recurrence_desc *d, int dtype) {
   int64_t n = 0;
   for (int w : {1, 2, 4}) {  // (whichever the alignment gives)
     for (int groups : {kGroups, kGroupsBf16Backward}) {
-      const Cut c = cut_of(d, w, groups);
+      const Cut c = cut_of(d, w, dtype == MCX_BF16 ? 2 : 4, groups);
       if (c.segments > 1) n = std::max<int64_t>(n, c.parts + 1);
     }
   }
   return (size_t)(d->B * n * 2 * d->C) * sizeof(float);
 }
-RecurParams params_of(const mcx_recurrence_desc *d, int word, int groups, void *workspace) {
+RecurParams params_of(const mcx_recurrence_desc *d, int word, int size, int groups, void *workspace) {
   RecurParams p = {};
   for (int k = 0; k < 2; k++) p.vs[k] = d->v_stride[k], p.fs[k] = d->f_stride[k], p.gs[k] = d->g_stride[k];
   p.L = (int)d->L, p.C = (int)d->C;
   p.tiles = (int)((d->C + kRowLanes * word - 1) / (kRowLanes * word));
-  const Cut c = cut_of(d, word, groups);
+  const Cut c = cut_of(d, word, size, groups);
   p.segment = c.segment, p.segments = c.segments, p.parts = c.parts, p.each = c.each, p.share = c.share;
   p.spans = (int)((d->L + kSpan - 1) / kSpan);
   p.reverse = d->reverse != 0;
@@ -740,7 +742,7 @@ int64_t mcx_gated_recurrence_spans(int64_t L) { return L < 0 ? 0 : (L + mcx::kSp
 size_t mcx_gated_recurrence_workspace(const mcx_recurrence_desc *desc, int dtype) {
   using namespace mcx;
   if (check_desc(desc, dtype) != MCX_OK || !desc->B || !desc->L) return 0;
-  return part_bytes(desc);
+  return part_bytes(desc, dtype);
 }
 
 int mcx_gated_recurrence_forward(const void *value, const void *forget, const void *gate,
@@ -751,11 +753,12 @@ int mcx_gated_recurrence_forward(const void *value, const void *forget, const vo
   if (int e = check_desc(desc, dtype)) return e;
   if (!desc->B || !desc->L) return MCX_OK;
   if (!value || !forget || !out || !final) return MCX_E_NULL;
-  const size_t need = part_bytes(desc);
+  const size_t need = part_bytes(desc, dtype);
   if (need && (!workspace || workspace_bytes < need)) return MCX_E_WORKSPACE;
-  const int word = word_of(desc, dtype == MCX_BF16 ? 2 : 4, gate != nullptr,
+  const int size = dtype == MCX_BF16 ? 2 : 4;
+  const int word = word_of(desc, size, gate != nullptr,
                            (uintptr_t)value | (uintptr_t)forget | (uintptr_t)gate | (uintptr_t)out);
-  RecurParams p = params_of(desc, word, kGroups, workspace);
+  RecurParams p = params_of(desc, word, size, kGroups, workspace);
   p.v = value, p.f = forget, p.g = gate, p.initial = initial, p.lengths = lengths;
   p.out = out, p.final = final, p.states = states;
   return dtype == MCX_BF16 ? launch<__bf16, true>(p, desc->B, word, (hipStream_t)stream)
@@ -771,12 +774,13 @@ int mcx_gated_recurrence_backward(const void *gout, const float *gfinal, const v
   if (int e = check_desc(desc, dtype)) return e;
   if (!desc->B || !desc->L) return MCX_OK;
   if (!gout || !value || !forget || !states) return MCX_E_NULL;
-  const size_t need = part_bytes(desc);
+  const size_t need = part_bytes(desc, dtype);
   if (need && (!workspace || workspace_bytes < need)) return MCX_E_WORKSPACE;
-  const int word = word_of(desc, dtype == MCX_BF16 ? 2 : 4, gate != nullptr,
+  const int size = dtype == MCX_BF16 ? 2 : 4;
+  const int word = word_of(desc, size, gate != nullptr,
                            (uintptr_t)value | (uintptr_t)forget | (uintptr_t)gate | (uintptr_t)gout |
                                (uintptr_t)gvalue | (uintptr_t)gforget | (uintptr_t)ggate);
-  RecurParams p = params_of(desc, word, dtype == MCX_BF16 ? kGroupsBf16Backward : kGroups, workspace);
+  RecurParams p = params_of(desc, word, size, size == 2 ? kGroupsBf16Backward : kGroups, workspace);
   p.v = value, p.f = forget, p.g = gate, p.go = gout, p.gfinal = gfinal, p.lengths = lengths;
   p.gv = gvalue, p.gf = gforget, p.gg = ggate, p.ginitial = ginitial;
   p.states = const_cast<float *>(states);
