@@ -1162,17 +1162,12 @@ def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
 # ---- a gated linear recurrence along a sequence ---------------------------------------------
 
 _two = _lib._i64 * 2
-
-
-def _pair(t):
-    return _two(t.stride(0), t.stride(1))
-
-
 _RECURRENCE_STRIDE = 1 << 22
 
 
-def _recurrence_args(value, forget, gate, lengths, reverse):
-    """(dtype code, descriptor, the tensors as the library takes them) of a recurrence call."""
+def _recurrence_args(value, forget, gate, lengths, reverse, states=(), **others):
+    """(dtype code, descriptor, the tensors as the library takes them) of a recurrence call; `states`:
+    the names of those of the others that are states."""
     shape = value.shape
     if len(shape) != 3 or shape[2] < 1:
         raise RuntimeError("value must have 3 dimensions [B, L, C], got %s" % (tuple(shape),))
@@ -1181,26 +1176,29 @@ def _recurrence_args(value, forget, gate, lengths, reverse):
             raise RuntimeError("%s must have value's shape %s, got %s" %
                                (name, tuple(shape), tuple(t.shape)))
     dt = _attention_dtype(value, forget=forget, gate=gate)
-    _on_gpu("value", value, forget=forget, gate=gate, lengths=lengths)
+    _on_gpu("value", value, forget=forget, gate=gate, lengths=lengths, **others)
     B, L, C = shape
+    for name in states:
+        t = others[name]
+        if t is not None and (t.dtype != torch.float32 or t.shape != (B, C)):
+            raise RuntimeError("%s must be float32 of shape (%d, %d), got %s %s" %
+                               (name, B, C, t.dtype, tuple(t.shape)))
     if lengths is not None:
         if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,):
             raise RuntimeError("lengths must be int32 of shape (%d,), got %s %s" %
                                (B, lengths.dtype, tuple(lengths.shape)))
         lengths = lengths.contiguous()
     # (steps further apart than the kernels' addresses reach are copied)
-    value, forget, gate = (
-        t if t is None or ((t.stride(2) == 1 or C == 1) and t.stride(1) <= _RECURRENCE_STRIDE)
-        else t.contiguous() for t in (value, forget, gate))
-    desc = _lib.RecurrenceDesc(B, L, C, _pair(value), _pair(forget),
-                               _two(0, 0) if gate is None else _pair(gate), int(bool(reverse)), 0)
-    return dt, desc, value, forget, gate, lengths
-
-
-def _state(name, t, like):
-    if t is not None and (t.dtype != torch.float32 or t.shape != (like.shape[0], like.shape[2])):
-        raise RuntimeError("%s must be float32 of shape (%d, %d), got %s %s" %
-                           (name, like.shape[0], like.shape[2], t.dtype, tuple(t.shape)))
+    tensors, strides = [], []
+    for t in (value, forget, gate):
+        stride = (0, 0, 1) if t is None else t.stride()
+        if (stride[2] != 1 and C != 1) or stride[1] > _RECURRENCE_STRIDE:
+            t = t.contiguous()
+            stride = t.stride()
+        tensors.append(t)
+        strides.append(stride[:2])
+    desc = _lib.RecurrenceDesc(B, L, C, *strides, int(bool(reverse)), 0)
+    return (dt, desc, *tensors, lengths)
 
 
 def gated_recurrence_forward(value, forget, gate=None, initial=None, lengths=None, reverse=False,
@@ -1217,11 +1215,9 @@ def gated_recurrence_forward(value, forget, gate=None, initial=None, lengths=Non
     -> [out [B, L, C], final, saved]: the state after the last step float32 [B, C], in the tensor `final`
     where one is given (it may be `initial`, for a state that is kept from call to call); `saved`, for
     gated_recurrence_backward, is None unless `for_backward`: states at some of the steps, float32."""
-    dt, desc, value, forget, gate, lengths = _recurrence_args(value, forget, gate, lengths, reverse)
+    dt, desc, value, forget, gate, lengths = _recurrence_args(
+        value, forget, gate, lengths, reverse, ("initial", "final"), initial=initial, final=final)
     B, L, C = value.shape
-    _state("initial", initial, value)
-    _state("final", final, value)
-    _on_gpu("value", value, initial=initial, final=final)
     _contig(final=final)
     if initial is not None:
         initial = initial.contiguous()
@@ -1254,18 +1250,18 @@ def gated_recurrence_backward(grad_output, value, forget, gate, saved, grad_fina
     same arguments and `for_backward`, from the gradients of out and (float32, zeros by default) of
     final; a gradient that `needs` leaves out, or that of a gate that there is not, is None.  The same
     bits from call to call."""
-    dt, desc, value, forget, gate, lengths = _recurrence_args(value, forget, gate, lengths, reverse)
+    dt, desc, value, forget, gate, lengths = _recurrence_args(
+        value, forget, gate, lengths, reverse, ("grad_final",), grad_final=grad_final,
+        grad_output=grad_output, saved=saved)
     B, L, C = value.shape
     lib = _lib.load()
     if grad_output.shape != value.shape:
         raise RuntimeError("grad_output must have shape %s, got %s" %
                            (tuple(value.shape), tuple(grad_output.shape)))
     _attention_dtype(value, grad_output=grad_output)
-    _state("grad_final", grad_final, value)
     if saved is None or saved.dtype != torch.float32 or \
             tuple(saved.shape) != (B, lib.mcx_gated_recurrence_spans(L), C):
         raise RuntimeError("saved must be what gated_recurrence_forward returned with for_backward")
-    _on_gpu("value", value, grad_output=grad_output, grad_final=grad_final, saved=saved)
     _contig(saved=saved)
     grad_output = grad_output.contiguous()
     if grad_final is not None:
@@ -1333,7 +1329,7 @@ def group_norm_forward(x, groups, weight=None, bias=None, eps=1e-5, activation=N
     ws = _workspace(nbytes, x.device)
     with _device(x):
         rc = lib.mcx_group_norm_forward(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(stats),
-                                        _ptr(ws), nbytes, _pair(x), B, N, C,
+                                        _ptr(ws), nbytes, _two(*x.stride()[:2]), B, N, C,
                                         groups, eps, act, dt, _stream(x))
     _lib.check(rc, "group_norm_forward")
     return [y, stats]
@@ -1369,7 +1365,7 @@ def group_norm_backward(grad_output, x, saved, groups, weight=None, bias=None, a
     with _device(x):
         rc = lib.mcx_group_norm_backward(_ptr(grad_output), _ptr(x), _ptr(saved), _ptr(weight),
                                          _ptr(bias), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), nbytes,
-                                         _pair(x), B, N, C, groups, act, dt,
+                                         _two(*x.stride()[:2]), B, N, C, groups, act, dt,
                                          _stream(x))
     _lib.check(rc, "group_norm_backward")
     return [gx, gw, gb]
