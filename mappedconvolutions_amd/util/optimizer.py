@@ -58,6 +58,12 @@ class AdamW(torch.optim.Optimizer):
                     dense[p.grad] = p.grad.contiguous()
         if not dense:
             return loss
+        if torch.cuda.is_current_stream_capturing():
+            if not self.capturable:
+                raise RuntimeError('Only a capturable AdamW counts the steps of a captured one')
+            if any(p.grad is not None and not self.state[p] for group in self.param_groups
+                   for p in group['params']):
+                raise RuntimeError('The first step of a parameter makes its moments and is not captured')
         norm = None
         if self.max_norm is not None:
             norm = self.grad_norm = _C.grad_norm(list(dense.values()))

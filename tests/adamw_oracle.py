@@ -36,7 +36,8 @@ def decode(code, scale, second):
 
 def held(x, chance, second):
     """(what is held of float64 values x, the step of each, how far each is from being rounded the
-    other way, in steps); `chance`: numbers below 2^16."""
+    other way, in steps, how far its block's largest value is from a power of two, at which the scale
+    doubles, over that value); `chance`: numbers below 2^16."""
     low, n = (-30 if second else -14), x.numel()
     top = per_block(x.abs()).amax(1, keepdim=True)
     scale = torch.where(top > 0, 2 ** (torch.floor(torch.log2(top.clamp_min(1e-300))) + 1), 1.0)
@@ -51,7 +52,10 @@ def held(x, chance, second):
     def wide(t):
         return (per_block(t) * scale).view(-1)[:n]
 
-    return wide(count * step) * torch.sign(x), wide(step), near
+    part = top / scale  # in [1/2, 1)
+    edge = torch.where(top > 0, torch.minimum(part - 0.5, 1 - part) / part.clamp_min(0.5), 1.0)
+    return (wide(count * step) * torch.sign(x), wide(step), near,
+            edge.expand(-1, 256).reshape(-1)[:n])
 
 
 def step(p, g, m, v, number, lr, betas=(0.9, 0.999), eps=1e-8, decay=0.0, factor=1.0):

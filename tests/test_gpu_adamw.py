@@ -7,7 +7,10 @@ anything cancels, and in 8 bits, where root and reciprocal are off by a unit in 
 and the quotient is a product more, 15 u; p's product and the difference: 3 u of p.  bf16 parameters: 2^-8 of the result
 besides.  Clipping: the factor is off by 1e-6 (the norm) and a rounding: 1.2e-6 of g, 2.4e-6 of v.
 In 8 bits what is held is equal to the definition's, but where the exact sum of value and chance lies
-nearer to a border than 32 bits tell (4 u of the parts over the step, and 2^-19 for up to 16 steps)."""
+nearer to a border than 32 bits tell (4 u of the parts over the step, and 2^-19 for up to 16 steps), and in
+blocks whose largest value is as near to a power of two (5 u of its parts, which are at most 2^4 of it
+unless they cancel: 2^-16 is far outside): the scale, and with it the smallest steps, may be twice as
+large there, so that what is held is off by two of these steps and the oracle's by one."""
 import pytest
 import torch
 
@@ -93,11 +96,11 @@ class Problem:
                 chance = oracle.words(number, seed, first, n)
                 for now, exact, part, second in ((m_now, m1, chance & 65535, False),
                                                  (v_now, v1, chance >> 16, True)):
-                    want, step, near = oracle.held(exact, part, second)
+                    want, step, near, edge = oracle.held(exact, part, second)
                     room = ((5 * U + 2 * more) * (v1 if second else size) / step) + 2.0 ** -19
-                    sure = near > room
+                    sure = (near > room) & (edge > 2.0 ** -16)
                     assert torch.equal(now[sure], want[sure])
-                    assert ((now - want).abs() <= 1.001 * step).all()
+                    assert ((now - want).abs() <= torch.where(edge > 2.0 ** -16, 1.001, 3.001) * step).all()
                 first += 256 * oracle.blocks(n)
 
 
@@ -249,6 +252,12 @@ def test_moments_in_8_bits_follow_on_average(device):
     assert first.abs().mean() < 0.3 and abs(first.mean().item()) < 0.01
     _, later = run(1000, 3000, 0.0)
     assert abs(later.mean().item() / (second.mean().item() * 0.999 ** 1000) - 1) < 0.02
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_than_the_cache_holds(device, bits):
+    # (enough values that they pass the cache by)
+    Problem(11, [300, 10000001 if bits == 32 else 27000001], bits, (F32,), (F32, BF16)).check()
 
 
 @pytest.mark.parametrize("second", [False, True])

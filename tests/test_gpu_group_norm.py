@@ -101,7 +101,8 @@ CASES = [  # B, N, C, groups
     (1, 1, 8, 2), (2, 1, 64, 8), (1, 7, 30, 6), (3, 50, 48, 16), (2, 100, 90, 6), (1, 1000, 64, 64),
     (2, 333, 24, 1), (1, 65, 512, 32), (2, 40, 2048, 2048), (1, 130, 2056, 8), (1, 20, 4096, 1),
     (1, 9, 4104, 3), (2, 17, 1001, 7), (1, 33, 6000, 6), (1, 5, 3, 3), (4, 8, 1, 1), (1, 4099, 6, 2),
-    (300, 12, 16, 4), (1, 70001, 16, 4), (1, 12, 10008, 8), (2, 9, 8200, 8)]
+    (300, 12, 16, 4), (1, 70001, 16, 4), (1, 12, 10008, 8), (2, 9, 8200, 8), (70000, 3, 8, 2),
+    (1, 8192, 8, 1), (1, 8193, 8, 1), (2, 2048, 8, 8), (200, 300, 40, 5), (130, 1025, 24, 3)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -246,6 +247,25 @@ def test_in_a_graph_and_on_another_stream(device, dtype):
             for a, c in zip(held, both()):
                 assert torch.equal(a, c)
             torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_results_past_the_cache(device, dtype):
+    """Two samples whose tensors are larger than those whose results stay in the cache, and each alone."""
+    N = 300000 if dtype == BF16 else 150000
+    x, w, b, go = (t.cuda() for t in make(11, 2, N, 64, dtype))
+    y, saved = _C.group_norm_forward(x, 16, w, b, activation="silu", for_backward=True)
+    gx, gw, gb = _C.group_norm_backward(go, x, saved, 16, w, b, activation="silu")
+    sums = 0
+    for i in range(2):
+        one, kept = _C.group_norm_forward(x[i:i + 1], 16, w, b, activation="silu", for_backward=True)
+        assert torch.equal(one[0], y[i]) and torch.equal(kept[0], saved[i])
+        g = _C.group_norm_backward(go[i:i + 1], x[i:i + 1], kept, 16, w, b, activation="silu")
+        assert torch.equal(g[0][0], gx[i])
+        sums = sums + torch.stack(g[1:]).double()
+    # the halves' sums are rounded once more
+    half = 2.0 ** -8 if dtype == BF16 else 2 * U
+    assert ((torch.stack((gw, gb)).double() - sums).abs() <= half * (4 * sums.abs() + 2 * N ** 0.5)).all()
 
 
 def test_more_than_32_bits_of_values(device):

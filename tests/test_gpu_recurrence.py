@@ -118,7 +118,7 @@ def check(v, f, z, go, first, last, lengths=None, reverse=False, views=lambda *t
 
 SIZES = [(1, 1, 1), (2, 2, 3), (3, 7, 64), (2, 8, 60), (2, 9, 66), (1, 127, 16), (2, 128, 4), (1, 129, 130),
          (2, 255, 20), (1, 256, 64), (3, 257, 5), (1, 513, 192), (2, 1025, 12), (1, 4097, 68),
-         (600, 40, 64), (1, 1300, 2)]
+         (600, 40, 64), (1, 1300, 2), (1, 9000, 160), (3, 5000, 33), (1, 70, 20000), (9000, 12, 8)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -281,6 +281,34 @@ def test_the_same_bits_on_two_streams_and_in_a_graph(device):
             for a, b in zip(held, run()):
                 assert torch.equal(a, b)
             torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_results_past_the_cache(device, dtype):
+    """A batch whose tensors are larger than those whose results stay in the cache, and its halves, which
+    are not: each sequence is computed alike."""
+    B = 6000 if dtype == BF16 else 3000
+    v, f, z, go, first, last = (t.cuda() for t in make(10, B, 100, 64, dtype))
+    whole = call(v, f, z, go, first, last, None, False)
+    for half in (slice(0, B // 2), slice(B // 2, B)):
+        for a, b in zip(call(*(t[half] for t in (v, f, z, go, first, last)), None, False), whole):
+            assert torch.equal(a, b[half])
+
+
+def test_steps_far_apart(device):
+    # further than the kernels' addresses reach from a tile's first: copied
+    v, f, z, go, first, last = make(11, 2, 70, 16, BF16)
+
+    def apart(*ts):
+        wide = torch.zeros(70, (1 << 22) + 64, dtype=BF16, device="cuda")
+        out = []
+        for k, t in enumerate(ts):
+            view = wide[:, 32 * k:32 * k + 32].unflatten(1, (2, 16)).transpose(0, 1)
+            view.copy_(t)
+            out.append(view)
+        return out
+
+    check(v, f, z, go, first, last, views=apart)
 
 
 def test_empty(device):

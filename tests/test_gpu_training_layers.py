@@ -319,6 +319,24 @@ def test_a_captured_training_step(device, bits):
     assert optimizer.state[params[0]]["step"].item() == 5
 
 
+def test_steps_that_a_graph_would_not_replay_are_refused(device):
+    for capturable, steps, words in ((False, 1, "capturable"), (True, 0, "first step")):
+        p = torch.nn.Parameter(torch.ones(10, device=device))
+        p.grad = torch.ones(10, device=device)
+        optimizer = util.AdamW([p], capturable=capturable)
+        for _ in range(steps):
+            optimizer.step()
+        graph = torch.cuda.CUDAGraph()
+        refused = False
+        with torch.cuda.graph(graph):
+            try:
+                optimizer.step()
+            except RuntimeError as error:
+                refused = words in str(error)
+            p.grad.add_(0)
+        assert refused
+
+
 # ---- the example --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("bits", [32, 8])
