@@ -317,35 +317,40 @@ __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurPa
   const Place at = place_of<E>(p, gridDim.x - 1 - blockIdx.x, p.segments);
   const int begin = at.segment * p.segment, end = min(p.L, begin + p.segment);
   Raw<T, E> rv[N], rf[N], rz[N];
-  // the tile's values, the next one's while this one is worked on
+  // the tile's values, the next one's while this one is worked on; gates when the tile's are used up
   const auto load = [&](int s0) {
     const auto v = Rows<T>::template of<kTile>(p, at, s0, p.v, p.vs[0], p.vs[1], run * N);
     const auto f = Rows<T>::template of<kTile>(p, at, s0, p.f, p.fs[0], p.fs[1], run * N);
-    const auto g = Rows<T>::template of<kTile>(p, at, s0, p.g, p.gs[0], p.gs[1], run * N);
     const int s = s0 + run * N;
-    const bool whole = s0 + kTile <= at.len;
-    if (whole) {
+    if (s0 + kTile <= at.len) {
 #pragma unroll
-      for (int i = 0; i < N; i++) {
-        rv[i].load(v.at(i));
-        rf[i].load(f.at(i));
-        if (Gated) rz[i].load(g.at(i));
-      }
+      for (int i = 0; i < N; i++) rv[i].load(v.at(i)), rf[i].load(f.at(i));
       return;
     }
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      if (s + i < at.len) {
-        rv[i].load(v.at(i));
-        rf[i].load(f.at(i));
-        if (Gated) rz[i].load(g.at(i));
-      } else {  // a step that leaves the state as it is
-        rv[i].fill(0.f), rf[i].fill(__builtin_inff());
-        if (Gated) rz[i].fill(0.f);
-      }
+      // a step that leaves the state as it is
+      rv[i].fill(0.f), rf[i].fill(__builtin_inff());
+      if (s + i < at.len) rv[i].load(v.at(i)), rf[i].load(f.at(i));
+    }
+  };
+  const auto load_gates = [&](int s0) {
+    if (!Gated) return;
+    const auto g = Rows<T>::template of<kTile>(p, at, s0, p.g, p.gs[0], p.gs[1], run * N);
+    const int s = s0 + run * N;
+    if (s0 + kTile <= at.len) {
+#pragma unroll
+      for (int i = 0; i < N; i++) rz[i].load(g.at(i));
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      rz[i].fill(0.f);
+      if (s + i < at.len) rz[i].load(g.at(i));
     }
   };
   load(begin);
+  load_gates(begin);
   float carry[E];
 #pragma unroll
   for (int e = 0; e < E; e++) carry[e] = 0.f;
@@ -363,12 +368,10 @@ __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurPa
     const int s = s0 + run * N;
     const bool whole = s0 + kTile <= at.len;
     float a[N][E], u[N][E], A[E], H[E], before_a[E], before_h[E];
-    Raw<T, E> z[N];
 #pragma unroll
     for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      if (Gated) z[i] = rz[i];
 #pragma unroll
       for (int e = 0; e < E; e++) {
         float away;
@@ -406,11 +409,12 @@ __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurPa
       for (int e = 0; e < E; e++) {
         h[e] = fmaf(a[i][e], h[e], u[i][e]);
         y[e] = h[e];
-        if (Gated) y[e] *= z[i][e] * sigmoid<kFine<T>>(z[i][e]);
+        if (Gated) y[e] *= rz[i][e] * sigmoid<kFine<T>>(rz[i][e]);
       }
       if (at.here && (whole || s + i < at.len)) put<T, E, Passing>(out.at(i), y);
     }
     if (!whole) put_zeros<T, E>(p, at, p.out, s, N);
+    if (s0 + kTile < end) load_gates(s0 + kTile);
   }
   if (at.here && at.segment == p.segments - 1 && threadIdx.x < kRowLanes)
 #pragma unroll
@@ -430,21 +434,33 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
   const int last = begin + (end - begin - 1) / kTile * kTile;
   Raw<T, E> rv[N], rf[N], rg[N], ro[N];
   float kept[E];
+  // (as forward: what is used up first is fetched first)
   const auto load = [&](int s0) {
     const auto v = Rows<T>::template of<kTile>(p, at, s0, p.v, p.vs[0], p.vs[1], run * N);
     const auto f = Rows<T>::template of<kTile>(p, at, s0, p.f, p.fs[0], p.fs[1], run * N);
-    const auto g = Rows<T>::template of<kTile>(p, at, s0, p.g, p.gs[0], p.gs[1], run * N);
-    const auto o = Rows<T>::template of<kTile>(p, at, s0, p.go, (int64_t)p.L * p.C, p.C, run * N);
     const int s = s0 + run * N;
-    const bool whole = s0 + kTile <= at.len;
 #pragma unroll
     for (int e = 0; e < E; e++)
       kept[e] = p.states[((int64_t)at.b * p.spans + s0 / kSpan) * p.C + at.c + e];
-    if (whole) {
+    if (s0 + kTile <= at.len) {
+#pragma unroll
+      for (int i = 0; i < N; i++) rv[i].load(v.at(i)), rf[i].load(f.at(i));
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      // a step that leaves the state and its gradient as they are
+      rv[i].fill(0.f), rf[i].fill(__builtin_inff());
+      if (s + i < at.len) rv[i].load(v.at(i)), rf[i].load(f.at(i));
+    }
+  };
+  const auto load_gradients = [&](int s0) {
+    const auto g = Rows<T>::template of<kTile>(p, at, s0, p.g, p.gs[0], p.gs[1], run * N);
+    const auto o = Rows<T>::template of<kTile>(p, at, s0, p.go, (int64_t)p.L * p.C, p.C, run * N);
+    const int s = s0 + run * N;
+    if (s0 + kTile <= at.len) {
 #pragma unroll
       for (int i = 0; i < N; i++) {
-        rv[i].load(v.at(i));
-        rf[i].load(f.at(i));
         if (Gated) rg[i].load(g.at(i));
         ro[i].load(o.at(i));
       }
@@ -452,18 +468,16 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
     }
 #pragma unroll
     for (int i = 0; i < N; i++) {
+      ro[i].fill(0.f);
+      if (Gated) rg[i].fill(0.f);
       if (s + i < at.len) {
-        rv[i].load(v.at(i));
-        rf[i].load(f.at(i));
         if (Gated) rg[i].load(g.at(i));
         ro[i].load(o.at(i));
-      } else {  // a step that leaves the state and its gradient as they are
-        rv[i].fill(0.f), rf[i].fill(__builtin_inff()), ro[i].fill(0.f);
-        if (Gated) rg[i].fill(0.f);
       }
     }
   };
   load(last);
+  load_gradients(last);
   float carry[E];
 #pragma unroll
   for (int e = 0; e < E; e++) carry[e] = p.gfinal ? p.gfinal[(int64_t)at.b * p.C + at.c + e] : 0.f;
@@ -517,7 +531,10 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
       }
       if (Gated && p.gg && at.here && (whole || s + i < at.len)) put<T, E, Passing>(gg.at(i), y);
     }
+    // (all at once in bf16; in single precision, whose words take twice the registers, the gradients later: 43 ->
+    // 39 us of 3 sequences of up to 31250 steps of 90 channels)
     if (s0 > begin) load(s0 - kTile);
+    if (!kFine<T> && s0 > begin) load_gradients(s0 - kTile);
 #pragma unroll
     for (int e = 0; e < E; e++) A[e] = 1.f, H[e] = 0.f;
 #pragma unroll
@@ -560,6 +577,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
       if (p.gf) put_zeros<T, E>(p, at, p.gf, s, N);
       if (Gated && p.gg) put_zeros<T, E>(p, at, p.gg, s, N);
     }
+    if (kFine<T> && s0 > begin) load_gradients(s0 - kTile);
   }
   if (p.ginitial && at.here && at.segment == 0 && threadIdx.x < kRowLanes)
 #pragma unroll
