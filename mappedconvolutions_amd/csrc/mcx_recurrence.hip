@@ -33,8 +33,9 @@ constexpr int kSpan = kRuns * 4;             // steps from one kept state to the
 constexpr int kFew = 8;                 // steps that a thread walks alone
 // Workgroups aimed at by segments: as many as are resident at a time (forward, float32 backward, bf16 back-
 // ward; 768 there: 2 sequences of 32768 steps of 1024 channels 440 -> 542 us), and by the parts of the first
-// launch; workgroups from which on there are no segments.
-constexpr int kGroups = 768, kGroupsBf16Backward = 512, kSums = 8192, kAlone = 512;
+// launch; workgroups from which on there are no segments (16 sequences of 4096 steps of 1024 bf16 channels, 256 of
+// them, 388 us with and 403 without; 24 of 3000, 384 of them, 470 and 430).
+constexpr int kGroups = 768, kGroupsBf16Backward = 512, kSums = 8192, kAlone = 257;
 constexpr int kWideRow = 40;           // words of a row from which on the first launch reads rows of 64 lanes
 // Tensors whose results would push out of the last-level cache what is read a second time (2 sequences of
 // 32768 steps of 1024 channels 473 -> 440 us); only whole lines are written past it (rows of 360 bytes: 50 -> 66).
