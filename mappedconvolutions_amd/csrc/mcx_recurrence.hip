@@ -30,7 +30,9 @@ constexpr int kRuns = kThreads / kRowLanes;  // runs of steps of a tile
 // that all fits the registers.
 constexpr int run_steps(int word, int size) { return word == 4 || size == 4 ? 4 : 8; }
 constexpr int kSpan = kRuns * 4;             // steps from one kept state to the next, a part of every tile
-constexpr int kFew = 8;                 // steps that a thread walks alone
+// Steps that a thread walks alone, forward (8192 sequences of 16 steps of 256 bf16 channels 54 us, in a tile 74; 512 of
+// 32 steps 20 and 13).
+constexpr int kFew = 16;
 // Workgroups aimed at by segments: as many as are resident at a time (forward, float32 backward, bf16 back-
 // ward; 768 there: 2 sequences of 32768 steps of 1024 channels 440 -> 542 us), and by the parts of the first
 // launch; workgroups from which on there are no segments (16 sequences of 4096 steps of 1024 bf16 channels, 256 of
@@ -307,9 +309,9 @@ __global__ __launch_bounds__(kThreads) void recurrence_parts_kernel(RecurParams 
   }
 }
 
-template <typename T, int E, bool Gated, bool Passing>
+template <typename T, int E, int N, bool Gated, bool Passing>
 __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurParams p) {
-  constexpr int N = run_steps(E, sizeof(T)), kTile = kRuns * N;
+  constexpr int kTile = kRuns * N;
   __shared__ Exchange<E> both[2];
   __shared__ Ranges<E> ranges;
   const int lane = threadIdx.x & (kRowLanes - 1), run = threadIdx.x / kRowLanes;
@@ -422,9 +424,9 @@ __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurPa
     for (int e = 0; e < E; e++) p.final[(int64_t)at.b * p.C + at.c + e] = carry[e];
 }
 
-template <typename T, int E, bool Gated, bool Passing>
+template <typename T, int E, int N, bool Gated, bool Passing>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurParams p) {
-  constexpr int N = run_steps(E, sizeof(T)), kTile = kRuns * N;
+  constexpr int kTile = kRuns * N;
   __shared__ Exchange<E> ahead[2], back[2];
   __shared__ Ranges<E> ranges;
   const int lane = threadIdx.x & (kRowLanes - 1), run = threadIdx.x / kRowLanes;
@@ -721,11 +723,27 @@ template <typename T, int E> bool passing(const RecurParams &p, int64_t B) {
   return p.C * (int)sizeof(T) % kLine == 0 && B * p.L * p.C * (int64_t)sizeof(T) >= kPassingBytes;
 }
 
-template <typename T, int E, bool Gated>
-int forward(const RecurParams &p, int64_t B, hipStream_t s) {
-  const unsigned groups = (unsigned)(B * p.tiles);
-  const dim3 threads(kThreads);
-  if (p.L <= kFew) {
+// Few steps take a tile of as few (8192 sequences of 16 steps of 256 bf16 channels forward and backward 451 -> 208 us,
+// of 32 steps 651 -> 451).
+template <typename T, int E, int N, bool Gated, bool Backward>
+int launch_tiles(const RecurParams &p, int64_t B, hipStream_t s) {
+  constexpr bool kWord = E * sizeof(T) == 8;
+  const bool past = passing<T, E>(p, B);
+  const dim3 groups((unsigned)(B * p.tiles * p.segments));
+  if constexpr (Backward)
+    hipLaunchKernelGGL((past ? recurrence_backward_kernel<T, E, N, Gated, kWord>
+                             : recurrence_backward_kernel<T, E, N, Gated, false>),
+                       groups, dim3(kThreads), 0, s, p);
+  else
+    hipLaunchKernelGGL((past ? recurrence_forward_kernel<T, E, N, Gated, kWord>
+                             : recurrence_forward_kernel<T, E, N, Gated, false>),
+                       groups, dim3(kThreads), 0, s, p);
+  MCX_HIP_CHECK_LAUNCH();
+  return MCX_OK;
+}
+template <typename T, int E, bool Gated, bool Backward>
+int launch_steps(const RecurParams &p, int64_t B, hipStream_t s) {
+  if (!Backward && p.L <= kFew) {
     const int64_t words = B * (p.C / E);
     hipLaunchKernelGGL((recurrence_few_kernel<T, E, Gated>), dim3((unsigned)((words + 255) / 256)), dim3(256),
                        0, s, p, words);
@@ -733,30 +751,16 @@ int forward(const RecurParams &p, int64_t B, hipStream_t s) {
     return MCX_OK;
   }
   if (p.segments > 1)
-    if (int e = sum_parts<T, E, false, false>(p, B, s)) return e;
-  hipLaunchKernelGGL((passing<T, E>(p, B) ? recurrence_forward_kernel<T, E, Gated, E * sizeof(T) == 8>
-                                          : recurrence_forward_kernel<T, E, Gated, false>),
-                     dim3(groups * p.segments), threads, 0, s, p);
-  MCX_HIP_CHECK_LAUNCH();
-  return MCX_OK;
-}
-template <typename T, int E, bool Gated>
-int backward(const RecurParams &p, int64_t B, hipStream_t s) {
-  const unsigned groups = (unsigned)(B * p.tiles);
-  const dim3 threads(kThreads);
-  if (p.segments > 1)
-    if (int e = sum_parts<T, E, Gated, true>(p, B, s)) return e;
-  hipLaunchKernelGGL((passing<T, E>(p, B) ? recurrence_backward_kernel<T, E, Gated, E * sizeof(T) == 8>
-                                          : recurrence_backward_kernel<T, E, Gated, false>),
-                     dim3(groups * p.segments), threads, 0, s, p);
-  MCX_HIP_CHECK_LAUNCH();
-  return MCX_OK;
+    if (int e = sum_parts<T, E, Backward && Gated, Backward>(p, B, s)) return e;
+  if constexpr (Backward)
+    if (p.L <= kRuns) return launch_tiles<T, E, 1, Gated, true>(p, B, s);
+  if (p.L <= 2 * kRuns) return launch_tiles<T, E, 2, Gated, Backward>(p, B, s);
+  return launch_tiles<T, E, run_steps(E, sizeof(T)), Gated, Backward>(p, B, s);
 }
 template <typename T, bool Forward>
 int launch(const RecurParams &p, int64_t B, int word, hipStream_t s) {
-#define MCX_RECUR(E)                                                                                 \
-  (Forward ? (p.g ? forward<T, E, true>(p, B, s) : forward<T, E, false>(p, B, s))                    \
-           : (p.g ? backward<T, E, true>(p, B, s) : backward<T, E, false>(p, B, s)))
+#define MCX_RECUR(E) \
+  (p.g ? launch_steps<T, E, true, !Forward>(p, B, s) : launch_steps<T, E, false, !Forward>(p, B, s))
   if constexpr (sizeof(T) == 2)
     if (word == 4) return MCX_RECUR(4);
   return word == 2 ? MCX_RECUR(2) : MCX_RECUR(1);

@@ -130,6 +130,17 @@ def test_sizes(device, size, dtype):
         check(v, f, None, go, None, None, reverse=reverse)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("L", [15, 16, 17, 31, 32, 33])
+def test_tiles_of_few_steps(device, L, dtype):
+    for C in (5, 36, 66, 72):
+        for reverse in (False, True):
+            v, f, z, go, first, last = make(12, 3, L, C, dtype)
+            check(v, f, z, go, first, last, reverse=reverse)
+            check(v, f, z, go, first, last, [L, 0, L - 9], reverse)
+            check(v, f, None, go, None, None, [3, L - 1, 1], reverse)
+
+
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_lengths(device, dtype, reverse):
