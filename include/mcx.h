@@ -498,7 +498,7 @@ int mcx_clip_grad_norm(const void *const *in, void *const *out, const int64_t *s
  * No counterpart in the reference.  F32 and BF16; states are float and so is every sum.  Strides (of
  * sequence and step, in values) of value, forget and gate [B, L, C], the last axis dense; any alignment
  * goes, rows of whole 8-byte words are read in those.  The stride of a step is at most 2^22,
- * C <= 2^22, B * ceil(C / 16) <= 2^21. */
+ * C <= 2^22, B * ceil(C / 16) < 2^23. */
 typedef struct mcx_recurrence_desc {
   int64_t B, L, C;
   int64_t v_stride[2], f_stride[2], g_stride[2];

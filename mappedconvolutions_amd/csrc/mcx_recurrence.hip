@@ -634,7 +634,7 @@ int check_desc(const mcx_recurrence_desc *d, int dtype) {
   if (!d) return MCX_E_NULL;
   if (dtype != MCX_F32 && dtype != MCX_BF16) return MCX_E_DTYPE;
   if (d->B < 0 || d->L < 0 || d->C < 1 || d->L > 0x3fffffff || d->C > (1 << 22) || d->B > (1 << 24) ||
-      d->B * ((d->C + 15) / 16) > (1 << 21))
+      d->B * ((d->C + 15) / 16) >= (1 << 23))  // workgroups of 256 threads, their threads in 32 bits
     return MCX_E_SHAPE;
   // (a tile's addresses are 32 bits from its first)
   for (int64_t stride : {d->v_stride[1], d->f_stride[1], d->g_stride[1]})

@@ -306,6 +306,15 @@ def test_results_past_the_cache(device, dtype):
             assert torch.equal(a, b[half])
 
 
+def test_many_short_sequences(device):
+    B = 1 << 21  # of 48 channels: 3 tiles each
+    v, f, z, go, first, last = make(13, 64, 2, 48, BF16)
+    few = call(*(t.cuda() for t in (v, f, z, go, first, last)), None, False)
+    many = [t.cuda().repeat(B // 64, *[1] * (t.dim() - 1)) for t in (v, f, z, go, first, last)]
+    for a, b in zip(call(*many, None, False), few):
+        assert torch.equal(a.view(B // 64, *b.shape), b.expand(B // 64, *b.shape))
+
+
 def test_steps_far_apart(device):
     # further than the kernels' addresses reach from a tile's first: copied
     v, f, z, go, first, last = make(11, 2, 70, 16, BF16)
