@@ -58,10 +58,11 @@ class AdamW(torch.optim.Optimizer):
                     dense[p.grad] = p.grad.contiguous()
         if not dense:
             return loss
-        if torch.cuda.is_current_stream_capturing():
+        capturing = torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+        if capturing:
             if not self.capturable:
                 raise RuntimeError('Only a capturable AdamW counts the steps of a captured one')
-            if any(p.grad is not None and not self.state[p] for group in self.param_groups
+            if any(p.grad is not None and not self.state.get(p) for group in self.param_groups
                    for p in group['params']):
                 raise RuntimeError('The first step of a parameter makes its moments and is not captured')
         norm = None
@@ -77,36 +78,49 @@ class AdamW(torch.optim.Optimizer):
                     made.append(torch.zeros((), dtype=torch.int64, device=group['params'][0].device))
                 return made[0]
 
-            alike = {}
+            alike, absent = {}, {}
             for p in group['params']:
                 if p.grad is None:
+                    if self.capturable and self.state.get(p):
+                        absent.setdefault(id(self.state[p]['step']), []).append(self.state[p])
                     continue
                 state = self._state_of(p, group['bits'], counter)
                 step = state['step']
                 key = id(step) if isinstance(step, torch.Tensor) else step
                 alike.setdefault(key, (step, []))[1].append((p, state))
-            for step, members in alike.values():
+            for key, (step, members) in alike.items():
+                if key in absent:  # whose counter stays behind
+                    if capturing:
+                        raise RuntimeError('Parameters without gradients share a counter with others: take '
+                                           'a step without them before the captured one')
+                    behind = step.clone()
+                    for state in absent[key]:
+                        state['step'] = behind
                 self._update(group, step, members, dense, norm, call)
                 call += 1
         return loss
 
     def _update(self, group, step, members, dense, norm, call):
-        if isinstance(step, torch.Tensor):
-            step += 1
-        else:
-            step += 1
-            for _, state in members:
-                state['step'] = step
+        counted = isinstance(step, torch.Tensor)
+        step = step.add_(1) if counted else step + 1
         params = [p if p.is_contiguous() else p.contiguous() for p, _ in members]
         scales = {}
         if group['bits'] == 8:
             scales = dict(first_scales=[s['first_scale'] for _, s in members],
                           second_scales=[s['second_scale'] for _, s in members],
                           seed=self.seed + 0x9E3779B1 * call)
-        _C.adamw_step(params, [dense[p.grad] for p, _ in members], [s['first'] for _, s in members],
-                      [s['second'] for _, s in members], step, group['lr'], group['betas'],
-                      group['eps'], group['weight_decay'], grad_norm=norm,
-                      max_norm=None if norm is None else self.max_norm, **scales)
+        try:
+            _C.adamw_step(params, [dense[p.grad] for p, _ in members], [s['first'] for _, s in members],
+                          [s['second'] for _, s in members], step, group['lr'], group['betas'],
+                          group['eps'], group['weight_decay'], grad_norm=norm,
+                          max_norm=None if norm is None else self.max_norm, **scales)
+        except RuntimeError:  # a step that is refused is none
+            if counted:
+                step.sub_(1)
+            raise
+        if not counted:
+            for _, state in members:
+                state['step'] = step
         for changed, (p, _) in zip(params, members):
             if changed is not p:
                 p.copy_(changed)
@@ -119,7 +133,7 @@ class AdamW(torch.optim.Optimizer):
             counters = {}
             for p in group['params']:
                 saved = state_dict['state'].get(ids.pop(0))
-                if saved is None:
+                if not saved:
                     continue
                 state = {name: value.to(p.device, copy=True) for name, value in saved.items()
                          if name != 'step'}

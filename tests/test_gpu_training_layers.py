@@ -337,6 +337,34 @@ def test_steps_that_a_graph_would_not_replay_are_refused(device):
         assert refused
 
 
+def test_parameters_without_gradients_keep_their_count(device):
+    """Counters on the GPU are shared: what has no gradient for some steps is counted as on the host."""
+    ours, other = parameters(), parameters()
+    counted, host = util.AdamW(ours, lr=0.1, capturable=True), util.AdamW(other, lr=0.1)
+    for k, skip in enumerate(((), (1, 3), (), (3,), (0, 1, 2, 4), ())):
+        give_gradients(ours, k, skip)
+        give_gradients(other, k, skip)
+        counted.step()
+        host.step()
+        for p, q in zip(ours, other):
+            assert torch.equal(p, q) and int(counted.state[p]["step"]) == host.state[q]["step"]
+    assert [host.state[q]["step"] for q in other] == [5, 4, 5, 4, 5]
+    # a graph would count those that come back later
+    one, two = (torch.nn.Parameter(torch.ones(10, device=device)) for _ in range(2))
+    one.grad, two.grad = torch.ones(10, device=device), torch.ones(10, device=device)
+    optimizer = util.AdamW([one, two], capturable=True)
+    optimizer.step()
+    two.grad = None
+    refused = False
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        try:
+            optimizer.step()
+        except RuntimeError as error:
+            refused = "share a counter" in str(error)
+        one.grad.add_(0)
+    assert refused
+
+
 # ---- the example --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("bits", [32, 8])

@@ -186,3 +186,23 @@ def test_optimizer_arguments():
     assert optimizer.step() is None  # no gradients yet
     assert optimizer.step(lambda: 7) == 7
     assert not optimizer.state and optimizer.param_groups[0]["bits"] == 8
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_is_not_counted(capturable, monkeypatch):
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    opt = util.AdamW([p], capturable=capturable)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="one GPU"):
+            opt.step()
+        assert int(opt.state[p]["step"]) == 0
+    # a first step that would be captured leaves nothing behind
+    opt = util.AdamW([p], capturable=capturable)
+    for name in ("is_initialized", "is_current_stream_capturing"):
+        monkeypatch.setattr(torch.cuda, name, lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()
+    monkeypatch.undo()
+    assert opt.state_dict()["state"] == {}
+    assert util.AdamW([p]).load_state_dict(opt.state_dict()) is None
