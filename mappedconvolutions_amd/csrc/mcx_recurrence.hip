@@ -25,11 +25,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kRowLanes = 16;           // lanes of a step's channels
-constexpr int kRuns = kThreads / kRowLanes;  // runs of steps of a tile
+constexpr int kNarrowLanes = 4;         // the same where channels are few
+// Runs of steps of a tile
+template <int Lanes> constexpr int kRuns = kThreads / Lanes;
 // Steps of a run: 16 values a lane, 8 in single precision (whose words hold 2) and where no words can be read, so
 // that all fits the registers.
 constexpr int run_steps(int word, int size) { return word == 4 || size == 4 ? 4 : 8; }
-constexpr int kSpan = kRuns * 4;             // steps from one kept state to the next, a part of every tile
+constexpr int kSpan = kRuns<kRowLanes> * 4;  // steps from one kept state to the next, a part of every tile
 // Steps that a thread walks alone, forward (8192 sequences of 16 steps of 256 bf16 channels 54 us, in a tile 74; 512 of
 // 32 steps 20 and 13).
 constexpr int kFew = 16;
@@ -56,6 +58,7 @@ struct RecurParams {
   int segments, segment;             // steps of a segment
   int parts, each, share;            // parts of all steps, their steps, parts of a segment
   int spans, reverse;
+  int lanes;                         // of a row
   int together;                      // neighbours go to the same XCD
 };
 
@@ -117,7 +120,7 @@ struct Place {
   bool here;
 };
 // (what all lanes have in common in scalar registers: the addresses are these, and 32 bits a lane)
-template <int E, int RowLanes = kRowLanes>
+template <int E, int RowLanes>
 __device__ inline Place place_of(const RecurParams &p, int index, int segments) {
   Place a;
   if (p.together) index = xcd_contiguous_tile(index, gridDim.x);
@@ -139,19 +142,19 @@ __device__ inline int64_t token_of(const RecurParams &p, const Place &a, int s) 
 // first step and the way to the next step.
 template <typename T> struct Rows {
   const char *base;
-  int first, step;
+  unsigned first, step;
   template <int Tile>
   static __device__ inline Rows of(const RecurParams &p, const Place &a, int s0, const void *x,
                                    int64_t sequence, int64_t stride, int j) {
     const int64_t t0 = p.reverse ? (int64_t)a.len - Tile - s0 : s0;
-    const int bytes = (int)stride * (int)sizeof(T);
+    const unsigned bytes = (unsigned)stride * (unsigned)sizeof(T);
     Rows r;
     r.base = (const char *)x + (a.b * sequence + t0 * stride) * (int64_t)sizeof(T);
-    r.first = (p.reverse ? Tile - 1 - j : j) * bytes + a.c * (int)sizeof(T);
-    r.step = p.reverse ? -bytes : bytes;
+    r.first = (unsigned)(p.reverse ? Tile - 1 - j : j) * bytes + (unsigned)a.c * (unsigned)sizeof(T);
+    r.step = p.reverse ? 0u - bytes : bytes;
     return r;
   }
-  __device__ inline T *at(int i) const { return (T *)(base + (unsigned)(first + i * step)); }
+  __device__ inline T *at(int i) const { return (T *)(base + (first + (unsigned)i * step)); }
 };
 
 // Zeros at those of steps s to s + n that are not in use.
@@ -166,43 +169,44 @@ __device__ inline void put_zeros(const RecurParams &p, const Place &a, void *x, 
 
 // (A, H) of the runs before (Up) or behind a lane's in its wave, and of the whole wave in its
 // last (first) row.
-template <int E, bool Up>
+template <int E, int RowLanes, bool Up>
 __device__ inline void wave_scan(int row, float *A, float *H, float *before_a, float *before_h) {
 #pragma unroll
-  for (int d = 1; d < 64 / kRowLanes; d *= 2) {
-    const bool take = Up ? row >= d : row + d < 64 / kRowLanes;
+  for (int d = 1; d < 64 / RowLanes; d *= 2) {
+    const bool take = Up ? row >= d : row + d < 64 / RowLanes;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const float pa = Up ? __shfl_up(A[e], d * kRowLanes) : __shfl_down(A[e], d * kRowLanes);
-      const float ph = Up ? __shfl_up(H[e], d * kRowLanes) : __shfl_down(H[e], d * kRowLanes);
+      const float pa = Up ? __shfl_up(A[e], d * RowLanes) : __shfl_down(A[e], d * RowLanes);
+      const float ph = Up ? __shfl_up(H[e], d * RowLanes) : __shfl_down(H[e], d * RowLanes);
       H[e] = take ? fmaf(A[e], ph, H[e]) : H[e];
       A[e] = take ? A[e] * pa : A[e];
     }
   }
-  const bool first = Up ? row == 0 : row == 64 / kRowLanes - 1;
+  const bool first = Up ? row == 0 : row == 64 / RowLanes - 1;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    const float pa = Up ? __shfl_up(A[e], kRowLanes) : __shfl_down(A[e], kRowLanes);
-    const float ph = Up ? __shfl_up(H[e], kRowLanes) : __shfl_down(H[e], kRowLanes);
+    const float pa = Up ? __shfl_up(A[e], RowLanes) : __shfl_down(A[e], RowLanes);
+    const float ph = Up ? __shfl_up(H[e], RowLanes) : __shfl_down(H[e], RowLanes);
     before_a[e] = first ? 1.f : pa, before_h[e] = first ? 0.f : ph;
   }
 }
 
 // Whole waves' (A, H) of a tile.
-template <int E> struct Exchange {
-  float a[kWaves][kRowLanes][E], h[kWaves][kRowLanes][E];
+template <int E, int RowLanes> struct Exchange {
+  float a[kWaves][RowLanes][E], h[kWaves][RowLanes][E];
 };
 
 // The state that a segment begins with: (A, H) of the parts before it (Backward: behind it) over `carry`.  A row of
 // lanes goes over some of them, then all over the rows.
-template <int E> struct Ranges {
-  float a[kRuns][kRowLanes][E], h[kRuns][kRowLanes][E];
+template <int E, int RowLanes> struct Ranges {
+  float a[kRuns<RowLanes>][RowLanes][E], h[kRuns<RowLanes>][RowLanes][E];
 };
-template <int E, bool Backward>
-__device__ inline void carry_in(const RecurParams &p, const Place &at, Ranges<E> &x, float *carry) {
-  const int lane = threadIdx.x & (kRowLanes - 1), row = threadIdx.x / kRowLanes;
+template <int E, int RowLanes, bool Backward>
+__device__ inline void carry_in(const RecurParams &p, const Place &at, Ranges<E, RowLanes> &x, float *carry) {
+  const int lane = threadIdx.x & (RowLanes - 1), row = threadIdx.x / RowLanes;
   const int n = Backward ? max(0, p.parts - (at.segment + 1) * p.share) : at.segment * p.share;
-  const int each = (n + kRuns - 1) / kRuns;
+  constexpr int kRows = kRuns<RowLanes>;
+  const int each = (n + kRows - 1) / kRows;
   const float *part = p.part + (int64_t)at.b * (p.parts + 1) * 2 * p.C + at.c;
   float A[E], H[E];
 #pragma unroll
@@ -221,7 +225,7 @@ __device__ inline void carry_in(const RecurParams &p, const Place &at, Ranges<E>
   for (int e = 0; e < E; e++) x.a[row][lane][e] = A[e], x.h[row][lane][e] = H[e];
   __syncthreads();
 #pragma unroll 4
-  for (int k = 0; k < kRuns; k++)
+  for (int k = 0; k < kRows; k++)
 #pragma unroll
     for (int e = 0; e < E; e++) carry[e] = fmaf(x.a[k][lane][e], carry[e], x.h[k][lane][e]);
 }
@@ -281,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void recurrence_parts_kernel(RecurParams 
   for (; i < hi - lo; i++) steps(std::integral_constant<int, 1>(), i);
   if constexpr (RowLanes < 64) {
     float before_a[E], before_h[E];
-    wave_scan<E, !Backward>(row, A, H, before_a, before_h);
+    wave_scan<E, RowLanes, !Backward>(row, A, H, before_a, before_h);
   }
   if (row == (Backward ? 0 : 64 / RowLanes - 1))
 #pragma unroll
@@ -309,15 +313,15 @@ __global__ __launch_bounds__(kThreads) void recurrence_parts_kernel(RecurParams 
   }
 }
 
-template <typename T, int E, int N, bool Gated, bool Passing>
+template <typename T, int E, int N, int RowLanes, bool Gated, bool Passing>
 __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurParams p) {
-  constexpr int kTile = kRuns * N;
-  __shared__ Exchange<E> both[2];
-  __shared__ Ranges<E> ranges;
-  const int lane = threadIdx.x & (kRowLanes - 1), run = threadIdx.x / kRowLanes;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = (threadIdx.x & 63) / kRowLanes;
+  constexpr int kTile = kRuns<RowLanes> * N;
+  __shared__ Exchange<E, RowLanes> both[2];
+  __shared__ Ranges<E, RowLanes> ranges;
+  const int lane = threadIdx.x & (RowLanes - 1), run = threadIdx.x / RowLanes;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = (threadIdx.x & 63) / RowLanes;
   // (from the end, which the first launch read last)
-  const Place at = place_of<E>(p, gridDim.x - 1 - blockIdx.x, p.segments);
+  const Place at = place_of<E, RowLanes>(p, gridDim.x - 1 - blockIdx.x, p.segments);
   const int begin = at.segment * p.segment, end = min(p.L, begin + p.segment);
   Raw<T, E> rv[N], rf[N], rz[N];
   // the tile's values, the next one's while this one is worked on; gates when the tile's are used up
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurPa
 #pragma unroll
     for (int e = 0; e < E; e++)
       carry[e] = p.part[((int64_t)at.b * (p.parts + 1) + p.parts) * 2 * p.C + at.c + e];
-    carry_in<E, false>(p, at, ranges, carry);
+    carry_in<E, RowLanes, false>(p, at, ranges, carry);
   } else if (p.initial) {
 #pragma unroll
     for (int e = 0; e < E; e++) carry[e] = p.initial[(int64_t)at.b * p.C + at.c + e];
@@ -383,9 +387,9 @@ __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurPa
         A[e] *= a[i][e], H[e] = fmaf(a[i][e], H[e], u[i][e]);
       }
     }
-    wave_scan<E, true>(row, A, H, before_a, before_h);
-    Exchange<E> &x = both[turn];
-    if (row == 64 / kRowLanes - 1)
+    wave_scan<E, RowLanes, true>(row, A, H, before_a, before_h);
+    Exchange<E, RowLanes> &x = both[turn];
+    if (row == 64 / RowLanes - 1)
 #pragma unroll
       for (int e = 0; e < E; e++) x.a[wave][lane][e] = A[e], x.h[wave][lane][e] = H[e];
     __syncthreads();
@@ -419,20 +423,20 @@ __global__ __launch_bounds__(kThreads, 3) void recurrence_forward_kernel(RecurPa
     if (!whole) put_zeros<T, E>(p, at, p.out, s, N);
     if (s0 + kTile < end) load_gates(s0 + kTile);
   }
-  if (at.here && at.segment == p.segments - 1 && threadIdx.x < kRowLanes)
+  if (at.here && at.segment == p.segments - 1 && threadIdx.x < RowLanes)
 #pragma unroll
     for (int e = 0; e < E; e++) p.final[(int64_t)at.b * p.C + at.c + e] = carry[e];
 }
 
-template <typename T, int E, int N, bool Gated, bool Passing>
+template <typename T, int E, int N, int RowLanes, bool Gated, bool Passing>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurParams p) {
-  constexpr int kTile = kRuns * N;
-  __shared__ Exchange<E> ahead[2], back[2];
-  __shared__ Ranges<E> ranges;
-  const int lane = threadIdx.x & (kRowLanes - 1), run = threadIdx.x / kRowLanes;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = (threadIdx.x & 63) / kRowLanes;
+  constexpr int kTile = kRuns<RowLanes> * N;
+  __shared__ Exchange<E, RowLanes> ahead[2], back[2];
+  __shared__ Ranges<E, RowLanes> ranges;
+  const int lane = threadIdx.x & (RowLanes - 1), run = threadIdx.x / RowLanes;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = (threadIdx.x & 63) / RowLanes;
   // (from the beginning, which the first launch read last)
-  const Place at = place_of<E>(p, blockIdx.x, p.segments);
+  const Place at = place_of<E, RowLanes>(p, blockIdx.x, p.segments);
   const int begin = at.segment * p.segment, end = min(p.L, begin + p.segment);
   const int last = begin + (end - begin - 1) / kTile * kTile;
   Raw<T, E> rv[N], rf[N], rg[N], ro[N];
@@ -484,7 +488,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
   float carry[E];
 #pragma unroll
   for (int e = 0; e < E; e++) carry[e] = p.gfinal ? p.gfinal[(int64_t)at.b * p.C + at.c + e] : 0.f;
-  if (p.segments > 1) carry_in<E, true>(p, at, ranges, carry);
+  if (p.segments > 1) carry_in<E, RowLanes, true>(p, at, ranges, carry);
   int turn = 0;
   for (int s0 = last; s0 >= begin; s0 -= kTile, turn ^= 1) {
     const int s = s0 + run * N;
@@ -499,9 +503,9 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
         a[i][e] = logistic<kFine<T>>(rf[i][e], away[i][e]);
         A[e] *= a[i][e], H[e] = fmaf(a[i][e], H[e], away[i][e] * rv[i][e]);
       }
-    wave_scan<E, true>(row, A, H, before_a, before_h);
-    Exchange<E> &x = ahead[turn];
-    if (row == 64 / kRowLanes - 1)
+    wave_scan<E, RowLanes, true>(row, A, H, before_a, before_h);
+    Exchange<E, RowLanes> &x = ahead[turn];
+    if (row == 64 / RowLanes - 1)
 #pragma unroll
       for (int e = 0; e < E; e++) x.a[wave][lane][e] = A[e], x.h[wave][lane][e] = H[e];
     __syncthreads();
@@ -544,8 +548,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
     for (int i = N - 1; i >= 0; i--)
 #pragma unroll
       for (int e = 0; e < E; e++) H[e] = a[i][e] * (d[i][e] + H[e]), A[e] *= a[i][e];
-    wave_scan<E, false>(row, A, H, before_a, before_h);
-    Exchange<E> &y = back[turn];
+    wave_scan<E, RowLanes, false>(row, A, H, before_a, before_h);
+    Exchange<E, RowLanes> &y = back[turn];
     if (row == 0)
 #pragma unroll
       for (int e = 0; e < E; e++) y.a[wave][lane][e] = A[e], y.h[wave][lane][e] = H[e];
@@ -582,7 +586,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
     }
     if (kFine<T> && s0 > begin) load_gradients(s0 - kTile);
   }
-  if (p.ginitial && at.here && at.segment == 0 && threadIdx.x < kRowLanes)
+  if (p.ginitial && at.here && at.segment == 0 && threadIdx.x < RowLanes)
 #pragma unroll
     for (int e = 0; e < E; e++) p.ginitial[(int64_t)at.b * p.C + at.c + e] = carry[e];
 }
@@ -636,7 +640,8 @@ int check_desc(const mcx_recurrence_desc *d, int dtype) {
   if (d->B < 0 || d->L < 0 || d->C < 1 || d->L > 0x3fffffff || d->C > (1 << 22) || d->B > (1 << 24) ||
       d->B * ((d->C + 15) / 16) >= (1 << 23))  // workgroups of 256 threads, their threads in 32 bits
     return MCX_E_SHAPE;
-  // (a tile's addresses are 32 bits from its first)
+  // (a tile's addresses are 32 bits from its first: 512 steps of 2 bytes or 256 of 4 where channels are few, 128
+  // and 64 of up to 2^22 channels)
   for (int64_t stride : {d->v_stride[1], d->f_stride[1], d->g_stride[1]})
     if (d->L > 1 && (stride < 0 || stride > (1 << 22))) return MCX_E_SHAPE;
   return MCX_OK;
@@ -662,15 +667,26 @@ int word_of(const mcx_recurrence_desc *d, int size, uint64_t bits) {
 int split_lines(const mcx_recurrence_desc *d, int size, uint64_t bits) {
   return bits % kLine != 0 || d->C * size % kLine != 0;
 }
+// Two tiles of kNarrowLanes channels' words at most, where that makes fewer tiles of channels and steps than
+// kRowLanes (250 sequences of 6000 steps of 8 bf16 channels, forward and gradients, 413 -> 159 us; three tiles:
+// 1091 of 1000 steps of 11 float32 channels 165 -> 199).
+int lanes_of(const mcx_recurrence_desc *d, int word, int size) {
+  const auto tiles = [&](int lanes) {
+    const int64_t tile = kThreads / lanes * run_steps(word, size);
+    return (d->C + lanes * word - 1) / (lanes * word) * ((d->L + tile - 1) / tile);
+  };
+  return d->C <= 2 * kNarrowLanes * word && tiles(kNarrowLanes) < tiles(kRowLanes) ? kNarrowLanes : kRowLanes;
+}
 // Segments make kGroups workgroups of the second launch, parts of them kSums of the first, which has less to
 // do and so needs more under way; two tiles and one at least.
 struct Cut {
   int segments, segment, parts, each, share;
 };
 Cut cut_of(const mcx_recurrence_desc *d, int word, int size, int groups) {
-  const int64_t columns = std::max<int64_t>(1, d->B * ((d->C + kRowLanes * word - 1) / (kRowLanes * word)));
+  const int lanes = lanes_of(d, word, size);
+  const int64_t columns = std::max<int64_t>(1, d->B * ((d->C + lanes * word - 1) / (lanes * word)));
   int64_t n = columns >= kAlone ? 1 : (groups + columns - 1) / columns;
-  const int64_t tile = kRuns * run_steps(word, size);
+  const int64_t tile = kThreads / lanes * run_steps(word, size);
   n = std::max<int64_t>(1, std::min(n, d->L / (2 * tile)));
   // in tiles
   const int64_t segment = ((d->L + n - 1) / n + tile - 1) / tile;
@@ -695,7 +711,8 @@ RecurParams params_of(const mcx_recurrence_desc *d, int word, int size, int grou
   RecurParams p = {};
   for (int k = 0; k < 2; k++) p.vs[k] = d->v_stride[k], p.fs[k] = d->f_stride[k], p.gs[k] = d->g_stride[k];
   p.L = (int)d->L, p.C = (int)d->C;
-  p.tiles = (int)((d->C + kRowLanes * word - 1) / (kRowLanes * word));
+  p.lanes = lanes_of(d, word, size);
+  p.tiles = (int)((d->C + p.lanes * word - 1) / (p.lanes * word));
   const Cut c = cut_of(d, word, size, groups);
   p.segment = c.segment, p.segments = c.segments, p.parts = c.parts, p.each = c.each, p.share = c.share;
   p.spans = (int)((d->L + kSpan - 1) / kSpan);
@@ -715,8 +732,9 @@ int launch_parts(RecurParams p, int64_t B, hipStream_t s) {
 }
 template <typename T, int E, bool Gated, bool Backward>
 int sum_parts(const RecurParams &p, int64_t B, hipStream_t s) {
+  if (p.lanes == kNarrowLanes) return launch_parts<T, E, kNarrowLanes, Gated, Backward>(p, B, s);
   return p.C / E >= kWideRow ? launch_parts<T, E, 64, Gated, Backward>(p, B, s)
-                       : launch_parts<T, E, kRowLanes, Gated, Backward>(p, B, s);
+                             : launch_parts<T, E, kRowLanes, Gated, Backward>(p, B, s);
 }
 
 template <typename T, int E> bool passing(const RecurParams &p, int64_t B) {
@@ -725,18 +743,18 @@ template <typename T, int E> bool passing(const RecurParams &p, int64_t B) {
 
 // Few steps take a tile of as few (8192 sequences of 16 steps of 256 bf16 channels forward and backward 451 -> 208 us,
 // of 32 steps 651 -> 451).
-template <typename T, int E, int N, bool Gated, bool Backward>
+template <typename T, int E, int N, int RowLanes, bool Gated, bool Backward>
 int launch_tiles(const RecurParams &p, int64_t B, hipStream_t s) {
   constexpr bool kWord = E * sizeof(T) == 8;
   const bool past = passing<T, E>(p, B);
   const dim3 groups((unsigned)(B * p.tiles * p.segments));
   if constexpr (Backward)
-    hipLaunchKernelGGL((past ? recurrence_backward_kernel<T, E, N, Gated, kWord>
-                             : recurrence_backward_kernel<T, E, N, Gated, false>),
+    hipLaunchKernelGGL((past ? recurrence_backward_kernel<T, E, N, RowLanes, Gated, kWord>
+                             : recurrence_backward_kernel<T, E, N, RowLanes, Gated, false>),
                        groups, dim3(kThreads), 0, s, p);
   else
-    hipLaunchKernelGGL((past ? recurrence_forward_kernel<T, E, N, Gated, kWord>
-                             : recurrence_forward_kernel<T, E, N, Gated, false>),
+    hipLaunchKernelGGL((past ? recurrence_forward_kernel<T, E, N, RowLanes, Gated, kWord>
+                             : recurrence_forward_kernel<T, E, N, RowLanes, Gated, false>),
                        groups, dim3(kThreads), 0, s, p);
   MCX_HIP_CHECK_LAUNCH();
   return MCX_OK;
@@ -752,10 +770,12 @@ int launch_steps(const RecurParams &p, int64_t B, hipStream_t s) {
   }
   if (p.segments > 1)
     if (int e = sum_parts<T, E, Backward && Gated, Backward>(p, B, s)) return e;
+  constexpr int kSteps = run_steps(E, sizeof(T));
+  if (p.lanes == kNarrowLanes) return launch_tiles<T, E, kSteps, kNarrowLanes, Gated, Backward>(p, B, s);
   if constexpr (Backward)
-    if (p.L <= kRuns) return launch_tiles<T, E, 1, Gated, true>(p, B, s);
-  if (p.L <= 2 * kRuns) return launch_tiles<T, E, 2, Gated, Backward>(p, B, s);
-  return launch_tiles<T, E, run_steps(E, sizeof(T)), Gated, Backward>(p, B, s);
+    if (p.L <= kRuns<kRowLanes>) return launch_tiles<T, E, 1, kRowLanes, Gated, true>(p, B, s);
+  if (p.L <= 2 * kRuns<kRowLanes>) return launch_tiles<T, E, 2, kRowLanes, Gated, Backward>(p, B, s);
+  return launch_tiles<T, E, kSteps, kRowLanes, Gated, Backward>(p, B, s);
 }
 template <typename T, bool Forward>
 int launch(const RecurParams &p, int64_t B, int word, hipStream_t s) {

@@ -315,6 +315,35 @@ def test_many_short_sequences(device):
         assert torch.equal(a.view(B // 64, *b.shape), b.expand(B // 64, *b.shape))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("C", [1, 2, 3, 6, 8, 10, 13, 24, 32])
+def test_few_channels(device, C, dtype):
+    for L, lengths in ((100, [100, 37, 0]), (257, [257, 1, 256]), (700, [3, 699, 700]), (5000, [5000, 4097, 1025])):
+        v, f, z, go, first, last = make(14, 3, L, C, dtype)
+        for reverse in (False, True):
+            check(v, f, z, go, first, last, lengths, reverse)
+            check(v, f, None, go, None, None, None, reverse)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_channels_far_apart(device, dtype):
+    # as far as the kernels' addresses reach: the last step of a tile lies close to 2^32 bytes from its first
+    L = 600 if dtype == BF16 else 300
+    v, f, z, go, first, last = make(15, 2, L, 5, dtype)
+    wide = torch.zeros(L, 1 << 22, dtype=dtype, device="cuda")
+
+    def apart(*ts):
+        out = []
+        for k, t in enumerate(ts):
+            view = wide[:, 10 * k:10 * k + 10].unflatten(1, (2, 5)).transpose(0, 1)
+            view.copy_(t)
+            out.append(view)
+        return out
+
+    for reverse in (False, True):
+        check(v, f, z, go, first, last, [L, L - 7], reverse, views=apart)
+
+
 def test_steps_far_apart(device):
     # further than the kernels' addresses reach from a tile's first: copied
     v, f, z, go, first, last = make(11, 2, 70, 16, BF16)
