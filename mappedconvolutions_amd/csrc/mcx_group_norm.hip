@@ -785,24 +785,28 @@ Split split_of(int64_t B, int64_t N, int64_t C, int64_t G, int size, uint64_t by
 // The slab of the held form: as wide as a workgroup holds, but no wider than 128 bytes unless that leaves
 // more than kHeldGroups workgroups; 0: a sample does not fit.  threads: of that workgroup.
 // Workgroups of 1024 threads leave nothing to load beside those that compute: they are for calls that other-
-// wise wait for launches (forward and gradients of 4096 tokens of 256 channels 36 -> 32 us; 16 of them 80 -> 96).
-constexpr int kHeldGroups = 512, kHeldAlone = 128;
+// wise wait for launches (forward and gradients of 4096 tokens of 256 channels 36 -> 32 us; 16 of them 80 -> 96);
+// others get a slab that 256 hold, 32 bytes of a row at least (219 x 606 tokens of 128 bf16 channels, which
+// 1024 threads held 64 bytes of, 93 -> 74 us; 128 x 512 of 256 channels 83 -> 56).
+constexpr int kHeldGroups = 512, kHeldAlone = 128, kHeldBytes = 32;
 int held_slab(int64_t B, int64_t N, int64_t C, int64_t G, int word, int size, int *threads) {
   const int per = (int)(C / G), least = word / common(per % word ? per : word, word);
   const int64_t unit = (int64_t)least * per / word;  // words
   if (unit > kHeldWords || N > 1024 * kHeld || (int64_t)least > G) return 0;
-  int64_t best = 0;
-  for (int64_t k = 1; k * least < G + least && k * unit <= kHeldWords; k++) {
-    const int64_t words = std::min(k * unit, C / word);
-    if (N > 1024 / words * kHeld) break;
-    if (best && (words * word * size > 128 || B * ((G + k * least - 1) / (k * least)) < kHeldGroups)) break;
-    best = k;
+  for (int most : {1024, 256}) {
+    int64_t best = 0;
+    for (int64_t k = 1; k * least < G + least && k * unit <= kHeldWords; k++) {
+      const int64_t words = std::min(k * unit, C / word);
+      if (N > most / words * kHeld) break;
+      if (best && (words * word * size > 128 || B * ((G + k * least - 1) / (k * least)) < kHeldGroups)) break;
+      best = k;
+    }
+    const int64_t slab = std::min(best * least, G), words = slab * per / word;
+    if (!best || (most == 256 && slab < G && words * word * size < kHeldBytes)) return 0;
+    *threads = N <= 256 / words * kHeld ? 256 : 1024;
+    if (*threads == 256 || B * ((G + slab - 1) / slab) <= kHeldAlone) return (int)slab;
   }
-  if (!best) return 0;
-  const int64_t slab = std::min(best * least, G), words = slab * per / word;
-  *threads = N <= 256 / words * kHeld ? 256 : 1024;
-  if (*threads > 256 && B * ((G + slab - 1) / slab) > kHeldAlone) return 0;
-  return (int)slab;
+  return 0;
 }
 
 int check_sizes(int64_t B, int64_t N, int64_t C, int64_t G, int dtype) {

@@ -114,6 +114,15 @@ def test_sizes(device, size, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [(130, 512, 64, 16), (40, 606, 128, 32), (70, 700, 96, 12), (129, 300, 72, 6),
+                                  (65, 1023, 40, 20), (50, 257, 264, 33)])
+def test_samples_held_in_parts(device, size, dtype):
+    B, N, C, groups = size
+    check(*make(12, B, N, C, dtype), groups, "silu")
+    check(*make(13, B, N, C, dtype), groups, None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_without_weight_or_bias(device, dtype):
     x, w, b, go = make(2, 2, 40, 32, dtype)
     for W, b_ in ((None, None), (w, None), (None, b)):
