@@ -33,8 +33,9 @@ template <int Lanes> constexpr int kRuns = kThreads / Lanes;
 constexpr int run_steps(int word, int size) { return word == 4 || size == 4 ? 4 : 8; }
 constexpr int kSpan = kRuns<kRowLanes> * 4;  // steps from one kept state to the next, a part of every tile
 // Steps that a thread walks alone, forward (8192 sequences of 16 steps of 256 bf16 channels 54 us, in a tile 74; 512 of
-// 32 steps 20 and 13).
-constexpr int kFew = 16;
+// 32 steps 20 and 13), and backward, which holds them all in registers (20000 of 8 steps of 66, forward and gradients,
+// 64 and 154; 1500 of one step of 1661 35 and 350).
+constexpr int kFew = 16, kFewBackward = 8;
 // Workgroups aimed at by segments: as many as are resident at a time (forward, float32 backward, bf16 back-
 // ward; 768 there: 2 sequences of 32768 steps of 1024 channels 440 -> 542 us), and by the parts of the first
 // launch; workgroups from which on there are no segments (16 sequences of 4096 steps of 1024 bf16 channels, 256 of
@@ -591,7 +592,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_backward_kernel(RecurP
     for (int e = 0; e < E; e++) p.ginitial[(int64_t)at.b * p.C + at.c + e] = carry[e];
 }
 
-// Up to kFew steps: a thread walks them all.
+// Up to kFew steps, and kFewBackward backward: a thread walks them all.
 template <typename T, int E, bool Gated>
 __global__ __launch_bounds__(256) void recurrence_few_kernel(RecurParams p, int64_t words) {
   const int64_t index = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -630,6 +631,76 @@ __global__ __launch_bounds__(256) void recurrence_few_kernel(RecurParams p, int6
   }
 #pragma unroll
   for (int e = 0; e < E; e++) p.final[state + e] = h[e];
+}
+
+template <typename T, int E, bool Gated>
+__global__ __launch_bounds__(256) void recurrence_few_backward_kernel(RecurParams p, int64_t words) {
+  constexpr int K = kFewBackward;
+  const int64_t index = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (index >= words) return;
+  const int row = p.C / E;
+  Place at;
+  at.b = (int)(index / row), at.c = (int)(index % row) * E;
+  at.len = p.lengths ? min(max(p.lengths[at.b], 0), p.L) : p.L;
+  Raw<T, E> rv[K], rf[K], rg[K], ro[K];
+  int64_t to[K];
+#pragma unroll
+  for (int s = 0; s < K; s++) {
+    const int64_t t = token_of(p, at, s);
+    to[s] = ((int64_t)at.b * p.L + t) * p.C + at.c;
+    if (s < at.len) {
+      rv[s].load((const T *)p.v + at.b * p.vs[0] + t * p.vs[1] + at.c);
+      rf[s].load((const T *)p.f + at.b * p.fs[0] + t * p.fs[1] + at.c);
+      ro[s].load((const T *)p.go + to[s]);
+      if (Gated) rg[s].load((const T *)p.g + at.b * p.gs[0] + t * p.gs[1] + at.c);
+    }
+  }
+  const int64_t state = (int64_t)at.b * p.C + at.c;
+  float h[E], push[E], a[K][E], away[K][E], before[K][E], d[K][E];
+#pragma unroll
+  for (int e = 0; e < E; e++) h[e] = p.states[state + e], push[e] = p.gfinal ? p.gfinal[state + e] : 0.f;
+#pragma unroll
+  for (int s = 0; s < K; s++) {
+    float y[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) y[e] = 0.f;
+    if (s < at.len) {
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        a[s][e] = logistic<kFine<T>>(rf[s][e], away[s][e]);
+        const float x = rv[s][e];
+        before[s][e] = h[e] - x;
+        h[e] = fmaf(a[s][e], h[e], away[s][e] * x);
+        d[s][e] = ro[s][e];
+        if (Gated) {
+          const float z = rg[s][e], sg = sigmoid<kFine<T>>(z);
+          y[e] = d[s][e] * h[e] * (sg * fmaf(z, 1.f - sg, 1.f));
+          d[s][e] *= z * sg;
+        }
+      }
+    }
+    if (Gated && p.gg && s < p.L) put<T, E>((T *)p.gg + to[s], y);
+  }
+#pragma unroll
+  for (int s = K - 1; s >= 0; s--) {
+    float y1[E], y2[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) y1[e] = y2[e] = 0.f;
+    if (s < at.len) {
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float D = d[s][e] + push[e];
+        push[e] = a[s][e] * D;
+        y1[e] = away[s][e] * D;
+        y2[e] = push[e] * (before[s][e] * away[s][e]);
+      }
+    }
+    if (p.gv && s < p.L) put<T, E>((T *)p.gv + to[s], y1);
+    if (p.gf && s < p.L) put<T, E>((T *)p.gf + to[s], y2);
+  }
+  if (p.ginitial)
+#pragma unroll
+    for (int e = 0; e < E; e++) p.ginitial[state + e] = push[e];
 }
 
 // ---- host ----
@@ -761,10 +832,10 @@ int launch_tiles(const RecurParams &p, int64_t B, hipStream_t s) {
 }
 template <typename T, int E, bool Gated, bool Backward>
 int launch_steps(const RecurParams &p, int64_t B, hipStream_t s) {
-  if (!Backward && p.L <= kFew) {
+  if (p.L <= (Backward ? kFewBackward : kFew)) {
     const int64_t words = B * (p.C / E);
-    hipLaunchKernelGGL((recurrence_few_kernel<T, E, Gated>), dim3((unsigned)((words + 255) / 256)), dim3(256),
-                       0, s, p, words);
+    hipLaunchKernelGGL((Backward ? recurrence_few_backward_kernel<T, E, Gated> : recurrence_few_kernel<T, E, Gated>),
+                       dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, p, words);
     MCX_HIP_CHECK_LAUNCH();
     return MCX_OK;
   }

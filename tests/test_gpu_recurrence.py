@@ -344,6 +344,23 @@ def test_few_channels_far_apart(device, dtype):
         check(v, f, z, go, first, last, [L, L - 7], reverse, views=apart)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_steps_backward(device, dtype):
+    for L in range(1, 10):
+        for C in (1, 6, 20, 68):
+            v, f, z, go, first, last = make(16, 5, L, C, dtype)
+            for reverse in (False, True):
+                check(v, f, z, go, first, last, [L, 0, L - 1, 1, L + 3], reverse)
+                check(v, f, None, go, first, None, None, reverse)
+    for L in (1, 8):
+        args = [t.cuda() for t in make(17, 3, L, 24, dtype)]
+        _, _, saved = _C.gated_recurrence_forward(*args[:3], args[4], for_backward=True)
+        every = _C.gated_recurrence_backward(args[3], *args[:3], saved, args[5])
+        for k in range(4):
+            some = _C.gated_recurrence_backward(args[3], *args[:3], saved, args[5], needs=[n == k for n in range(4)])
+            assert all(t is None for n, t in enumerate(some) if n != k) and torch.equal(some[k], every[k])
+
+
 def test_steps_far_apart(device):
     # further than the kernels' addresses reach from a tile's first: copied
     v, f, z, go, first, last = make(11, 2, 70, 16, BF16)
