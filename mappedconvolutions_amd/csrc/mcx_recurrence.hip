@@ -13,7 +13,11 @@
 //   Where sequences and channels are too few to fill the card the steps are cut into segments, and a first
 // launch sums up the (A, H) of each: it reads two streams of four, or three of seven, a second time.  (Tiles
 // that wait for the state of the tile before them read everything once and took longer: 2 sequences of 32768
-// steps of 1024 bf16 channels forward 165 us and backward 312.)
+// steps of 1024 bf16 channels forward 165 us and backward 312.)  Few steps have a tile of as few or a thread to
+// themselves, few channels four lanes a row instead of 16.
+//   Measured in bf16 with an output gate, forward and gradients: 2048 sequences of 512 steps of 128 channels 214
+// and 384 us, 5.0 and 4.9 TB/s; 2 of 32768 steps of 1024 channels 51 + 119 and 66 + 212 us, 4.7 and 4.8 TB/s
+// with the second read (vector units 63 % of the time).  One step of 16 x 1024 channels 3.4 us.
 #include <algorithm>
 #include <type_traits>
 
