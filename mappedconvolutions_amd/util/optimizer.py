@@ -130,6 +130,8 @@ class AdamW(torch.optim.Optimizer):
         # moments keep their own types (the base class casts them to the parameters')
         ids = [i for group in state_dict['param_groups'] for i in group['params']]
         for group in self.param_groups:
+            if isinstance(group['lr'], torch.Tensor) and group['params']:
+                group['lr'] = group['lr'].to(group['params'][0].device)
             counters = {}
             for p in group['params']:
                 saved = state_dict['state'].get(ids.pop(0))

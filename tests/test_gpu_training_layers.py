@@ -251,6 +251,23 @@ def test_optimizer_goes_on_from_a_file(device, dtype, bits, capturable):
             assert value.equal(other) if isinstance(value, torch.Tensor) else value == other
 
 
+def test_a_rate_on_the_gpu_comes_back_from_a_file(device):
+    make = lambda: torch.nn.Parameter(torch.ones(10, device=device))  # noqa: E731
+    p, q = make(), make()
+    first, again = (util.AdamW([x], lr=torch.tensor(0.25, device=device), capturable=True) for x in (p, q))
+    p.grad = q.grad = torch.ones(10, device=device)
+    first.step()
+    file = io.BytesIO()
+    torch.save(first.state_dict(), file)
+    file.seek(0)
+    again.load_state_dict(torch.load(file, weights_only=True, map_location="cpu"))
+    with torch.no_grad():
+        q.copy_(p)
+    first.step()
+    again.step()
+    assert torch.equal(p, q) and again.param_groups[0]["lr"].is_cuda
+
+
 def test_optimizer_shares_a_gradient_and_copies(device):
     a, b = (torch.nn.Parameter(torch.ones(10, device=device)) for _ in range(2))
     a.grad = b.grad = torch.full((10,), 3.0, device=device)
