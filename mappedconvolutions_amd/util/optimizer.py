@@ -29,18 +29,14 @@ class AdamW(torch.optim.Optimizer):
         own = ('max_norm', 'capturable', 'seed', 'grad_norm')
         return dict(super().__getstate__(), **{name: getattr(self, name) for name in own})
 
-    def _state_of(self, p, bits, counter):
+    def _make(self, state, p, bits, counter):
         """The moments of a parameter, zeros when it first has a gradient."""
-        state = self.state[p]
-        if not state:
-            zeros = {32: torch.float32, 8: torch.uint8}[bits]
-            state['step'] = counter() if self.capturable else 0
-            for name in ('first', 'second'):
-                state[name] = torch.zeros(p.shape, dtype=zeros, device=p.device)
-                if bits == 8:
-                    state[name + '_scale'] = torch.zeros(-(-p.numel() // _C.ADAMW_BLOCK),
-                                                         device=p.device)
-        return state
+        zeros = {32: torch.float32, 8: torch.uint8}[bits]
+        state['step'] = counter() if self.capturable else 0
+        for name in ('first', 'second'):
+            state[name] = torch.zeros(p.shape, dtype=zeros, device=p.device)
+            if bits == 8:
+                state[name + '_scale'] = torch.zeros(-(-p.numel() // _C.ADAMW_BLOCK), device=p.device)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -48,28 +44,31 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        # (the same gradient of several parameters is read, and counts in the norm, once)
-        dense = {}
+        # (hundreds of parameters: each is looked at as rarely as can be.  The same gradient of several
+        # parameters is read, and counts in the norm, once)
+        dense, given = {}, []
         for group in self.param_groups:
-            for p in group['params']:
-                if p.grad is not None and p.grad not in dense:
-                    if p.grad.is_sparse:
+            gradients = [p.grad for p in group['params']]
+            given.append(gradients)
+            for g in gradients:
+                if g is not None and id(g) not in dense:
+                    if g.is_sparse:
                         raise RuntimeError('AdamW does not support sparse gradients')
-                    dense[p.grad] = p.grad.contiguous()
+                    dense[id(g)] = g.contiguous()
         if not dense:
             return loss
         capturing = torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
         if capturing:
             if not self.capturable:
                 raise RuntimeError('Only a capturable AdamW counts the steps of a captured one')
-            if any(p.grad is not None and not self.state.get(p) for group in self.param_groups
-                   for p in group['params']):
+            if any(g is not None and not self.state.get(p) for group, gradients in zip(self.param_groups, given)
+                   for p, g in zip(group['params'], gradients)):
                 raise RuntimeError('The first step of a parameter makes its moments and is not captured')
         norm = None
         if self.max_norm is not None:
             norm = self.grad_norm = _C.grad_norm(list(dense.values()))
         call = 0
-        for group in self.param_groups:
+        for group, gradients in zip(self.param_groups, given):
             made = []
 
             def counter():
@@ -79,16 +78,23 @@ class AdamW(torch.optim.Optimizer):
                 return made[0]
 
             alike, absent = {}, {}
-            for p in group['params']:
-                if p.grad is None:
+            for p, g in zip(group['params'], gradients):
+                if g is None:
                     if self.capturable and self.state.get(p):
                         absent.setdefault(id(self.state[p]['step']), []).append(self.state[p])
                     continue
-                state = self._state_of(p, group['bits'], counter)
+                state = self.state[p]
+                if not state:
+                    self._make(state, p, group['bits'], counter)
                 step = state['step']
-                key = id(step) if isinstance(step, torch.Tensor) else step
-                alike.setdefault(key, (step, []))[1].append((p, state))
-            for key, (step, members) in alike.items():
+                key = id(step) if self.capturable else step
+                if key not in alike:
+                    alike[key] = (step, [], [], [])
+                _, params, grads, states = alike[key]
+                params.append(p)
+                grads.append(dense[id(g)])
+                states.append(state)
+            for key, (step, params, grads, states) in alike.items():
                 if key in absent:  # whose counter stays behind
                     if capturing:
                         raise RuntimeError('Parameters without gradients share a counter with others: take '
@@ -96,32 +102,31 @@ class AdamW(torch.optim.Optimizer):
                     behind = step.clone()
                     for state in absent[key]:
                         state['step'] = behind
-                self._update(group, step, members, dense, norm, call)
+                self._update(group, step, params, grads, states, norm, call)
                 call += 1
         return loss
 
-    def _update(self, group, step, members, dense, norm, call):
+    def _update(self, group, step, params, grads, states, norm, call):
         counted = isinstance(step, torch.Tensor)
         step = step.add_(1) if counted else step + 1
-        params = [p if p.is_contiguous() else p.contiguous() for p, _ in members]
+        dense = list(map(torch.Tensor.contiguous, params))
         scales = {}
         if group['bits'] == 8:
-            scales = dict(first_scales=[s['first_scale'] for _, s in members],
-                          second_scales=[s['second_scale'] for _, s in members],
+            scales = dict(first_scales=[s['first_scale'] for s in states],
+                          second_scales=[s['second_scale'] for s in states],
                           seed=self.seed + 0x9E3779B1 * call)
         try:
-            _C.adamw_step(params, [dense[p.grad] for p, _ in members], [s['first'] for _, s in members],
-                          [s['second'] for _, s in members], step, group['lr'], group['betas'],
-                          group['eps'], group['weight_decay'], grad_norm=norm,
+            _C.adamw_step(dense, grads, [s['first'] for s in states], [s['second'] for s in states], step,
+                          group['lr'], group['betas'], group['eps'], group['weight_decay'], grad_norm=norm,
                           max_norm=None if norm is None else self.max_norm, **scales)
         except RuntimeError:  # a step that is refused is none
             if counted:
                 step.sub_(1)
             raise
         if not counted:
-            for _, state in members:
+            for state in states:
                 state['step'] = step
-        for changed, (p, _) in zip(params, members):
+        for changed, p in zip(dense, params):
             if changed is not p:
                 p.copy_(changed)
 
