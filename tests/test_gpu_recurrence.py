@@ -316,9 +316,9 @@ def test_many_short_sequences(device):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("C", [1, 2, 3, 6, 8, 10, 13, 24, 32])
+@pytest.mark.parametrize("C", [1, 2, 3, 4, 6, 8, 10, 13, 24, 32])
 def test_few_channels(device, C, dtype):
-    for L, lengths in ((100, [100, 37, 0]), (257, [257, 1, 256]), (700, [3, 699, 700]), (5000, [5000, 4097, 1025])):
+    for L, lengths in ((64, [64, 1, 33]), (65, [65, 64, 3]), (100, [100, 37, 0]), (257, [257, 1, 256]), (700, [3, 699, 700]), (5000, [5000, 4097, 1025])):
         v, f, z, go, first, last = make(14, 3, L, C, dtype)
         for reverse in (False, True):
             check(v, f, z, go, first, last, lengths, reverse)
