@@ -235,8 +235,8 @@ __device__ inline void carry_in(const RecurParams &p, const Place &at, Ranges<E,
     for (int e = 0; e < E; e++) carry[e] = fmaf(x.a[k][lane][e], carry[e], x.h[k][lane][e]);
 }
 
-// (A, H) of every part but those of the last segment, forward, and of the first, backward.  Gates below -20.79
-// count as that here: what they leave of the state, 10^-9, is below what 32 bits tell.
+// (A, H) of every part but those of the last segment, forward, and of the first, backward.  As in the tiles what
+// values are multiplied by is at most 1: the largest overflow nothing, whatever the gates.
 template <typename T, int E, int RowLanes, bool Gated, bool Backward>
 __global__ __launch_bounds__(kThreads) void recurrence_parts_kernel(RecurParams p) {
   constexpr int N = 4;  // steps under way
@@ -267,23 +267,47 @@ __global__ __launch_bounds__(kThreads) void recurrence_parts_kernel(RecurParams 
       rv[k].load(v + (i + k) * vs);
       if (Backward && Gated) rg[k].load(g + (i + k) * gs);
     }
+    const auto added = [&](int k, int e) {
+      const float x = rv[k][e];
+      return Backward && Gated ? x * (rg[k][e] * sigmoid<kFine<T>>(rg[k][e])) : x;
+    };
+    // one reciprocal for K steps: with x = e^-f the product of all 1 / a is D, and a value's share of the state
+    // x (backward: 1) times D of the steps before it over the last D, at most 1
+    float share[K][E], D[E];
+    bool fits = true;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      // over a common denominator, the product of all 1 / a = 1 + x, x = e^-f held below 2^30
-      float D = 1.f, M = H[e];
+      D[e] = 1.f;
 #pragma unroll
       for (int k = 0; k < K; k++) {
-        float f = __builtin_elementwise_maximum((float)rf[k][e], -20.79f);
+        float f = __builtin_elementwise_maximum((float)rf[k][e], -80.f);
         if (kFine<T>) f = __builtin_elementwise_minimum(f, 200.f);
         const float x = exponential<kFine<T>>(f);
-        float d = rv[k][e];
-        if (!Backward) d *= x;  // h = (h + x v) / (1 + x)
-        else if (Gated) d *= rg[k][e] * sigmoid<kFine<T>>(rg[k][e]);
-        M = fmaf(d, D, M), D = fmaf(x, D, D);
+        share[k][e] = Backward ? D[e] : x * D[e];
+        D[e] = fmaf(x, D[e], D[e]);
       }
-      const float r = reciprocal(D);
-      H[e] = M * r, A[e] *= r;
+      fits &= D[e] <= 0x1p120f;
     }
+    if (fits) {
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float r = reciprocal(D[e]);
+        H[e] *= r, A[e] *= r;
+#pragma unroll
+        for (int k = 0; k < K; k++) H[e] = fmaf(share[k][e] * r, added(k, e), H[e]);
+      }
+      return;
+    }
+    // (several shut gates, or one that is no number: step by step)
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        float away;
+        const float a = logistic<kFine<T>>(rf[k][e], away);
+        H[e] = Backward ? a * (added(k, e) + H[e]) : fmaf(a, H[e], away * added(k, e));
+        A[e] *= a;
+      }
   };
   int i = 0;
   for (; i + N <= hi - lo; i += N) steps(std::integral_constant<int, N>(), i);

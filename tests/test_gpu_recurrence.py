@@ -407,3 +407,69 @@ def test_more_than_32_bits_of_values(device):
     gv = _C.gated_recurrence_backward(v, v, f, None, saved, needs=(True, False, False, False))[0]
     assert (gv[0, -4:, 0] == torch.tensor([2., 4., 0., 0.], device="cuda")).all()
     assert (gv[0, 4:6, 127] == torch.tensor([1., 2.], device="cuda")).all()
+
+
+def check_at_the_ends(v, f, z, go, first, last, reverse):
+    """As check(), where gates lie far outside: forget gates below -80 count as that (a is 1.9e-35), and of the
+    output gate's silu and slope, which are below 10^-36 from -90 on, nothing need be left.  Both clamps'
+    whole effect is added to the bounds for the clamped gates: what is computed is then near c, and rounding
+    takes half a step of that."""
+    got = call(*(None if t is None else t.cuda() for t in (v, f, z, go, first, last)), None, reverse)
+    near, bounds = oracle(v, f.clamp(min=-80), None if z is None else z.clamp(min=-90), go, first, last, None, reverse)
+    far = (f < -80).any() or (z is not None and (z < -90).any())
+    want = oracle(v, f, z, go, first, last, None, reverse)[0] if far else near
+    for k, (a, b, c, e) in enumerate(zip(got, want, near, bounds)):
+        half = 2.0 ** -8 if a.dtype == BF16 else U
+        off, bound = (a.double().cpu() - b).abs(), e + (b - c).abs() + half * c.abs() + 1e-30
+        assert (off <= bound).all(), (k, (off / bound).max().item())
+
+
+# a tile; segments of four lanes, of 16, of 64 in the first launch, of words that are not whole
+SHUT_SIZES = [(2, 300, 64), (3, 2100, 8), (1, 1300, 64), (2, 700, 320), (2, 1100, 33)]
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", SHUT_SIZES)
+def test_shut_gates_and_large_values(device, size, dtype, reverse):
+    B, L, C = size
+    for gated, shut, large in ((True, -21.0, 1e3), (False, -25.0, 1e4), (True, -1e30, 1e30),
+                               (False, -float("inf"), 300.0)):
+        v, f, z, go, first, last = make(18, B, L, C, dtype)
+        v *= large
+        first *= large
+        # runs of shut gates of many lengths, one of hundreds of steps
+        at = torch.arange(L)[:, None] + 7 * torch.arange(C)
+        f[:, (at % 64) % 11 < 5] = shut
+        f[:, L // 2:L // 2 + 150] = shut
+        check_at_the_ends(v, f, z if gated else None, go, first, last, reverse)
+    f[:] = -30.0  # all of them
+    check_at_the_ends(v, f, z, go, first, last, reverse)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", SHUT_SIZES)
+def test_a_shut_gate_resets_a_large_state(device, size, dtype, reverse):
+    B, L, C = size
+    for gated, shut in ((False, -60.0), (True, -100.0)):
+        v, f, z, go, first, last = make(19, B, L, C, dtype)
+        f[:, L // 2] = shut  # e^-60 = 9e-27 of the state is left
+        if gated:  # and at the ends, where the states come in
+            f[:, 0], f[:, -1] = shut, shut
+        check_at_the_ends(v, f, z if gated else None, go, 1e12 * first, 1e12 * last, reverse)
+
+
+def test_a_batch_does_not_change_its_sequences(device):
+    """The same sequences in a batch that is cut into segments and in one that is not, where gates are shut and
+    values large: both are within the same bound of the exact state."""
+    v, f, z, go, first, last = make(21, 1, 1300, 64, BF16)
+    f[:, ::2], f[:, 40:90] = -30.0, -30.0
+    v *= 500
+    few, many = ([t.cuda().repeat(B, *[1] * (t.dim() - 1)) for t in (v, f, z, go, first, last)] for B in (1, 300))
+    bounds = oracle(v, f, z, go, first, last, None, False)
+    for k, (a, b, want, e) in enumerate(zip(call(*few, None, False), call(*many, None, False), *bounds)):
+        half = 2.0 ** -8 if a.dtype == BF16 else U
+        off = (a.double() - b[:1].double()).abs().cpu()
+        assert (off <= 2 * (e + half * want.abs()) + 1e-30).all(), k
+        assert torch.equal(b, b[:1].expand_as(b))
