@@ -112,10 +112,12 @@ template <bool Fine> __device__ inline float logistic(float x, float &away) {
   away = e * a;
   return a;
 }
-// The same for an output gate, which nothing adds up over.
+// The same for an output gate, which nothing adds up over and which is multiplied by it: nothing is left of it
+// where e^-x leaves the range (x below -87, where x sigmoid(x) is above -1.5e-36).
 template <bool Fine> __device__ inline float sigmoid(float x) {
-  float away;
-  return Fine ? logistic<true>(x, away) : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504f));
+  if (!Fine) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504f));
+  const float y = __builtin_elementwise_minimum(__builtin_elementwise_maximum(x, -87.f), 200.f);
+  return x < -87.f ? 0.f : reciprocal(1.f + exponential<true>(y));
 }
 template <typename T> constexpr bool kFine = sizeof(T) == 4;
 

@@ -473,3 +473,17 @@ def test_a_batch_does_not_change_its_sequences(device):
         off = (a.double() - b[:1].double()).abs().cpu()
         assert (off <= 2 * (e + half * want.abs()) + 1e-30).all(), k
         assert torch.equal(b, b[:1].expand_as(b))
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [(3, 1, 24), (3, 6, 24), (3, 14, 24)] + SHUT_SIZES)
+def test_output_gates_far_from_zero(device, size, dtype, reverse):
+    v, f, z, go, first, last = make(20, *size, dtype)
+    for i, far in enumerate((-88.0, -100.0, -1e30, torch.finfo(dtype).min, 100.0, 1e4)):
+        z[..., i::8] = far
+    check_at_the_ends(v, f, z, go, first, last, reverse)
+    # what is no number stays none, and stays where it is
+    z[0, 0, 0] = float("nan")
+    out, final, _ = _C.gated_recurrence_forward(v.cuda(), f.cuda(), z.cuda(), first.cuda(), None, reverse)
+    assert torch.isnan(out[0, 0, 0]) and torch.isnan(out).sum() == 1 and torch.isfinite(final).all()
