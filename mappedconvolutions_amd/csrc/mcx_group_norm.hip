@@ -80,16 +80,18 @@ template <bool Fine> __device__ inline float exponential(float x) {
   return Fine ? fmaf(e, 0.69314718f * fmaf(x, kRest, fmaf(x, kLog2e, -t)), e) : e;
 }
 template <bool Fine> __device__ inline float logistic(float x) {
-  if (Fine) {  // (an infinite power has no rounding to put back; what is no number stays none)
-    x = x < -80.f ? -80.f : x;
-    x = x > 80.f ? 80.f : x;
-  }
-  return __builtin_amdgcn_rcpf(1.f + exponential<Fine>(-x));
+  if (!Fine) return __builtin_amdgcn_rcpf(1.f + exponential<false>(-x));
+  // (an infinite power has no rounding to put back: 0 where e^-x leaves the range, since u is multiplied by it;
+  // what is no number stays none)
+  const float y = __builtin_elementwise_minimum(__builtin_elementwise_maximum(x, -87.f), 80.f);
+  return x < -87.f ? 0.f : __builtin_amdgcn_rcpf(1.f + exponential<true>(-y));
 }
 // (1 + erf(u / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun, off by 7.5e-8 at most; `bell` is
-// e^(-u^2 / 2).  It costs a third of the library's erf, which the vector units took longer for than memory.
+// e^(-u^2 / 2), down to 0: the slope multiplies it by u.  It costs a third of the library's erf, which the vector
+// units took longer for than memory.
 template <bool Fine> __device__ inline float normal(float u, float &bell) {
-  const float q = Fine ? fminf(u * u, 170.f) : u * u;
+  // (an infinite power has no rounding to put back)
+  const float q = Fine ? fminf(u * u, 1000.f) : u * u;
   bell = Fine ? exponential<true>(-0.5f * q) : __builtin_amdgcn_exp2f(-0.72134752f * q);
   const float t = __builtin_amdgcn_rcpf(fmaf(0.23164190f, fabsf(u), 1.f));
   float s = fmaf(0.5307027145f, t, -0.7265760135f);

@@ -291,3 +291,32 @@ def test_more_than_32_bits_of_values(device):
     # all others: zero but for the mean's error
     assert (y.abs() > 64 * U * 8 * r).sum().item() == 8 and (y[..., :60] == 0).all()
     assert abs(saved[0, 15, 1].item() - r) < 1e-4 * r
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [(2, 60, 32), (1, 1, 32), (2, 20000, 32)])
+def test_biases_that_shut_or_open_a_channel(device, size, dtype, activation):
+    """Far below zero an activation and its slope vanish, far above it they are u and 1: gradients are those
+    of channels whose gradient is zero, or of no activation, to the bit."""
+    x, w, b, go = (t.cuda() for t in make(14, *size, dtype))
+    for far in (-1e30, -torch.finfo(dtype).max, 1e30, torch.finfo(dtype).max):
+        bias = b.clone()
+        bias[::5] = far
+        shut = torch.zeros(size[2], dtype=torch.bool, device="cuda")
+        shut[::5] = True
+        y, saved = _C.group_norm_forward(x, 4, w, bias, activation=activation, for_backward=True)
+        gx, gw, gb = _C.group_norm_backward(go, x, saved, 4, w, bias, activation=activation)
+        y0, _ = _C.group_norm_forward(x, 4, w, b, activation=activation)
+        assert torch.equal(y[..., ~shut], y0[..., ~shut])
+        assert all(torch.isfinite(t).all() for t in (gx, gw, gb))
+        if far < 0:
+            assert (y[..., shut] == 0).all() and (gw[shut] == 0).all() and (gb[shut] == 0).all()
+            none = torch.where(shut, 0.0, go).to(dtype)
+            gx0, gw0, gb0 = _C.group_norm_backward(none, x, saved, 4, w, b, activation=activation)
+            assert torch.equal(gx, gx0) and torch.equal(gw, gw0) and torch.equal(gb, gb0)
+        else:
+            # (n w is lost next to the bias)
+            assert torch.equal(y[..., shut], bias[shut].expand_as(y[..., shut]))
+            gb0 = _C.group_norm_backward(go, x, saved, 4, w, b)[2]
+            assert torch.equal(gb[shut], gb0[shut])
