@@ -104,6 +104,12 @@ def _stream(t):
     return _raw_stream(t.get_device())
 
 
+def _changed(tensors):
+    """Tells torch which tensors a kernel has written in place: graphs that have saved them refuse their
+    backward pass then, and plans of a map are made anew."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 _here = contextlib.nullcontext()
 
 
@@ -1156,6 +1162,7 @@ def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
         rc = lib.mcx_clip_grad_norm(*hosts, n, max_norm, eps, _ptr(norm), _ptr(ws), nbytes,
                                     _stream(norm))
     _lib.check(rc, "clip_grad_norm")
+    _changed(every[-n:])
     return norm
 
 
@@ -1222,7 +1229,8 @@ def gated_recurrence_forward(value, forget, gate=None, initial=None, lengths=Non
     if initial is not None:
         initial = initial.contiguous()
     out = value.new_empty((B, L, C))
-    if final is None:
+    given = final is not None
+    if not given:
         final = torch.empty((B, C), dtype=torch.float32, device=value.device)
     lib = _lib.load()
     states = None
@@ -1241,6 +1249,8 @@ def gated_recurrence_forward(value, forget, gate=None, initial=None, lengths=Non
                                               _ptr(lengths), _ptr(out), _ptr(final), _ptr(states),
                                               _ptr(ws), nbytes, desc, dt, _stream(value))
     _lib.check(rc, "gated_recurrence_forward")
+    if given:
+        _changed(final)
     return [out, final, states]
 
 
@@ -1476,7 +1486,8 @@ def adamw_step(params, grads, first_moments, second_moments, step, lr, betas=(0.
     if not wide and [-(-k // ADAMW_BLOCK) for k in sizes[:n]] * 2 != sizes[4 * n:]:
         raise RuntimeError("there must be one scale for %d values of a tensor" % ADAMW_BLOCK)
     written = at[:n] + at[2 * n:]
-    if len(set(written)) != len(written) or not set(written).isdisjoint(at[n:2 * n]):
+    places = set(written)
+    if len(places) != len(written) or not places.isdisjoint(at[n:2 * n]):
         # (tensors without values may share an address)
         full = [a for a, k in zip(written, sizes[:n] + sizes[2 * n:]) if k]
         if len(set(full)) != len(full) or \
@@ -1498,6 +1509,7 @@ def adamw_step(params, grads, first_moments, second_moments, step, lr, betas=(0.
         rc = _lib.load().mcx_adamw_step(*hosts, sizes.buffer_info()[0], types_at, types_at + 4 * n, n,
                                         options, _stream(first))
     _lib.check(rc, "adamw_step")
+    _changed(lists[0] + every[2 * n:])
 
 
 def adamw_moment(codes, scales, second, dtype=torch.float32):

@@ -425,3 +425,77 @@ def test_gradient_of_the_example_against_differences(device):
             for p, w in zip(params, way):
                 p.sub_(w, alpha=sign * h)
     assert abs((values[0] - values[1]) / (2 * h) - slope) <= 1e-2 * (1 + abs(slope))
+
+
+# ---- what is changed in place ---------------------------------------------------------------
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_graph_refuses_weights_that_a_step_has_changed(device, bits):
+    for p in parameters():
+        optimizer = util.AdamW([p], lr=0.1, bits=bits, max_norm=1.0)
+        x = torch.randn_like(p, requires_grad=True)
+        loss = (p * x).square().sum()
+        loss.backward(retain_graph=True)
+        before = p._version
+        optimizer.step()
+        assert p._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    # moments and scales are changed too, gradients are not
+    p, g, m, v = (torch.ones(300, device=device) for _ in range(4))
+    _C.adamw_step([p], [g], [m], [v], 1, 1e-3)
+    assert p._version and m._version and v._version and not g._version
+    with torch.inference_mode():
+        p, g, m, v = (torch.ones(300, device=device) for _ in range(4))
+        _C.adamw_step([p], [g], [m], [v], 1, 1e-3)
+
+
+def test_a_graph_refuses_a_state_that_a_step_has_changed(device):
+    scan = nn.GatedRecurrence()
+    for L in (0, 1, 30):
+        x = torch.randn(2, L, 8, device=device)
+        state, weight = torch.randn(2, 8, device=device), torch.randn(2, 8, device=device, requires_grad=True)
+        y = (weight * state).sum()
+        scan.step(state, x, x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        first = torch.randn(2, 8, device=device, requires_grad=True)
+        _, final = scan(x, x, initial=first)  # (a state of its own)
+        final.sum().backward()
+        assert first.grad is not None
+
+
+def test_a_graph_refuses_gradients_that_were_clipped(device):
+    p = torch.nn.Parameter(torch.randn(300, device=device))
+    p.grad = torch.randn(300, device=device)
+    weight = torch.randn(300, device=device, requires_grad=True)
+    y = (weight * p.grad).sum()
+    util.clip_grad_norm_([p], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    x, out = torch.randn(300, device=device), torch.empty(300, device=device)
+    _C.clip_grad_norm([x], 1.0, out=[out])
+    assert not x._version and out._version
+
+
+def test_a_plan_follows_a_map_that_a_step_has_changed(device):
+    torch.manual_seed(1)
+    layer = nn.MappedConvolution(4, 4, 9, cache_plan=True).to(device)
+    plain = nn.MappedConvolution(4, 4, 9).to(device)
+    plain.load_state_dict(layer.state_dict())
+    sample_map = torch.nn.Parameter(util.latitude_map(16, 32).to(device))
+    x = torch.randn(2, 4, 16, 32, device=device)
+    optimizer = util.AdamW([sample_map], lr=0.5, weight_decay=0.0)
+    gy = torch.randn(2, 4, 16, 32, device=device)
+    for k in range(3):
+        outs = []
+        for one in (layer, plain):
+            image = x.clone().requires_grad_()
+            y = one(image, sample_map.detach())
+            y.backward(gy)
+            outs.append((y.detach(), image.grad))
+        for a, b in zip(*outs):
+            # sums of 9 x 4 products of values below 8, in an order that a plan may change
+            assert (a - b).abs().max().item() <= 64 * 36 * 8 * U
+        sample_map.grad = torch.randn_like(sample_map)
+        optimizer.step()
