@@ -1450,6 +1450,14 @@ def adamw_step(params, grads, first_moments, second_moments, step, lr, betas=(0.
     value on the GPU; both are read there when the kernels run, so that a captured step can be replayed.
     What is changed must not share memory with any other tensor: one that stands in the lists twice
     is refused, parts that overlap are not looked for."""
+    _adamw_call(params, grads, first_moments, second_moments, step, lr, betas, eps, weight_decay,
+                first_scales, second_scales, seed, grad_norm, max_norm)()
+
+
+def _adamw_call(params, grads, first_moments, second_moments, step, lr, betas, eps, weight_decay,
+                first_scales=None, second_scales=None, seed=0, grad_norm=None, max_norm=None):
+    """adamw_step's checks -> what launches the step, so that a caller can have several steps checked before
+    the first of them changes anything."""
     if (first_scales is None) != (second_scales is None):
         raise RuntimeError("first_scales and second_scales go together")
     if (grad_norm is None) != (max_norm is None):
@@ -1472,7 +1480,7 @@ def adamw_step(params, grads, first_moments, second_moments, step, lr, betas=(0.
     if set(map(len, lists)) != {n}:
         raise RuntimeError("every list must have as many tensors: %s" % list(map(len, lists)))
     if not n:
-        return
+        return lambda: None
     every = sum(lists, [])
     at, sizes = _together(every)
     dtypes = [t.dtype for t in every]
@@ -1503,13 +1511,16 @@ def adamw_step(params, grads, first_moments, second_moments, step, lr, betas=(0.
         int(seed) & 0xFFFFFFFF, 32 if wide else 8)
     # (host arrays of the library's types, which live until it has returned)
     at, sizes = array.array("Q", at), array.array("q", sizes[:n])
-    hosts = [at.buffer_info()[0] + 8 * n * k for k in range(4 if wide else 6)] + [None] * (2 * wide)
-    types_at = types.buffer_info()[0]
-    with _device(first):
-        rc = _lib.load().mcx_adamw_step(*hosts, sizes.buffer_info()[0], types_at, types_at + 4 * n, n,
-                                        options, _stream(first))
-    _lib.check(rc, "adamw_step")
-    _changed(lists[0] + every[2 * n:])
+
+    def run():
+        types_at = types.buffer_info()[0]
+        hosts = [at.buffer_info()[0] + 8 * n * k for k in range(4 if wide else 6)] + [None] * (2 * wide)
+        with _device(first):
+            rc = _lib.load().mcx_adamw_step(*hosts, sizes.buffer_info()[0], types_at, types_at + 4 * n, n,
+                                            options, _stream(first))
+        _lib.check(rc, "adamw_step")
+        _changed(lists[0] + every[2 * n:])
+    return run
 
 
 def adamw_moment(codes, scales, second, dtype=torch.float32):

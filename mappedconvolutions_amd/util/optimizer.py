@@ -67,7 +67,8 @@ class AdamW(torch.optim.Optimizer):
         norm = None
         if self.max_norm is not None:
             norm = self.grad_norm = _C.grad_norm(list(dense.values()))
-        call = 0
+        # (all are checked before the first changes anything: a step that is refused leaves all as it was)
+        updates = []
         for group, gradients in zip(self.param_groups, given):
             made = []
 
@@ -102,33 +103,41 @@ class AdamW(torch.optim.Optimizer):
                     behind = step.clone()
                     for state in absent[key]:
                         state['step'] = behind
-                self._update(group, step, params, grads, states, norm, call)
-                call += 1
+                updates.append(self._update(group, step, params, grads, states, norm, len(updates)))
+        for update in updates:
+            update()
         return loss
 
     def _update(self, group, step, params, grads, states, norm, call):
+        """-> what changes parameters that share a count."""
         counted = isinstance(step, torch.Tensor)
-        step = step.add_(1) if counted else step + 1
         dense = list(map(torch.Tensor.contiguous, params))
         scales = {}
         if group['bits'] == 8:
             scales = dict(first_scales=[s['first_scale'] for s in states],
                           second_scales=[s['second_scale'] for s in states],
                           seed=self.seed + 0x9E3779B1 * call)
-        try:
-            _C.adamw_step(dense, grads, [s['first'] for s in states], [s['second'] for s in states], step,
-                          group['lr'], group['betas'], group['eps'], group['weight_decay'], grad_norm=norm,
-                          max_norm=None if norm is None else self.max_norm, **scales)
-        except RuntimeError:  # a step that is refused is none
+        number = step if counted else step + 1
+        launch = _C._adamw_call(dense, grads, [s['first'] for s in states], [s['second'] for s in states], number,
+                                group['lr'], group['betas'], group['eps'], group['weight_decay'], grad_norm=norm,
+                                max_norm=None if norm is None else self.max_norm, **scales)
+
+        def update():
             if counted:
-                step.sub_(1)
-            raise
-        if not counted:
-            for state in states:
-                state['step'] = step
-        for changed, p in zip(dense, params):
-            if changed is not p:
-                p.copy_(changed)
+                step.add_(1)
+            try:
+                launch()
+            except RuntimeError:  # a step that is not launched is none
+                if counted:
+                    step.sub_(1)
+                raise
+            if not counted:
+                for state in states:
+                    state['step'] = number
+            for changed, p in zip(dense, params):
+                if changed is not p:
+                    p.copy_(changed)
+        return update
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)

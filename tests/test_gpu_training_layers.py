@@ -499,3 +499,39 @@ def test_a_plan_follows_a_map_that_a_step_has_changed(device):
             assert (a - b).abs().max().item() <= 64 * 36 * 8 * U
         sample_map.grad = torch.randn_like(sample_map)
         optimizer.step()
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_step_changes_nothing_in_any_group(device, bits, capturable):
+    """What is refused in the last list, and taken again once it is mended, is the step that was never
+    refused."""
+    def make():
+        ps = parameters()
+        groups = [dict(params=ps[:2]), dict(params=ps[2:4]), dict(params=ps[4:], lr=0.01)]
+        return ps, util.AdamW(groups, lr=0.1, bits=bits, max_norm=1.0, capturable=capturable)
+
+    (ours, optimizer), (other, twin) = make(), make()
+    for k, skip in enumerate(((3,), (), ())):  # counts differ within a group: four lists
+        give_gradients(ours, k, skip)
+        give_gradients(other, k, skip)
+        if k:
+            before = [[p.clone()] + [t.clone() if isinstance(t, torch.Tensor) else t
+                                     for t in optimizer.state[p].values()] for p in ours]
+            optimizer.param_groups[2]["lr"] = float("nan")
+            with pytest.raises(RuntimeError, match="finite"):
+                optimizer.step()
+            optimizer.param_groups[2]["lr"] = 0.01
+            good, optimizer.state[ours[4]]["first"] = optimizer.state[ours[4]]["first"], ours[4].detach().half()
+            with pytest.raises(RuntimeError, match="moments"):
+                optimizer.step()
+            optimizer.state[ours[4]]["first"] = good
+            for p, kept in zip(ours, before):
+                for a, b in zip([p] + list(optimizer.state[p].values()), kept):
+                    assert torch.equal(a, b) if isinstance(a, torch.Tensor) else a == b
+        optimizer.step()
+        twin.step()
+    for p, q in zip(ours, other):
+        assert torch.equal(p, q) and int(optimizer.state[p]["step"]) == int(twin.state[q]["step"])
+        for name in ("first", "second"):
+            assert torch.equal(optimizer.state[p][name], twin.state[q][name])

@@ -206,3 +206,28 @@ def test_a_refused_step_is_not_counted(capturable, monkeypatch):
     monkeypatch.undo()
     assert opt.state_dict()["state"] == {}
     assert util.AdamW([p]).load_state_dict(opt.state_dict()) is None
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_nothing_is_launched_before_all_is_checked(capturable, monkeypatch):
+    params = [torch.nn.Parameter(torch.zeros(n)) for n in (3, 4, 5)]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt = util.AdamW([dict(params=params[:2]), dict(params=params[2:], lr=0.5)], capturable=capturable)
+    seen = []
+
+    def checked(ps, grads, first, second, step, lr, *rest, **kw):
+        if lr == 0.5 and refuse:
+            raise RuntimeError("refused")
+        seen.append("checked")
+        return lambda: seen.append("launched")
+
+    monkeypatch.setattr(_C, "_adamw_call", checked)
+    refuse = True
+    with pytest.raises(RuntimeError, match="refused"):
+        opt.step()
+    assert seen == ["checked"] and [int(opt.state[p]["step"]) for p in params] == [0, 0, 0]
+    refuse = False
+    opt.step()
+    assert seen[1:] == ["checked", "checked", "launched", "launched"]
+    assert [int(opt.state[p]["step"]) for p in params] == [1, 1, 1]
