@@ -36,7 +36,8 @@ class AdamW(torch.optim.Optimizer):
         for name in ('first', 'second'):
             state[name] = torch.zeros(p.shape, dtype=zeros, device=p.device)
             if bits == 8:
-                state[name + '_scale'] = torch.zeros(-(-p.numel() // _C.ADAMW_BLOCK), device=p.device)
+                state[name + '_scale'] = torch.zeros(-(-p.numel() // _C.ADAMW_BLOCK), dtype=torch.float32,
+                                                     device=p.device)
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -535,3 +535,21 @@ def test_a_refused_step_changes_nothing_in_any_group(device, bits, capturable):
         assert torch.equal(p, q) and int(optimizer.state[p]["step"]) == int(twin.state[q]["step"])
         for name in ("first", "second"):
             assert torch.equal(optimizer.state[p][name], twin.state[q][name])
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float64])
+def test_a_step_in_8_bits_under_another_default(device, dtype):
+    def run():
+        p = torch.nn.Parameter(torch.ones(300, dtype=F32, device=device))
+        p.grad = torch.full((300,), 0.5, dtype=F32, device=device)
+        optimizer = util.AdamW([p], lr=0.1, bits=8, max_norm=1.0)
+        optimizer.step()
+        return p.detach()
+
+    want, before = run(), torch.get_default_dtype()
+    torch.set_default_dtype(dtype)
+    try:
+        got = run()
+    finally:
+        torch.set_default_dtype(before)
+    assert torch.equal(got, want)

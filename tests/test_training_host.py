@@ -231,3 +231,19 @@ def test_nothing_is_launched_before_all_is_checked(capturable, monkeypatch):
     opt.step()
     assert seen[1:] == ["checked", "checked", "launched", "launched"]
     assert [int(opt.state[p]["step"]) for p in params] == [1, 1, 1]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_moments_keep_their_types_under_another_default(dtype):
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(dtype)
+    try:
+        p = torch.nn.Parameter(torch.zeros(300, dtype=torch.float32))
+        p.grad = torch.ones_like(p)
+        opt = util.AdamW([p], bits=8)
+        with pytest.raises(RuntimeError, match="one GPU"):
+            opt.step()
+    finally:
+        torch.set_default_dtype(before)
+    assert {n: t.dtype for n, t in opt.state[p].items() if isinstance(t, torch.Tensor)} == dict(
+        first=torch.uint8, second=torch.uint8, first_scale=torch.float32, second_scale=torch.float32)
