@@ -297,3 +297,73 @@ def test_many_values(device):
     assert p[-1].item() == -0.5 and p[3].item() == 0.5 and p.count_nonzero().item() == 2
     tail = _C.adamw_moment(m[-300:].contiguous()[-44:].clone(), ms[-1:], False)
     assert abs(tail[-1].item() - 0.4) <= 0.4 / 8 and tail[:-1].abs().sum() == 0
+
+
+def equal(one, other, names="p m v ms vs", last=None):
+    for name in names.split():
+        for a, b in zip(getattr(one, name)[-last:] if last else getattr(one, name),
+                        getattr(other, name)[-last:] if last else getattr(other, name)):
+            assert torch.equal(a, b), name
+
+
+def test_parts_of_a_list_give_the_bits_of_the_whole(device):
+    """In 32 bits a tensor's result does not depend on what stands in the list beside it: in which launch it is,
+    and how long its chunks are (2048 values in a list of 9 million, 1024 alone)."""
+    sizes = [5000, 70, 100003, 1, 16385, 40000] + [300 + i for i in range(60)] + [9000001, 257, 2049]
+    types = (F32, BF16, F32), (BF16, F32)
+    whole, alone, parts = (Problem(12, sizes, 32, *types) for _ in range(3))
+    numbers = (3, 1e-2, (0.9, 0.999), 1e-8, 0.1)
+    clip = dict(grad_norm=_C.grad_norm(whole.g), max_norm=0.5)
+    _C.adamw_step(whole.p, whole.g, whole.m, whole.v, *numbers, **clip)
+    for t in range(len(sizes)):
+        _C.adamw_step(alone.p[t:t + 1], alone.g[t:t + 1], alone.m[t:t + 1], alone.v[t:t + 1], *numbers, **clip)
+    for part in (slice(0, 7), slice(7, 66), slice(66, None)):
+        _C.adamw_step(parts.p[part], parts.g[part], parts.m[part], parts.v[part], *numbers, **clip)
+    equal(whole, alone)
+    equal(whole, parts)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_address_does_not_change_the_bits(device, bits):
+    sizes = [300, 5000, 1, 256, 16385] + [77] * 60
+    problems = [Problem(13, sizes, bits, (F32, BF16, F32), (BF16, F32), at) for at in (0, 1, 2, 4)]
+    for one in problems:
+        _C.adamw_step(one.p, one.g, one.m, one.v, 5, 1e-3, weight_decay=0.1, **one.scales(seed=9))
+    for one in problems[1:]:
+        equal(problems[0], one)
+
+
+def test_places_in_8_bits_count_on_over_launches(device):
+    """A value's place is counted in blocks of 256 from the list's first: behind 60 tensors of 90 blocks in all,
+    in a second launch, tensors are rounded as behind one of 90 blocks, and otherwise than behind none."""
+    tail = [700, 256, 4097, 3]
+    many, one, none = ([300] * 30 + [40] * 30, [90 * 256 - 1], [])
+    problems = []
+    for lead in (many, one, none):
+        problem = Problem(14, lead + tail, 8)
+        last = Problem(15, tail, 8)  # the same tensors at the end of every list
+        for name in ("p", "g", "m", "v", "ms", "vs"):
+            getattr(problem, name)[len(lead):] = getattr(last, name)
+        _C.adamw_step(problem.p, problem.g, problem.m, problem.v, 5, 1e-3, **problem.scales(seed=9))
+        problems.append(problem)
+    assert sum(map(oracle.blocks, many)) == sum(map(oracle.blocks, one)) == 90
+    equal(problems[0], problems[1], last=len(tail))
+    equal(problems[0], problems[2], "p ms vs", last=len(tail))  # (what is not rounded at random)
+    assert not torch.equal(problems[0].m[-2], problems[2].m[-2])
+
+
+def test_scales_of_8_bits(device):
+    """Twice the power of two below a block's largest value, where that is not so near to a power of two (see
+    above) that 32 bits tell otherwise; zero where all are."""
+    problem = Problem(16, [1000, 256, 257, 5, 40000], 8)
+    problem.m[1].zero_(), problem.v[1].zero_(), problem.g[1].zero_()
+    before = [(p.double().cpu(), g.cpu(), m, v) for p, g, (m, v) in zip(problem.p, problem.g, problem.moments())]
+    _C.adamw_step(problem.p, problem.g, problem.m, problem.v, 5, 1e-3, **problem.scales())
+    for (p, g, m, v), ms, vs in zip(before, problem.ms, problem.vs):
+        _, m, v, _, _ = oracle.step(p, g, m, v, 5, 1e-3)
+        for exact, got in ((m, ms), (v, vs)):
+            top = oracle.per_block(exact.abs()).amax(1)
+            want = torch.where(top > 0, 2 ** (torch.floor(torch.log2(top.clamp_min(1e-300))) + 1), 0.0)
+            part = top / want.clamp_min(1e-300)
+            sure = (top == 0) | (torch.minimum(part - 0.5, 1 - part) > 2.0 ** -16)
+            assert sure.float().mean() > 0.9 and torch.equal(got.double().cpu()[sure], want[sure])
