@@ -19,11 +19,14 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32,
                  max_norm=None, capturable=False, seed=0):
-        if bits not in (32, 8):
-            raise ValueError('Moments are held in 32 or 8 bits')
         self.max_norm, self.capturable, self.seed, self.grad_norm = max_norm, capturable, seed, None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                                       bits=bits))
+
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict) and param_group.get('bits', self.defaults['bits']) not in (32, 8):
+            raise ValueError('Moments are held in 32 or 8 bits')
+        super().add_param_group(param_group)
 
     def __getstate__(self):
         own = ('max_norm', 'capturable', 'seed', 'grad_norm')

@@ -247,3 +247,14 @@ def test_moments_keep_their_types_under_another_default(dtype):
         torch.set_default_dtype(before)
     assert {n: t.dtype for n, t in opt.state[p].items() if isinstance(t, torch.Tensor)} == dict(
         first=torch.uint8, second=torch.uint8, first_scale=torch.float32, second_scale=torch.float32)
+
+
+def test_a_group_of_other_bits_is_refused():
+    a, b = (torch.nn.Parameter(torch.zeros(3)) for _ in range(2))
+    with pytest.raises(ValueError, match="32 or 8"):
+        util.AdamW([dict(params=[a]), dict(params=[b], bits=16)])
+    opt = util.AdamW([a], bits=8)
+    with pytest.raises(ValueError, match="32 or 8"):
+        opt.add_param_group(dict(params=[b], bits=4))
+    opt.add_param_group(dict(params=[b], bits=32))
+    assert [g["bits"] for g in opt.param_groups] == [8, 32]
