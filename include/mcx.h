@@ -507,7 +507,7 @@ typedef struct mcx_recurrence_desc {
 } mcx_recurrence_desc;
 
 /* a_t = sigmoid(forget_t),  h_t = a_t h_{t-1} + (1 - a_t) value_t,
- * out_t = h_t gate_t sigmoid(gate_t), or h_t where gate is NULL
+ * out_t = h_t gate_t sigmoid(gate_t), or h_t where gate is NULL (forget gates below -80 count as -80)
  * over the steps t < lengths[b] (int32 [B], or NULL: L; clamped to [0, L]), from `initial` (float [B,
  * C], or NULL: zeros).  What lies behind the steps in use is not read, and out is zero there.
  * out [B, L, C] is contiguous; final float [B, C] is the state after the last step in use, and may be

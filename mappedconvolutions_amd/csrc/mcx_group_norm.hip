@@ -10,7 +10,9 @@
 // of kRows tokens about each block's own mean and merged (counts, means and squared deviations), so a
 // mean far from zero costs nothing.  Statistics of the parts, then products: two launches forward, and
 // a third between them backward that joins the parts' sums.  No atomics: the same bits from call to call.
-// Samples that a workgroup's registers hold a slab of take one launch and are read once.
+// Samples that a workgroup's threads hold a slab of take one launch and are read once; every sample has a work-
+// group of its own at least, most of whose threads are idle where samples are a token or a few (65536 samples of a
+// token of 128 channels 576 us).
 //   Measured in bf16: 8 x 131072 tokens of 64 channels with silu statistics 33 us, products 50, sums 52, their join
 // 5, gradients 68 (4.1, 5.4, 5.2 and 5.9 TB/s; a large copy 4.8: what was read last is read first from the cache).  32 x
 // 2048 tokens of 512 channels with gelu 14, 31, 35, 5 and 42 us: there the vector units are busy 74 to 85 %
@@ -86,9 +88,9 @@ template <bool Fine> __device__ inline float logistic(float x) {
   const float y = __builtin_elementwise_minimum(__builtin_elementwise_maximum(x, -87.f), 80.f);
   return x < -87.f ? 0.f : __builtin_amdgcn_rcpf(1.f + exponential<true>(-y));
 }
-// (1 + erf(u / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun, off by 7.5e-8 at most; `bell` is
-// e^(-u^2 / 2), down to 0: the slope multiplies it by u.  It costs a third of the library's erf, which the vector
-// units took longer for than memory.
+// (1 + erf(u / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun, off by 7.5e-8 at most (in all: far below zero
+// few digits are right); `bell` is e^(-u^2 / 2), down to 0: the slope multiplies it by u.  It costs a third of the
+// library's erf, which the vector units took longer for than memory.
 template <bool Fine> __device__ inline float normal(float u, float &bell) {
   // (an infinite power has no rounding to put back)
   const float q = Fine ? fminf(u * u, 1000.f) : u * u;
@@ -544,8 +546,10 @@ __global__ __launch_bounds__(kThreads) void group_gradient_kernel(GroupParams p)
 
 // ---- samples whose slab a workgroup holds ----
 //
-// Up to kHeld words a thread stay in registers between the statistics and the products, so that everything
-// is read once, by one launch (and a second small one for the sums over the samples).
+// Up to kHeld words a thread stay there between the statistics and the products, so that everything is read
+// once, by one launch (and a second small one for the sums over the samples).  They stay in registers but for some
+// kernels of 1024 threads, which have 128 each, and words of 8 bf16 values: those whose words lie in several
+// groups, and gradients with an activation, keep 12 to 132 bytes a lane in scratch memory.
 
 constexpr int kHeld = 8;
 constexpr int kHeldWords = 32;            // words of a slab at most

@@ -16,7 +16,7 @@
 // steps of 1024 bf16 channels forward 165 us and backward 312.)  Few steps have a tile of as few or a thread to
 // themselves, few channels four lanes a row instead of 16.
 //   Measured in bf16 with an output gate, forward and gradients: 2048 sequences of 512 steps of 128 channels 214
-// and 384 us, 5.0 and 4.9 TB/s; 2 of 32768 steps of 1024 channels 51 + 119 and 66 + 212 us, 4.7 and 4.8 TB/s
+// and 384 us, 5.0 and 4.9 TB/s; 2 of 32768 steps of 1024 channels 51 + 119 and 65 + 212 us, 4.7 and 4.8 TB/s
 // with the second read (vector units 63 % of the time).  One step of 16 x 1024 channels 3.4 us.
 #include <algorithm>
 #include <type_traits>
